@@ -86,6 +86,24 @@ SIGNATURES = {
     "nrq_model_load_nrm": ([_vp, _i, _i, C.POINTER(_vp)], _i),
 }
 
+# element types of include/nrq_serve.h, and its symbols
+F32, F16, BF16 = 0, 16, 17
+_i64, _f, _szp = C.c_int64, C.c_float, C.POINTER(C.c_size_t)
+SERVE_SIGNATURES = {
+    "nrq_dev_rope": ([_vp, _vp, _i, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _i, _f, _vp], _i),
+    "nrq_dev_rope_append": ([_vp, _vp, _vp, _vp, _i, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _i, _f, _vp, _vp, _vp], _i),
+    "nrq_paged_attention_workspace": ([_sz, _sz, _vp, _szp], _i),
+    "nrq_dev_paged_attention": ([_vp, _vp, _i, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _f, C.c_int32, _vp, _vp, _sz, _vp],
+                                _i),
+    "nrq_verify_workspace": ([_sz, _sz, _szp], _i),
+    "nrq_dev_verify_drafts": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp], _i),
+    "nrq_dev_quantize_mxfp4": ([_vp, _i, _sz, _sz, _i64, _vp, _vp, _vp], _i),
+    "nrq_dev_dequantize_mxfp4": ([_vp, _vp, _sz, _sz, _vp, _i, _i64, _vp], _i),
+    "nrq_dev_matmul_mxfp4": ([_vp, _i, _i64, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp], _i),
+    "nrq_linear_mxfp4_workspace": ([_sz, _sz, _szp], _i),
+    "nrq_dev_linear_mxfp4": ([_vp, _i, _i64, _vp, _vp, _vp, _i, _i64, _sz, _sz, _sz, _vp, _sz, _vp], _i),
+}
+
 
 class NrqError(RuntimeError):
     def __init__(self, code: int, msg: str):
@@ -114,7 +132,7 @@ def lib():
         import torch  # noqa: F401
 
         L = C.CDLL(LIB_PATH)
-        for name, (args, res) in SIGNATURES.items():
+        for name, (args, res) in {**SIGNATURES, **SERVE_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, res
         _lib = L

@@ -207,6 +207,7 @@ int dev_check(const char* name, int dtype, int order) {
 
 namespace nrq {
 void set_last_error(const char* msg) { g_err = msg; }
+int init_device() { return S().init ? S().device : -1; }
 }  // namespace nrq
 
 extern "C" {

@@ -151,6 +151,8 @@ int launch_pf_attention(const PfAttnLaunch& L);
 
 // Sets the message nrq_last_error() returns on this thread (nrq_api.hip).
 void set_last_error(const char* msg);
+// The device nrq_init took, -1 before it (nrq_api.hip).
+int init_device();
 // The model frees `dev` (a hipMalloc'd buffer its tensors point into) when destroyed.
 void model_adopt_buffer(nrq_model* m, void* dev);
 // Looks up the current device's address of the sampler's fixed scratch
