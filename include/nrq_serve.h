@@ -35,7 +35,7 @@ extern "C" {
  * position t of a sequence, KV head h, dimension d is at
  *   v[page * page_stride + h * head_stride + (t % page_size) * pos_stride + d]
  * with page = table[sequence][t / page_size]. Strides are multiples of 8, the
- * pools 16-byte aligned. Any page size from 1. */
+ * pools 16-byte aligned, a pool at most 2^35 elements. Any page size from 1. */
 typedef struct {
   void *k, *v;
   int64_t page_stride, head_stride, pos_stride;

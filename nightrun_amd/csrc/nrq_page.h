@@ -14,16 +14,19 @@
 
 namespace nrq {
 
-// The place (in elements from the pool's start) of position t on the pages of one
-// sequence, -1 where there is none: outside the table, or on an entry that is no page.
-NRQ_HD int64_t page_place(const int* pages, int width, int page_size, int n_pages, int64_t page_stride,
-                          int64_t pos_stride, int t) {
-  if (t < 0) return -1;
+constexpr uint32_t kNoPlace = 0xffffffffu;
+
+// The place (in units of 8 elements from the pool's start, as the strides are given) of
+// position t on the pages of one sequence, kNoPlace where there is none: outside
+// the table, or on an entry that is no page.
+NRQ_HD uint32_t page_place(const int* pages, int width, int page_size, int n_pages, uint32_t page_stride8,
+                           uint32_t pos_stride8, int t) {
+  if (t < 0) return kNoPlace;
   const uint32_t p = (uint32_t)t / (uint32_t)page_size;
-  if (p >= (uint32_t)width) return -1;
+  if (p >= (uint32_t)width) return kNoPlace;
   const int page = pages[p];
-  if (page < 0 || page >= n_pages) return -1;
-  return page * page_stride + (int64_t)((uint32_t)t - p * (uint32_t)page_size) * pos_stride;
+  if (page < 0 || page >= n_pages) return kNoPlace;
+  return (uint32_t)page * page_stride8 + ((uint32_t)t - p * (uint32_t)page_size) * pos_stride8;
 }
 
 // A sequence of the attention: its positions and new tokens (clamped), the first
@@ -44,9 +47,16 @@ NRQ_HD SeqSpan seq_span(int len, int count, int n_new, int64_t held, int window,
   return s;
 }
 
-// Workgroup w of `wgs` takes tiles [line_start(w), line_start(w + 1)) of `total` >= wgs.
-NRQ_HD int64_t line_start(int64_t w, int64_t total, int64_t wgs) { return w * total / wgs; }
-// The workgroup that takes tile g: the last w with line_start(w) <= g.
-NRQ_HD int64_t line_owner(int64_t g, int64_t total, int64_t wgs) { return ((g + 1) * wgs - 1) / total; }
+// The line of `total` tiles among `wgs` <= total workgroups: the first total % wgs
+// take one tile more. line_start(wgs) is total.
+NRQ_HD int line_start(int w, int total, int wgs) {
+  const int each = total / wgs, more = total - each * wgs;
+  return w * each + (w < more ? w : more);
+}
+// The workgroup that takes tile g.
+NRQ_HD int line_owner(int g, int total, int wgs) {
+  const int each = total / wgs, more = total - each * wgs, big = more * (each + 1);
+  return g < big ? g / (each + 1) : more + (g - big) / each;
+}
 
 }  // namespace nrq

@@ -29,7 +29,7 @@ namespace nrq {
 
 constexpr int kPaNT = 256;        // threads: four waves
 constexpr int kTile = 128;        // positions of a tile, 32 a wave
-constexpr int kPaMaxWgs = 1024;   // four workgroups on each of 256 CUs
+constexpr int kPaMaxWgs = 768;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct PaArgs {
@@ -39,6 +39,7 @@ struct PaArgs {
   int units_per_seq;
   int wgs;
   int slots;            // rows of a unit that there are: min(rows, per)
+  int wide_q;           // q in 16-byte loads
   float* part_o;        // [2 * wgs][slots][hd]
   float2* part_ml;      // [2 * wgs][slots]: maximum (log2 units), sum
 };
@@ -48,6 +49,7 @@ inline int pa_per(int hd, size_t rows) { return hd <= 128 && rows > 16 ? 32 : 16
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ SeqSpan pa_seq(const PagedAttnLaunch& L, int b) {
@@ -55,44 +57,39 @@ __device__ __forceinline__ SeqSpan pa_seq(const PagedAttnLaunch& L, int b) {
                   L.window, kTile);
 }
 
-// All tiles of a sequence's units, and of the sequences before it: a wave's own
-// scan over the lengths.
-__device__ __forceinline__ int64_t pa_total(const PaArgs& A) {
+// All tiles of the line, summed by each wave for itself.
+__device__ __forceinline__ int pa_total(const PaArgs& A) {
   const int lane = threadIdx.x & 63;
-  int64_t t = 0;
+  int t = 0;
   for (int b = lane; b < A.L.table.seqs; b += 64) t += pa_seq(A.L, b).tiles;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) t += __shfl_xor(t, m);
-  return t * A.units_per_seq;
+  return __builtin_amdgcn_readfirstlane(t) * A.units_per_seq;
 }
 
 // The sequence whose tiles hold tile g of the line, and its first tile's place.
-__device__ __forceinline__ int pa_find(const PaArgs& A, int64_t g, int64_t* first) {
+__device__ __forceinline__ int pa_find(const PaArgs& A, int g, int* first) {
   const int lane = threadIdx.x & 63;
-  int64_t base = 0;
+  int base = 0;
   for (int b0 = 0; b0 < A.L.table.seqs; b0 += 64) {
     const int b = b0 + lane;
-    int64_t own = b < A.L.table.seqs ? (int64_t)pa_seq(A.L, b).tiles * A.units_per_seq : 0, sum = own;
+    const int own = b < A.L.table.seqs ? pa_seq(A.L, b).tiles * A.units_per_seq : 0;
+    int sum = own;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
-      const int64_t y = __shfl_up(sum, m);
+      const int y = __shfl_up(sum, m);
       if (lane >= m) sum += y;
     }
     const unsigned long long over = __ballot(base + sum > g);
     if (over) {
       const int at = __ffsll(over) - 1;
-      *first = base + __shfl(sum, at) - __shfl(own, at);
+      *first = base + __builtin_amdgcn_readlane(sum - own, at);
       return b0 + at;
     }
-    base += __shfl(sum, 63);
+    base += __builtin_amdgcn_readlane(sum, 63);
   }
   *first = base;
   return A.L.table.seqs;
-}
-
-__device__ __forceinline__ float pa_load_q(const void* q, int dtype, int64_t at) {
-  if (dtype == kF32) return ((const float*)q)[at];
-  return dtype == kF16 ? (float)((const _Float16*)q)[at] : (float)((const __bf16*)q)[at];
 }
 
 __device__ __forceinline__ void pa_store(void* o, int dtype, int64_t at, float v) {
@@ -109,6 +106,8 @@ struct PaType;
 template <>
 struct PaType<_Float16> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+  static constexpr int kId = kF16;
+  static constexpr int kPieces = 2;  // of an f32 value: 22 bits
   static constexpr uint32_t kExp = 0x7c00u;
   static constexpr float kOffset = 12.0f;  // weights up to 2^12: pieces down to 2^-36 of the largest
   static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) {
@@ -118,12 +117,40 @@ struct PaType<_Float16> {
 template <>
 struct PaType<__bf16> {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  static constexpr int kId = kBF16;
+  static constexpr int kPieces = 3;
   static constexpr uint32_t kExp = 0x7f80u;
   static constexpr float kOffset = 0.0f;
   static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
+
+// Eight consecutive values of a query.
+template <typename Q>
+__device__ __forceinline__ void pa_load8(const Q* p, bool wide, float* f) {
+  constexpr int V = 16 / sizeof(Q);
+  struct alignas(16) Vec {
+    Q v[V];
+  };
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 8; i += V) {
+      const Vec a = *(const Vec*)(p + i);
+#pragma unroll
+      for (int j = 0; j < V; j++) f[i + j] = (float)a.v[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = (float)p[i];
+  }
+}
+
+template <typename Q, int KS>
+__device__ __forceinline__ void pa_load_q(const void* q, int64_t at, bool wide, float (*f)[8]) {
+#pragma unroll
+  for (int s = 0; s < KS; s++) pa_load8((const Q*)q + at + 32 * s, wide, f[s]);
+}
 
 // Pieces of eight f32 values, each the rest of the ones before it.
 template <typename T, int N>
@@ -141,14 +168,114 @@ __device__ __forceinline__ void pa_split(const float* f, typename PaType<T>::v8*
     }
 }
 
-__device__ __forceinline__ int64_t pa_place(const PagedAttnLaunch& L, const int* pages, int t, int begin, int end) {
-  if (t < begin || t >= end) return -1;
-  return page_place(pages, L.table.width, L.kv.page_size, L.kv.n_pages, L.kv.page_stride, L.kv.pos_stride, t);
+__device__ __forceinline__ uint32_t pa_place(const PagedAttnLaunch& L, const int* pages, int t, int begin, int end) {
+  if (t < begin || t >= end) return kNoPlace;
+  return page_place(pages, L.table.width, L.kv.page_size, L.kv.n_pages, L.kv.page_stride8, L.kv.pos_stride8, t);
+}
+
+// A wave's 32 positions of a tile in registers: what lane l holds is said above.
+template <int HD>
+struct PaTile {
+  static constexpr int KS = HD / 32, DV = HD / 16;
+  u32x4 k[2][KS];
+  uint32_t v[8][DV / 2];
+
+  // here: lane p % 32 has the place of position p. Positions without one read the pool's first
+  // (any; their scores are masked, their values cleared): no load is conditional.
+  __device__ __forceinline__ void load_k(const uint16_t* pool, uint32_t here, int c, int g) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const uint32_t a = __shfl((int)here, 16 * u + c);
+      const uint16_t* p = pool + (uint64_t)a * 8 + 8 * g;
+#pragma unroll
+      for (int s = 0; s < KS; s++) k[u][s] = *(const u32x4*)(p + 32 * s);
+    }
+  }
+  __device__ __forceinline__ void load_v(const uint16_t* pool, uint32_t here, int c, int g) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t a = __shfl((int)here, (j < 4 ? 0 : 16) + 4 * g + (j & 3));
+      const uint16_t* p = pool + (uint64_t)a * 8 + DV * c;
+      if constexpr (DV % 8 == 0) {
+#pragma unroll
+        for (int d = 0; d < DV / 8; d++) {
+          const u32x4 x = *(const u32x4*)(p + 8 * d);
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[j][4 * d + i] = x[i];
+        }
+      } else if constexpr (DV == 4) {
+        const u32x2 x = *(const u32x2*)p;
+        v[j][0] = x[0], v[j][1] = x[1];
+      } else {
+#pragma unroll
+        for (int d = 0; d < DV / 2; d++) v[j][d] = ((const uint32_t*)p)[d];
+      }
+    }
+  }
+  __device__ __forceinline__ void clear_v(uint32_t live, int g) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const bool on = live >> ((j < 4 ? 0 : 16) + 4 * g + (j & 3)) & 1;
+#pragma unroll
+      for (int d = 0; d < DV / 2; d++) v[j][d] = on ? v[j][d] : 0u;
+    }
+  }
+};
+
+// Workgroups a CU holds: registers for the tile, the accumulators and the queries.
+constexpr int pa_resident(int hd, int nt) { return hd > 128 ? 1 : (nt == 2 || hd > 96 ? 2 : 3); }
+
+// The same stretch of one wave without matrix instructions, position by position and row by
+// row, for values that hold an infinity or a NaN: there the products of weights
+// that are 0 (rows that do not see a position) or of the pieces of a weight would give
+// NaN. Dimension lane + 64 e is the lane's.
+template <typename T, int HD>
+__device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int row0, int rows, int p0, int stop, int len,
+                                      int n, float* ex_o, float (*ex_ml)[2], int os) {
+  constexpr int E = (HD + 63) / 64;
+  const PagedAttnLaunch& L = A.L;
+  const int lane = threadIdx.x & 63;
+  const int* pages = L.table.pages + b * L.table.stride;
+  for (int r = 0; r < rows; r++) {
+    const int rr = row0 + r, tok = rr / A.group, hi = len - n + tok;
+    const int lo = L.window > 0 ? max(0, hi - L.window + 1) : 0;
+    const int64_t qa = b * L.qb + tok * L.qt + (head * A.group + rr - tok * A.group) * L.qh;
+    float q[E], o[E], m = -INFINITY, l = 0;
+    for (int e = 0; e < E; e++) {
+      const int d = 64 * e + lane;
+      o[e] = 0;
+      q[e] = 0;
+      if (d < HD)
+        q[e] = L.dtype == kF32   ? ((const float*)L.q)[qa + d]
+               : L.dtype == kF16 ? (float)((const _Float16*)L.q)[qa + d]
+                                 : (float)((const __bf16*)L.q)[qa + d];
+    }
+    for (int t0 = p0; t0 < stop; t0 += kTile)
+      for (int t = max(t0, lo); t < min(t0 + 32, hi + 1); t++) {
+        const uint32_t place = pa_place(L, pages, t, lo, min(len, hi + 1));
+        if (place == kNoPlace) continue;
+        const int64_t at = (int64_t)place * 8 + head * L.kv.head_stride;
+        float s = 0;
+        for (int e = 0; e < E; e++)
+          if (64 * e + lane < HD) s = fmaf((float)((const T*)L.kv.k)[at + 64 * e + lane], q[e], s);
+        for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+        s *= L.scale * kLog2e;
+        const float mn = fmaxf(m, s), by = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;
+        const float p = __builtin_amdgcn_exp2f(s - (mn == -INFINITY ? 0.0f : mn) + PaType<T>::kOffset);
+        l = l * by + p;
+        for (int e = 0; e < E; e++)
+          if (64 * e + lane < HD) o[e] = o[e] * by + p * (float)((const T*)L.kv.v)[at + 64 * e + lane];
+        m = mn;
+      }
+    for (int e = 0; e < E; e++)
+      if (64 * e + lane < HD) ex_o[(64 * e + lane) * os + r] = o[e];
+    if (lane == 0) ex_ml[r][0] = m, ex_ml[r][1] = l;
+  }
 }
 
 // T: the cache's type; HD; NT: groups of 16 rows; NQ, NP: pieces of a query and of a weight.
 template <typename T, int HD, int NT, int NQ, int NP>
-__global__ __launch_bounds__(kPaNT) void paged_kernel(PaArgs A) {
+__global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArgs A) {
   typedef typename PaType<T>::v8 v8;
   constexpr int KS = HD / 32;  // steps of K
   constexpr int DV = HD / 16;  // dimensions of a lane's values
@@ -158,22 +285,31 @@ __global__ __launch_bounds__(kPaNT) void paged_kernel(PaArgs A) {
   const PagedAttnLaunch& L = A.L;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
 
-  const int64_t total = pa_total(A);
-  const int64_t wgs = min<int64_t>(A.wgs, total);
-  if (blockIdx.x >= wgs) return;
-  int64_t at = line_start(blockIdx.x, total, wgs);
-  const int64_t stop = line_start((int64_t)blockIdx.x + 1, total, wgs);
-  int64_t first;
+  const int total = pa_total(A);
+  const int wgs = min(A.wgs, total);
+  if ((int)blockIdx.x >= wgs) return;
+  int at = line_start(blockIdx.x, total, wgs);
+  const int stop = line_start(blockIdx.x + 1, total, wgs);
+  int first;
   int b = pa_find(A, at, &first);
   while (at < stop) {
     const SeqSpan sq = pa_seq(L, b);
-    const int unit = (int)((at - first) / sq.tiles);
-    const int t_begin = (int)(at - first - (int64_t)unit * sq.tiles);
-    const int t_end = (int)min<int64_t>(sq.tiles, t_begin + (stop - at));
+    const int unit = (at - first) / sq.tiles;
+    const int t_begin = at - first - unit * sq.tiles;
+    const int t_end = min(sq.tiles, t_begin + (stop - at));
     const int head = unit / A.row_tiles, rt = unit - head * A.row_tiles;
     const int row0 = rt * 16 * NT, rows = min(16 * NT, sq.n * A.group - row0);
     const bool whole = t_begin == 0 && t_end == sq.tiles;
     if (rows > 0) {
+      const int first_hi = sq.len - sq.n + row0 / A.group;                // what the unit's first
+      const int last_hi = sq.len - sq.n + (row0 + rows - 1) / A.group;    // and last row see
+      const int last_lo = L.window > 0 ? max(0, last_hi - L.window + 1) : 0;
+      const int begin = L.window > 0 ? max(0, first_hi - L.window + 1) : 0, end = min(sq.len, last_hi + 1);
+      const int* pages = L.table.pages + b * L.table.stride;
+      const uint16_t* kp = L.kv.k + head * L.kv.head_stride;
+      const uint16_t* vp = L.kv.v + head * L.kv.head_stride;
+      const int pw = sq.start + 32 * w + (lane & 31);  // the lane's position in the first tile
+      uint32_t here = pa_place(L, pages, pw + t_begin * kTile, begin, end);
       // ---- queries, and what each row sees
       v8 q[NQ][NT][KS];
       float to_log2[NT];  // what brings a row's products to log2 units
@@ -183,17 +319,23 @@ __global__ __launch_bounds__(kPaNT) void paged_kernel(PaArgs A) {
         const int r = min(row0 + 16 * n + c, sq.n * A.group - 1), tok = r / A.group;
         hi[n] = sq.len - sq.n + tok;
         lo[n] = L.window > 0 ? max(0, hi[n] - L.window + 1) : 0;
-        const int64_t qa = b * L.qb + tok * L.qt + (head * A.group + r - tok * A.group) * L.qh;
-        float f[KS][8], big = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            f[s][i] = pa_load_q(L.q, L.dtype, qa + 32 * s + 8 * g + i);
-            big = fmaxf(big, fabsf(f[s][i]));
-          }
+        const int64_t qa = b * L.qb + tok * L.qt + (head * A.group + r - tok * A.group) * L.qh + 8 * g;
         to_log2[n] = L.scale * kLog2e;
+        float f[KS][8];
+        if (NQ == 1)
+          pa_load_q<T, KS>(L.q, qa, A.wide_q, f);  // 16 bits either way: the conversions cancel
+        else if (L.dtype == kF32)
+          pa_load_q<float, KS>(L.q, qa, A.wide_q, f);
+        else if (L.dtype == kF16)
+          pa_load_q<_Float16, KS>(L.q, qa, A.wide_q, f);
+        else
+          pa_load_q<__bf16, KS>(L.q, qa, A.wide_q, f);
         if (NQ > 1) {  // the largest magnitude of the row to [2^13, 2^14)
+          float big = 0.0f;
+#pragma unroll
+          for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(f[s][i]));
           big = fmaxf(big, __shfl_xor(big, 16));
           big = fmaxf(big, __shfl_xor(big, 32));
           const int e = min(max((int)(__float_as_uint(big) >> 23), 27), 253);  // small rows: as if 2^-100
@@ -212,24 +354,9 @@ __global__ __launch_bounds__(kPaNT) void paged_kernel(PaArgs A) {
           for (int k = 0; k < NQ; k++) q[k][n][s] = tmp[k];
         }
       }
-      const int first_row_hi = sq.len - sq.n + row0 / A.group;                 // of the unit's rows the
-      const int last_row_hi = sq.len - sq.n + (row0 + rows - 1) / A.group;     // nearest and farthest ends
-      const int last_row_lo = L.window > 0 ? max(0, last_row_hi - L.window + 1) : 0;
-      // positions that any of them sees
-      const int begin = L.window > 0 ? max(0, first_row_hi - L.window + 1) : 0, end = min(sq.len, last_row_hi + 1);
-
-      const int* pages = L.table.pages + b * L.table.stride;
-      const T* kp = (const T*)L.kv.k + head * L.kv.head_stride;
-      const T* vp = (const T*)L.kv.v + head * L.kv.head_stride;
 
       float m[NT], l[NT];
       f32x4 acc[NT][DV];
-      // With an infinity or a NaN among the values the plain sums go wrong: a weight of 0 (a
-      // row that does not see the position) or a negative piece of one times infinity is
-      // NaN. Such a stretch is done again, `apart`: row by row, each with the values that it sees,
-      // and the lower pieces with the finite ones only.
-      bool apart = false;
-    again:
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         m[n] = -INFINITY;
@@ -237,167 +364,118 @@ __global__ __launch_bounds__(kPaNT) void paged_kernel(PaArgs A) {
 #pragma unroll
         for (int d = 0; d < DV; d++) acc[n][d] = f32x4{0, 0, 0, 0};
       }
+      PaTile<HD> tile;
+      uint32_t live = (uint32_t)__ballot(here != kNoPlace), next = kNoPlace, next_live = 0;
+      if (live) {  // else the pool may be empty
+        tile.load_k(kp, here == kNoPlace ? 0 : here, c, g);
+        tile.load_v(vp, here == kNoPlace ? 0 : here, c, g);
+      }
+      if (t_begin + 1 < t_end) {
+        next = pa_place(L, pages, pw + (t_begin + 1) * kTile, begin, end);
+        next_live = (uint32_t)__ballot(next != kNoPlace);
+      }
       int p0 = sq.start + t_begin * kTile + 32 * w;
-      int64_t place = pa_place(L, pages, p0 + (lane & 31), begin, end);
       for (int t = t_begin; t < t_end; t++, p0 += kTile) {
-        if (p0 >= end) break;
-        const int64_t here = place;
-        if (t + 1 < t_end) place = pa_place(L, pages, p0 + kTile + (lane & 31), begin, end);
-        // ---- loads: 32 positions of K and V
-        u32x4 kr[2][KS];
+        uint32_t after = kNoPlace;
+        if (t + 2 < t_end) after = pa_place(L, pages, pw + (t + 2) * kTile, begin, end);
+        // ---- scores: 8 positions for query c of each group
+        f32x4 x[NT][2];
+        if (live) {
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const int64_t a = __shfl(here, 16 * u + c);
+          for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int s = 0; s < KS; s++)
-            kr[u][s] = a >= 0 ? *(const u32x4*)(kp + a + 32 * s + 8 * g) : u32x4{0, 0, 0, 0};
-        }
-        uint32_t vr[8][DV / 2];
+            for (int u = 0; u < 2; u++) {
+              x[n][u] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const int64_t a = __shfl(here, (j < 4 ? 0 : 16) + 4 * g + (j & 3));
+              for (int k = NQ - 1; k >= 0; k--)
 #pragma unroll
-          for (int d = 0; d < DV / 2; d++) vr[j][d] = 0;
-          if (a >= 0) {
-            if constexpr (DV % 8 == 0) {
-#pragma unroll
-              for (int d = 0; d < DV / 8; d++) *(u32x4*)&vr[j][4 * d] = *(const u32x4*)(vp + a + DV * c + 8 * d);
-            } else {
-              struct alignas(4) Row {
-                uint32_t x[DV / 2];
-              };
-              const Row r = *(const Row*)(vp + a + DV * c);
-#pragma unroll
-              for (int d = 0; d < DV / 2; d++) vr[j][d] = r.x[d];
+                for (int s = 0; s < KS; s++) x[n][u] = PaType<T>::mfma(*(v8*)&tile.k[u][s], q[k][n][s], x[n][u]);
             }
-          }
         }
-        // which of the 32 positions are on a page
-        const uint32_t live = (uint32_t)__ballot(here >= 0);
-        const bool inside = live == 0xffffffffu && p0 + 31 <= first_row_hi && p0 >= last_row_lo;
+        const uint32_t ahead = next == kNoPlace ? 0 : next;
+        if (next_live) tile.load_k(kp, ahead, c, g);
+        if (live) {
+          const bool inside = live == 0xffffffffu && p0 + 31 <= first_hi && p0 >= last_lo;
+          v8 pp[NT][NP];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          // ---- scores of 8 positions for query c, in log2 units
-          float s[8];
+          for (int n = 0; n < NT; n++) {
+            float s[8];
 #pragma unroll
-          for (int u = 0; u < 2; u++) {
-            f32x4 x = {0, 0, 0, 0};
+            for (int i = 0; i < 8; i++) s[i] = x[n][i >> 2][i & 3] * to_log2[n];
+            if (!inside) {
 #pragma unroll
-            for (int k = NQ - 1; k >= 0; k--)
+              for (int i = 0; i < 8; i++) {
+                const int o = (i < 4 ? 0 : 16) + 4 * g + (i & 3), p = p0 + o;
+                s[i] = p >= lo[n] && p <= hi[n] && (live >> o & 1) ? s[i] : -INFINITY;
+              }
+            }
+            // ---- running maximum and sum
+            float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float mn = fmaxf(m[n], top);
+            const float ref = mn == -INFINITY ? 0.0f : mn;
+            if (__any(mn > m[n])) {
+              const float by = __builtin_amdgcn_exp2f(m[n] - ref);
+              l[n] *= by;
 #pragma unroll
-              for (int st = 0; st < KS; st++) x = PaType<T>::mfma(*(v8*)&kr[u][st], q[k][n][st], x);
-#pragma unroll
-            for (int i = 0; i < 4; i++) s[4 * u + i] = x[i] * to_log2[n];
-          }
-          if (!inside) {
+              for (int d = 0; d < DV; d++) acc[n][d] *= by;
+              m[n] = mn;
+            }
+            float p[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-              const int o = (i < 4 ? 0 : 16) + 4 * g + (i & 3), p = p0 + o;
-              s[i] = p >= lo[n] && p <= hi[n] && (live >> o & 1) ? s[i] : -INFINITY;
+              p[i] = __builtin_amdgcn_exp2f(s[i] - ref + PaType<T>::kOffset);
+              l[n] += p[i];
             }
+            pa_split<T, NP>(p, pp[n]);
           }
-          // ---- running maximum and sum
-          float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const float mn = fmaxf(m[n], top);
-          const float ref = mn == -INFINITY ? 0.0f : mn;
-          if (__any(mn > m[n])) {
-            const float by = __builtin_amdgcn_exp2f(m[n] - ref);
-            l[n] *= by;
-#pragma unroll
-            for (int d = 0; d < DV; d++) acc[n][d] *= by;
-            m[n] = mn;
-          }
-          float p[8];
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            p[i] = __builtin_amdgcn_exp2f(s[i] - ref + PaType<T>::kOffset);
-            l[n] += p[i];
-          }
-          v8 pp[NP];
-          pa_split<T, NP>(p, pp);
+          if (live != 0xffffffffu) tile.clear_v(live, g);
           // ---- O^T += V^T P^T
-          if (!apart) {
 #pragma unroll
-            for (int d = 0; d < DV; d++) {
-              u32x4 a;
+          for (int d = 0; d < DV; d++) {
+            u32x4 a;
 #pragma unroll
-              for (int j = 0; j < 4; j++) {
-                const uint32_t x = vr[2 * j][d / 2], y = vr[2 * j + 1][d / 2];
-                a[j] = d & 1 ? (x >> 16) | (y & 0xffff0000u) : (x & 0xffffu) | (y << 16);
-              }
+            for (int j = 0; j < 4; j++)  // a pair of positions of one dimension
+              a[j] = __builtin_amdgcn_perm(tile.v[2 * j + 1][d / 2], tile.v[2 * j][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
-              for (int k = NP - 1; k >= 0; k--) acc[n][d] = PaType<T>::mfma(*(v8*)&a, pp[k], acc[n][d]);
-            }
-          } else {
-            for (int j = 0; j < 8; j++)  // a weight above 0 is not lost in the first piece
-              if (p[j] > 0.0f && (float)pp[0][j] == 0.0f) pp[0][j] = (T)6e-8f;
-#pragma unroll 1
-            for (int only = 0; only < 16; only++) {
-              const int l0 = __shfl(lo[n], only), h0 = __shfl(hi[n], only);
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-              for (int d = 0; d < DV; d++) {
-                u32x4 a, fin;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                  uint32_t h[2];
-#pragma unroll
-                  for (int i = 0; i < 2; i++) {
-                    const int pos = p0 + (j < 2 ? 0 : 16) + 4 * g + (2 * j & 3) + i;
-                    h[i] = (d & 1 ? vr[2 * j + i][d / 2] >> 16 : vr[2 * j + i][d / 2]) & 0xffffu;
-                    if (pos < l0 || pos > h0) h[i] = 0;
-                  }
-                  a[j] = h[0] | h[1] << 16;
-#pragma unroll
-                  for (int i = 0; i < 2; i++)
-                    if ((h[i] & PaType<T>::kExp) == PaType<T>::kExp) h[i] = 0;
-                  fin[j] = h[0] | h[1] << 16;
-                }
-                f32x4 x = acc[n][d];
-#pragma unroll
-                for (int k = NP - 1; k >= 0; k--) x = PaType<T>::mfma(k ? *(v8*)&fin : *(v8*)&a, pp[k], x);
-                if (c == only) acc[n][d] = x;
-              }
-            }
+              for (int k = NP - 1; k >= 0; k--) acc[n][d] = PaType<T>::mfma(*(v8*)&a, pp[n][k], acc[n][d]);
           }
         }
+        if (next_live) tile.load_v(vp, ahead, c, g);
+        live = next_live;
+        next = after;
+        next_live = (uint32_t)__ballot(next != kNoPlace);
       }
-      if (!apart) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-          for (int d = 0; d < DV; d++) sum += (acc[n][d][0] * 0.0f + acc[n][d][1] * 0.0f) + (acc[n][d][2] * 0.0f + acc[n][d][3] * 0.0f);
-        if (__any(sum != sum)) {
-          apart = true;
-          goto again;
-        }
-      }
-
       // ---- the four waves' results together
-      __syncthreads();  // the exchange of the unit before is read
+      float sum = 0.0f;
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         l[n] += __shfl_xor(l[n], 16);
         l[n] += __shfl_xor(l[n], 32);
-        if (g == 0) {
-          ex_ml[w][16 * n + c][0] = m[n];
-          ex_ml[w][16 * n + c][1] = l[n];
-        }
-      }
-      __syncthreads();
-      float* mine = ex_o[w];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        float mm = ex_ml[0][16 * n + c][0];
-#pragma unroll
-        for (int i = 1; i < 4; i++) mm = fmaxf(mm, ex_ml[i][16 * n + c][0]);
-        const float by = __builtin_amdgcn_exp2f(m[n] - (mm == -INFINITY ? 0.0f : mm));
 #pragma unroll
         for (int d = 0; d < DV; d++)
+          sum += (acc[n][d][0] * 0.0f + acc[n][d][1] * 0.0f) + (acc[n][d][2] * 0.0f + acc[n][d][3] * 0.0f);
+      }
+      __syncthreads();  // the exchange of the unit before is read
+      if (__any(sum != sum)) {
+        pa_plain<T, HD>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, sq.len,
+                        sq.n, ex_o[w], ex_ml[w], OS);
+      } else {
 #pragma unroll
-          for (int i = 0; i < 4; i++) mine[((4 * g + i) * DV + d) * OS + 16 * n + c] = acc[n][d][i] * by;
+        for (int n = 0; n < NT; n++)
+          if (16 * n + c < rows) {
+            if (g == 0) {
+              ex_ml[w][16 * n + c][0] = m[n];
+              ex_ml[w][16 * n + c][1] = l[n];
+            }
+#pragma unroll
+            for (int d = 0; d < DV; d++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) ex_o[w][((4 * g + i) * DV + d) * OS + 16 * n + c] = acc[n][d][i];
+          }
       }
       __syncthreads();
       const int64_t slot = 2 * (int64_t)blockIdx.x + (t_begin == 0 ? 1 : 0);
@@ -409,8 +487,9 @@ __global__ __launch_bounds__(kPaNT) void paged_kernel(PaArgs A) {
         const float ref = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-          o += ex_o[k][d * OS + r];
-          ll += ex_ml[k][r][1] * __builtin_amdgcn_exp2f(ex_ml[k][r][0] - ref);
+          const float by = __builtin_amdgcn_exp2f(ex_ml[k][r][0] - ref);
+          if (by > 0.0f || ref != ref) o += ex_o[k][d * OS + r] * by;  // a wave that saw nothing, or nothing of weight
+          ll += ex_ml[k][r][1] * by;
         }
         if (!whole) {
           A.part_o[(slot * A.slots + r) * HD + d] = o;
@@ -426,63 +505,94 @@ __global__ __launch_bounds__(kPaNT) void paged_kernel(PaArgs A) {
       }
     }
     at += t_end - t_begin;
-    if (at == first + (int64_t)sq.tiles * A.units_per_seq) {
+    if (at == first + sq.tiles * A.units_per_seq) {
       first = at;
       b++;
     }
   }
 }
 
-// The stretches of one row of a unit that more than one workgroup shared, in order.
+// The stretches of one row of a unit that several workgroups shared, in order: four waves take
+// every fourth of them, then add up.
 template <typename T, int HD>
-__global__ __launch_bounds__((HD + 63) / 64 * 64) void paged_join_kernel(PaArgs A) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PaArgs A) {
+  constexpr int E = (HD + 63) / 64;  // dimensions of a lane: lane + 64 e
+  __shared__ float ex_o[4][64 * E], ex_l[4];
   const PagedAttnLaunch& L = A.L;
   const int u = blockIdx.x, b = u / A.units_per_seq, unit = u - b * A.units_per_seq;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const SeqSpan sq = pa_seq(L, b);
   const int head = unit / A.row_tiles, rt = unit - head * A.row_tiles;
   const int r = blockIdx.y, rr = rt * A.per + r;
   if (rr >= sq.n * A.group) return;
-  int64_t before = 0;
-  for (int i = lane; i < b; i += 64) before += pa_seq(L, i).tiles;
+  int before = 0, all = 0;  // tiles of the sequences before, and of all
+  for (int i = lane; i < L.table.seqs; i += 64) {
+    const int t = pa_seq(L, i).tiles;
+    all += t;
+    if (i < b) before += t;
+  }
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m);
-  const int64_t total = pa_total(A), wgs = min<int64_t>(A.wgs, total);
-  const int64_t g0 = before * A.units_per_seq + (int64_t)unit * sq.tiles, g1 = g0 + sq.tiles;
-  const int64_t w0 = line_owner(g0, total, wgs), w1 = line_owner(g1 - 1, total, wgs);
+  for (int m = 1; m < 64; m <<= 1) {
+    before += __shfl_xor(before, m);
+    all += __shfl_xor(all, m);
+  }
+  const int total = all * A.units_per_seq, wgs = min(A.wgs, total);
+  const int g0 = before * A.units_per_seq + unit * sq.tiles, g1 = g0 + sq.tiles;
+  const int w0 = line_owner(g0, total, wgs), w1 = line_owner(g1 - 1, total, wgs);
   if (w0 == w1) return;
-  const int d = threadIdx.x;
+  // the maximum over all stretches
   float mm = -INFINITY;
-  for (int64_t k = w0; k <= w1; k++) mm = fmaxf(mm, A.part_ml[(2 * k + (k == w0 ? 1 : 0)) * A.slots + r].x);
+  for (int k = w0 + lane; k <= w1; k += 64) mm = fmaxf(mm, A.part_ml[(2 * k + (k == w0 ? 1 : 0)) * A.slots + r].x);
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) mm = fmaxf(mm, __shfl_xor(mm, m));
   const float ref = mm == -INFINITY ? 0.0f : mm;
-  float o = 0, l = 0;
-  for (int64_t k = w0; k <= w1; k++) {
+  float o[E], l = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = 0;
+#pragma unroll 4
+  for (int k = w0 + w; k <= w1; k += 4) {
     const int64_t slot = (2 * k + (k == w0 ? 1 : 0)) * A.slots + r;
     const float2 ml = A.part_ml[slot];
     const float by = __builtin_amdgcn_exp2f(ml.x - ref);
     l += ml.y * by;
-    if (d < HD) o += A.part_o[slot * HD + d] * by;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (64 * e + lane < HD) o[e] += A.part_o[slot * HD + 64 * e + lane] * by;
   }
+#pragma unroll
+  for (int e = 0; e < E; e++) ex_o[w][64 * e + lane] = o[e];
+  if (lane == 0) ex_l[w] = l;
+  __syncthreads();
+  l = ((ex_l[0] + ex_l[1]) + (ex_l[2] + ex_l[3]));
   const int tok = rr / A.group, h = head * A.group + rr - tok * A.group;
   const bool none = mm == -INFINITY && l == 0.0f;
-  if (d < HD) pa_store(L.out, L.dtype, b * L.ob + tok * L.ot + h * L.oh + d, none ? 0.0f : o / l);
-  if (L.lse && d == 0)
+  for (int d = threadIdx.x; d < HD; d += 256) {
+    const float x = (ex_o[0][d] + ex_o[1][d]) + (ex_o[2][d] + ex_o[3][d]);
+    pa_store(L.out, L.dtype, b * L.ob + tok * L.ot + h * L.oh + d, none ? 0.0f : x / l);
+  }
+  if (L.lse && threadIdx.x == 0)
     L.lse[((int64_t)b * L.n_new + tok) * L.heads + h] =
         none ? -INFINITY : (mm - PaType<T>::kOffset + log2f(l)) * 0.69314718055994531f;
 }
 
 template <typename T, int HD, int NT, int NQ, int NP>
-hipError_t pa_launch(PaArgs& A, bool join) {
+hipError_t pa_launch(PaArgs& A) {
+  const int64_t units = (int64_t)A.units_per_seq * A.L.table.seqs;
+  const int64_t tiles = ((int64_t)A.L.table.width * A.L.kv.page_size + kTile - 1) / kTile;
+  const int64_t most = units * (tiles > 0 ? tiles : 1), fill = 256 * pa_resident(HD, NT);
+  static_assert(256 * pa_resident(HD, NT) <= kPaMaxWgs, "workspace");
+  A.wgs = (int)(most < fill ? most : fill);
+  A.part_o = (float*)A.L.workspace;
+  A.part_ml = (float2*)(A.part_o + (size_t)2 * A.wgs * A.slots * HD);
   hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ, NP>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
-  if (join)
-    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(A.units_per_seq * A.L.table.seqs, A.slots),
-                       dim3((HD + 63) / 64 * 64), 0, A.L.stream, A);
+  if (tiles > 1)
+    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)units, A.slots), dim3(256), 0, A.L.stream, A);
   return hipGetLastError();
 }
 
 template <typename T, int HD>
 hipError_t pa_launch_hd(const PagedAttnLaunch& L) {
-  constexpr int kMany = sizeof(T) == 2 && PaType<T>::kOffset > 0 ? 2 : 3;  // f16: 2 pieces of 11 bits, bf16: 3 of 8
+  constexpr int kMany = PaType<T>::kPieces;
   PaArgs A;
   A.L = L;
   A.group = L.heads / L.kv.n_kv;
@@ -490,18 +600,13 @@ hipError_t pa_launch_hd(const PagedAttnLaunch& L) {
   A.per = pa_per(HD, A.rows);
   A.row_tiles = (A.rows + A.per - 1) / A.per;
   A.units_per_seq = L.kv.n_kv * A.row_tiles;
-  const int64_t units = (int64_t)A.units_per_seq * L.table.seqs;
-  const int64_t tiles = ((int64_t)L.table.width * L.kv.page_size + kTile - 1) / kTile;
-  A.wgs = (int)(units * (tiles > 0 ? tiles : 1) < kPaMaxWgs ? units * (tiles > 0 ? tiles : 1) : kPaMaxWgs);
   A.slots = A.rows < A.per ? A.rows : A.per;
-  A.part_o = (float*)L.workspace;
-  A.part_ml = (float2*)(A.part_o + (size_t)2 * A.wgs * A.slots * HD);
-  const bool join = tiles > 1;
-  const bool same = L.dtype == (PaType<T>::kOffset > 0 ? kF16 : kBF16);
+  const int v = L.dtype == kF32 ? 4 : 8;
+  A.wide_q = ((uintptr_t)L.q & 15) == 0 && L.qb % v == 0 && L.qt % v == 0 && L.qh % v == 0;
+  const bool same = L.dtype == PaType<T>::kId;
   if constexpr (HD <= 128)
-    if (A.per == 32)
-      return same ? pa_launch<T, HD, 2, 1, 2>(A, join) : pa_launch<T, HD, 2, kMany, kMany>(A, join);
-  return same ? pa_launch<T, HD, 1, 1, 2>(A, join) : pa_launch<T, HD, 1, kMany, kMany>(A, join);
+    if (A.per == 32) return same ? pa_launch<T, HD, 2, 1, 2>(A) : pa_launch<T, HD, 2, kMany, kMany>(A);
+  return same ? pa_launch<T, HD, 1, 1, 2>(A) : pa_launch<T, HD, 1, kMany, kMany>(A);
 }
 
 template <typename T>

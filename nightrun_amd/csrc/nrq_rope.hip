@@ -102,11 +102,11 @@ __global__ __launch_bounds__(kRopeNT) void rope_kernel(RopeLaunch L, int tpw) {
       } else {
         const bool isk = h < L.heads + L.kv.n_kv;
         const int hh = h - L.heads - (isk ? 0 : L.kv.n_kv);
-        const int64_t place = page_place(L.table.pages + seq * L.table.stride, L.table.width, L.kv.page_size,
-                                         L.kv.n_pages, L.kv.page_stride, L.kv.pos_stride, pos);
-        if (place < 0) continue;
+        const uint32_t place = page_place(L.table.pages + seq * L.table.stride, L.table.width, L.kv.page_size,
+                                          L.kv.n_pages, L.kv.page_stride8, L.kv.pos_stride8, pos);
+        if (place == kNoPlace) continue;
         row.src = isk ? (const T*)L.k + t * L.kt + hh * L.kh : (const T*)L.v + t * L.vt + hh * L.vh;
-        row.c = (isk ? L.kv.k : L.kv.v) + place + hh * L.kv.head_stride;
+        row.c = (isk ? L.kv.k : L.kv.v) + (uint64_t)place * 8 + hh * L.kv.head_stride;
         turn = isk;
       }
     }

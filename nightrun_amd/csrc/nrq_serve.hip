@@ -60,8 +60,14 @@ int kv_check(const char* name, const nrq_paged_kv* kv, const nrq_page_table* tab
   if (kv->page_stride < 0 || kv->head_stride < 0 || kv->pos_stride < 0 || kv->page_stride % 8 || kv->head_stride % 8 ||
       kv->pos_stride % 8)
     return fail(NRQ_ERR_ARG, name, "cache strides are not multiples of 8");
-  *okv = nrq::PagedKv{(uint16_t*)kv->k, (uint16_t*)kv->v, kv->page_stride, kv->head_stride, kv->pos_stride,
-                      kv->n_pages,      kv->page_size,    kv->n_kv_heads,  kv->head_dim,    kv->dtype};
+  // places count 8 elements in 32 bits, the last is no place; within a page there is no more than a page
+  const double last = ((double)(kv->n_pages ? kv->n_pages - 1 : 0) * (double)kv->page_stride +
+                       (double)(kv->page_size - 1) * (double)kv->pos_stride) / 8;
+  if (last >= 4294967295.0 || kv->page_stride / 8 > 0xffffffffll || kv->pos_stride / 8 > 0xffffffffll)
+    return fail(NRQ_ERR_UNSUPPORTED, name, "cache of more than 2^35 elements in a pool");
+  *okv = nrq::PagedKv{(uint16_t*)kv->k, (uint16_t*)kv->v, kv->head_stride, (uint32_t)(kv->page_stride / 8),
+                      (uint32_t)(kv->pos_stride / 8), kv->n_pages, kv->page_size, kv->n_kv_heads, kv->head_dim,
+                      kv->dtype};
   if (!table) return NRQ_OK;
   if (table->seqs < 0 || table->width < 0) return fail(NRQ_ERR_SHAPE, name, "table of %d by %d", table->seqs, table->width);
   if (table->seqs && table->width && !table->pages) return fail(NRQ_ERR_ARG, name, "null table");
@@ -205,6 +211,9 @@ int nrq_dev_paged_attention(void* out, const void* q, int dtype, size_t n_new, s
       n_new * heads * (size_t)table->seqs > (size_t)1 << 30)
     return fail(NRQ_ERR_UNSUPPORTED, name, "%d sequences of %zu rows of %zu heads", table->seqs, n_new, heads);
   if (!strides || !out || !q || !lens) return fail(NRQ_ERR_ARG, name, "null pointer");
+  if ((double)table->seqs * (double)(n_new * heads) * ((double)table->width * kv->page_size / 128 + 1) >= 2147483647.0)
+    return fail(NRQ_ERR_UNSUPPORTED, name, "%d sequences of %d pages of %d: too much work for a call", table->seqs,
+                table->width, kv->page_size);
   const size_t e = bytes_of(dtype);
   if (!aligned(out, e) || !aligned(q, e) || !aligned(lens, 4) || !aligned(counts, 4) || !aligned(lse, 4))
     return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");

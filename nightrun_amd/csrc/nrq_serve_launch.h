@@ -12,7 +12,8 @@ enum { kF32 = 0, kF16 = 16, kBF16 = 17 };
 
 struct PagedKv {
   uint16_t *k, *v;
-  int64_t page_stride, head_stride, pos_stride;
+  int64_t head_stride;
+  uint32_t page_stride8, pos_stride8;  // in units of 8 elements
   int n_pages, page_size, n_kv, hd;
   int dtype;
 };

@@ -354,8 +354,10 @@ def test_attention_masked_garbage(gpu):
             y = torch.empty_like(q)
             kp, vp, table, lens = c.dev()
             serve.paged_attention(y, q, kp, vp, table, lens, 128 ** -0.5, window=window)
-            # the rows before keep their values (but for the order of additions, which stays)
-            assert torch.equal(y[:, :new - 2], clean[:, :new - 2])
+            # the rows before keep their values (the order of additions may be another one)
+            want, tol, _ = attention(f64(q), c, [new] * 3, 128 ** -0.5, window)
+            tol += PIECES["f16", "f16"] * max(float(v.abs().max()) for v in c.v) + half_step("f16") * np.abs(want)
+            assert np.all(np.abs(f64(y) - want)[:, :new - 2] <= tol[:, :new - 2])
             assert torch.isinf(y[:, new - 2]).all() and torch.isnan(y[:, new - 1]).all()
         if window:  # before every row's window
             for b, n in enumerate(c.lens):

@@ -144,6 +144,9 @@ REFUSED = [
     ("nrq_dev_paged_attention", dict(ws=None), ARG, "workspace"),
     ("nrq_dev_paged_attention", dict(ws=P + 8), ARG, "aligned"),
     ("nrq_dev_paged_attention", dict(n_new=70000), UNSUPPORTED, "rows"),
+    ("nrq_dev_paged_attention", dict(kv=_kv(n_pages=2 ** 31 - 1)), UNSUPPORTED, "elements"),
+    ("nrq_dev_paged_attention", dict(table=_table(width=2 ** 28, stride=2 ** 28)), UNSUPPORTED, "too much"),
+    ("nrq_dev_rope_append", dict(kv=_kv(page_size=2 ** 31 - 1)), UNSUPPORTED, "elements"),
     ("nrq_dev_verify_drafts", dict(n_new=65), UNSUPPORTED, "64"),
     ("nrq_dev_verify_drafts", dict(vocab=0), SHAPE, "vocabulary"),
     ("nrq_dev_verify_drafts", dict(target=None), ARG, "null"),
@@ -208,13 +211,13 @@ def page(tmp_path_factory):
     src = d / "page.cpp"
     src.write_text('''#include "nrq_page.h"
 extern "C" {
-int64_t place(const int* p, int w, int ps, int n, int64_t a, int64_t b, int t) { return nrq::page_place(p, w, ps, n, a, b, t); }
+uint32_t place(const int* p, int w, int ps, int n, uint32_t a, uint32_t b, int t) { return nrq::page_place(p, w, ps, n, a, b, t); }
 void span(int len, int count, int n_new, int64_t held, int window, int tile, int* o) {
   nrq::SeqSpan s = nrq::seq_span(len, count, n_new, held, window, tile);
   o[0] = s.len; o[1] = s.n; o[2] = s.start; o[3] = s.tiles;
 }
-int64_t start(int64_t w, int64_t t, int64_t n) { return nrq::line_start(w, t, n); }
-int64_t owner(int64_t g, int64_t t, int64_t n) { return nrq::line_owner(g, t, n); }
+int start(int w, int t, int n) { return nrq::line_start(w, t, n); }
+int owner(int g, int t, int n) { return nrq::line_owner(g, t, n); }
 }
 ''')
     so = d / "page.so"
@@ -222,11 +225,11 @@ int64_t owner(int64_t g, int64_t t, int64_t n) { return nrq::line_owner(g, t, n)
                     "-fno-sanitize-recover", "-static-libubsan", "-I", os.path.join(ROOT, "nightrun_amd", "csrc"),
                     str(src), "-o", str(so)], check=True)
     L = C.CDLL(str(so))
-    i, q = C.c_int, C.c_int64
-    L.place.argtypes, L.place.restype = [C.c_void_p, i, i, i, q, q, i], q
+    i, q, u = C.c_int, C.c_int64, C.c_uint32
+    L.place.argtypes, L.place.restype = [C.c_void_p, i, i, i, u, u, i], u
     L.span.argtypes = [i, i, i, q, i, i, C.c_void_p]
-    L.start.argtypes, L.start.restype = [q, q, q], q
-    L.owner.argtypes, L.owner.restype = [q, q, q], q
+    L.start.argtypes, L.start.restype = [i, i, i], i
+    L.owner.argtypes, L.owner.restype = [i, i, i], i
     return L
 
 
@@ -234,13 +237,13 @@ int64_t owner(int64_t g, int64_t t, int64_t n) { return nrq::line_owner(g, t, n)
 def test_places(page, size):
     """Every position of a table with bad entries: the page's place, or none."""
     table = np.array([3, -1, 7, 8, 0, -2 ** 31, 2 ** 31 - 1, 5], np.int32)
-    n_pages, ps, ts = 8, 3 * 2 ** 32, 136
+    n_pages, ps, ts, none = 8, 3 * 2 ** 27, 17, 2 ** 32 - 1
     for t in list(range(-3, 8 * size + 3)) + [2 ** 31 - 1, -2 ** 31]:
-        want = -1
+        want = none
         if 0 <= t < 8 * size and 0 <= table[t // size] < n_pages:
             want = int(table[t // size]) * ps + (t % size) * ts
         assert page.place(table.ctypes.data, 8, size, n_pages, ps, ts, t) == want, t
-    assert page.place(table.ctypes.data, 0, size, n_pages, ps, ts, 0) == -1
+    assert page.place(table.ctypes.data, 0, size, n_pages, ps, ts, 0) == none
 
 
 def test_spans(page):
@@ -262,7 +265,7 @@ def test_spans(page):
 
 
 @pytest.mark.parametrize("total,wgs", [(1, 1), (7, 3), (7, 7), (1000, 64), (1023, 1024), (999983, 1024),
-                                       (2 ** 40 + 11, 1024)])
+                                       (2 ** 31 - 1, 1024), (2 ** 31 - 1024, 1023)])
 def test_line(page, total, wgs):
     """Every tile has one owner, whose stretch holds it; every workgroup has a stretch."""
     wgs = min(total, wgs)
