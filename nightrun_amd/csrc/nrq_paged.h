@@ -280,8 +280,12 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
   constexpr int KS = HD / 32;  // steps of K
   constexpr int DV = HD / 16;  // dimensions of a lane's values
   constexpr int OS = 16 * NT + 1;  // row stride of the exchange: odd
-  __shared__ float ex_ml[4][NT * 16][2];
-  __shared__ float ex_o[4][HD * OS];
+  __shared__ float ex_ml[4][NT * 16][2], unit_log2[NT * 16];
+  // the queries' pieces while a stretch runs, the waves' results behind it
+  constexpr int QB = NQ * NT * KS * 64 * 16, OB = 4 * HD * OS * 4;
+  __shared__ __align__(16) uint8_t shared[QB > OB ? QB : OB];
+  float (*ex_o)[HD * OS] = (float (*)[HD * OS])shared;
+  u32x4* qs = (u32x4*)shared;  // [k][n][s][lane]
   const PagedAttnLaunch& L = A.L;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
 
@@ -310,18 +314,23 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       const uint16_t* vp = L.kv.v + head * L.kv.head_stride;
       const int pw = sq.start + 32 * w + (lane & 31);  // the lane's position in the first tile
       uint32_t here = pa_place(L, pages, pw + t_begin * kTile, begin, end);
-      // ---- queries, and what each row sees
-      v8 q[NQ][NT][KS];
-      float to_log2[NT];  // what brings a row's products to log2 units
-      int lo[NT], hi[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        const int r = min(row0 + 16 * n + c, sq.n * A.group - 1), tok = r / A.group;
-        hi[n] = sq.len - sq.n + tok;
-        lo[n] = L.window > 0 ? max(0, hi[n] - L.window + 1) : 0;
+      PaTile<HD> tile;
+      uint32_t live = (uint32_t)__ballot(here != kNoPlace), next = kNoPlace, next_live = 0;
+      if (live) {  // else the pool may be empty
+        tile.load_k(kp, here == kNoPlace ? 0 : here, c, g);
+        tile.load_v(vp, here == kNoPlace ? 0 : here, c, g);
+      }
+      if (t_begin + 1 < t_end) {
+        next = pa_place(L, pages, pw + (t_begin + 1) * kTile, begin, end);
+        next_live = (uint32_t)__ballot(next != kNoPlace);
+      }
+      // ---- queries: wave n brings the pieces of group n to LDS, in registers they would cost the
+      // workgroups of a CU that hide the loads
+      __syncthreads();  // the exchange of the unit before is read
+      if (w < NT) {
+        const int r = min(row0 + 16 * w + c, sq.n * A.group - 1), tok = r / A.group;
         const int64_t qa = b * L.qb + tok * L.qt + (head * A.group + r - tok * A.group) * L.qh + 8 * g;
-        to_log2[n] = L.scale * kLog2e;
-        float f[KS][8];
+        float f[KS][8], unit = L.scale * kLog2e;
         if (NQ == 1)
           pa_load_q<T, KS>(L.q, qa, A.wide_q, f);  // 16 bits either way: the conversions cancel
         else if (L.dtype == kF32)
@@ -344,15 +353,25 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
           for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int i = 0; i < 8; i++) f[s][i] *= up;
-          to_log2[n] *= 1.0f / up;
+          unit *= 1.0f / up;
         }
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           v8 tmp[NQ];
           pa_split<T, NQ>(f[s], tmp);
 #pragma unroll
-          for (int k = 0; k < NQ; k++) q[k][n][s] = tmp[k];
+          for (int k = 0; k < NQ; k++) qs[((k * NT + w) * KS + s) * 64 + lane] = *(u32x4*)&tmp[k];
         }
+        if (g == 0) unit_log2[16 * w + c] = unit;
+      }
+      __syncthreads();
+      float to_log2[NT];  // what brings a row's products to log2 units
+      int lo[NT], hi[NT];  // what the row sees
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        to_log2[n] = unit_log2[16 * n + c];
+        hi[n] = sq.len - sq.n + min(row0 + 16 * n + c, sq.n * A.group - 1) / A.group;
+        lo[n] = L.window > 0 ? max(0, hi[n] - L.window + 1) : 0;
       }
 
       float m[NT], l[NT];
@@ -364,16 +383,6 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
 #pragma unroll
         for (int d = 0; d < DV; d++) acc[n][d] = f32x4{0, 0, 0, 0};
       }
-      PaTile<HD> tile;
-      uint32_t live = (uint32_t)__ballot(here != kNoPlace), next = kNoPlace, next_live = 0;
-      if (live) {  // else the pool may be empty
-        tile.load_k(kp, here == kNoPlace ? 0 : here, c, g);
-        tile.load_v(vp, here == kNoPlace ? 0 : here, c, g);
-      }
-      if (t_begin + 1 < t_end) {
-        next = pa_place(L, pages, pw + (t_begin + 1) * kTile, begin, end);
-        next_live = (uint32_t)__ballot(next != kNoPlace);
-      }
       int p0 = sq.start + t_begin * kTile + 32 * w;
       for (int t = t_begin; t < t_end; t++, p0 += kTile) {
         uint32_t after = kNoPlace;
@@ -381,16 +390,19 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
         // ---- scores: 8 positions for query c of each group
         f32x4 x[NT][2];
         if (live) {
+          asm volatile("" ::: "memory");  // the queries stay in LDS
 #pragma unroll
-          for (int n = 0; n < NT; n++)
+          for (int n = 0; n < NT; n++) {
+            x[n][0] = x[n][1] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-              x[n][u] = f32x4{0, 0, 0, 0};
+            for (int k = NQ - 1; k >= 0; k--)
 #pragma unroll
-              for (int k = NQ - 1; k >= 0; k--)
-#pragma unroll
-                for (int s = 0; s < KS; s++) x[n][u] = PaType<T>::mfma(*(v8*)&tile.k[u][s], q[k][n][s], x[n][u]);
-            }
+              for (int s = 0; s < KS; s++) {
+                const u32x4 q = qs[((k * NT + n) * KS + s) * 64 + lane];
+                x[n][0] = PaType<T>::mfma(*(v8*)&tile.k[0][s], *(v8*)&q, x[n][0]);
+                x[n][1] = PaType<T>::mfma(*(v8*)&tile.k[1][s], *(v8*)&q, x[n][1]);
+              }
+          }
         }
         const uint32_t ahead = next == kNoPlace ? 0 : next;
         if (next_live) tile.load_k(kp, ahead, c, g);
@@ -459,7 +471,7 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
         for (int d = 0; d < DV; d++)
           sum += (acc[n][d][0] * 0.0f + acc[n][d][1] * 0.0f) + (acc[n][d][2] * 0.0f + acc[n][d][3] * 0.0f);
       }
-      __syncthreads();  // the exchange of the unit before is read
+      __syncthreads();  // the queries are read
       if (__any(sum != sum)) {
         pa_plain<T, HD>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, sq.len,
                         sq.n, ex_o[w], ex_ml[w], OS);
