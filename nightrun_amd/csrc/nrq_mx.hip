@@ -227,6 +227,7 @@ hipError_t launch_mx_dequantize(const void* q, const void* s, size_t rows, size_
 }
 
 hipError_t launch_mx_matmul(const MxMatmul& L) {
+  if (L.batch > 64 && L.cols >= 64) return launch_mx_gemm(L);
   const int tiles = (L.batch + 15) / 16;
   const unsigned gx = (unsigned)((L.rows + 15) / 16);
   if (tiles == 1)

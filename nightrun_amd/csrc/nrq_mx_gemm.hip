@@ -1,0 +1,166 @@
+// The MXFP4 product over many tokens: tiles of 128 rows of w by 128 tokens.
+//
+// A stage holds 256 columns (128 bytes) of the tile's 128 + 128 rows, 32 KiB; two
+// stages take turns, filled by direct loads to LDS while the other is
+// multiplied, two workgroups a CU. 16-byte chunk c of row r lies at c ^ (r / 2 & 7): the 16
+// rows that a matrix instruction's quarter reads at one chunk fall on 16 different
+// places of the 64 banks. A wave multiplies 64 rows by 64 tokens; of lane l's
+// two steps in a stage, step s takes block 2 (l / 16) + s, so that both scale bytes of a
+// row come as one 16-bit load and the instruction picks the byte. Chunks behind
+// the last column come from zeros; rows behind the last are the last once more and are not stored.
+#include "nrq_serve_launch.h"
+
+namespace nrq {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kGemmTile = 128;
+
+__device__ const uint32_t mx_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
+
+// 16 bytes a lane from memory to LDS, lane after lane from byte address m0 (wave-uniform)
+__device__ __forceinline__ void mx_dma16(const void* g, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
+}
+
+template <int S>
+__device__ __forceinline__ f32x4 mx_step(i32x4 a, int sa, i32x4 b, int sb, f32x4 c) {
+  const i32x8 x = {a.x, a.y, a.z, a.w, 0, 0, 0, 0}, y = {b.x, b.y, b.z, b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, S, sa, S, sb);
+}
+
+template <typename T>
+struct alignas(sizeof(T) * 4) Out4 {
+  T v[4];
+};
+
+template <typename T>
+__device__ __forceinline__ void mx_out(void* y, int64_t at, int n, bool wide, f32x4 v) {
+  T* p = (T*)y + at;
+  if (wide && n >= 4) {
+    Out4<T> o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o.v[i] = (T)v[i];
+    *(Out4<T>*)p = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (i < n) p[i] = (T)v[i];
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 2) void mx_gemm_kernel(MxMatmul L, int row_tiles, int tok_tiles, int wide) {
+  __shared__ __align__(16) uint8_t stage[2][256][128];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int blocks = L.cols / 32, tiles_k = (blocks + 7) / 8;
+  // workgroups go round the eight XCDs: each XCD gets a run of tiles, row tile by row
+  // tile, so that its share of w and the tokens stay in its L2
+  const int all = row_tiles * tok_tiles, x = blockIdx.x & 7;
+  const int t = x * (all >> 3) + min(x, all & 7) + (int)(blockIdx.x >> 3);
+  const int r0 = t / tok_tiles * kGemmTile, b0 = t % tok_tiles * kGemmTile;
+
+  // this lane's chunks of a stage: row 32 j + 8 w + lane / 8, j < 4 of w, then of the tokens
+  const int sub = 8 * w + (lane >> 3), chunk = (lane & 7) ^ (((w & 1) << 2 | lane >> 4) & 7);
+  const uint8_t* src[8];
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const int r = 32 * (j & 3) + sub;
+    src[j] = j < 4 ? L.w + (int64_t)min(r0 + r, L.rows - 1) * blocks * 16 : L.x + (int64_t)min(b0 + r, L.batch - 1) * blocks * 16;
+    src[j] += chunk * 16;
+  }
+  const uint32_t base = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&stage[0][0][0] + (uint32_t)w * 1024u);
+  auto fill = [&](int kt) {
+    const bool live = 8 * kt + chunk < blocks;
+    const uint32_t to = base + (uint32_t)(kt & 1) * 32768u;
+#pragma unroll
+    for (int j = 0; j < 8; j++) mx_dma16(live ? src[j] + (int64_t)kt * 128 : (const uint8_t*)mx_zeros, to + (uint32_t)j * 4096u);
+  };
+  // scale bytes of this wave's rows and tokens
+  const int wr = 64 * (w & 1), wb = 64 * (w >> 1);
+  const uint8_t *ss[8];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    ss[i] = L.ws + (int64_t)min(r0 + wr + 16 * i + c, L.rows - 1) * blocks + 2 * g;
+    ss[4 + i] = L.xs + (int64_t)min(b0 + wb + 16 * i + c, L.batch - 1) * blocks + 2 * g;
+  }
+  // both bytes of a stage's two steps, from the last two where the row has ended (at least two blocks): no
+  // load is conditional, what it gives is put right when it is used
+  uint16_t sc[8];
+  auto scales = [&](int kt) {
+    const int b = min(8 * kt, blocks - 2 - 2 * g);
+#pragma unroll
+    for (int i = 0; i < 8; i++) __builtin_memcpy(&sc[i], ss[i] + b, 2);
+  };
+
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+  fill(0);
+  scales(0);
+  const int swz = (c >> 1) & 7;
+  for (int kt = 0; kt < tiles_k; kt++) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int now[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int left = blocks - 8 * kt - 2 * g;  // blocks from this one on
+      now[i] = left >= 2 ? (int)sc[i] : (left == 1 ? 0x7f00 | sc[i] >> 8 : 0x7f7f);
+    }
+    if (kt + 1 < tiles_k) {
+      fill(kt + 1);
+      scales(kt + 1);
+    }
+    const uint8_t(*rows)[128] = stage[kt & 1];
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const int at = ((2 * g + s) ^ swz) * 16;
+      i32x4 a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        a[i] = *(const i32x4*)&rows[wr + 16 * i + c][at];
+        b[i] = *(const i32x4*)&rows[128 + wb + 16 * i + c][at];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          acc[i][j] = s ? mx_step<1>(a[i], now[i], b[j], now[4 + j], acc[i][j]) : mx_step<0>(a[i], now[i], b[j], now[4 + j], acc[i][j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int tok = b0 + wb + 16 * j + c;
+    if (tok >= L.batch) continue;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int r = r0 + wr + 16 * i + 4 * g;
+      if (r < L.rows) mx_out<T>(L.y, tok * L.ldy + r, L.rows - r, wide, acc[i][j]);
+    }
+  }
+}
+
+template <typename T>
+hipError_t gemm_t(const MxMatmul& L) {
+  const int rt = (L.rows + kGemmTile - 1) / kGemmTile, tt = (L.batch + kGemmTile - 1) / kGemmTile;
+  const int wide = ((uintptr_t)L.y & (4 * sizeof(T) - 1)) == 0 && L.ldy % 4 == 0;
+  hipLaunchKernelGGL((mx_gemm_kernel<T>), dim3((unsigned)(rt * tt)), dim3(256), 0, L.stream, L, rt, tt, wide);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// At least two blocks a row (the scale bytes come in pairs).
+hipError_t launch_mx_gemm(const MxMatmul& L) {
+  if (L.dtype == kF32) return gemm_t<float>(L);
+  return L.dtype == kF16 ? gemm_t<_Float16>(L) : gemm_t<__bf16>(L);
+}
+
+}  // namespace nrq

@@ -86,5 +86,6 @@ struct MxMatmul {
   hipStream_t stream;
 };
 hipError_t launch_mx_matmul(const MxMatmul& L);
+hipError_t launch_mx_gemm(const MxMatmul& L);  // many tokens (nrq_mx_gemm.hip)
 
 }  // namespace nrq
