@@ -26,6 +26,11 @@ __device__ __forceinline__ void mx_dma16(const void* g, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
 }
 
+// the same with 4 bytes a lane
+__device__ __forceinline__ void mx_dma4(const void* g, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(m0), "v"(g) : "memory");
+}
+
 template <int S>
 __device__ __forceinline__ f32x4 mx_step(i32x4 a, int sa, i32x4 b, int sb, f32x4 c) {
   const i32x8 x = {a.x, a.y, a.z, a.w, 0, 0, 0, 0}, y = {b.x, b.y, b.z, b.w, 0, 0, 0, 0};
@@ -147,11 +152,101 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(MxMatmul L, int row_til
   }
 }
 
+// The same for whole steps of 128 columns: four stages of one step each (64 bytes and one dword
+// of scales a row, 17 KiB), three of them on their way while the fourth is multiplied. Chunk c of
+// row r lies at c ^ (r / 4 & 3).
+template <typename T>
+__global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_tiles, int tok_tiles, int wide) {
+  constexpr int NS = 4, SB = 256 * 64 + 256 * 4;
+  __shared__ __align__(16) uint8_t stage[NS][SB];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+  const int blocks = L.cols / 32, steps = blocks / 4;
+  const int all = row_tiles * tok_tiles, x = blockIdx.x & 7;
+  const int t = x * (all >> 3) + min(x, all & 7) + (int)(blockIdx.x >> 3);
+  const int r0 = t / tok_tiles * kGemmTile, b0 = t % tok_tiles * kGemmTile;
+
+  const uint8_t* src[5];
+  const int chunk = (lane & 3) ^ (lane >> 4);
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    const int r = 32 * w + 16 * j + (lane >> 2);
+    src[j] = L.w + (int64_t)min(r0 + r, L.rows - 1) * blocks * 16 + chunk * 16;
+    src[2 + j] = L.x + (int64_t)min(b0 + r, L.batch - 1) * blocks * 16 + chunk * 16;
+  }
+  {
+    const int r = 64 * (w & 1) + lane;
+    src[4] = w < 2 ? L.ws + (int64_t)min(r0 + r, L.rows - 1) * blocks : L.xs + (int64_t)min(b0 + r, L.batch - 1) * blocks;
+  }
+  const uint32_t base = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&stage[0][0]);
+  auto fill = [&](int k) {
+    const uint32_t to = base + (uint32_t)(k & (NS - 1)) * SB;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      mx_dma16(src[j] + k * 64, to + (uint32_t)(32 * w + 16 * j) * 64);
+      mx_dma16(src[2 + j] + k * 64, to + (uint32_t)(128 + 32 * w + 16 * j) * 64);
+    }
+    mx_dma4(src[4] + k * 4, to + 256 * 64 + (uint32_t)w * 256);
+  };
+
+  f32x4 acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+  const int wr = 64 * (w & 1), wb = 128 + 64 * (w >> 1);
+  const int at = (g ^ (c >> 2)) * 16;
+#pragma unroll
+  for (int k = 0; k < NS - 1; k++)
+    if (k < steps) fill(k);
+  for (int k = 0; k < steps; k++) {
+    // five loads a stage: this one's are there when those of the two behind it may be missing
+    if (k + 2 < steps)
+      asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    else if (k + 1 < steps)
+      asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // everyone's are there, and the stage before has been read
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + NS - 1 < steps) fill(k + NS - 1);
+    const uint8_t* st = stage[k & (NS - 1)];
+    const uint8_t* sc = st + 256 * 64;
+    i32x4 a[4], b[4];
+    int sa[4], sb[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      a[i] = *(const i32x4*)(st + (wr + 16 * i + c) * 64 + at);
+      b[i] = *(const i32x4*)(st + (wb + 16 * i + c) * 64 + at);
+      sa[i] = sc[(wr + 16 * i + c) * 4 + g];
+      sb[i] = sc[(wb + 16 * i + c) * 4 + g];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) acc[i][j] = mx_step<0>(a[i], sa[i], b[j], sb[j], acc[i][j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int tok = b0 + wb - 128 + 16 * j + c;
+    if (tok >= L.batch) continue;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int r = r0 + wr + 16 * i + 4 * g;
+      if (r < L.rows) mx_out<T>(L.y, tok * L.ldy + r, L.rows - r, wide, acc[i][j]);
+    }
+  }
+}
+
 template <typename T>
 hipError_t gemm_t(const MxMatmul& L) {
   const int rt = (L.rows + kGemmTile - 1) / kGemmTile, tt = (L.batch + kGemmTile - 1) / kGemmTile;
   const int wide = ((uintptr_t)L.y & (4 * sizeof(T) - 1)) == 0 && L.ldy % 4 == 0;
-  hipLaunchKernelGGL((mx_gemm_kernel<T>), dim3((unsigned)(rt * tt)), dim3(256), 0, L.stream, L, rt, tt, wide);
+  const bool steps = L.cols % 128 == 0 && ((uintptr_t)L.ws & 3) == 0 && ((uintptr_t)L.xs & 3) == 0;
+  if (steps)
+    hipLaunchKernelGGL((mx_gemm128_kernel<T>), dim3((unsigned)(rt * tt)), dim3(256), 0, L.stream, L, rt, tt, wide);
+  else
+    hipLaunchKernelGGL((mx_gemm_kernel<T>), dim3((unsigned)(rt * tt)), dim3(256), 0, L.stream, L, rt, tt, wide);
   return hipGetLastError();
 }
 
