@@ -26,11 +26,6 @@ __device__ __forceinline__ void mx_dma16(const void* g, uint32_t m0) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
 }
 
-// the same with 4 bytes a lane
-__device__ __forceinline__ void mx_dma4(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(m0), "v"(g) : "memory");
-}
-
 template <int S>
 __device__ __forceinline__ f32x4 mx_step(i32x4 a, int sa, i32x4 b, int sb, f32x4 c) {
   const i32x8 x = {a.x, a.y, a.z, a.w, 0, 0, 0, 0}, y = {b.x, b.y, b.z, b.w, 0, 0, 0, 0};
@@ -38,18 +33,17 @@ __device__ __forceinline__ f32x4 mx_step(i32x4 a, int sa, i32x4 b, int sb, f32x4
 }
 
 template <typename T>
-struct alignas(sizeof(T) * 4) Out4 {
-  T v[4];
-};
-
-template <typename T>
 __device__ __forceinline__ void mx_out(void* y, int64_t at, int n, bool wide, f32x4 v) {
   T* p = (T*)y + at;
   if (wide && n >= 4) {
-    Out4<T> o;
-#pragma unroll
-    for (int i = 0; i < 4; i++) o.v[i] = (T)v[i];
-    *(Out4<T>*)p = o;
+    // past the caches, which w and the tokens fill: 16384 x 2048 at 2048 tokens takes 92 us so, 117 through them
+    if constexpr (sizeof(T) == 4) {
+      __builtin_nontemporal_store(v, (f32x4*)p);
+    } else {
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      const t4 o = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+      __builtin_nontemporal_store(o, (t4*)p);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -57,16 +51,28 @@ __device__ __forceinline__ void mx_out(void* y, int64_t at, int n, bool wide, f3
   }
 }
 
+// Which tile a workgroup takes. Workgroups go round the eight XCDs; each XCD gets a run of the
+// tiles, which go by groups of up to 16 row tiles, within a group by tokens, and for the same
+// tokens by rows. So an XCD keeps its rows of w in its L2, and what it writes at a time lies
+// together: by tokens first, 16384 x 2048 at 2048 tokens takes 94 us, so 75.
+struct GemmTile {
+  int r, b;
+};
+__device__ __forceinline__ GemmTile gemm_tile(int row_tiles, int tok_tiles) {
+  const int all = row_tiles * tok_tiles, x = blockIdx.x & 7;
+  const int t = x * (all >> 3) + min(x, all & 7) + (int)(blockIdx.x >> 3);
+  const int group = min(16, (row_tiles + 7) >> 3), q = t / (group * tok_tiles), i = t - q * group * tok_tiles;
+  const int rows = min(group, row_tiles - q * group), b = i / rows;
+  return GemmTile{q * group + i - b * rows, b};
+}
+
 template <typename T>
 __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(MxMatmul L, int row_tiles, int tok_tiles, int wide) {
   __shared__ __align__(16) uint8_t stage[2][256][128];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int blocks = L.cols / 32, tiles_k = (blocks + 7) / 8;
-  // workgroups go round the eight XCDs: each XCD gets a run of tiles, row tile by row
-  // tile, so that its share of w and the tokens stay in its L2
-  const int all = row_tiles * tok_tiles, x = blockIdx.x & 7;
-  const int t = x * (all >> 3) + min(x, all & 7) + (int)(blockIdx.x >> 3);
-  const int r0 = t / tok_tiles * kGemmTile, b0 = t % tok_tiles * kGemmTile;
+  const GemmTile tile = gemm_tile(row_tiles, tok_tiles);
+  const int r0 = tile.r * kGemmTile, b0 = tile.b * kGemmTile;
 
   // this lane's chunks of a stage: row 32 j + 8 w + lane / 8, j < 4 of w, then of the tokens
   const int sub = 8 * w + (lane >> 3), chunk = (lane & 7) ^ (((w & 1) << 2 | lane >> 4) & 7);
@@ -152,18 +158,19 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(MxMatmul L, int row_til
   }
 }
 
-// The same for whole steps of 128 columns: four stages of one step each (64 bytes and one dword
-// of scales a row, 17 KiB), three of them on their way while the fourth is multiplied. Chunk c of
-// row r lies at c ^ (r / 4 & 3).
+// The same for whole steps of 128 columns: four stages of one step each (64 bytes a row, 16
+// KiB), three of them on their way while the fourth is multiplied. Chunk c of row r
+// lies at c ^ (r / 4 & 3). The scale bytes come for four steps at a time, 16 bytes of a
+// row in one piece: by the step they would be as many requests to L2 as the values.
 template <typename T>
 __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_tiles, int tok_tiles, int wide) {
-  constexpr int NS = 4, SB = 256 * 64 + 256 * 4;
+  constexpr int NS = 4, SB = 256 * 64;
   __shared__ __align__(16) uint8_t stage[NS][SB];
+  __shared__ __align__(16) uint8_t scale[2][256][16];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int blocks = L.cols / 32, steps = blocks / 4;
-  const int all = row_tiles * tok_tiles, x = blockIdx.x & 7;
-  const int t = x * (all >> 3) + min(x, all & 7) + (int)(blockIdx.x >> 3);
-  const int r0 = t / tok_tiles * kGemmTile, b0 = t % tok_tiles * kGemmTile;
+  const GemmTile tile = gemm_tile(row_tiles, tok_tiles);
+  const int r0 = tile.r * kGemmTile, b0 = tile.b * kGemmTile;
 
   const uint8_t* src[5];
   const int chunk = (lane & 3) ^ (lane >> 4);
@@ -179,14 +186,17 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
   }
   const uint32_t base = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&stage[0][0]);
+  const uint32_t sbase = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&scale[0][0][0]);
   auto fill = [&](int k) {
+    // the last 16 of the row where fewer are left (at least 16 blocks)
+    if ((k & 3) == 0) mx_dma16(src[4] + min(4 * k, blocks - 16), sbase + (uint32_t)(k >> 2 & 1) * 4096 + (uint32_t)w * 1024);
     const uint32_t to = base + (uint32_t)(k & (NS - 1)) * SB;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       mx_dma16(src[j] + k * 64, to + (uint32_t)(32 * w + 16 * j) * 64);
       mx_dma16(src[2 + j] + k * 64, to + (uint32_t)(128 + 32 * w + 16 * j) * 64);
     }
-    mx_dma4(src[4] + k * 4, to + 256 * 64 + (uint32_t)w * 256);
   };
 
   f32x4 acc[4][4];
@@ -200,26 +210,26 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
   for (int k = 0; k < NS - 1; k++)
     if (k < steps) fill(k);
   for (int k = 0; k < steps; k++) {
-    // five loads a stage: this one's are there when those of the two behind it may be missing
+    // at least four loads a stage: this one's are there when those of the two behind it may be missing
     if (k + 2 < steps)
-      asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     else if (k + 1 < steps)
-      asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     else
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // everyone's are there, and the stage before has been read
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (k + NS - 1 < steps) fill(k + NS - 1);
     const uint8_t* st = stage[k & (NS - 1)];
-    const uint8_t* sc = st + 256 * 64;
+    const uint8_t* sc = &scale[k >> 2 & 1][0][4 * k + g - min(4 * (k & ~3), blocks - 16)];
     i32x4 a[4], b[4];
     int sa[4], sb[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       a[i] = *(const i32x4*)(st + (wr + 16 * i + c) * 64 + at);
       b[i] = *(const i32x4*)(st + (wb + 16 * i + c) * 64 + at);
-      sa[i] = sc[(wr + 16 * i + c) * 4 + g];
-      sb[i] = sc[(wb + 16 * i + c) * 4 + g];
+      sa[i] = sc[(wr + 16 * i + c) * 16];
+      sb[i] = sc[(wb + 16 * i + c) * 16];
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -242,7 +252,7 @@ template <typename T>
 hipError_t gemm_t(const MxMatmul& L) {
   const int rt = (L.rows + kGemmTile - 1) / kGemmTile, tt = (L.batch + kGemmTile - 1) / kGemmTile;
   const int wide = ((uintptr_t)L.y & (4 * sizeof(T) - 1)) == 0 && L.ldy % 4 == 0;
-  const bool steps = L.cols % 128 == 0 && ((uintptr_t)L.ws & 3) == 0 && ((uintptr_t)L.xs & 3) == 0;
+  const bool steps = L.cols % 128 == 0 && L.cols >= 512 && ((uintptr_t)L.ws & 3) == 0 && ((uintptr_t)L.xs & 3) == 0;
   if (steps)
     hipLaunchKernelGGL((mx_gemm128_kernel<T>), dim3((unsigned)(rt * tt)), dim3(256), 0, L.stream, L, rt, tt, wide);
   else
