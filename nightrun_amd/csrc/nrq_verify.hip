@@ -2,23 +2,28 @@
 //
 // Per sequence one row decides: the first refused draft's, or the one behind the
 // last draft. The first launch finds it (a few gathers and a ballot, done again
-// by every workgroup) and sums its weights over spans of the vocabulary, the
-// second adds the spans up, finds the one in which the drawn point lies and scans
+// by every workgroup, which takes a run of spans so that this is not most of its time) and sums its
+// weights over spans of 1024 tokens, the second adds the spans up, finds the one in which the drawn point lies and scans
 // it. All sums are f64 in a fixed order: cumulative sums of 10^5 f32 weights in
 // f32 would be off by more than the gap between neighbouring tokens.
 #include "nrq_serve_launch.h"
+
+#include <climits>
 
 namespace nrq {
 namespace {
 
 constexpr int kVerNT = 256;
-constexpr int kVerPer = 8;                     // values of a thread
-constexpr int kVerSpan = kVerNT * kVerPer;     // values of a workgroup
+constexpr int kVerPer = 4;                  // values of a thread: 16 bytes
+constexpr int kVerSpan = kVerNT * kVerPer;  // values of a span
+constexpr int kVerMost = 32;                // spans of a workgroup at most
+constexpr int kVerFill = 2048;              // workgroups that the card holds
 
 struct VerArgs {
   VerifyLaunch L;
-  double* sums;  // [seqs][spans][2]: of the residual, of the target
-  int spans;
+  double* sums;  // [seqs][spans]
+  int* counts;   // [seqs]: drafts accepted
+  int spans, per;  // of a row, of a workgroup
 };
 
 struct VerRow {
@@ -56,29 +61,21 @@ __device__ __forceinline__ VerRow verify_row(const VerifyLaunch& L, int b) {
   return r;
 }
 
-// weights of value v: of the residual and of the target; NaN and negative ones are none
-__device__ __forceinline__ double2 ver_weight(const VerRow& r, float p, float q, int v) {
-  const double tp = p > 0.0f ? (double)p : 0.0;
-  double res = tp;
+// weight of value v; NaN and negative ones are none
+__device__ __forceinline__ double ver_weight(const VerRow& r, float p, float q, int v) {
   if (r.q) {
     const double diff = (double)p - (double)q;
-    res = diff > 0.0 ? diff : 0.0;
-  } else if (v == r.without) {
-    res = 0.0;
+    return diff > 0.0 ? diff : 0.0;
   }
-  return make_double2(res, tp);
+  return p > 0.0f && v != r.without ? (double)p : 0.0;
 }
 
 __device__ __forceinline__ void ver_load(const VerRow& r, int v0, int vocab, float* p, float* q) {
   const bool wide = v0 + kVerPer <= vocab && (((uintptr_t)r.p | (uintptr_t)r.q) & 15) == 0;
   if (wide) {
-#pragma unroll
-    for (int i = 0; i < kVerPer; i += 4) {
-      const float4 a = *(const float4*)(r.p + v0 + i);
-      const float4 c = r.q ? *(const float4*)(r.q + v0 + i) : make_float4(0, 0, 0, 0);
-      p[i] = a.x, p[i + 1] = a.y, p[i + 2] = a.z, p[i + 3] = a.w;
-      q[i] = c.x, q[i + 1] = c.y, q[i + 2] = c.z, q[i + 3] = c.w;
-    }
+    const float4 a = *(const float4*)(r.p + v0), c = r.q ? *(const float4*)(r.q + v0) : make_float4(0, 0, 0, 0);
+    p[0] = a.x, p[1] = a.y, p[2] = a.z, p[3] = a.w;
+    q[0] = c.x, q[1] = c.y, q[2] = c.z, q[3] = c.w;
   } else {
 #pragma unroll
     for (int i = 0; i < kVerPer; i++) {
@@ -88,134 +85,153 @@ __device__ __forceinline__ void ver_load(const VerRow& r, int v0, int vocab, flo
   }
 }
 
+// Sum over the wave, in a fixed order.
+__device__ __forceinline__ double ver_wave_sum(double s) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) s += __shfl_xor(s, m);
+  return s;
+}
+
 __global__ __launch_bounds__(kVerNT) void verify_sums_kernel(VerArgs A) {
-  __shared__ double part[kVerNT / 64][2];
-  const int b = blockIdx.y, span = blockIdx.x;
+  __shared__ double part[kVerMost][kVerNT / 64];
+  const int b = blockIdx.y, s0 = blockIdx.x * A.per, s1 = min(s0 + A.per, A.spans), t = threadIdx.x;
   const VerRow r = verify_row(A.L, b);
-  const int v0 = span * kVerSpan + threadIdx.x * kVerPer;
-  double2 s = make_double2(0, 0);
-  if (v0 < A.L.vocab) {
-    float p[kVerPer], q[kVerPer];
-    ver_load(r, v0, A.L.vocab, p, q);
+  if (s0 == 0 && t == 0) A.counts[b] = r.count;
+  float p[kVerPer], q[kVerPer], pn[kVerPer] = {0, 0, 0, 0}, qn[kVerPer] = {0, 0, 0, 0};
+  ver_load(r, s0 * kVerSpan + t * kVerPer, A.L.vocab, p, q);
+  for (int k = s0; k < s1; k++) {  // the next span is on its way while this one is added up
+    const int v0 = k * kVerSpan + t * kVerPer;
+    if (k + 1 < s1) ver_load(r, v0 + kVerSpan, A.L.vocab, pn, qn);
+    double s = 0;
 #pragma unroll
-    for (int i = 0; i < kVerPer; i++) {
-      const double2 w = ver_weight(r, p[i], q[i], v0 + i);
-      s.x += w.x;
-      s.y += w.y;
-    }
-  }
+    for (int i = 0; i < kVerPer; i++)
+      if (v0 + i < A.L.vocab) s += ver_weight(r, p[i], q[i], v0 + i);
+    s = ver_wave_sum(s);
+    if ((t & 63) == 0) part[k - s0][t >> 6] = s;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    s.x += __shfl_xor(s.x, m);
-    s.y += __shfl_xor(s.y, m);
-  }
-  if ((threadIdx.x & 63) == 0) {
-    part[threadIdx.x >> 6][0] = s.x;
-    part[threadIdx.x >> 6][1] = s.y;
+    for (int i = 0; i < kVerPer; i++) p[i] = pn[i], q[i] = qn[i];
   }
   __syncthreads();
-  if (threadIdx.x < 2) {
-    double t = 0;
-    for (int w = 0; w < kVerNT / 64; w++) t += part[w][threadIdx.x];
-    A.sums[((int64_t)b * A.spans + span) * 2 + threadIdx.x] = t;
+  if (t < s1 - s0) {
+    double s = 0;
+    for (int w = 0; w < kVerNT / 64; w++) s += part[t][w];
+    A.sums[(int64_t)b * A.spans + s0 + t] = s;
   }
 }
 
-// Inclusive sums over the workgroup's threads; *total gets the whole.
-__device__ __forceinline__ double ver_scan(double x, double* lds, double* total) {
+// Sums over the workgroup's threads up to and before each; one thread's `upto` is the next one's
+// `before` to the bit, so that exactly one thread holds a point between them.
+struct VerSum {
+  double before, upto, total;
+};
+__device__ __forceinline__ VerSum ver_scan(double own, double* lds) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  double x = own;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     const double y = __shfl_up(x, m);
     if (lane >= m) x += y;
   }
-  __syncthreads();  // lds may still be read from the scan before
   if (lane == 63) lds[w] = x;
+  double y = __shfl_up(x, 1);
+  if (lane == 0) y = 0;
   __syncthreads();
   double before = 0, all = 0;
   for (int i = 0; i < kVerNT / 64; i++) {
-    if (i < w) before += lds[i];
+    if (i == w) before = all;
     all += lds[i];
   }
-  *total = all;
-  return before + x;
+  return VerSum{before + y, before + x, all};
 }
 
 __global__ __launch_bounds__(kVerNT) void verify_draw_kernel(VerArgs A) {
-  __shared__ double lds[kVerNT / 64];
-  __shared__ int first, last;
+  __shared__ double lds[3][kVerNT / 64], base;
+  __shared__ int found, last[2], drawn;
   const VerifyLaunch& L = A.L;
   const int b = blockIdx.x, t = threadIdx.x;
-  VerRow r = verify_row(L, b);
-  const double* sums = A.sums + (int64_t)b * A.spans * 2;
-  // the whole sums, in span order by threads; of the residual, else of the target
-  double all[2];
-  for (int k = 0; k < 2; k++) {
-    double s = 0;
-    for (int i = t; i < A.spans; i += kVerNT) s += sums[2 * i + k];
-    ver_scan(s, lds, &all[k]);
-  }
-  const int which = all[0] > 0.0 ? 0 : 1;
-  if (which) r.q = nullptr, r.without = -1;
-  const double point = (double)L.uniforms[(int64_t)b * (L.n_new + 1) + L.n_new] * all[which];
-  // the first span whose cumulative sum is above the point, else the last with any weight
-  double base = 0;
-  if (t == 0) first = A.spans, last = -1;
-  int span = -1;
-  double before = 0;
-  for (int i0 = 0; i0 < A.spans; i0 += kVerNT) {
-    const int i = i0 + t;
-    const double x = i < A.spans ? sums[2 * i + which] : 0.0;
-    double total;
-    const double c = ver_scan(x, lds, &total);  // its barriers order first and last too
-    if (i < A.spans && base + c > point) atomicMin(&first, i);
-    if (x > 0.0) atomicMax(&last, i);
-    __syncthreads();
-    const int f = first;
-    if (f < A.spans) {  // the sum before it: from the thread that holds it
-      if (i == f) lds[0] = base + (c - x);
-      __syncthreads();
-      span = f;
-      before = lds[0];
-      break;
+  double* sums = A.sums + (int64_t)b * A.spans;
+  // each thread adds up a run of spans (one, up to 262144 tokens)
+  const int per = (A.spans + kVerNT - 1) / kVerNT, s0 = min(t * per, A.spans), s1 = min(s0 + per, A.spans);
+  double own = 0;
+  for (int i = s0; i < s1; i++) own += sums[i];
+  const int n = L.counts ? min(max(L.counts[b], 0), L.n_new) : L.n_new;
+  VerRow r;
+  r.count = A.counts[b];
+  r.p = L.target + b * L.tb + r.count * L.tr;
+  r.q = r.count < n && L.draft ? L.draft + b * L.db + r.count * L.dr : nullptr;
+  r.without = r.count < n && !L.draft ? L.drafted[(int64_t)b * L.n_new + r.count] : -1;
+  const double u = (double)L.uniforms[(int64_t)b * (L.n_new + 1) + L.n_new];
+  if (t == 0) found = drawn = -1;
+  if (t < 2) last[t] = -1;
+  VerSum c = ver_scan(own, lds[0]);
+  if (!(c.total > 0.0) && (r.q || r.without >= 0)) {  // nothing left: the target itself (rare, by this workgroup alone)
+    r.q = nullptr;
+    r.without = -1;
+    own = 0;
+    for (int i = s0; i < s1; i++) {
+      double s = 0;
+      for (int v = i * kVerSpan; v < min((i + 1) * kVerSpan, L.vocab); v++) s += ver_weight(r, r.p[v], 0.0f, v);
+      sums[i] = s;  // read again by this thread only
+      own += s;
     }
-    base += total;
+    c = ver_scan(own, lds[1]);
+  }
+  // the first span whose cumulative sum is above the point
+  const double point = u * c.total;
+  if (c.before <= point && c.upto > point) {
+    double before = c.before;
+    int i = s0;
+    for (; i + 1 < s1; i++) {
+      const double s = sums[i];
+      if (before + s > point) break;
+      before += s;
+    }
+    found = i;
+    base = before;
   }
   __syncthreads();
+  int span = found;
   const bool past = span < 0;
-  if (past) span = last;
+  if (past) {  // no sum is above the point (a uniform of 1, or no weight): the last span with any
+    for (int i = s0; i < s1; i++)
+      if (sums[i] > 0.0) atomicMax(&last[0], i);
+    __syncthreads();
+    span = last[0];
+  }
   int token = -1;
   if (span >= 0) {
-    __syncthreads();
-    if (t == 0) first = kVerSpan, last = -1;
     const int v0 = span * kVerSpan + t * kVerPer;
     double w[kVerPer], s = 0;
-    if (v0 < L.vocab) {
-      float p[kVerPer], q[kVerPer];
-      ver_load(r, v0, L.vocab, p, q);
-#pragma unroll
-      for (int i = 0; i < kVerPer; i++) w[i] = which ? ver_weight(r, p[i], q[i], v0 + i).y : ver_weight(r, p[i], q[i], v0 + i).x;
-    } else {
-#pragma unroll
-      for (int i = 0; i < kVerPer; i++) w[i] = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < kVerPer; i++) s += w[i];
-    double total;
-    double c = before + (ver_scan(s, lds, &total) - s);
-    int above = kVerSpan, weight = -1;
+    float p[kVerPer], q[kVerPer];
+    ver_load(r, v0, L.vocab, p, q);
 #pragma unroll
     for (int i = 0; i < kVerPer; i++) {
-      c += w[i];
-      if (w[i] > 0.0) {
-        weight = t * kVerPer + i;
-        if (!past && c > point && above == kVerSpan) above = t * kVerPer + i;
-      }
+      w[i] = v0 + i < L.vocab ? ver_weight(r, p[i], q[i], v0 + i) : 0.0;
+      s += w[i];
     }
-    if (above < kVerSpan) atomicMin(&first, above);
-    if (weight >= 0) atomicMax(&last, weight);
+    const VerSum e = ver_scan(s, lds[2]);
+    const double point1 = past ? INFINITY : point - base;
+    int lastw = -1;
+#pragma unroll
+    for (int i = 0; i < kVerPer; i++)
+      if (w[i] > 0.0) lastw = v0 + i;
+    if (e.before <= point1 && e.upto > point1) {
+      double at = e.before;
+      int v = -1;
+#pragma unroll
+      for (int i = 0; i < kVerPer; i++) {
+        at += w[i];
+        if (v < 0 && w[i] > 0.0 && at > point1) v = v0 + i;
+      }
+      drawn = v < 0 ? lastw : v;  // the scan's rounding and this sum's may differ
+    }
     __syncthreads();
-    token = span * kVerSpan + (first < kVerSpan ? first : last);
+    token = drawn;
+    if (token < 0) {  // past the last weight, or what the span's sums differ by
+      if (lastw >= 0) atomicMax(&last[1], lastw);
+      __syncthreads();
+      token = last[1];
+    }
   }
   if (t == 0) L.accepted[b] = r.count;
   for (int j = t; j <= L.n_new; j += kVerNT)
@@ -226,11 +242,16 @@ __global__ __launch_bounds__(kVerNT) void verify_draw_kernel(VerArgs A) {
 }  // namespace
 
 size_t verify_workspace(size_t seqs, size_t vocab) {
-  return seqs * ((vocab + kVerSpan - 1) / kVerSpan) * 2 * sizeof(double);
+  return seqs * ((vocab + kVerSpan - 1) / kVerSpan * sizeof(double) + sizeof(int));
 }
 
 hipError_t launch_verify(const VerifyLaunch& L) {
-  VerArgs A{L, (double*)L.workspace, (L.vocab + kVerSpan - 1) / kVerSpan};
+  const int spans = (L.vocab + kVerSpan - 1) / kVerSpan;
+  VerArgs A{L, (double*)L.workspace, (int*)((double*)L.workspace + (size_t)L.seqs * spans), spans, 1};
+  // as many workgroups as the card holds, with equal runs of spans
+  int groups = kVerFill / L.seqs;
+  if (groups < (spans + kVerMost - 1) / kVerMost) groups = (spans + kVerMost - 1) / kVerMost;
+  A.per = (spans + groups - 1) / groups;
   for (int b0 = 0; b0 < L.seqs; b0 += 65535) {  // gridDim.y
     VerArgs P = A;
     const int n = L.seqs - b0 < 65535 ? L.seqs - b0 : 65535;
@@ -241,8 +262,9 @@ hipError_t launch_verify(const VerifyLaunch& L) {
     P.L.drafted += (int64_t)b0 * L.n_new;
     P.L.uniforms += (int64_t)b0 * (L.n_new + 1);
     if (L.counts) P.L.counts += b0;
-    P.sums += (int64_t)b0 * A.spans * 2;
-    hipLaunchKernelGGL(verify_sums_kernel, dim3(A.spans, n), dim3(kVerNT), 0, L.stream, P);
+    P.sums += (int64_t)b0 * A.spans;
+    P.counts += b0;
+    hipLaunchKernelGGL(verify_sums_kernel, dim3((A.spans + A.per - 1) / A.per, n), dim3(kVerNT), 0, L.stream, P);
     hipLaunchKernelGGL(verify_draw_kernel, dim3(n), dim3(kVerNT), 0, L.stream, P);
   }
   return hipGetLastError();
