@@ -40,122 +40,135 @@ struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
 
-// One head of one token: where its row comes from and goes to. kind 0: q, 1: k, 2: v.
-template <typename T>
-struct RopeRow {
-  const T* src;
-  T* y;         // q
-  uint16_t* c;  // k, v: the cache row, nullptr if there is none
-};
-
-template <typename T, typename C, int V>
-__device__ __forceinline__ void rope_put(const RopeRow<T>& r, int d, const float* f) {
-  if (r.y) {
-    Vec<T, V> o;
-#pragma unroll
-    for (int i = 0; i < V; i++) o.v[i] = (T)f[i];
-    *(Vec<T, V>*)(r.y + d) = o;
-  } else if (r.c) {
-    Vec<C, V> o;
-#pragma unroll
-    for (int i = 0; i < V; i++) o.v[i] = (C)f[i];
-    *(Vec<C, V>*)((C*)r.c + d) = o;
-  }
-}
+constexpr int kRopeTokens = 64;  // tokens of a workgroup at most
+constexpr int kRopeAhead = 4;    // rows of a thread whose loads are on their way together
 
 // T: the rows' type, C: the cache's, V: elements of one access (16 bytes of T
-// where strides, addresses and the rotated part allow it, else 1 or, for
-// adjacent pairs, 2 by scalar accesses).
+// where strides, addresses and the rotated part allow it, else 1).
+//
+// An item is an access of one head's row (with NEOX pairs an access of each half), 256 / items
+// rows at a time: a thread keeps its place in the row and goes from row to row.
 template <typename T, typename C, int V, bool APPEND>
 __global__ __launch_bounds__(kRopeNT) void rope_kernel(RopeLaunch L, int tpw) {
   __shared__ float2 cs[kRopePairs];
-  const int t0 = blockIdx.x * tpw, nt = min(tpw, L.tokens - t0);
-  for (int i = threadIdx.x; i < nt * L.nf; i += kRopeNT) {
-    const float2 v = sincos_turn(L.pos[t0 + i / L.nf], L.freqs[i % L.nf]);
+  __shared__ uint32_t place[kRopeTokens];
+  __shared__ bool pad[kRopeTokens];
+  const int t0 = blockIdx.x * tpw, nt = min(tpw, L.tokens - t0), half = L.nf;
+  for (int i = threadIdx.x; i < nt * half; i += kRopeNT) {
+    const float2 v = sincos_turn(L.pos[t0 + i / half], L.freqs[i % half]);
     cs[i] = make_float2(v.x * L.scale, v.y * L.scale);
   }
+  if (APPEND)
+    for (int i = threadIdx.x; i < nt; i += kRopeNT) {
+      const int seq = L.seq[t0 + i], pos = L.pos[t0 + i];
+      const bool p = seq < 0 || seq >= L.table.seqs || pos < 0;
+      pad[i] = p;
+      place[i] = p ? kNoPlace
+                   : page_place(L.table.pages + seq * L.table.stride, L.table.width, L.kv.page_size, L.kv.n_pages,
+                                L.kv.page_stride8, L.kv.pos_stride8, pos);
+    }
   __syncthreads();
   const int heads = APPEND ? L.heads + 2 * L.kv.n_kv : L.heads;
-  const int half = L.nf, rot = 2 * half;
-  // items of a head: with NEOX pairs an access of each half, else one access; then the rest of the head
-  const int rest0 = rot / V, chunks = L.hd / V;
+  const int rest0 = 2 * half / V, chunks = L.hd / V;  // accesses of the rotated part, of a row
   const int pairs = L.neox ? half / V : (V == 1 ? half : rest0);  // items that rotate
   const int items = pairs + chunks - rest0;
-  const int per_token = heads * items, total = nt * per_token;
-  const int step = kRopeNT * gridDim.y;
-  for (int it = blockIdx.y * kRopeNT + threadIdx.x; it < total; it += step) {
-    const int tt = it / per_token, r = it - tt * per_token, h = r / items, c = r - h * items;
-    const int t = t0 + tt;
-    RopeRow<T> row;
-    row.y = nullptr;
-    row.c = nullptr;
-    bool turn = true;
-    if (!APPEND) {
-      row.src = (const T*)L.x + t * L.xt + h * L.xh;
-      row.y = (T*)L.y + t * L.yt + h * L.yh;
-    } else {
-      const int seq = L.seq[t], pos = L.pos[t];
-      if (seq < 0 || seq >= L.table.seqs || pos < 0) continue;  // padding
-      if (h < L.heads) {
-        row.src = (const T*)L.x + t * L.xt + h * L.xh;
-        row.y = (T*)L.y + t * L.yt + h * L.yh;
-      } else {
-        const bool isk = h < L.heads + L.kv.n_kv;
-        const int hh = h - L.heads - (isk ? 0 : L.kv.n_kv);
-        const uint32_t place = page_place(L.table.pages + seq * L.table.stride, L.table.width, L.kv.page_size,
-                                          L.kv.n_pages, L.kv.page_stride8, L.kv.pos_stride8, pos);
-        if (place == kNoPlace) continue;
-        row.src = isk ? (const T*)L.k + t * L.kt + hh * L.kh : (const T*)L.v + t * L.vt + hh * L.vh;
-        row.c = (isk ? L.kv.k : L.kv.v) + (uint64_t)place * 8 + hh * L.kv.head_stride;
-        turn = isk;
-      }
-    }
-    const float2* w = cs + tt * half;
-    if (c >= pairs) {  // behind the rotated part
-      const int d = (rest0 + c - pairs) * V;
-      const Vec<T, V> a = *(const Vec<T, V>*)(row.src + d);
-      float o[V];
+  const int across = max(1, kRopeNT / items), lanes = min(items, kRopeNT);  // rows at a time; items over 256: one, in turns
+  const int row0 = (int)threadIdx.x / lanes;
+  if (row0 >= across) return;
+  const int step = across * gridDim.y, dt = step / heads, dh = step - dt * heads;
+  for (int c = (int)threadIdx.x - row0 * lanes; c < items; c += kRopeNT) {
+    const bool turning = c < pairs;
+    const int d = !turning ? (rest0 + c - pairs) * V : (L.neox ? c * V : (V == 1 ? 2 * c : c * V));
+    const int d1 = !turning ? d : (L.neox ? d + half : d + 1);  // the second access, if any
+    const bool two = turning && (L.neox || V == 1);
+    int r = row0 + across * blockIdx.y, tt = r / heads, h = r - tt * heads;
+    while (tt < nt) {
+      Vec<T, V> a[kRopeAhead], b[kRopeAhead];
+      const T* from[kRopeAhead];
+      T* y[kRopeAhead];
+      C* cache[kRopeAhead];
+      int tok[kRopeAhead];
+      bool turn[kRopeAhead];
 #pragma unroll
-      for (int i = 0; i < V; i++) o[i] = (float)a.v[i];
-      rope_put<T, C, V>(row, d, o);
-    } else if (L.neox) {
-      const int d = c * V;
-      const Vec<T, V> a = *(const Vec<T, V>*)(row.src + d), b = *(const Vec<T, V>*)(row.src + d + half);
-      float o0[V], o1[V];
-#pragma unroll
-      for (int i = 0; i < V; i++) {
-        const float x0 = (float)a.v[i], x1 = (float)b.v[i];
-        const float2 k = turn ? w[d + i] : make_float2(1.0f, 0.0f);
-        o0[i] = turn ? fmaf(x0, k.x, -(x1 * k.y)) : x0;
-        o1[i] = turn ? fmaf(x0, k.y, x1 * k.x) : x1;
+      for (int k = 0; k < kRopeAhead; k++) {
+        const int t = t0 + tt;
+        bool on = tt < nt;
+        tok[k] = tt;
+        from[k] = nullptr;
+        y[k] = nullptr;
+        cache[k] = nullptr;
+        turn[k] = turning;
+        if (on) {
+          if (!APPEND || h < L.heads) {
+            on = !APPEND || !pad[tt];
+            from[k] = (const T*)L.x + t * L.xt + h * L.xh;
+            y[k] = (T*)L.y + t * L.yt + h * L.yh;
+          } else {
+            const bool isk = h < L.heads + L.kv.n_kv;
+            const int hh = h - L.heads - (isk ? 0 : L.kv.n_kv);
+            on = place[tt] != kNoPlace;
+            from[k] = isk ? (const T*)L.k + t * L.kt + hh * L.kh : (const T*)L.v + t * L.vt + hh * L.vh;
+            cache[k] = (C*)(isk ? L.kv.k : L.kv.v) + (uint64_t)place[tt] * 8 + hh * L.kv.head_stride;
+            turn[k] = turning && isk;
+          }
+        }
+        if (on) {
+          a[k] = *(const Vec<T, V>*)(from[k] + d);
+          if (two) b[k] = *(const Vec<T, V>*)(from[k] + d1);
+        } else {
+          from[k] = nullptr;
+        }
+        h += dh;
+        tt += dt;
+        if (h >= heads) h -= heads, tt++;
       }
-      rope_put<T, C, V>(row, d, o0);
-      rope_put<T, C, V>(row, d + half, o1);
-    } else {
-      constexpr int P = V == 1 ? 2 : V;  // scalar accesses: the item is one pair
-      const int d = V == 1 ? 2 * c : c * V;
-      T x[P];
-      if constexpr (V == 1) {
-        x[0] = row.src[d];
-        x[1] = row.src[d + 1];
-      } else {
-        const Vec<T, V> a = *(const Vec<T, V>*)(row.src + d);
 #pragma unroll
-        for (int i = 0; i < V; i++) x[i] = a.v[i];
-      }
-      float o[P];
+      for (int k = 0; k < kRopeAhead; k++) {
+        if (!from[k]) continue;
+        const float2* w = cs + tok[k] * half;
+        float o0[V], o1[V];
 #pragma unroll
-      for (int i = 0; i < P; i += 2) {
-        const float x0 = (float)x[i], x1 = (float)x[i + 1];
-        const float2 k = w[(d + i) >> 1];
-        o[i] = turn ? fmaf(x0, k.x, -(x1 * k.y)) : x0;
-        o[i + 1] = turn ? fmaf(x0, k.y, x1 * k.x) : x1;
-      }
-      if constexpr (V == 1) {
-        rope_put<T, C, 1>(row, d, o);
-        rope_put<T, C, 1>(row, d + 1, o + 1);
-      } else {
-        rope_put<T, C, V>(row, d, o);
+        for (int i = 0; i < V; i++) o0[i] = (float)a[k].v[i], o1[i] = two ? (float)b[k].v[i] : 0.0f;
+        if (turn[k]) {
+          if (two) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+              const float2 q = w[L.neox ? d + i : c];
+              const float x0 = o0[i], x1 = o1[i];
+              o0[i] = fmaf(x0, q.x, -(x1 * q.y));
+              o1[i] = fmaf(x0, q.y, x1 * q.x);
+            }
+          } else if constexpr (V > 1) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+              const float2 q = w[(d + i) >> 1];
+              const float x0 = o0[i], x1 = o0[i + 1];
+              o0[i] = fmaf(x0, q.x, -(x1 * q.y));
+              o0[i + 1] = fmaf(x0, q.y, x1 * q.x);
+            }
+          }
+        }
+        if (y[k]) {
+          Vec<T, V> v;
+#pragma unroll
+          for (int i = 0; i < V; i++) v.v[i] = (T)o0[i];
+          *(Vec<T, V>*)(y[k] + d) = v;
+          if (two) {
+#pragma unroll
+            for (int i = 0; i < V; i++) v.v[i] = (T)o1[i];
+            *(Vec<T, V>*)(y[k] + d1) = v;
+          }
+        } else {
+          Vec<C, V> v;
+#pragma unroll
+          for (int i = 0; i < V; i++) v.v[i] = (C)o0[i];
+          *(Vec<C, V>*)(cache[k] + d) = v;
+          if (two) {
+#pragma unroll
+            for (int i = 0; i < V; i++) v.v[i] = (C)o1[i];
+            *(Vec<C, V>*)(cache[k] + d1) = v;
+          }
+        }
       }
     }
   }
@@ -169,12 +182,13 @@ hipError_t launch_t(const RopeLaunch& L) {
   };
   bool wide = fits(L.x, L.xt, L.xh) && fits(L.y, L.yt, L.yh) && L.hd % V == 0 && (L.neox ? L.nf : 2 * L.nf) % V == 0;
   if (APPEND) wide = wide && fits(L.k, L.kt, L.kh) && fits(L.v, L.vt, L.vh);
-  // tokens of a workgroup: as many as make one angle a thread
-  const int tpw = L.nf > kRopeNT ? 1 : kRopeNT / L.nf;
-  const int t = tpw < L.tokens ? tpw : L.tokens;
+  // Tokens of a workgroup: as many as make one angle a thread, fewer where the card (2048 workgroups) would not
+  // be full; with few tokens their rows are spread over more workgroups, an access a thread in each.
+  int t = kRopeNT / L.nf;
+  t = t < 1 ? 1 : (t > kRopeTokens ? kRopeTokens : t);
+  if (t > (L.tokens + 2047) / 2048) t = (L.tokens + 2047) / 2048;
   const int64_t work = (int64_t)t * (L.heads + (APPEND ? 2 * L.kv.n_kv : 0)) * L.hd;
   const int tw = (L.tokens + t - 1) / t;
-  // few tokens: their heads are spread over more workgroups, at least an access a thread in each
   int64_t gy = tw >= 512 ? 1 : (512 + tw - 1) / tw;
   if (gy * kRopeNT * V > work) gy = work < kRopeNT * V ? 1 : work / (kRopeNT * V);
   const dim3 grid(tw, (unsigned)gy);
