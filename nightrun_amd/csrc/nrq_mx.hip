@@ -20,11 +20,19 @@ struct alignas(16) Half16 {
   T v[16 / sizeof(T)];
 };
 
-// Eight values of a row: 16 bytes or, for unaligned rows, one by one.
+// Eight values of a row: 16 bytes (wide 2: streamed past the caches) or, for unaligned rows, one by one.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool wide, float* f) {
+__device__ __forceinline__ void load8(const T* p, int wide, float* f) {
   constexpr int V = 16 / sizeof(T);
-  if (wide) {
+  if (wide == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; i += V) {
+      const i32x4 x = __builtin_nontemporal_load((const i32x4*)(p + i));
+      const Half16<T> a = *(const Half16<T>*)&x;
+#pragma unroll
+      for (int j = 0; j < V; j++) f[i + j] = (float)a.v[j];
+    }
+  } else if (wide) {
 #pragma unroll
     for (int i = 0; i < 8; i += V) {
       const Half16<T> a = *(const Half16<T>*)(p + i);
@@ -61,66 +69,81 @@ __device__ __forceinline__ uint32_t mx_quantize8(float* f, uint32_t* scale) {
   return r;
 }
 
+constexpr int kMxOwn = 16384;  // values that a product's workgroups quantize for themselves
+constexpr int kMxAhead = 2;  // accesses of a thread that are on their way together
+
+// Eight values an access, four lanes a block: cols / 8 is a multiple of four and a workgroup
+// starts at a multiple of four, so a block's lanes stay together. dense: rows without gaps.
 template <typename T>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* src, int64_t stride, uint32_t cols8, int64_t items,
-                                                          uint32_t* q, uint8_t* sc, int wide) {
-  // grid-stride over groups of 8 values; four lanes a block, and the grid's size
-  // is a multiple of four, so a block's lanes stay together
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / cols8;
-    const int c = (int)(i - row * cols8) * 8;
-    float f[8];
-    load8(src + row * stride + c, wide, f);
+                                                          uint32_t* q, uint8_t* sc, int wide, int dense) {
+  const int64_t i0 = (int64_t)blockIdx.x * (256 * kMxAhead) + threadIdx.x;
+  float f[kMxAhead][8];
+#pragma unroll
+  for (int k = 0; k < kMxAhead; k++) {
+    const int64_t i = min(i0 + 256 * k, items - 1);  // no load is conditional
+    const int64_t row = dense ? 0 : i / cols8;
+    load8(src + (dense ? i * 8 : row * stride + (i - row * cols8) * 8), wide, f[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kMxAhead; k++) {
+    const int64_t i = i0 + 256 * k;
+    if (i >= items) break;
     uint32_t s;
-    q[i] = mx_quantize8(f, &s);
+    q[i] = mx_quantize8(f[k], &s);
     if ((threadIdx.x & 3) == 0) sc[i >> 2] = (uint8_t)s;
   }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* q, const uint8_t* sc, int64_t stride,
-                                                            uint32_t cols8, int64_t items, T* dst, int wide) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / cols8;
-    const int c = (int)(i - row * cols8) * 8;
-    const uint32_t w = q[i], s = sc[i >> 2];
-    const float by = __uint_as_float(s == 255u ? 0x7fc00000u : (s ? s << 23 : 0x00400000u));
+                                                            uint32_t cols8, int64_t items, T* dst, int wide, int dense) {
+  const int64_t i0 = (int64_t)blockIdx.x * (256 * kMxAhead) + threadIdx.x;
+  uint32_t w[kMxAhead], s[kMxAhead];
+#pragma unroll
+  for (int k = 0; k < kMxAhead; k++) {
+    const int64_t i = min(i0 + 256 * k, items - 1);
+    w[k] = q[i];
+    s[k] = sc[i >> 2];
+  }
+#pragma unroll
+  for (int k = 0; k < kMxAhead; k++) {
+    const int64_t i = i0 + 256 * k;
+    if (i >= items) break;
+    const float by = __uint_as_float(s[k] == 255u ? 0x7fc00000u : (s[k] ? s[k] << 23 : 0x00400000u));
     float f[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-      // code eem of 2^(ee - 1) (1 + m / 2), or m / 2: times 4 an integer
-      const uint32_t n = (w >> (4 * k)) & 15u, ee = (n >> 1) & 3u, m = n & 1u;
+    for (int e = 0; e < 8; e++) {
+      // code eem: 2^(ee - 1) (1 + m / 2), or m / 2
+      const uint32_t n = (w[k] >> (4 * e)) & 15u, ee = (n >> 1) & 3u, m = n & 1u;
       const float mag = ee ? __uint_as_float(((ee + 126u) << 23) | (m << 22)) : 0.5f * m;
-      f[k] = (n & 8u ? -mag : mag) * by;
+      f[e] = (n & 8u ? -mag : mag) * by;
     }
-    T* d = dst + row * stride + c;
+    const int64_t row = dense ? 0 : i / cols8;
+    T* d = dst + (dense ? i * 8 : row * stride + (i - row * cols8) * 8);
     constexpr int V = 16 / sizeof(T);
     if (wide) {
 #pragma unroll
-      for (int k = 0; k < 8; k += V) {
+      for (int e = 0; e < 8; e += V) {
         Half16<T> o;
 #pragma unroll
-        for (int j = 0; j < V; j++) o.v[j] = (T)f[k + j];
-        *(Half16<T>*)(d + k) = o;
+        for (int j = 0; j < V; j++) o.v[j] = (T)f[e + j];
+        // streamed: 9728 x 2560 bf16 takes 11.6 us so, 17.7 with ordinary stores
+        __builtin_nontemporal_store(*(i32x4*)&o, (i32x4*)(d + e));
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; k++) d[k] = (T)f[k];
+      for (int e = 0; e < 8; e++) d[e] = (T)f[e];
     }
   }
 }
 
-// One lane's block: 16 bytes and its scale; zeros with scale 1 for none.
+// One lane's block: 16 bytes and its scale.
 struct MxBlock {
   i32x4 q;
   int s;
 };
-__device__ __forceinline__ MxBlock mx_block(const uint8_t* q, const uint8_t* s, bool live) {
-  MxBlock b;
-  b.q = live ? *(const i32x4*)q : i32x4{0, 0, 0, 0};
-  b.s = live ? (int)*s : 127;
-  return b;
-}
+__device__ __forceinline__ MxBlock mx_block(const uint8_t* q, const uint8_t* s) { return MxBlock{*(const i32x4*)q, (int)*s}; }
 
 __device__ __forceinline__ f32x4 mx_mfma(const MxBlock& a, const MxBlock& b, f32x4 c) {
   const i32x8 x = {a.q.x, a.q.y, a.q.z, a.q.w, 0, 0, 0, 0}, y = {b.q.x, b.q.y, b.q.z, b.q.w, 0, 0, 0, 0};
@@ -143,42 +166,109 @@ __device__ __forceinline__ void mx_store(void* y, int dtype, int64_t at, int n, 
     put4((__bf16*)y, at, n, v);
 }
 
-// 16 rows of w times 16 NT tokens per workgroup; its four waves take every
-// fourth step of 128 columns, then add up in LDS.
-template <int NT>
-__global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L) {
-  __shared__ f32x4 part[3][NT][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+// Tiles of 16 rows of w by 16 NT tokens. A workgroup's four waves take every
+// fourth step of 128 columns and add up in LDS; it goes from one row tile to another, the next
+// weights on their way while these are multiplied. With X the activation is not in MXFP4
+// yet but [batch][cols] of X: every workgroup quantizes it once into LDS, behind the loads of its
+// first weights, which saves a launch (for a token or a few: see mx_linear_fits).
+template <int NT, typename X>
+__global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, const X* act, int64_t stride, int wide) {
+  constexpr bool kOwn = !__is_same(X, void);
+  constexpr int U = NT == 1 ? 5 : 2;  // steps on their way together: 2560 columns in one go
+  __shared__ f32x4 part[2][4][NT][64];
+  extern __shared__ __align__(16) uint8_t own[];  // with X: [batch][cols / 2], then [batch][cols / 32]
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const int blocks = L.cols / 32, steps = (blocks + 3) / 4;
-  const int row = blockIdx.x * 16 + i;
-  const uint8_t* wq = L.w + (int64_t)min(row, L.rows - 1) * blocks * 16;
-  const uint8_t* wsc = L.ws + (int64_t)min(row, L.rows - 1) * blocks;
-  f32x4 acc[NT];
+  MxBlock a[U];
+  auto load = [&](int tile, int s0) {
+    const int row = tile * 16 + i;
+    const int64_t r = (int64_t)min(row, L.rows - 1) * blocks;
 #pragma unroll
-  for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
-  for (int s = w; s < steps; s += 4) {
-    const int b = 4 * s + g;
-    const MxBlock a = mx_block(wq + (int64_t)b * 16, wsc + b, b < blocks && row < L.rows);
+    for (int u = 0; u < U; u++) {
+      // blocks behind the last read the last again, no load is conditional; they are cleared when used
+      const int64_t b = r + min(4 * (s0 + 4 * u) + g, blocks - 1);
+      a[u] = mx_block(L.w + b * 16, L.ws + b);
+    }
+  };
+  const uint8_t *xq = L.x, *xs = L.xs;
+  if constexpr (kOwn) {
+    // the first two accesses of each thread are asked for before the weights: loads come back in order
+    uint8_t* oq = own;
+    uint8_t* os = own + (size_t)L.batch * blocks * 16;
+    const int cols8 = L.cols / 8, items = L.batch * cols8;
+    auto value = [&](int k, float* f) {
+      const int t = L.batch == 1 ? 0 : k / cols8;
+      load8(act + t * stride + (k - t * cols8) * 8, wide, f);
+    };
+    auto put = [&](int k, float* f) {
+      uint32_t s;
+      ((uint32_t*)oq)[k] = mx_quantize8(f, &s);
+      if ((k & 3) == 0) os[k >> 2] = (uint8_t)s;
+    };
+    float f[2][8];
+    const int t = threadIdx.x;
+    value(min(t, items - 1), f[0]);
+    value(min(t + 256, items - 1), f[1]);
+    load(blockIdx.x, w);
+    if (t < items) put(t, f[0]);
+    if (t + 256 < items) put(t + 256, f[1]);
+    for (int k = t + 512; k < items; k += 256) {
+      value(k, f[0]);
+      put(k, f[0]);
+    }
+    __syncthreads();
+    xq = oq, xs = os;
+  } else if (blocks) {
+    load(blockIdx.x, w);
+  }
+  int round = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, round++) {
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
+    for (int s0 = w; s0 < steps; s0 += 4 * U) {
+      MxBlock now[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) now[u] = a[u];
+      if (s0 + 4 * U < steps)
+        load(tile, s0 + 4 * U);
+      else if (tile + (int)gridDim.x < tiles)
+        load(tile + gridDim.x, w);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int b = 4 * (s0 + 4 * u) + g;
+        const bool none = b >= blocks;
+        if (none) now[u] = MxBlock{{0, 0, 0, 0}, 127};
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const int tok = min((int)(blockIdx.y * NT + t) * 16 + i, L.batch - 1);  // tokens behind the last are not stored
+          const int64_t at = (int64_t)tok * blocks + min(b, blocks - 1);
+          MxBlock x = mx_block(xq + at * 16, xs + at);
+          if (none) x.s = 127;
+          acc[t] = mx_mfma(now[u], x, acc[t]);
+        }
+      }
+    }
+    // one barrier a tile: the wave that adds a tile up has done so before the barrier of the next, after
+    // which its place is written again
+    auto& p = part[round & 1];
+#pragma unroll
+    for (int t = 0; t < NT; t++) p[w][t][lane] = acc[t];
+    __syncthreads();
+    if (w != (round & 3)) continue;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const int tok = (blockIdx.y * NT + t) * 16 + i;
-      const int64_t at = (int64_t)tok * blocks + b;
-      acc[t] = mx_mfma(a, mx_block(L.x + at * 16, L.xs + at, b < blocks && tok < L.batch), acc[t]);
+      const f32x4 y = ((p[0][t][lane] + p[1][t][lane]) + p[2][t][lane]) + p[3][t][lane];
+      const int tok = (blockIdx.y * NT + t) * 16 + i, r = tile * 16 + 4 * g;
+      if (tok < L.batch && r < L.rows) mx_store(L.y, L.dtype, tok * L.ldy + r, L.rows - r, y);
     }
   }
-  if (w)
-#pragma unroll
-    for (int t = 0; t < NT; t++) part[w - 1][t][lane] = acc[t];
-  __syncthreads();
-  if (w) return;
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    acc[t] += part[0][t][lane];
-    acc[t] += part[1][t][lane];
-    acc[t] += part[2][t][lane];
-    const int tok = (blockIdx.y * NT + t) * 16 + i, r = blockIdx.x * 16 + 4 * g;
-    if (tok < L.batch && r < L.rows) mx_store(L.y, L.dtype, tok * L.ldy + r, L.rows - r, acc[t]);
-  }
+}
+
+// Workgroups for `tiles` row tiles: all of them up to `most`, else few enough that each has as many.
+inline unsigned mx_matvec_grid(int tiles, int most) {
+  const int rounds = (tiles + most - 1) / most;
+  return (unsigned)((tiles + rounds - 1) / rounds);
 }
 
 template <typename T>
@@ -186,20 +276,33 @@ bool wide_rows(const void* p, int64_t stride) {
   return ((uintptr_t)p & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
 }
 
+inline unsigned mx_grid(int64_t items) { return (unsigned)((items + 256 * kMxAhead - 1) / (256 * kMxAhead)); }
+
 template <typename T>
 void quantize_t(const void* src, size_t rows, size_t cols, int64_t stride, void* q, void* s, hipStream_t st) {
   const int64_t items = (int64_t)rows * (cols / 8);
-  const unsigned grid = (unsigned)(items + 255 < 256 * (int64_t)8192 ? (items + 255) / 256 : 8192);
-  hipLaunchKernelGGL((mx_quantize_kernel<T>), dim3(grid), dim3(256), 0, st, (const T*)src, stride, (uint32_t)(cols / 8),
-                     items, (uint32_t*)q, (uint8_t*)s, wide_rows<T>(src, stride) ? 1 : 0);
+  // more than the L2s hold is streamed: 9728 x 2560 bf16 and back takes 22.0 us so, 23.9 through them; less stays in
+  // them (2048 x 2048 f32 before its product: 73.4 us streamed, 72.4 not)
+  const bool big = items * 8 * (int64_t)sizeof(T) > 32 << 20;
+  hipLaunchKernelGGL((mx_quantize_kernel<T>), dim3(mx_grid(items)), dim3(256), 0, st, (const T*)src, stride,
+                     (uint32_t)(cols / 8), items, (uint32_t*)q, (uint8_t*)s, wide_rows<T>(src, stride) ? (big ? 2 : 1) : 0,
+                     stride == (int64_t)cols || rows == 1);
 }
 
 template <typename T>
 void dequantize_t(const void* q, const void* s, size_t rows, size_t cols, void* dst, int64_t stride, hipStream_t st) {
   const int64_t items = (int64_t)rows * (cols / 8);
-  const unsigned grid = (unsigned)(items + 255 < 256 * (int64_t)8192 ? (items + 255) / 256 : 8192);
-  hipLaunchKernelGGL((mx_dequantize_kernel<T>), dim3(grid), dim3(256), 0, st, (const uint32_t*)q, (const uint8_t*)s,
-                     stride, (uint32_t)(cols / 8), items, (T*)dst, wide_rows<T>(dst, stride) ? 1 : 0);
+  hipLaunchKernelGGL((mx_dequantize_kernel<T>), dim3(mx_grid(items)), dim3(256), 0, st, (const uint32_t*)q,
+                     (const uint8_t*)s, stride, (uint32_t)(cols / 8), items, (T*)dst, wide_rows<T>(dst, stride) ? 1 : 0,
+                     stride == (int64_t)cols || rows == 1);
+}
+
+template <typename X>
+void linear_t(const MxMatmul& L, const void* x, int64_t stride) {
+  const size_t lds = (size_t)L.batch * (L.cols / 2 + L.cols / 32);
+  const int tiles = (L.rows + 15) / 16;
+  hipLaunchKernelGGL((mx_matvec_kernel<1, X>), dim3(mx_matvec_grid(tiles, 4096)), dim3(256), lds, L.stream, L, tiles,
+                     (const X*)x, stride, wide_rows<X>(x, stride) ? 1 : 0);
 }
 
 }  // namespace
@@ -226,14 +329,29 @@ hipError_t launch_mx_dequantize(const void* q, const void* s, size_t rows, size_
   return hipGetLastError();
 }
 
+// A token or a few are quantized by every workgroup of the product: up to 16384 values (LDS for 4 workgroups a
+// CU).
+bool mx_linear_fits(int cols, int batch) { return batch <= 16 && (int64_t)cols * batch <= kMxOwn; }
+
+hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64_t stride) {
+  if (x_dtype == kF32)
+    linear_t<float>(L, x, stride);
+  else if (x_dtype == kF16)
+    linear_t<_Float16>(L, x, stride);
+  else
+    linear_t<__bf16>(L, x, stride);
+  return hipGetLastError();
+}
+
 hipError_t launch_mx_matmul(const MxMatmul& L) {
   if (L.batch > 64 && L.cols >= 64) return launch_mx_gemm(L);
-  const int tiles = (L.batch + 15) / 16;
-  const unsigned gx = (unsigned)((L.rows + 15) / 16);
-  if (tiles == 1)
-    hipLaunchKernelGGL((mx_matvec_kernel<1>), dim3(gx), dim3(256), 0, L.stream, L);
+  const int tokens = (L.batch + 15) / 16, tiles = (L.rows + 15) / 16;
+  if (tokens == 1)
+    hipLaunchKernelGGL((mx_matvec_kernel<1, void>), dim3(mx_matvec_grid(tiles, 4096)), dim3(256), 0, L.stream, L, tiles,
+                       (const void*)nullptr, (int64_t)0, 0);
   else
-    hipLaunchKernelGGL((mx_matvec_kernel<4>), dim3(gx, (tiles + 3) / 4), dim3(256), 0, L.stream, L);
+    hipLaunchKernelGGL((mx_matvec_kernel<4, void>), dim3(mx_matvec_grid(tiles, 4096), (tokens + 3) / 4), dim3(256), 0,
+                       L.stream, L, tiles, (const void*)nullptr, (int64_t)0, 0);
   return hipGetLastError();
 }
 

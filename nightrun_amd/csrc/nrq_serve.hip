@@ -116,6 +116,11 @@ int mx_check(const char* name, size_t rows, size_t cols) {
   return NRQ_OK;
 }
 
+size_t linear_bytes(size_t cols, size_t batch) {
+  if (batch <= INT_MAX && nrq::mx_linear_fits((int)cols, (int)batch)) return 0;
+  return up16(batch * (cols / 2)) + up16(batch * (cols / 32));
+}
+
 int mx_matmul(const char* name, void* y, int dtype, int64_t ldy, const void* w, const void* ws, const void* x,
               const void* xs, size_t rows, size_t cols, size_t batch, void* stream) {
   nrq::MxMatmul L{y,         dtype,      ldy,        (const uint8_t*)w, (const uint8_t*)ws, (const uint8_t*)x, (const uint8_t*)xs,
@@ -304,7 +309,8 @@ int nrq_linear_mxfp4_workspace(size_t cols, size_t batch, size_t* bytes) {
   if (!bytes) return fail(NRQ_ERR_ARG, name, "null pointer");
   int rc = mx_check(name, batch, cols);
   if (rc) return rc;
-  *bytes = up16(batch * (cols / 2)) + up16(batch * (cols / 32));
+  // the product's workgroups quantize few values for themselves
+  *bytes = linear_bytes(cols, batch);
   return NRQ_OK;
 }
 
@@ -318,10 +324,14 @@ int nrq_dev_linear_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, co
   if (!bytes_of(x_dtype)) return fail(NRQ_ERR_ARG, name, "unknown type %d", x_dtype);
   if (cols && !x) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(x, bytes_of(x_dtype))) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
-  const size_t qb = up16(batch * (cols / 2));
-  if ((rc = workspace_check(name, workspace, workspace_bytes, qb + up16(batch * (cols / 32))))) return rc;
+  if ((rc = workspace_check(name, workspace, workspace_bytes, linear_bytes(cols, batch)))) return rc;
   if ((rc = device_check(name, stream))) return rc;
-  uint8_t* xs = (uint8_t*)workspace + qb;
+  if (cols && nrq::mx_linear_fits((int)cols, (int)batch)) {
+    nrq::MxMatmul L{y,         dtype,      y_stride,   (const uint8_t*)w, (const uint8_t*)w_scales, nullptr, nullptr,
+                    (int)rows, (int)cols, (int)batch, (hipStream_t)stream};
+    return launched(name, nrq::launch_mx_linear(L, x, x_dtype, x_stride));
+  }
+  uint8_t* xs = (uint8_t*)workspace + up16(batch * (cols / 2));
   if (cols && (rc = launched(name, nrq::launch_mx_quantize(x, x_dtype, batch, cols, x_stride, workspace, xs, (hipStream_t)stream))))
     return rc;
   return mx_matmul(name, y, dtype, y_stride, w, w_scales, workspace, xs, rows, cols, batch, stream);

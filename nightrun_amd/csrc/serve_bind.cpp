@@ -283,9 +283,10 @@ BIND(linear_mxfp4, 4) {
   size_t need;
   const int rc = nrq_linear_mxfp4_workspace(w.cols, batch, &need);
   if (rc) return rc;
-  const at::Tensor ws = workspace(need, x);
-  return nrq_dev_linear_mxfp4(yp, yk, y.stride(0), w.q, w.s, xp, xk, x.stride(0), w.rows, w.cols, batch, ws.data_ptr(),
-                              need, stream);
+  at::Tensor ws;
+  if (need) ws = workspace(need, x);
+  return nrq_dev_linear_mxfp4(yp, yk, y.stride(0), w.q, w.s, xp, xk, x.stride(0), w.rows, w.cols, batch,
+                              need ? ws.data_ptr() : nullptr, need, stream);
 }
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
