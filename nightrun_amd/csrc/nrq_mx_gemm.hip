@@ -167,22 +167,23 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(MxMatmul L, int row_til
   }
 }
 
-// The same for whole steps of 128 columns (at least four): four stages of one step each (64 bytes a
-// row, 16 KiB), three of them on their way while the fourth is multiplied. Chunk c
-// of row r lies at c ^ (r / 4 & 3). The scale bytes come for four steps at a time, 16
-// bytes of a row in one piece (by the step they would be as many requests to L2 as the values), and go
-// to registers so.
+// The same on stages of one step of 128 columns (four steps a row at least): 64 bytes a row, 16 KiB;
+// while one is multiplied the others are on their way. Chunk c of row r lies at c ^ (r / 4 & 3).
+// The scale bytes come for four steps at a time (by the step they would be as many requests to
+// L2 as the values) and go to registers so: WHOLE where each row's 16 are an aligned 16-byte piece
+// (multiples of 512 columns), else the two aligned pieces that hold them are fetched, the second only
+// where the row reaches into it. Two workgroups a CU: with the first four stages fit, else three.
 //
 // A workgroup takes tile after tile; the stages run on from one to the next, so that the next
 // tile's are on their way while this one's outputs are written, and a CU's two workgroups drift apart, one
 // writing while the other multiplies.
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_tiles, int tok_tiles, int wide) {
-  constexpr int NS = 4, SB = 256 * 64;
+  constexpr int NS = WHOLE ? 4 : 3, SB = 256 * 64, SP = WHOLE ? 16 : 32;  // stages, bytes of one, scale bytes of a row
   __shared__ __align__(16) uint8_t stage[NS][SB];
-  __shared__ __align__(16) uint8_t scale[2][256][16];
+  __shared__ __align__(16) uint8_t scale[2][256][SP];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-  const int blocks = L.cols / 32, steps = blocks / 4;
+  const int blocks = L.cols / 32, steps = (blocks + 3) / 4;
   const GemmRun run = gemm_run(row_tiles * tok_tiles);
   if (run.first >= run.stop) return;
 
@@ -192,8 +193,9 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&stage[0][0]);
   const uint32_t sbase = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&scale[0][0][0]);
-  const uint8_t* src[5];
-  int ft = run.first, fk = 0, filled = 0, groups = 0;
+  const uint8_t* src[4];
+  uintptr_t sfrom[2], send[2];  // the scale bytes' 16-byte piece, the row's end
+  int ft = run.first, fk = 0, filled = 0, groups = 0, fslot = 0;
   auto aim = [&]() {
     const GemmTile tile = gemm_tile(ft, row_tiles, tok_tiles);
     const int r0 = tile.r * kGemmTile, b0 = tile.b * kGemmTile;
@@ -202,22 +204,31 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
       const int r = 32 * w + 16 * j + (lane >> 2);
       src[j] = L.w + (int64_t)min(r0 + r, L.rows - 1) * blocks * 16 + chunk * 16;
       src[2 + j] = L.x + (int64_t)min(b0 + r, L.batch - 1) * blocks * 16 + chunk * 16;
+      const int q = WHOLE ? 64 * (w & 1) + lane : 64 * (w & 1) + 32 * j + (lane >> 1);
+      const uintptr_t s = (uintptr_t)(w < 2 ? L.ws + (int64_t)min(r0 + q, L.rows - 1) * blocks
+                                            : L.xs + (int64_t)min(b0 + q, L.batch - 1) * blocks);
+      sfrom[j] = s & ~(uintptr_t)15;
+      send[j] = s + blocks;
     }
-    const int r = 64 * (w & 1) + lane;
-    src[4] = w < 2 ? L.ws + (int64_t)min(r0 + r, L.rows - 1) * blocks : L.xs + (int64_t)min(b0 + r, L.batch - 1) * blocks;
   };
   auto fill = [&]() {
     if (ft >= run.stop) return;
     if ((fk & 3) == 0) {
-      // the last 16 of the row where fewer are left
-      mx_dma16(src[4] + min(4 * fk, blocks - 16), sbase + (uint32_t)(groups & 1) * 4096 + (uint32_t)w * 1024);
+#pragma unroll
+      for (int j = 0; j < (WHOLE ? 1 : 2); j++) {
+        const uintptr_t p = sfrom[j] + 4 * fk, next = p + 16;
+        mx_dma16((const void*)(!WHOLE && (lane & 1) && next < send[j] ? next : p),
+                 sbase + (uint32_t)(groups & 1) * (256 * SP) + (uint32_t)(64 * w + 32 * j) * SP);
+      }
       groups++;
     }
-    const uint32_t to = base + (uint32_t)(filled & (NS - 1)) * SB;
+    const uint32_t to = base + (uint32_t)fslot * SB;
+    fslot = fslot + 1 == NS ? 0 : fslot + 1;
+    const bool live = WHOLE || 4 * fk + chunk < blocks;  // chunks behind the last are zeros
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      mx_dma16(src[j] + fk * 64, to + (uint32_t)(32 * w + 16 * j) * 64);
-      mx_dma16(src[2 + j] + fk * 64, to + (uint32_t)(128 + 32 * w + 16 * j) * 64);
+      mx_dma16(live ? src[j] + fk * 64 : (const uint8_t*)mx_zeros, to + (uint32_t)(32 * w + 16 * j) * 64);
+      mx_dma16(live ? src[2 + j] + fk * 64 : (const uint8_t*)mx_zeros, to + (uint32_t)(128 + 32 * w + 16 * j) * 64);
     }
     filled++;
     if (++fk == steps) {
@@ -237,71 +248,74 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
     for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0, 0, 0, 0};
   const int wr = 64 * (w & 1), wb = 128 + 64 * (w >> 1);
   const int at = (g ^ (c >> 2)) * 16;
-  int done = 0, group = 0, stores = 0;  // steps and groups of four; steps for which 16 stores are newer than a stage
+  int done = 0, slot = 0, group = 0, stores = 0;  // steps and groups of four; steps for which 16 stores are newer than a stage
   uint32_t sa[4][4], sb[4][4];
   auto wait = [&]() {
-    // at least four loads a stage: this one's are there when those of the two behind it may be missing, and
-    // the outputs' stores that were issued between them
+    // at least four loads a stage: this one's are there when those of the NS - 2 behind it may be missing,
+    // and the outputs' stores that were issued between them
     const int behind = filled - done - 1;
     if (behind < 1)
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    else if (behind < 2)
+    else if (behind < NS - 2)
       asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     else if (stores > 0)
-      asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * (NS - 2) + 16) : "memory");
     else
-      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * (NS - 2)) : "memory");
     stores--;
     // everyone's are there, and the stage before has been read
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     fill();
   };
-  auto multiply = [&](const uint32_t* va, const uint32_t* vb) {
-    const uint8_t* st = stage[done & (NS - 1)];
-    i32x4 a[4], b[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      a[i] = *(const i32x4*)(st + (wr + 16 * i + c) * 64 + at);
-      b[i] = *(const i32x4*)(st + (wb + 16 * i + c) * 64 + at);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) acc[i][j] = mx_step<0>(a[i], (int)va[i], b[j], (int)vb[j], acc[i][j]);
-    done++;
-  };
   for (int t = run.first; t < run.stop; t += run.step) {
     const GemmTile tile = gemm_tile(t, row_tiles, tok_tiles);
     const int r0 = tile.r * kGemmTile, b0 = tile.b * kGemmTile;
-    int k = 0;
-    for (; k + 4 <= steps; k += 4) {
+    // where the scale bytes of this lane's rows start in the fetched pieces
+    int oa[4], ob[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      oa[i] = (wr + 16 * i + c) * SP + (WHOLE ? 0 : 1) * (int)(((uintptr_t)L.ws + (int64_t)min(r0 + wr + 16 * i + c, L.rows - 1) * blocks) & 15);
+      ob[i] = (wb + 16 * i + c) * SP + (WHOLE ? 0 : 1) * (int)(((uintptr_t)L.xs + (int64_t)min(b0 + wb - 128 + 16 * i + c, L.batch - 1) * blocks) & 15);
+    }
+    auto scales = [&](int o, uint32_t* out) {
+      const uint32_t* p = (const uint32_t*)(&scale[group & 1][0][0] + (o & ~3));
+      if constexpr (WHOLE) {
+        const u32x4 d = *(const u32x4*)p;
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e] = d[e] >> (8 * g);
+      } else {
+        uint32_t d[5];
+#pragma unroll
+        for (int e = 0; e < 5; e++) d[e] = p[e];
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e] = __builtin_amdgcn_alignbyte(d[e + 1], d[e], o & 3) >> (8 * g);
+      }
+    };
+    for (int k = 0; k < steps; k += 4, group++) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
+        if (!WHOLE && k + e >= steps) break;
         wait();
-        if (e == 0) {
+        if (e == 0)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            *(u32x4*)sa[i] = *(const u32x4*)scale[group & 1][wr + 16 * i + c];
-            *(u32x4*)sb[i] = *(const u32x4*)scale[group & 1][wb + 16 * i + c];
-          }
+          for (int i = 0; i < 4; i++) scales(oa[i], sa[i]), scales(ob[i], sb[i]);
+        if (!WHOLE && 4 * (k + e) + 4 > blocks && 4 * (k + e) + g >= blocks)  // behind the last block: zeros of scale 1
+#pragma unroll
+          for (int i = 0; i < 4; i++) sa[i][e] = sb[i][e] = 127;
+        const uint8_t* st = stage[slot];
+        slot = slot + 1 == NS ? 0 : slot + 1;
+        i32x4 a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          a[i] = *(const i32x4*)(st + (wr + 16 * i + c) * 64 + at);
+          b[i] = *(const i32x4*)(st + (wb + 16 * i + c) * 64 + at);
         }
-        uint32_t va[4], vb[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) va[i] = sa[i][e] >> (8 * g), vb[i] = sb[i][e] >> (8 * g);
-        multiply(va, vb);
-      }
-      group++;
-    }
-    if (k < steps) {
-      const uint8_t* sc = &scale[group & 1][0][16 - 4 * (steps - k) + g];  // the last 16 bytes of the row
-      for (; k < steps; k++, sc += 4) {
-        wait();
-        uint32_t va[4], vb[4];
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) va[i] = sc[(wr + 16 * i + c) * 16], vb[i] = sc[(wb + 16 * i + c) * 16];
-        multiply(va, vb);
+          for (int j = 0; j < 4; j++) acc[i][j] = mx_step<0>(a[i], (int)sa[i][e], b[j], (int)sb[j][e], acc[i][j]);
+        done++;
       }
-      group++;
     }
     const bool inner = wide && r0 + kGemmTile <= L.rows && b0 + kGemmTile <= L.batch;  // then 16 stores, no more
 #pragma unroll
@@ -318,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
 #pragma unroll
       for (int i = 0; i < 4; i++) acc[i][j] = f32x4{0, 0, 0, 0};
     }
-    stores = inner ? 3 : 0;
+    stores = inner ? NS - 1 : 0;
   }
 }
 
@@ -327,9 +341,11 @@ hipError_t gemm_t(const MxMatmul& L) {
   const int rt = (L.rows + kGemmTile - 1) / kGemmTile, tt = (L.batch + kGemmTile - 1) / kGemmTile;
   const int wide = ((uintptr_t)L.y & (4 * sizeof(T) - 1)) == 0 && L.ldy % 4 == 0;
   const unsigned all = (unsigned)((rt * tt + 7) / 8 * 8);
-  const bool steps = L.cols % 128 == 0 && L.cols >= 512 && ((uintptr_t)L.ws & 3) == 0 && ((uintptr_t)L.xs & 3) == 0;
-  if (steps)
-    hipLaunchKernelGGL((mx_gemm128_kernel<T>), dim3(all < 512 ? all : 512), dim3(256), 0, L.stream, L, rt, tt, wide);
+  const dim3 grid(all < 512 ? all : 512);
+  if (L.cols % 512 == 0 && ((uintptr_t)L.ws & 15) == 0 && ((uintptr_t)L.xs & 15) == 0)
+    hipLaunchKernelGGL((mx_gemm128_kernel<T, true>), grid, dim3(256), 0, L.stream, L, rt, tt, wide);
+  else if (L.cols > 384)  // four steps
+    hipLaunchKernelGGL((mx_gemm128_kernel<T, false>), grid, dim3(256), 0, L.stream, L, rt, tt, wide);
   else
     hipLaunchKernelGGL((mx_gemm_kernel<T>), dim3(all), dim3(256), 0, L.stream, L, rt, tt, wide);
   return hipGetLastError();

@@ -698,7 +698,9 @@ def check_product(y, xc, xs, wc, ws, kind):
 
 @pytest.mark.parametrize("batch,rows,cols", [(1, 1, 32), (1, 40, 64), (1, 4100, 2560), (3, 16, 96), (16, 33, 512),
                                              (17, 70, 160), (64, 300, 1024), (65, 129, 352), (130, 257, 288),
-                                             (300, 512, 2048), (257, 1000, 128), (512, 24, 4128), (1000, 515, 256)])
+                                             (300, 512, 2048), (257, 1000, 128), (512, 24, 4128), (1000, 515, 256), (300, 700, 640),
+                                             (200, 150, 416), (513, 130, 480), (129, 1030, 1312), (1100, 600, 544),
+                                             (70, 3000, 2080)])
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 def test_mx_matmul(gpu, kind, batch, rows, cols):
     import torch
