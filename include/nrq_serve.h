@@ -151,7 +151,7 @@ int nrq_dev_matmul_mxfp4(void *y, int dtype, int64_t y_stride, const void *w, co
  * rows x_stride apart; the result is that of nrq_dev_quantize_mxfp4 and
  * nrq_dev_matmul_mxfp4. workspace: nrq_linear_mxfp4_workspace bytes, 16-byte
  * aligned, as for the attention. */
-int nrq_linear_mxfp4_workspace(size_t cols, size_t batch, size_t *bytes);
+int nrq_linear_mxfp4_workspace(size_t rows, size_t cols, size_t batch, size_t *bytes);
 int nrq_dev_linear_mxfp4(void *y, int dtype, int64_t y_stride, const void *w, const void *w_scales, const void *x,
                          int x_dtype, int64_t x_stride, size_t rows, size_t cols, size_t batch, void *workspace,
                          size_t workspace_bytes, void *stream);

@@ -171,10 +171,9 @@ __device__ __forceinline__ void mx_store(void* y, int dtype, int64_t at, int n, 
 // weights on their way while these are multiplied. With X the activation is not in MXFP4
 // yet but [batch][cols] of X: every workgroup quantizes it once into LDS, behind the loads of its
 // first weights, which saves a launch (for a token or a few: see mx_linear_fits).
-template <int NT, typename X>
+template <int NT, int U, typename X>
 __global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, const X* act, int64_t stride, int wide) {
   constexpr bool kOwn = !__is_same(X, void);
-  constexpr int U = NT == 1 ? 5 : 2;  // steps on their way together: 2560 columns in one go
   __shared__ f32x4 part[2][4][NT][64];
   extern __shared__ __align__(16) uint8_t own[];  // with X: [batch][cols / 2], then [batch][cols / 32]
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
@@ -265,10 +264,23 @@ __global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, c
   }
 }
 
-// Workgroups for `tiles` row tiles: all of them up to `most`, else few enough that each has as many.
-inline unsigned mx_matvec_grid(int tiles, int most) {
-  const int rounds = (tiles + most - 1) / most;
+// Workgroups for `tiles` row tiles: all of them up to 2048, else few enough that each has as many (128256 x 2048
+// by eight tokens: 51 us, 62 with one tile a workgroup; 19456 x 2560 by one is all of them: 7.8, with 768 8.9).
+inline unsigned mx_matvec_grid(int tiles) {
+  const int rounds = (tiles + 2047) / 2048;
   return (unsigned)((tiles + rounds - 1) / rounds);
+}
+
+// Steps of a wave on their way together (U): four or five, whichever divides its steps with less rest (2048 columns
+// are four steps a wave, 2560 five: with five for both, 128256 x 2048 takes 42 us for 38).
+template <typename X>
+void matvec_t(const MxMatmul& L, size_t lds, const X* x, int64_t stride, int wide) {
+  const int tiles = (L.rows + 15) / 16, steps = (L.cols + 511) / 512;
+  const dim3 grid(mx_matvec_grid(tiles));
+  if ((steps + 3) / 4 * 4 < (steps + 4) / 5 * 5)
+    hipLaunchKernelGGL((mx_matvec_kernel<1, 4, X>), grid, dim3(256), lds, L.stream, L, tiles, x, stride, wide);
+  else
+    hipLaunchKernelGGL((mx_matvec_kernel<1, 5, X>), grid, dim3(256), lds, L.stream, L, tiles, x, stride, wide);
 }
 
 template <typename T>
@@ -300,9 +312,7 @@ void dequantize_t(const void* q, const void* s, size_t rows, size_t cols, void* 
 template <typename X>
 void linear_t(const MxMatmul& L, const void* x, int64_t stride) {
   const size_t lds = (size_t)L.batch * (L.cols / 2 + L.cols / 32);
-  const int tiles = (L.rows + 15) / 16;
-  hipLaunchKernelGGL((mx_matvec_kernel<1, X>), dim3(mx_matvec_grid(tiles, 4096)), dim3(256), lds, L.stream, L, tiles,
-                     (const X*)x, stride, wide_rows<X>(x, stride) ? 1 : 0);
+  matvec_t<X>(L, lds, (const X*)x, stride, wide_rows<X>(x, stride) ? 1 : 0);
 }
 
 }  // namespace
@@ -329,9 +339,19 @@ hipError_t launch_mx_dequantize(const void* q, const void* s, size_t rows, size_
   return hipGetLastError();
 }
 
-// A token or a few are quantized by every workgroup of the product: up to 16384 values (LDS for 4 workgroups a
-// CU).
-bool mx_linear_fits(int cols, int batch) { return batch <= 16 && (int64_t)cols * batch <= kMxOwn; }
+// The tiles of 128 x 128: from 65 tokens on, or where there are many rows (64 x 9728 x 2560: 14.8 us on them, 20.5
+// not; 32 x 2560 x 9728, 20 row tiles: 36.4 and 24.7; 4 x 128256 x 2048: 35.8 and 40.9, but 1 x 32768 x 2560: 14.8 and
+// 10.9). Their scales come in pairs at least.
+static bool mx_wants_gemm(int rows, int cols, int batch) {
+  return cols >= 64 && (batch > 64 || (batch > 16 && rows >= 8192) || (batch > 3 && rows >= 32768));
+}
+
+// A token or a few are quantized by every workgroup of the product, up to 16384 values: 9728 x 2560 by one, four,
+// eight tokens takes 6.3, 7.7, 10.1 us so and 9.7, 10.2, 10.1 in two launches, 2560 x 9728 by one and two 8.2, 10.8 and
+// 10.1, 10.1.
+bool mx_linear_fits(int rows, int cols, int batch) {
+  return batch <= 16 && (int64_t)cols * batch <= kMxOwn && !mx_wants_gemm(rows, cols, batch);
+}
 
 hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64_t stride) {
   if (x_dtype == kF32)
@@ -344,13 +364,12 @@ hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64
 }
 
 hipError_t launch_mx_matmul(const MxMatmul& L) {
-  if (L.batch > 64 && L.cols >= 64) return launch_mx_gemm(L);
+  if (mx_wants_gemm(L.rows, L.cols, L.batch)) return launch_mx_gemm(L);
   const int tokens = (L.batch + 15) / 16, tiles = (L.rows + 15) / 16;
   if (tokens == 1)
-    hipLaunchKernelGGL((mx_matvec_kernel<1, void>), dim3(mx_matvec_grid(tiles, 4096)), dim3(256), 0, L.stream, L, tiles,
-                       (const void*)nullptr, (int64_t)0, 0);
+    matvec_t<void>(L, 0, nullptr, 0, 0);
   else
-    hipLaunchKernelGGL((mx_matvec_kernel<4, void>), dim3(mx_matvec_grid(tiles, 4096), (tokens + 3) / 4), dim3(256), 0,
+    hipLaunchKernelGGL((mx_matvec_kernel<4, 2, void>), dim3(mx_matvec_grid(tiles), (tokens + 3) / 4), dim3(256), 0,
                        L.stream, L, tiles, (const void*)nullptr, (int64_t)0, 0);
   return hipGetLastError();
 }

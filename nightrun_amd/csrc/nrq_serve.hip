@@ -116,8 +116,8 @@ int mx_check(const char* name, size_t rows, size_t cols) {
   return NRQ_OK;
 }
 
-size_t linear_bytes(size_t cols, size_t batch) {
-  if (batch <= INT_MAX && nrq::mx_linear_fits((int)cols, (int)batch)) return 0;
+size_t linear_bytes(size_t rows, size_t cols, size_t batch) {
+  if (nrq::mx_linear_fits((int)rows, (int)cols, (int)batch)) return 0;
   return up16(batch * (cols / 2)) + up16(batch * (cols / 32));
 }
 
@@ -304,13 +304,14 @@ int nrq_dev_matmul_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, co
   return mx_matmul(name, y, dtype, y_stride, w, w_scales, x, x_scales, rows, cols, batch, stream);
 }
 
-int nrq_linear_mxfp4_workspace(size_t cols, size_t batch, size_t* bytes) {
+int nrq_linear_mxfp4_workspace(size_t rows, size_t cols, size_t batch, size_t* bytes) {
   static const char* name = "nrq_linear_mxfp4_workspace";
   if (!bytes) return fail(NRQ_ERR_ARG, name, "null pointer");
-  int rc = mx_check(name, batch, cols);
+  int rc = mx_check(name, rows, cols);
   if (rc) return rc;
+  if (batch > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "batch of %zu (at most 2^20)", batch);
   // the product's workgroups quantize few values for themselves
-  *bytes = linear_bytes(cols, batch);
+  *bytes = linear_bytes(rows, cols, batch);
   return NRQ_OK;
 }
 
@@ -324,9 +325,9 @@ int nrq_dev_linear_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, co
   if (!bytes_of(x_dtype)) return fail(NRQ_ERR_ARG, name, "unknown type %d", x_dtype);
   if (cols && !x) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(x, bytes_of(x_dtype))) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
-  if ((rc = workspace_check(name, workspace, workspace_bytes, linear_bytes(cols, batch)))) return rc;
+  if ((rc = workspace_check(name, workspace, workspace_bytes, linear_bytes(rows, cols, batch)))) return rc;
   if ((rc = device_check(name, stream))) return rc;
-  if (cols && nrq::mx_linear_fits((int)cols, (int)batch)) {
+  if (cols && nrq::mx_linear_fits((int)rows, (int)cols, (int)batch)) {
     nrq::MxMatmul L{y,         dtype,      y_stride,   (const uint8_t*)w, (const uint8_t*)w_scales, nullptr, nullptr,
                     (int)rows, (int)cols, (int)batch, (hipStream_t)stream};
     return launched(name, nrq::launch_mx_linear(L, x, x_dtype, x_stride));

@@ -86,7 +86,7 @@ struct MxMatmul {
   hipStream_t stream;
 };
 hipError_t launch_mx_matmul(const MxMatmul& L);
-bool mx_linear_fits(int cols, int batch);  // whether launch_mx_linear takes the activation as it is
+bool mx_linear_fits(int rows, int cols, int batch);  // whether launch_mx_linear takes the activation as it is
 hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64_t stride);
 hipError_t launch_mx_gemm(const MxMatmul& L);  // many tokens (nrq_mx_gemm.hip)
 

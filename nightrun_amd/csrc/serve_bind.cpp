@@ -281,7 +281,7 @@ BIND(linear_mxfp4, 4) {
   const int yk = kind(y, "y"), xk = kind(x, "x");
   void *yp = on(y, "y", dev), *xp = on(x, "x", dev);
   size_t need;
-  const int rc = nrq_linear_mxfp4_workspace(w.cols, batch, &need);
+  const int rc = nrq_linear_mxfp4_workspace(w.rows, w.cols, batch, &need);
   if (rc) return rc;
   at::Tensor ws;
   if (need) ws = workspace(need, x);

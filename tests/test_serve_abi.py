@@ -194,9 +194,9 @@ def test_workspaces():
     from nightrun_amd import _lib
 
     L, n = _lib.lib(), C.c_size_t()
-    assert L.nrq_linear_mxfp4_workspace(64, 505, C.byref(n)) == 0 and n.value == 505 * 32 + 1024
-    assert L.nrq_linear_mxfp4_workspace(64, 5, C.byref(n)) == 0 and n.value == 0  # quantized where it is used
-    assert L.nrq_linear_mxfp4_workspace(65, 5, C.byref(n)) == SHAPE
+    assert L.nrq_linear_mxfp4_workspace(40, 64, 505, C.byref(n)) == 0 and n.value == 505 * 32 + 1024
+    assert L.nrq_linear_mxfp4_workspace(40, 64, 5, C.byref(n)) == 0 and n.value == 0  # quantized where it is used
+    assert L.nrq_linear_mxfp4_workspace(40, 65, 5, C.byref(n)) == SHAPE
     assert L.nrq_verify_workspace(3, 5000, C.byref(n)) == 0 and 0 < n.value <= 3 * 5000 * 16
     assert L.nrq_paged_attention_workspace(1, 32, _kv(), C.byref(n)) == 0 and n.value >= 4 * 130 * 4
     assert L.nrq_paged_attention_workspace(1, 33, _kv(), C.byref(n)) == SHAPE
