@@ -100,7 +100,7 @@ int nrq_dev_rope_append(void *y, const void *q, const void *k, const void *v, in
  * workspace: nrq_paged_attention_workspace bytes, 16-byte aligned, its contents
  * of no meaning before and after; calls that may overlap, and graphs whose
  * replays may, need one each. */
-int nrq_paged_attention_workspace(size_t n_new, size_t heads, const nrq_paged_kv *kv, size_t *bytes);
+int nrq_paged_attention_workspace(size_t seqs, size_t n_new, size_t heads, const nrq_paged_kv *kv, size_t *bytes);
 int nrq_dev_paged_attention(void *out, const void *q, int dtype, size_t n_new, size_t heads, const int64_t strides[6],
                             const nrq_paged_kv *kv, const nrq_page_table *table, const int32_t *lens,
                             const int32_t *counts, float scale, int32_t window, float *lse, void *workspace,

@@ -92,7 +92,7 @@ _i64, _f, _szp = C.c_int64, C.c_float, C.POINTER(C.c_size_t)
 SERVE_SIGNATURES = {
     "nrq_dev_rope": ([_vp, _vp, _i, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _i, _f, _vp], _i),
     "nrq_dev_rope_append": ([_vp, _vp, _vp, _vp, _i, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _i, _f, _vp, _vp, _vp], _i),
-    "nrq_paged_attention_workspace": ([_sz, _sz, _vp, _szp], _i),
+    "nrq_paged_attention_workspace": ([_sz, _sz, _sz, _vp, _szp], _i),
     "nrq_dev_paged_attention": ([_vp, _vp, _i, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _f, C.c_int32, _vp, _vp, _sz, _vp],
                                 _i),
     "nrq_verify_workspace": ([_sz, _sz, _szp], _i),

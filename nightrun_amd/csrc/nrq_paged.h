@@ -42,6 +42,7 @@ struct PaArgs {
   int wide_q;           // q in 16-byte loads
   float* part_o;        // [2 * wgs][slots][hd]
   float2* part_ml;      // [2 * wgs][slots]: maximum (log2 units), sum
+  int4* share;          // [units]: first and last workgroup, rows
 };
 
 inline int pa_per(int hd, size_t rows) { return hd <= 128 && rows > 16 ? 32 : 16; }
@@ -57,39 +58,42 @@ __device__ __forceinline__ SeqSpan pa_seq(const PagedAttnLaunch& L, int b) {
                   L.window, kTile);
 }
 
-// All tiles of the line, summed by each wave for itself.
-__device__ __forceinline__ int pa_total(const PaArgs& A) {
-  const int lane = threadIdx.x & 63;
-  int t = 0;
-  for (int b = lane; b < A.L.table.seqs; b += 64) t += pa_seq(A.L, b).tiles;
+// All tiles of the line; the sequence whose tiles hold tile `g(total)`, and its first tile's place.
+// Each wave sums and scans the lengths for itself; up to 64 of them are read once.
+struct PaLine {
+  int total, wgs, at, b, first;
+};
+__device__ __forceinline__ PaLine pa_line(const PaArgs& A, int wg) {
+  const int lane = threadIdx.x & 63, seqs = A.L.table.seqs;
+  const int mine = lane < seqs ? pa_seq(A.L, lane).tiles * A.units_per_seq : 0;
+  int t = mine;
+  for (int b = lane + 64; b < seqs; b += 64) t += pa_seq(A.L, b).tiles * A.units_per_seq;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) t += __shfl_xor(t, m);
-  return __builtin_amdgcn_readfirstlane(t) * A.units_per_seq;
-}
-
-// The sequence whose tiles hold tile g of the line, and its first tile's place.
-__device__ __forceinline__ int pa_find(const PaArgs& A, int g, int* first) {
-  const int lane = threadIdx.x & 63;
+  PaLine p;
+  p.total = __builtin_amdgcn_readfirstlane(t);
+  p.wgs = min(A.wgs, p.total);
+  p.at = wg < p.wgs ? line_start(wg, p.total, p.wgs) : p.total;
   int base = 0;
-  for (int b0 = 0; b0 < A.L.table.seqs; b0 += 64) {
-    const int b = b0 + lane;
-    const int own = b < A.L.table.seqs ? pa_seq(A.L, b).tiles * A.units_per_seq : 0;
+  for (int b0 = 0; b0 < seqs; b0 += 64) {
+    const int own = b0 == 0 ? mine : (b0 + lane < seqs ? pa_seq(A.L, b0 + lane).tiles * A.units_per_seq : 0);
     int sum = own;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
       const int y = __shfl_up(sum, m);
       if (lane >= m) sum += y;
     }
-    const unsigned long long over = __ballot(base + sum > g);
+    const unsigned long long over = __ballot(base + sum > p.at);
     if (over) {
-      const int at = __ffsll(over) - 1;
-      *first = base + __builtin_amdgcn_readlane(sum - own, at);
-      return b0 + at;
+      const int k = __ffsll(over) - 1;
+      p.first = base + __builtin_amdgcn_readlane(sum - own, k);
+      p.b = b0 + k;
+      return p;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
   }
-  *first = base;
-  return A.L.table.seqs;
+  p.b = seqs, p.first = base;
+  return p;
 }
 
 __device__ __forceinline__ void pa_store(void* o, int dtype, int64_t at, float v) {
@@ -289,13 +293,11 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
   const PagedAttnLaunch& L = A.L;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
 
-  const int total = pa_total(A);
-  const int wgs = min(A.wgs, total);
+  const PaLine line = pa_line(A, blockIdx.x);
+  const int total = line.total, wgs = line.wgs;
   if ((int)blockIdx.x >= wgs) return;
-  int at = line_start(blockIdx.x, total, wgs);
+  int at = line.at, first = line.first, b = line.b;
   const int stop = line_start(blockIdx.x + 1, total, wgs);
-  int first;
-  int b = pa_find(A, at, &first);
   while (at < stop) {
     const SeqSpan sq = pa_seq(L, b);
     const int unit = (at - first) / sq.tiles;
@@ -304,6 +306,9 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
     const int head = unit / A.row_tiles, rt = unit - head * A.row_tiles;
     const int row0 = rt * 16 * NT, rows = min(16 * NT, sq.n * A.group - row0);
     const bool whole = t_begin == 0 && t_end == sq.tiles;
+    if (t_begin == 0 && threadIdx.x == 0)
+      A.share[b * A.units_per_seq + unit] =
+          make_int4(blockIdx.x, whole ? (int)blockIdx.x : line_owner(at + sq.tiles - 1, total, wgs), rows, 0);
     if (rows > 0) {
       const int first_hi = sq.len - sq.n + row0 / A.group;                // what the unit's first
       const int last_hi = sq.len - sq.n + (row0 + rows - 1) / A.group;    // and last row see
@@ -533,43 +538,41 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs A) {
   const PagedAttnLaunch& L = A.L;
   const int u = blockIdx.x, b = u / A.units_per_seq, unit = u - b * A.units_per_seq;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const SeqSpan sq = pa_seq(L, b);
-  const int head = unit / A.row_tiles, rt = unit - head * A.row_tiles;
-  const int r = blockIdx.y, rr = rt * A.per + r;
-  if (rr >= sq.n * A.group) return;
-  int before = 0, all = 0;  // tiles of the sequences before, and of all
-  for (int i = lane; i < L.table.seqs; i += 64) {
-    const int t = pa_seq(L, i).tiles;
-    all += t;
-    if (i < b) before += t;
-  }
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    before += __shfl_xor(before, m);
-    all += __shfl_xor(all, m);
-  }
-  const int total = all * A.units_per_seq, wgs = min(A.wgs, total);
-  const int g0 = before * A.units_per_seq + unit * sq.tiles, g1 = g0 + sq.tiles;
-  const int w0 = line_owner(g0, total, wgs), w1 = line_owner(g1 - 1, total, wgs);
-  if (w0 == w1) return;
-  // the maximum over all stretches
-  float mm = -INFINITY;
-  for (int k = w0 + lane; k <= w1; k += 64) mm = fmaxf(mm, A.part_ml[(2 * k + (k == w0 ? 1 : 0)) * A.slots + r].x);
+  const int4 share = A.share[u];
+  const int r = blockIdx.y, w0 = share.x, n = share.y - w0 + 1;
+  if (n < 2 || r >= share.z) return;
+  const int head = unit / A.row_tiles, rr = (unit - head * A.row_tiles) * A.per + r;
+  auto slot = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * A.slots + r; };
+  // the maximum over all stretches, then their sums; a lane keeps the first 64's
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (lane < n) ml = A.part_ml[slot(lane)];
+  float mm = ml.x;
+  for (int k = lane + 64; k < n; k += 64) mm = fmaxf(mm, A.part_ml[slot(k)].x);
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) mm = fmaxf(mm, __shfl_xor(mm, m));
   const float ref = mm == -INFINITY ? 0.0f : mm;
+  const float mine = __builtin_amdgcn_exp2f(ml.x - ref);
   float o[E], l = 0;
 #pragma unroll
   for (int e = 0; e < E; e++) o[e] = 0;
-#pragma unroll 4
-  for (int k = w0 + w; k <= w1; k += 4) {
-    const int64_t slot = (2 * k + (k == w0 ? 1 : 0)) * A.slots + r;
-    const float2 ml = A.part_ml[slot];
-    const float by = __builtin_amdgcn_exp2f(ml.x - ref);
-    l += ml.y * by;
+#pragma unroll 8
+  for (int k = w; k < min(n, 64); k += 4) {
+    const float by = __shfl(mine, k);
+    l += __shfl(ml.y, k) * by;
+    const int64_t s = slot(k);
 #pragma unroll
     for (int e = 0; e < E; e++)
-      if (64 * e + lane < HD) o[e] += A.part_o[slot * HD + 64 * e + lane] * by;
+      if (64 * e + lane < HD) o[e] += A.part_o[s * HD + 64 * e + lane] * by;
+  }
+#pragma unroll 4
+  for (int k = 64 + w; k < n; k += 4) {
+    const int64_t s = slot(k);
+    const float2 x = A.part_ml[s];
+    const float by = __builtin_amdgcn_exp2f(x.x - ref);
+    l += x.y * by;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (64 * e + lane < HD) o[e] += A.part_o[s * HD + 64 * e + lane] * by;
   }
 #pragma unroll
   for (int e = 0; e < E; e++) ex_o[w][64 * e + lane] = o[e];
@@ -596,6 +599,7 @@ hipError_t pa_launch(PaArgs& A) {
   A.wgs = (int)(most < fill ? most : fill);
   A.part_o = (float*)A.L.workspace;
   A.part_ml = (float2*)(A.part_o + (size_t)2 * A.wgs * A.slots * HD);
+  A.share = (int4*)(((uintptr_t)(A.part_ml + (size_t)2 * A.wgs * A.slots) + 15) & ~(uintptr_t)15);
   hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ, NP>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
   if (tiles > 1)
     hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)units, A.slots), dim3(256), 0, A.L.stream, A);

@@ -186,13 +186,13 @@ int nrq_dev_rope_append(void* y, const void* q, const void* k, const void* v, in
   return launched(name, nrq::launch_rope(L));
 }
 
-int nrq_paged_attention_workspace(size_t n_new, size_t heads, const nrq_paged_kv* kv, size_t* bytes) {
+int nrq_paged_attention_workspace(size_t seqs, size_t n_new, size_t heads, const nrq_paged_kv* kv, size_t* bytes) {
   static const char* name = "nrq_paged_attention_workspace";
   if (!bytes || !kv) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (kv->n_kv_heads < 1 || heads < 1 || heads % kv->n_kv_heads)
     return fail(NRQ_ERR_SHAPE, name, "%zu heads over %d KV heads", heads, kv->n_kv_heads);
   if (!paged_hd(kv->head_dim)) return fail(NRQ_ERR_UNSUPPORTED, name, "heads of %d", kv->head_dim);
-  *bytes = nrq::paged_attn_workspace(n_new, heads, kv->n_kv_heads, kv->head_dim);
+  *bytes = nrq::paged_attn_workspace(seqs, n_new, heads, kv->n_kv_heads, kv->head_dim);
   return NRQ_OK;
 }
 
@@ -226,7 +226,7 @@ int nrq_dev_paged_attention(void* out, const void* q, int dtype, size_t n_new, s
   if (!apart(strides[3], (size_t)table->seqs, strides[4], n_new, hd) || !apart(strides[5], heads, 0, 1, hd))
     return fail(NRQ_ERR_ARG, name, "output rows overlap");
   if ((rc = workspace_check(name, workspace, workspace_bytes,
-                            nrq::paged_attn_workspace(n_new, heads, kv->n_kv_heads, kv->head_dim))))
+                            nrq::paged_attn_workspace((size_t)table->seqs, n_new, heads, kv->n_kv_heads, kv->head_dim))))
     return rc;
   L.out = out, L.q = q, L.dtype = dtype, L.n_new = (int)n_new, L.heads = (int)heads;
   L.qb = strides[0], L.qt = strides[1], L.qh = strides[2], L.ob = strides[3], L.ot = strides[4], L.oh = strides[5];

@@ -56,7 +56,7 @@ struct PagedAttnLaunch {
   void* workspace;
   hipStream_t stream;
 };
-size_t paged_attn_workspace(size_t n_new, size_t heads, int n_kv, int hd);
+size_t paged_attn_workspace(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd);
 hipError_t launch_paged_attn(const PagedAttnLaunch& L);
 
 struct VerifyLaunch {

@@ -199,7 +199,7 @@ BIND(paged_attention, 10) {
   VALUE_CHECK(window >= 0 && window <= INT32_MAX, "window: ", window);
   void *yp = on(y, "y", dev), *qp = on(q, "q", dev);
   size_t need;
-  const int rc = nrq_paged_attention_workspace(n, heads, &kv, &need);
+  const int rc = nrq_paged_attention_workspace(q.size(0), n, heads, &kv, &need);
   if (rc) return rc;
   const at::Tensor ws = workspace(need, q);
   const int64_t s[6] = {q.stride(0), q.stride(1), q.stride(2), y.stride(0), y.stride(1), y.stride(2)};

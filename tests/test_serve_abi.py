@@ -198,9 +198,9 @@ def test_workspaces():
     assert L.nrq_linear_mxfp4_workspace(40, 64, 5, C.byref(n)) == 0 and n.value == 0  # quantized where it is used
     assert L.nrq_linear_mxfp4_workspace(40, 65, 5, C.byref(n)) == SHAPE
     assert L.nrq_verify_workspace(3, 5000, C.byref(n)) == 0 and 0 < n.value <= 3 * 5000 * 16
-    assert L.nrq_paged_attention_workspace(1, 32, _kv(), C.byref(n)) == 0 and n.value >= 4 * 130 * 4
-    assert L.nrq_paged_attention_workspace(1, 33, _kv(), C.byref(n)) == SHAPE
-    assert L.nrq_paged_attention_workspace(1, 32, _kv(), None) == ARG
+    assert L.nrq_paged_attention_workspace(3, 1, 32, _kv(), C.byref(n)) == 0 and n.value >= 4 * 130 * 4
+    assert L.nrq_paged_attention_workspace(3, 1, 33, _kv(), C.byref(n)) == SHAPE
+    assert L.nrq_paged_attention_workspace(3, 1, 32, _kv(), None) == ARG
 
 
 # ---- the paged cache's index arithmetic ---------------------------------------------------
