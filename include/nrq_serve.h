@@ -82,7 +82,8 @@ int nrq_dev_rope_append(void *y, const void *q, const void *k, const void *v, in
  * are [table.seqs][n_new][heads][head_dim] of `dtype` (NRQ_F32, NRQ_F16,
  * NRQ_BF16), strides = {q sequence, q token, q head, out sequence, out token, out
  * head}; heads is a multiple of the KV heads, query head h reads KV head h /
- * (heads / n_kv_heads). head_dim is 32, 64, 96, 128 or 256.
+ * (heads / n_kv_heads). head_dim is 32, 64, 96, 128 or 256; a table holds at
+ * most 2^30 positions of a sequence.
  *   lens[b]: positions of sequence b, its new tokens' among them (their keys and
  *     values are in the cache already); below 0 is 0, more than the table holds
  *     is what it holds.
@@ -134,7 +135,9 @@ int nrq_dev_verify_drafts(int32_t *tokens, int32_t *accepted, const float *targe
  * row share a scale 2^(s - 127), s a byte; each value is 4 bits: sign and 0,
  * .5, 1, 1.5, 2, 3, 4 or 6, two to a byte, the first in the low bits. q is
  * [rows][cols / 2] bytes, scales [rows][cols / 32] bytes, contiguous, q 16-byte
- * aligned; cols a multiple of 32. s - 127 = floor(log2(largest magnitude)) - 2,
+ * aligned; cols a multiple of 32. Scales have to be readable from the 16-byte
+ * boundary before their first byte to the one behind their last (true within any
+ * HIP allocation). s - 127 = floor(log2(largest magnitude)) - 2,
  * at least -127 (also for zeros); values to the nearest of those (ties to the even
  * code), at most 6. A block with an infinity or a NaN is s = 255 (NaN
  * throughout) with zeros. */

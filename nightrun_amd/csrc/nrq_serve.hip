@@ -216,7 +216,9 @@ int nrq_dev_paged_attention(void* out, const void* q, int dtype, size_t n_new, s
       n_new * heads * (size_t)table->seqs > (size_t)1 << 30)
     return fail(NRQ_ERR_UNSUPPORTED, name, "%d sequences of %zu rows of %zu heads", table->seqs, n_new, heads);
   if (!strides || !out || !q || !lens) return fail(NRQ_ERR_ARG, name, "null pointer");
-  if ((double)table->seqs * (double)(n_new * heads) * ((double)table->width * kv->page_size / 128 + 1) >= 2147483647.0)
+  const int64_t held = (int64_t)table->width * kv->page_size;  // positions of a sequence at most
+  if (held > (int64_t)1 << 30) return fail(NRQ_ERR_UNSUPPORTED, name, "%lld positions of a sequence (at most 2^30)", (long long)held);
+  if ((double)table->seqs * (double)(n_new * heads) * ((double)held / 128 + 1) >= 2147483647.0)
     return fail(NRQ_ERR_UNSUPPORTED, name, "%d sequences of %d pages of %d: too much work for a call", table->seqs,
                 table->width, kv->page_size);
   const size_t e = bytes_of(dtype);
@@ -230,7 +232,8 @@ int nrq_dev_paged_attention(void* out, const void* q, int dtype, size_t n_new, s
     return rc;
   L.out = out, L.q = q, L.dtype = dtype, L.n_new = (int)n_new, L.heads = (int)heads;
   L.qb = strides[0], L.qt = strides[1], L.qh = strides[2], L.ob = strides[3], L.ot = strides[4], L.oh = strides[5];
-  L.lens = lens, L.counts = counts, L.scale = scale, L.window = window, L.lse = lse;
+  // a window that no sequence outgrows is none (and position - window stays within 32 bits)
+  L.lens = lens, L.counts = counts, L.scale = scale, L.window = window < held ? window : 0, L.lse = lse;
   L.workspace = workspace, L.stream = (hipStream_t)stream;
   if ((rc = device_check(name, stream))) return rc;
   return launched(name, nrq::launch_paged_attn(L));

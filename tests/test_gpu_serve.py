@@ -391,6 +391,50 @@ def test_attention_bad_pages_and_lengths(gpu):
     assert torch.equal(z, torch.zeros_like(z))
 
 
+@pytest.mark.parametrize("window", [167, 168, 169, 2 ** 30, 2 ** 31 - 1])
+def test_attention_window_past_everything(gpu, window):
+    """Windows as long as the table and longer, with rows before the first position: as without one."""
+    import torch
+
+    c = Cache(gen(11), [3, 160, 0], 2, 64, 24, "f16", width=7)  # holds 168
+    y = check_attention(c, "f32", "f16", 6, 4, window=window)
+    assert torch.equal(y, check_attention(c, "f32", "f16", 6, 4))
+
+
+def test_two_threads(gpu):
+    """Calls from two host threads, each on a stream of its own, with errors in one of them."""
+    import threading
+
+    import torch
+
+    from nightrun_amd import NrPanic, serve
+
+    steps, out = [Step(5), Step(6)], [None, None]
+    for s in steps:
+        s.run()
+    torch.cuda.synchronize()
+    want = [s.results() for s in steps]
+
+    def work(i):
+        st = torch.cuda.Stream()
+        for _ in range(20):
+            steps[i].run(stream=st)
+            if i:
+                with pytest.raises(NrPanic):
+                    serve.rope(steps[i].x.view(-1, 4, 64), steps[i].x.view(-1, 4, 64), steps[i].pos,
+                               torch.ones(33, device="cuda"), stream=st)
+        st.synchronize()
+        out[i] = steps[i].results()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for o, w in zip(out, want):
+        assert all(torch.equal(a, b) for a, b in zip(o, w))
+
+
 def test_attention_extreme_scores(gpu):
     """Rows of very different sizes (weights that underflow, f32 queries past f16's range, zeros), a scale of zero."""
     import torch
@@ -700,7 +744,7 @@ def check_product(y, xc, xs, wc, ws, kind):
                                              (17, 70, 160), (64, 300, 1024), (65, 129, 352), (130, 257, 288),
                                              (300, 512, 2048), (257, 1000, 128), (512, 24, 4128), (1000, 515, 256), (300, 700, 640),
                                              (200, 150, 416), (513, 130, 480), (129, 1030, 1312), (1100, 600, 544),
-                                             (70, 3000, 2080)])
+                                             (70, 3000, 2080), (2100, 8300, 512), (4200, 4100, 544)])
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 def test_mx_matmul(gpu, kind, batch, rows, cols):
     import torch

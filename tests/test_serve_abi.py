@@ -145,7 +145,8 @@ REFUSED = [
     ("nrq_dev_paged_attention", dict(ws=P + 8), ARG, "aligned"),
     ("nrq_dev_paged_attention", dict(n_new=70000), UNSUPPORTED, "rows"),
     ("nrq_dev_paged_attention", dict(kv=_kv(n_pages=2 ** 31 - 1)), UNSUPPORTED, "elements"),
-    ("nrq_dev_paged_attention", dict(table=_table(width=2 ** 28, stride=2 ** 28)), UNSUPPORTED, "too much"),
+    ("nrq_dev_paged_attention", dict(table=_table(width=2 ** 25, stride=2 ** 25, seqs=20)), UNSUPPORTED, "too much"),
+    ("nrq_dev_paged_attention", dict(table=_table(width=2 ** 26 + 1, stride=2 ** 27)), UNSUPPORTED, "2^30"),
     ("nrq_dev_rope_append", dict(kv=_kv(page_size=2 ** 31 - 1)), UNSUPPORTED, "elements"),
     ("nrq_dev_verify_drafts", dict(n_new=65), UNSUPPORTED, "64"),
     ("nrq_dev_verify_drafts", dict(vocab=0), SHAPE, "vocabulary"),
