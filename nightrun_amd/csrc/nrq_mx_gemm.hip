@@ -3,7 +3,7 @@
 // y[b][r] = sum over blocks k of 2^(es + et - 254) * sum over the block's 32 columns of the E2M1
 // products, summed in 32 bits by the scaled matrix instruction (16 x 16 x 128, a scale byte per row and
 // block); rounded once, at the store. 2048 f32 tokens by 16384 x 2048, their quantization included, take
-// 70 us: 2.0 PFLOP/s and 1.9 TB/s of f32 outputs; 4096 x 4096 by 4096 tokens takes 75 us, 1.8 PFLOP/s. The
+// 61 us: 2.2 PFLOP/s and 2.2 TB/s of f32 outputs; 4096 x 4096 by 4096 tokens takes 75 us, 1.8 PFLOP/s. The
 // matrix units are busy a third of that: a step's loads, its reads from LDS (32 KiB for 128 x 128 x
 // 128) and its products overlap only as far as the CU's two workgroups drift apart.
 //
@@ -17,6 +17,8 @@
 // row come as one 16-bit load and the instruction picks the byte. Chunks behind
 // the last column come from zeros; rows behind the last are the last once more and are not stored.
 #include "nrq_serve_launch.h"
+
+#include <type_traits>
 
 namespace nrq {
 namespace {
@@ -185,9 +187,48 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(MxMatmul L, int row_til
 // A workgroup takes tile after tile; the stages run on from one to the next, so that the next
 // tile's are on their way while this one's outputs are written, and a CU's two workgroups drift apart, one
 // writing while the other multiplies.
+//
+// Row 16 (m / 4) + 4 i + m % 4 of a wave's 64 goes to row m of matrix instruction i, so that a lane ends with 16
+// neighbouring outputs of a token, P pieces of 16 bytes. P lanes, P tokens, then exchange
+// theirs: a store covers all 64 rows of its tokens, 256 or 128 bytes side by side (16384 x 2048 at 2048 tokens
+// takes 61 us so, 70 with stores of 64 bytes side by side).
+__device__ __forceinline__ int gemm_row(int q) { return (q & ~63) | (q & 12) << 2 | (q >> 4 & 3) << 2 | (q & 3); }
+
+template <typename T>
+__device__ __forceinline__ void mx_pack(f32x4 a, f32x4 b, f32x4 c, f32x4 d, u32x4* o) {
+  if constexpr (sizeof(T) == 4) {
+    o[0] = __builtin_bit_cast(u32x4, a), o[1] = __builtin_bit_cast(u32x4, b);
+    o[2] = __builtin_bit_cast(u32x4, c), o[3] = __builtin_bit_cast(u32x4, d);
+  } else {
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    o[0] = __builtin_bit_cast(u32x4, t8{(T)a[0], (T)a[1], (T)a[2], (T)a[3], (T)b[0], (T)b[1], (T)b[2], (T)b[3]});
+    o[1] = __builtin_bit_cast(u32x4, t8{(T)c[0], (T)c[1], (T)c[2], (T)c[3], (T)d[0], (T)d[1], (T)d[2], (T)d[3]});
+  }
+}
+
+// Piece k of lane l and piece l % P of lane (l / P) P + k change places.
+template <int P>
+__device__ __forceinline__ void mx_turn(u32x4* o, int c) {
+  auto swap = [](u32x4& x, u32x4& y, bool odd, auto perm) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? x[e] : y[e]), perm.value, 0xf, 0xf, true);
+      x[e] = odd ? got : x[e], y[e] = odd ? y[e] : got;
+    }
+  };
+  const std::integral_constant<int, 0xb1> by1;  // quad lanes 1 0 3 2
+  const std::integral_constant<int, 0x4e> by2;  // 2 3 0 1
+#pragma unroll
+  for (int k = 0; k < P; k += 2) swap(o[k], o[k + 1], c & 1, by1);
+  if constexpr (P == 4)
+#pragma unroll
+    for (int k = 0; k < 2; k++) swap(o[k], o[k + 2], c & 2, by2);
+}
+
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_tiles, int tok_tiles, int wide) {
   constexpr int NS = WHOLE ? 4 : 3, SB = 256 * 64, SP = WHOLE ? 16 : 32;  // stages, bytes of one, scale bytes of a row
+  constexpr int P = sizeof(T);  // 16-byte pieces of a lane's outputs for a token
   __shared__ __align__(16) uint8_t stage[NS][SB];
   __shared__ __align__(16) uint8_t scale[2][256][SP];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
@@ -196,7 +237,7 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
   if (run.first >= run.stop) return;
 
   // ---- the stages: what the next fill takes
-  const int chunk = (lane & 3) ^ (lane >> 4);
+  const int chunk = (lane & 3) ^ (lane >> 4), wchunk[2] = {(lane & 3) ^ (2 * w & 3), (lane & 3) ^ (2 * w & 3) ^ 1};
   const uint32_t base = __builtin_amdgcn_readfirstlane(
       (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)&stage[0][0]);
   const uint32_t sbase = __builtin_amdgcn_readfirstlane(
@@ -210,10 +251,10 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const int r = 32 * w + 16 * j + (lane >> 2);
-      src[j] = L.w + (int64_t)min(r0 + r, L.rows - 1) * blocks * 16 + chunk * 16;
+      src[j] = L.w + (int64_t)min(r0 + r, L.rows - 1) * blocks * 16 + wchunk[j] * 16;
       src[2 + j] = L.x + (int64_t)min(b0 + r, L.batch - 1) * blocks * 16 + chunk * 16;
       const int q = WHOLE ? 64 * (w & 1) + lane : 64 * (w & 1) + 32 * j + (lane >> 1);
-      const uintptr_t s = (uintptr_t)(w < 2 ? L.ws + (int64_t)min(r0 + q, L.rows - 1) * blocks
+      const uintptr_t s = (uintptr_t)(w < 2 ? L.ws + (int64_t)min(r0 + gemm_row(q), L.rows - 1) * blocks
                                             : L.xs + (int64_t)min(b0 + q, L.batch - 1) * blocks);
       sfrom[j] = s & ~(uintptr_t)15;
       send[j] = s + blocks;
@@ -235,7 +276,7 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
     const bool live = WHOLE || 4 * fk + chunk < blocks;  // chunks behind the last are zeros
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      mx_dma16(live ? src[j] + fk * 64 : (const uint8_t*)mx_zeros, to + (uint32_t)(32 * w + 16 * j) * 64);
+      mx_dma16(WHOLE || 4 * fk + wchunk[j] < blocks ? src[j] + fk * 64 : (const uint8_t*)mx_zeros, to + (uint32_t)(32 * w + 16 * j) * 64);
       mx_dma16(live ? src[2 + j] + fk * 64 : (const uint8_t*)mx_zeros, to + (uint32_t)(128 + 32 * w + 16 * j) * 64);
     }
     filled++;
@@ -255,8 +296,8 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
 #pragma unroll
     for (int j = 0; j < 4; j++) acc[i][j] = f32x4{0, 0, 0, 0};
   const int wr = 64 * (w & 1), wb = 128 + 64 * (w >> 1);
-  const int at = (g ^ (c >> 2)) * 16;
-  int done = 0, slot = 0, group = 0, stores = 0;  // steps and groups of four; steps for which 16 stores are newer than a stage
+  const int at = (g ^ (c >> 2)) * 16, wrow = wr + 16 * (c >> 2) + (c & 3);
+  int done = 0, slot = 0, group = 0, stores = 0;  // steps and groups of four; steps for which the outputs' stores are newer than a stage
   uint32_t sa[4][4], sb[4][4];
   auto wait = [&]() {
     // at least four loads a stage: this one's are there when those of the NS - 2 behind it may be missing,
@@ -267,7 +308,7 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
     else if (behind < NS - 2)
       asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     else if (stores > 0)
-      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * (NS - 2) + 16) : "memory");
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * (NS - 2) + 4 * P) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * (NS - 2)) : "memory");
     stores--;
@@ -281,7 +322,7 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
     int oa[4], ob[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      oa[i] = (wr + 16 * i + c) * SP + (WHOLE ? 0 : 1) * (int)(((uintptr_t)L.ws + (int64_t)min(r0 + wr + 16 * i + c, L.rows - 1) * blocks) & 15);
+      oa[i] = (wr + 16 * i + c) * SP + (WHOLE ? 0 : 1) * (int)(((uintptr_t)L.ws + (int64_t)min(r0 + wrow + 4 * i, L.rows - 1) * blocks) & 15);
       ob[i] = (wb + 16 * i + c) * SP + (WHOLE ? 0 : 1) * (int)(((uintptr_t)L.xs + (int64_t)min(b0 + wb - 128 + 16 * i + c, L.batch - 1) * blocks) & 15);
     }
     auto scales = [&](int o, uint32_t* out) {
@@ -314,7 +355,7 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
         i32x4 a[4], b[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          a[i] = *(const i32x4*)(st + (wr + 16 * i + c) * 64 + at);
+          a[i] = *(const i32x4*)(st + (wrow + 4 * i) * 64 + at);
           b[i] = *(const i32x4*)(st + (wb + 16 * i + c) * 64 + at);
         }
         // the next loads between the products, whose time hides their addresses: 4096 x 4096 at 4096 tokens
@@ -332,17 +373,21 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
         done++;
       }
     }
-    const bool inner = wide && r0 + kGemmTile <= L.rows && b0 + kGemmTile <= L.batch;  // then 16 stores, no more
+    const bool inner = wide == 2 && r0 + kGemmTile <= L.rows && b0 + kGemmTile <= L.batch;  // then 4 P stores, no more
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const int tok = b0 + wb - 128 + 16 * j + c, r = r0 + wr + 4 * g;
+      const int tok = b0 + wb - 128 + 16 * j + c, r = r0 + wr + 16 * g;
       if (inner) {
+        u32x4 o[P];
+        mx_pack<T>(acc[0][j], acc[1][j], acc[2][j], acc[3][j], o);
+        mx_turn<P>(o, c);
 #pragma unroll
-        for (int i = 0; i < 4; i++) mx_put<T>(L.y, tok * L.ldy + r + 16 * i, acc[i][j]);
+        for (int k = 0; k < P; k++)
+          __builtin_nontemporal_store(o[k], (u32x4*)((T*)L.y + (int64_t)((tok & ~(P - 1)) + k) * L.ldy + r + 16 / P * (c & (P - 1))));
       } else if (tok < L.batch) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          if (r + 16 * i < L.rows) mx_out<T>(L.y, tok * L.ldy + r + 16 * i, L.rows - r - 16 * i, wide, acc[i][j]);
+          if (r + 4 * i < L.rows) mx_out<T>(L.y, tok * L.ldy + r + 4 * i, L.rows - r - 4 * i, wide, acc[i][j]);
       }
 #pragma unroll
       for (int i = 0; i < 4; i++) acc[i][j] = f32x4{0, 0, 0, 0};
@@ -354,7 +399,10 @@ __global__ __launch_bounds__(256, 2) void mx_gemm128_kernel(MxMatmul L, int row_
 template <typename T>
 hipError_t gemm_t(const MxMatmul& L) {
   const int rt = (L.rows + kGemmTile - 1) / kGemmTile, tt = (L.batch + kGemmTile - 1) / kGemmTile;
-  const int wide = ((uintptr_t)L.y & (4 * sizeof(T) - 1)) == 0 && L.ldy % 4 == 0;
+  // outputs: 16 bytes at once, four values at once, or one by one
+  const int wide = ((uintptr_t)L.y & 15) == 0 && L.ldy * sizeof(T) % 16 == 0             ? 2
+                   : ((uintptr_t)L.y & (4 * sizeof(T) - 1)) == 0 && L.ldy % 4 == 0 ? 1
+                                                                                   : 0;
   const unsigned all = (unsigned)((rt * tt + 7) / 8 * 8);
   const dim3 grid(all < 512 ? all : 512);
   if (L.cols % 512 == 0 && ((uintptr_t)L.ws & 15) == 0 && ((uintptr_t)L.xs & 15) == 0)
