@@ -764,6 +764,46 @@ def test_mx_matmul(gpu, kind, batch, rows, cols):
     assert torch.equal(z, y)
 
 
+@pytest.mark.parametrize("kind,cols", [("f32", 2080), ("bf16", 2560), ("f16", 4032)])
+def test_mx_matmul_tiles_of_256(gpu, kind, cols):
+    """Sizes for which the larger tiles are taken, with rows and tokens that end inside one; odd output rows."""
+    import torch
+
+    from nightrun_amd import serve
+
+    batch, rows = 1030, 8201
+    g = gen(cols)
+    w, ws = mx_random(g, rows, cols)
+    x, xs = mx_random(g, batch, cols)
+    wide = torch.full((batch, rows + 6), 3.0, dtype=dt(kind), device="cuda")
+    y = wide[:, 1:1 + rows]
+    serve.matmul_mxfp4(y, w.cuda(), ws.cuda(), x.cuda(), xs.cuda())
+    check_product(y, unpack(x), xs.numpy(), unpack(w), ws.numpy(), kind)
+    assert torch.all(wide[:, :1] == 3) and torch.all(wide[:, 1 + rows:] == 3)
+    few = torch.empty(20, rows, dtype=dt(kind), device="cuda")  # the same sums in the same order on the smaller ones
+    serve.matmul_mxfp4(few, w.cuda(), ws.cuda(), x[:20].cuda(), xs[:20].cuda())
+    assert torch.equal(few, y[:20])
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 20, 96), (3, 40, 160), (70, 200, 96), (70, 200, 416), (70, 200, 480), (130, 130, 544),
+                                             (70, 300, 2080), (1030, 8201, 2080)])
+def test_mx_matmul_nan_rows_stay_alone(gpu, batch, rows, cols):
+    """A row of w, or a token, whose scales are all NaN: its outputs are NaN, no other changes."""
+    import torch
+
+    from nightrun_amd import serve
+
+    g = gen(cols + rows)
+    (w, ws), (x, xs) = ([t.cuda() for t in mx_random(g, n, cols)] for n in (rows, batch))
+    y, z = (torch.empty(batch, rows, device="cuda") for _ in range(2))
+    serve.matmul_mxfp4(y, w, ws, x, xs)
+    ws[5], xs[batch // 2] = 255, 255
+    serve.matmul_mxfp4(z, w, ws, x, xs)
+    lost = torch.zeros_like(y, dtype=torch.bool)
+    lost[:, 5] = lost[batch // 2] = True
+    assert torch.all(torch.isnan(z[lost])) and torch.equal(z[~lost], y[~lost])
+
+
 @pytest.mark.parametrize("batch,rows,cols", [(1, 512, 2560), (1, 100, 10016), (2, 300, 96), (13, 1531, 2048), (5, 8, 32),
                                              (100, 300, 1056), (300, 260, 512)])
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
