@@ -162,7 +162,7 @@ __global__ __launch_bounds__(kVerNT) void verify_draw_kernel(VerArgs A) {
   r.p = L.target + b * L.tb + r.count * L.tr;
   r.q = r.count < n && L.draft ? L.draft + b * L.db + r.count * L.dr : nullptr;
   r.without = r.count < n && !L.draft ? L.drafted[(int64_t)b * L.n_new + r.count] : -1;
-  const double u = (double)L.uniforms[(int64_t)b * (L.n_new + 1) + L.n_new];
+  const double drawn_u = (double)L.uniforms[(int64_t)b * (L.n_new + 1) + L.n_new], u = drawn_u < 0.0 ? 0.0 : drawn_u;
   if (t == 0) found = drawn = -1;
   if (t < 2) last[t] = -1;
   VerSum c = ver_scan(own, lds[0]);

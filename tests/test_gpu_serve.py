@@ -609,6 +609,20 @@ def test_verify_edges(gpu):
     assert tokens.tolist() == [[7, 8, 9], [7, 4, -1], [1, -1, -1]] and acc.tolist() == [2, 1, 0]
 
 
+def test_verify_uniforms_below_0_and_nan(gpu):
+    """Drawn with 0 and with nothing above: the first and the last token with weight."""
+    import torch
+
+    from nightrun_amd import serve
+
+    t = torch.zeros(2, 1, 3000, device="cuda")
+    t[:, 0, 11], t[:, 0, 2500] = 0.25, 0.75
+    u = torch.tensor([[-0.5], [float("nan")]], device="cuda")
+    tokens, accepted = (torch.full(n, 9, dtype=torch.int32, device="cuda") for n in ((2, 1), (2,)))
+    serve.verify_drafts(tokens, accepted, t, None, torch.zeros(2, 0, dtype=torch.int32, device="cuda"), u)
+    assert tokens.tolist() == [[11], [2500]] and accepted.tolist() == [0, 0]
+
+
 # ---- MXFP4 -----------------------------------------------------------------------------------------
 
 GRID = np.array([0, .5, 1, 1.5, 2, 3, 4, 6])
