@@ -71,7 +71,7 @@ int nrq_dev_rope(void *y, const void *x, int dtype, size_t tokens, size_t heads,
  * y token, y head}; y may be q. A token whose seq is outside [0, table.seqs) or
  * whose pos is negative is padding: its row of y stays as it was and nothing is
  * appended. A token whose position is behind the table, or on no page, is
- * rotated but not appended. Where two tokens name the same position the cache
+ * rotated but not appended. At least one head of q. Where two tokens name the same position the cache
  * gets values of one or the other. */
 int nrq_dev_rope_append(void *y, const void *q, const void *k, const void *v, int dtype, size_t tokens, size_t heads,
                         const int64_t strides[8], const int32_t *pos, const int32_t *seq, const float *freqs,
@@ -95,7 +95,7 @@ int nrq_dev_rope_append(void *y, const void *q, const void *k, const void *v, in
  * to nothing gives zeros. What the cache holds at positions that a row does not
  * attend to, infinities and NaN too, does not reach it. lse (or NULL):
  * f32 [table.seqs][n_new][heads] contiguous, log sum_t exp(scale q.k_t), -inf for nothing.
- * Scores, softmax and sums are in 32 bits. The results depend on how the work
+ * out may not overlap q. Scores, softmax and sums are in 32 bits. The results depend on how the work
  * is split, never on the order in which it runs: the same call gives the same
  * bits.
  * workspace: nrq_paged_attention_workspace bytes, 16-byte aligned, its contents
@@ -114,8 +114,8 @@ int nrq_dev_paged_attention(void *out, const void *q, int dtype, size_t n_new, s
  * refused a token is drawn from max(target[b][i] - draft[b][i], 0) (draft NULL:
  * target[b][i] without d_i; if that is zero throughout: target[b][i]); with all
  * accepted it is drawn from target[b][n]. Drawn is the smallest v whose
- * cumulative sum through v is above uniforms[b][n] * the whole sum, else the last v
- * with any weight; -1 if none has. Products, differences and sums are in 64 bits.
+ * cumulative sum through v is above uniforms[b][n] (below 0: 0) * the whole sum,
+ * else the last v with any weight; -1 if none has. Products, differences and sums are in 64 bits.
  * target is f32 [seqs][n_new + 1][vocab], draft f32 [seqs][n_new][vocab],
  * strides = {target sequence, target row, draft sequence, draft row}; drafted
  * int32 [seqs][n_new], uniforms f32 [seqs][n_new + 1], both contiguous; n =

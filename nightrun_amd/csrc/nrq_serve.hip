@@ -5,6 +5,7 @@
 #include <climits>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../include/nrq.h"
 #include "../../include/nrq_serve.h"
@@ -76,9 +77,26 @@ int kv_check(const char* name, const nrq_paged_kv* kv, const nrq_page_table* tab
   return NRQ_OK;
 }
 
-// Rows written must not overlap: the inner dimension's rows lie apart.
-bool apart(int64_t outer, size_t n_outer, int64_t inner, size_t n_inner, size_t dim) {
-  return (n_outer < 2 || outer >= (int64_t)dim) && (n_inner < 2 || inner >= (int64_t)dim);
+// Rows written must not overlap: sorted by their strides, each dimension steps over all of the ones inside it.
+struct Dim {
+  int64_t stride;
+  size_t n;
+};
+bool apart(size_t row, std::initializer_list<Dim> dims) {
+  Dim d[3];
+  int count = 0;
+  for (const Dim& x : dims) {
+    if (x.n < 2) continue;
+    int i = count++;
+    for (; i > 0 && d[i - 1].stride > x.stride; i--) d[i] = d[i - 1];
+    d[i] = x;
+  }
+  double extent = (double)row;  // of what lies inside; the strides may be anything
+  for (int i = 0; i < count; i++) {
+    if ((double)d[i].stride < extent) return false;
+    extent += (double)d[i].stride * (double)(d[i].n - 1);
+  }
+  return true;
 }
 
 int rope_check(const char* name, const nrq::RopeLaunch& L, size_t tokens, size_t heads, size_t hd, size_t nf,
@@ -93,7 +111,7 @@ int rope_check(const char* name, const nrq::RopeLaunch& L, size_t tokens, size_t
   const size_t e = bytes_of(L.dtype);
   if (!aligned(L.y, e) || !aligned(L.x, e) || !aligned(L.pos, 4) || !aligned(L.freqs, 4))
     return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
-  if (!apart(L.yt, tokens, L.yh, heads, hd)) return fail(NRQ_ERR_ARG, name, "output rows overlap");
+  if (!apart(hd, {{L.yt, tokens}, {L.yh, heads}})) return fail(NRQ_ERR_ARG, name, "output rows overlap");
   if (L.y == L.x && (L.yt != L.xt || L.yh != L.xh))
     return fail(NRQ_ERR_ARG, name, "in place, but with other strides");
   return NRQ_OK;
@@ -170,7 +188,8 @@ int nrq_dev_rope_append(void* y, const void* q, const void* k, const void* v, in
   nrq::RopeLaunch L{};
   if (!table) return fail(NRQ_ERR_ARG, name, "null table");
   if ((rc = kv_check(name, kv, table, &L.kv, &L.table))) return rc;
-  if (tokens == 0 || heads == 0) return device_check(name, stream);
+  if (heads == 0) return fail(NRQ_ERR_SHAPE, name, "no heads");
+  if (tokens == 0) return device_check(name, stream);
   if (!strides || !k || !v || !seq) return fail(NRQ_ERR_ARG, name, "null pointer");
   L.y = y, L.x = q, L.k = k, L.v = v, L.dtype = dtype, L.pos = pos, L.seq = seq, L.freqs = freqs;
   L.xt = strides[0], L.xh = strides[1], L.kt = strides[2], L.kh = strides[3];
@@ -178,6 +197,8 @@ int nrq_dev_rope_append(void* y, const void* q, const void* k, const void* v, in
   const size_t hd = (size_t)kv->head_dim;
   if ((rc = rope_check(name, L, tokens, heads, hd, n_freqs, style))) return rc;
   if ((size_t)kv->n_kv_heads * hd > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "%d KV heads", kv->n_kv_heads);
+  if (!apart(hd, {{kv->page_stride, (size_t)kv->n_pages}, {kv->head_stride, (size_t)kv->n_kv_heads}, {kv->pos_stride, (size_t)kv->page_size}}))
+    return fail(NRQ_ERR_ARG, name, "the cache's positions overlap");
   if (!aligned(k, bytes_of(dtype)) || !aligned(v, bytes_of(dtype)) || !aligned(seq, 4))
     return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
   L.tokens = (int)tokens, L.heads = (int)heads, L.hd = (int)hd, L.nf = (int)n_freqs;
@@ -225,7 +246,7 @@ int nrq_dev_paged_attention(void* out, const void* q, int dtype, size_t n_new, s
   if (!aligned(out, e) || !aligned(q, e) || !aligned(lens, 4) || !aligned(counts, 4) || !aligned(lse, 4))
     return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
   const size_t hd = (size_t)kv->head_dim;
-  if (!apart(strides[3], (size_t)table->seqs, strides[4], n_new, hd) || !apart(strides[5], heads, 0, 1, hd))
+  if (!apart(hd, {{strides[3], (size_t)table->seqs}, {strides[4], n_new}, {strides[5], heads}}))
     return fail(NRQ_ERR_ARG, name, "output rows overlap");
   if ((rc = workspace_check(name, workspace, workspace_bytes,
                             nrq::paged_attn_workspace((size_t)table->seqs, n_new, heads, kv->n_kv_heads, kv->head_dim))))

@@ -168,6 +168,16 @@ REFUSED = [
     ("nrq_dev_linear_mxfp4", dict(x_dtype=5), ARG, "unknown type"),
     ("nrq_dev_linear_mxfp4", dict(wk_bytes=100), ARG, "workspace"),
     ("nrq_dev_linear_mxfp4", dict(x=None), ARG, "null"),
+    # rows that would overlap although each stride alone is wide enough
+    ("nrq_dev_rope", dict(strides=_i64(512, 128, 256, 128)), ARG, "overlap"),
+    ("nrq_dev_rope", dict(strides=_i64(512, 128, 128, 512)), ARG, "overlap"),
+    ("nrq_dev_rope", dict(strides=_i64(512, 128, 512, -128)), ARG, "overlap"),
+    ("nrq_dev_paged_attention", dict(strides=_i64(8192, 4096, 128, 4096, 4096, 128)), ARG, "overlap"),
+    ("nrq_dev_paged_attention", dict(strides=_i64(8192, 4096, 128, 8192, 4000, 128)), ARG, "overlap"),
+    ("nrq_dev_rope_append", dict(kv=_kv(pos_stride=64)), ARG, "overlap"),
+    ("nrq_dev_rope_append", dict(kv=_kv(head_stride=0)), ARG, "overlap"),
+    ("nrq_dev_rope_append", dict(kv=_kv(page_stride=1024)), ARG, "overlap"),
+    ("nrq_dev_rope_append", dict(heads=0), SHAPE, "no heads"),
 ]
 
 
