@@ -147,9 +147,12 @@ int nrq_dev_quantize_mxfp4(const void *src, int dtype, size_t rows, size_t cols,
 int nrq_dev_dequantize_mxfp4(const void *q, const void *scales, size_t rows, size_t cols, void *dst, int dtype,
                              int64_t dst_stride, void *stream);
 /* y[b][r] = sum_c x[b][c] * w[r][c] with both in MXFP4, the products exact, sums in 32 bits,
- * y [batch][rows] of `dtype`, rows of y y_stride apart. */
+ * y [batch][rows] of `dtype`, rows of y y_stride apart. workspace: nrq_matmul_mxfp4_workspace
+ * bytes (0 for many sizes: then NULL will do), 16-byte aligned, as for the attention. */
+int nrq_matmul_mxfp4_workspace(size_t rows, size_t cols, size_t batch, size_t *bytes);
 int nrq_dev_matmul_mxfp4(void *y, int dtype, int64_t y_stride, const void *w, const void *w_scales, const void *x,
-                         const void *x_scales, size_t rows, size_t cols, size_t batch, void *stream);
+                         const void *x_scales, size_t rows, size_t cols, size_t batch, void *workspace,
+                         size_t workspace_bytes, void *stream);
 /* The same with the activation quantized on the way: x [batch][cols] of x_dtype,
  * rows x_stride apart; the result is that of nrq_dev_quantize_mxfp4 and
  * nrq_dev_matmul_mxfp4. workspace: nrq_linear_mxfp4_workspace bytes, 16-byte

@@ -99,7 +99,8 @@ SERVE_SIGNATURES = {
     "nrq_dev_verify_drafts": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp], _i),
     "nrq_dev_quantize_mxfp4": ([_vp, _i, _sz, _sz, _i64, _vp, _vp, _vp], _i),
     "nrq_dev_dequantize_mxfp4": ([_vp, _vp, _sz, _sz, _vp, _i, _i64, _vp], _i),
-    "nrq_dev_matmul_mxfp4": ([_vp, _i, _i64, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp], _i),
+    "nrq_matmul_mxfp4_workspace": ([_sz, _sz, _sz, _szp], _i),
+    "nrq_dev_matmul_mxfp4": ([_vp, _i, _i64, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp], _i),
     "nrq_linear_mxfp4_workspace": ([_sz, _sz, _sz, _szp], _i),
     "nrq_dev_linear_mxfp4": ([_vp, _i, _i64, _vp, _vp, _vp, _i, _i64, _sz, _sz, _sz, _vp, _sz, _vp], _i),
 }

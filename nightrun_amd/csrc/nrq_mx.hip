@@ -344,10 +344,11 @@ hipError_t launch_mx_dequantize(const void* q, const void* s, size_t rows, size_
 }
 
 // The tiles of 128 x 128: from 65 tokens on, or where there are many rows (64 x 9728 x 2560: 14.8 us on them, 20.5
-// not; 32 x 2560 x 9728, 20 row tiles: 36.4 and 24.7; 4 x 128256 x 2048: 35.8 and 40.9, but 1 x 32768 x 2560: 14.8 and
-// 10.9). Their scales come in pairs at least.
+// not; 4 x 128256 x 2048: 35.8 and 40.9, but 1 x 32768 x 2560: 14.8 and 10.9) or columns, which workgroups share
+// out (17 x 2560 x 9728: 14.4 and 21.3, 64: 15.5 and 34; but 17 x 2048 x 2560: 13.5 and 9.3). Their scales come in
+// pairs at least.
 static bool mx_wants_gemm(int rows, int cols, int batch) {
-  return cols >= 64 && (batch > 64 || (batch > 16 && rows >= 8192) || (batch > 3 && rows >= 32768));
+  return cols >= 64 && (batch > 64 || (batch > 16 && (rows >= 8192 || cols >= 4096)) || (batch > 3 && rows >= 32768));
 }
 
 // A token or a few are quantized by every workgroup of the product, up to 16384 values: 9728 x 2560 by one, four,
@@ -365,6 +366,10 @@ hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64
   else
     linear_t<__bf16>(L, x, stride);
   return hipGetLastError();
+}
+
+size_t mx_matmul_workspace(int rows, int cols, int batch) {
+  return mx_wants_gemm(rows, cols, batch) ? mx_gemm_workspace(rows, cols, batch) : 0;
 }
 
 hipError_t launch_mx_matmul(const MxMatmul& L) {

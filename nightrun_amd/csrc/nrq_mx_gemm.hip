@@ -252,8 +252,13 @@ __device__ __forceinline__ void mx_turn(u32x4* o, int c) {
     for (int k = 0; k < 2; k++) swap(o[k], o[k + 2], c & 2, by2);
 }
 
-template <typename T, bool WHOLE, int TILE>
-__global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int row_tiles, int tok_tiles) {
+// Part p of `parts` of a row's steps starts here: whole groups of four, the rest with the last.
+__device__ __forceinline__ int gemm_part(int p, int parts, int steps) {
+  return p == parts ? steps : __builtin_amdgcn_readfirstlane(4 * ((steps >> 2) * p / parts));
+}
+
+template <typename T, bool WHOLE, int TILE, bool PARTS>
+__global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int row_tiles, int tok_tiles, int parts, int64_t plane) {
   constexpr int NS = WHOLE ? 4 : 3, ROWS = 2 * TILE, SB = ROWS * 64, SP = WHOLE ? 16 : 32;  // stages, bytes of one, scale bytes of a row
   constexpr int HALF = TILE / 64, JT = TILE / 32;  // waves to a half of the tile's rows or tokens, products of a wave along the tokens
   constexpr int P = sizeof(T), E = 16 / sizeof(T);  // 16-byte pieces of a lane's outputs for a token, values of one
@@ -261,7 +266,8 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int
   __shared__ __align__(16) uint8_t scale[2][ROWS][SP];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
   const int blocks = L.cols / 32, steps = (blocks + 3) / 4;
-  const GemmRun run = gemm_run(row_tiles * tok_tiles);
+  const int tiles = row_tiles * tok_tiles;
+  const GemmRun run = gemm_run(PARTS ? tiles * parts : tiles);
   if (run.first >= run.stop) return;
 
   // ---- the stages: what the next fill takes
@@ -276,9 +282,12 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int
   const uint32_t row = (uint32_t)blocks * 16;
   const uint8_t *values, *sbytes;  // of the wave's first row; sbytes down to a multiple of 16
   uint32_t src[4], sfrom[2], send[2];  // from there: chunks of step 0; a row's first 16-byte piece of scales, its end
-  int ft = run.first, fk = 0, filled = 0, groups = 0, fslot = 0;
+  int ft = run.first, fk = 0, fstop = 0, filled = 0, groups = 0, fslot = 0;
   auto aim = [&]() {
-    const GemmTile tile = gemm_tile(ft, row_tiles, tok_tiles);
+    const int part = PARTS ? __builtin_amdgcn_readfirstlane(ft / tiles) : 0;
+    fk = PARTS ? gemm_part(part, parts, steps) : 0;
+    fstop = PARTS ? gemm_part(part + 1, parts, steps) : steps;
+    const GemmTile tile = gemm_tile(ft - part * tiles, row_tiles, tok_tiles);
     const int first = of_w ? tile.r * TILE + 64 * w : tile.b * TILE + 64 * (w - HALF), all = of_w ? L.rows : L.batch;
     const int from = min(first, all - 1), last = all - 1 - from;
     const uintptr_t s = (uintptr_t)(of_w ? L.ws : L.xs) + (int64_t)from * blocks;
@@ -311,8 +320,7 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int
     for (int j = 0; j < 4; j++)  // in place of chunks behind the last the step's first, cleared when used
       mx_dma16(values + fk * 64, WHOLE || 4 * fk + chunk[j] < blocks ? src[j] : src[j] - chunk[j] * 16, to + j * 1024);
     filled++;
-    if (++fk == steps) {
-      fk = 0;
+    if (++fk == fstop) {
       ft += run.step;
       if (ft < run.stop) aim();
     }
@@ -348,7 +356,9 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   };
   for (int t = run.first; t < run.stop; t += run.step) {
-    const GemmTile tile = gemm_tile(t, row_tiles, tok_tiles);
+    const int part = PARTS ? __builtin_amdgcn_readfirstlane(t / tiles) : 0;
+    const int from = PARTS ? gemm_part(part, parts, steps) : 0, to_step = PARTS ? gemm_part(part + 1, parts, steps) : steps;
+    const GemmTile tile = gemm_tile(t - part * tiles, row_tiles, tok_tiles);
     const int r0 = tile.r * TILE, b0 = tile.b * TILE;
     // where the scale bytes of this lane's rows start in the fetched pieces
     int oa[4], ob[JT];
@@ -372,10 +382,10 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int
       }
       return __builtin_amdgcn_perm(d[1], d[0], pick) | __builtin_amdgcn_perm(d[3], d[2], pick << 16 | pick >> 16);
     };
-    for (int k = 0; k < steps; k += 4, group++) {
+    for (int k = from; k < to_step; k += 4, group++) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        if (k + e >= steps) break;
+        if (k + e >= to_step) break;
         wait();
         if (e == 0) {
 #pragma unroll
@@ -418,7 +428,7 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int
       u32x4 o[P];
       mx_pack<T>(acc[0][j], acc[1][j], acc[2][j], acc[3][j], o);
       mx_turn<P>(o, c);
-      T* to = (T*)L.y + (int64_t)tok * L.ldy + r;
+      T* to = (T*)L.y + part * plane + (int64_t)tok * L.ldy + r;
 #pragma unroll
       for (int k = 0; k < P; k++)
         if (inner)
@@ -432,12 +442,54 @@ __global__ __launch_bounds__(2 * TILE, 2) void mx_gemm128_kernel(MxMatmul L, int
   }
 }
 
-template <typename T, bool WHOLE, int TILE>
-hipError_t gemm_run_tiles(const MxMatmul& L) {
+// The sums over the parts of the rows, in order: y from the planes, E values a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void mx_parts_kernel(MxMatmul L, const float* sums, int parts, int64_t plane, int ld) {
+  constexpr int E = 16 / sizeof(T);
+  const int each = ld / E;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, tok = i / each;
+  const int r = (int)(i - tok * each) * E;
+  if (tok >= L.batch || r >= L.rows) return;
+  f32x4 y[E / 4];
+#pragma unroll
+  for (int h = 0; h < E / 4; h++) y[h] = *(const f32x4*)(sums + tok * ld + r + 4 * h);
+#pragma unroll 4
+  for (int p = 1; p < parts; p++)
+#pragma unroll
+    for (int h = 0; h < E / 4; h++) y[h] += *(const f32x4*)(sums + p * plane + tok * ld + r + 4 * h);
+  typedef T te __attribute__((ext_vector_type(E)));
+  te o;
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = (T)y[e >> 2][e & 3];
+  mx_some<T>((T*)L.y + tok * L.ldy + r, L.rows - r, __builtin_bit_cast(u32x4, o));
+}
+
+template <typename T, bool WHOLE, int TILE, bool PARTS = false>
+hipError_t gemm_run_tiles(const MxMatmul& L, int parts = 1, int64_t plane = 0) {
   const int rt = (L.rows + TILE - 1) / TILE, tt = (L.batch + TILE - 1) / TILE;
-  const int all = (rt * tt + 7) / 8 * 8, most = 256 * 256 / TILE;  // as many workgroups as the card holds
-  hipLaunchKernelGGL((mx_gemm128_kernel<T, WHOLE, TILE>), dim3(all < most ? all : most), dim3(2 * TILE), 0, L.stream, L, rt, tt);
+  const int all = (rt * tt * parts + 7) / 8 * 8, most = 256 * 256 / TILE;  // as many workgroups as the card holds
+  hipLaunchKernelGGL((mx_gemm128_kernel<T, WHOLE, TILE, PARTS>), dim3(all < most ? all : most), dim3(2 * TILE), 0, L.stream, L, rt, tt, parts, plane);
   return hipGetLastError();
+}
+
+int gemm_ld(int rows) { return (rows + 7) & ~7; }
+
+// Parts of the rows: where tiles of 128 leave workgroups of the card idle, their steps are shared out, eight or more to
+// a part. A step takes a workgroup about 0.42 us; the parts' sums go to memory and back at about 4.5 TB/s, and adding
+// them up is a launch of 3 us. 2560 x 9728 by 64, 128 and 512 tokens takes 15, 18 and 29 us in parts, 34, 38 and 41
+// in whole rows; 9728 x 2560 by 256, for which two parts would take 24, 15 in whole ones.
+int gemm_parts(int rows, int cols, int batch) {
+  if (cols <= 384 || cols > 1 << 26) return 1;
+  const int64_t tiles = (int64_t)((rows + 127) / 128) * ((batch + 127) / 128);
+  const int most = (cols + 127) / 128 / 8;
+  if (tiles > 256 || most < 2) return 1;
+  const int fit = (int)(512 / tiles), top = fit < most ? fit : most;
+  const double whole = 0.42 * ((cols + 127) / 128), plane = (double)rows * batch * 8 / 4.5e6;
+  int parts = 1;
+  double best = whole;
+  for (int p = 2; p <= top; p++)
+    if (whole / p + plane * p + 3.0 < best) best = whole / p + plane * p + 3.0, parts = p;
+  return parts;
 }
 
 // Tiles of 256 where there are columns enough and tiles enough. A round of them (256 tiles) takes 1.7 times as long
@@ -461,11 +513,26 @@ hipError_t gemm_t(const MxMatmul& L) {
     return hipGetLastError();
   }
   const bool whole = L.cols % 512 == 0 && ((uintptr_t)L.ws & 15) == 0 && ((uintptr_t)L.xs & 15) == 0, big = gemm_big(L);
+  const int parts = gemm_parts(L.rows, L.cols, L.batch);
+  if (parts > 1) {
+    MxMatmul S = L;
+    S.y = L.workspace, S.ldy = gemm_ld(L.rows);
+    const int64_t plane = S.ldy * L.batch;
+    if (hipError_t e = whole ? gemm_run_tiles<float, true, 128, true>(S, parts, plane) : gemm_run_tiles<float, false, 128, true>(S, parts, plane)) return e;
+    const int64_t items = plane / (16 / (int)sizeof(T));
+    hipLaunchKernelGGL((mx_parts_kernel<T>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, L.stream, L, (const float*)L.workspace, parts, plane, (int)S.ldy);
+    return hipGetLastError();
+  }
   if (whole) return big ? gemm_run_tiles<T, true, 256>(L) : gemm_run_tiles<T, true, 128>(L);
   return big ? gemm_run_tiles<T, false, 256>(L) : gemm_run_tiles<T, false, 128>(L);
 }
 
 }  // namespace
+
+size_t mx_gemm_workspace(int rows, int cols, int batch) {
+  const int parts = gemm_parts(rows, cols, batch);
+  return parts > 1 ? (size_t)parts * batch * gemm_ld(rows) * sizeof(float) : 0;
+}
 
 // At least two blocks a row (the scale bytes come in pairs).
 hipError_t launch_mx_gemm(const MxMatmul& L) {

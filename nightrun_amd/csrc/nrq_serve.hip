@@ -134,15 +134,21 @@ int mx_check(const char* name, size_t rows, size_t cols) {
   return NRQ_OK;
 }
 
+size_t matmul_bytes(size_t rows, size_t cols, size_t batch) {
+  return nrq::mx_matmul_workspace((int)rows, (int)cols, (int)batch);
+}
+
+// The activation in MXFP4 and what the product needs; few values the product's workgroups quantize for themselves.
+size_t linear_own(size_t cols, size_t batch) { return up16(batch * (cols / 2)) + up16(batch * (cols / 32)); }
 size_t linear_bytes(size_t rows, size_t cols, size_t batch) {
   if (nrq::mx_linear_fits((int)rows, (int)cols, (int)batch)) return 0;
-  return up16(batch * (cols / 2)) + up16(batch * (cols / 32));
+  return linear_own(cols, batch) + matmul_bytes(rows, cols, batch);
 }
 
 int mx_matmul(const char* name, void* y, int dtype, int64_t ldy, const void* w, const void* ws, const void* x,
-              const void* xs, size_t rows, size_t cols, size_t batch, void* stream) {
+              const void* xs, size_t rows, size_t cols, size_t batch, void* workspace, void* stream) {
   nrq::MxMatmul L{y,         dtype,      ldy,        (const uint8_t*)w, (const uint8_t*)ws, (const uint8_t*)x, (const uint8_t*)xs,
-                  (int)rows, (int)cols, (int)batch, (hipStream_t)stream};
+                  (int)rows, (int)cols, (int)batch, (hipStream_t)stream, workspace};
   return launched(name, nrq::launch_mx_matmul(L));
 }
 
@@ -155,6 +161,16 @@ int mx_product_check(const char* name, const void* y, int dtype, int64_t ldy, co
   if (!y || (cols && (!w || !ws))) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(y, bytes_of(dtype)) || !aligned(w, 16)) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
   if (batch > 1 && ldy < (int64_t)rows) return fail(NRQ_ERR_ARG, name, "output rows overlap");
+  return NRQ_OK;
+}
+
+int mx_workspace(const char* name, size_t rows, size_t cols, size_t batch, size_t* bytes,
+                 size_t (*need)(size_t, size_t, size_t)) {
+  if (!bytes) return fail(NRQ_ERR_ARG, name, "null pointer");
+  int rc = mx_check(name, rows, cols);
+  if (rc) return rc;
+  if (batch > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "batch of %zu (at most 2^20)", batch);
+  *bytes = need(rows, cols, batch);
   return NRQ_OK;
 }
 
@@ -316,27 +332,26 @@ int nrq_dev_dequantize_mxfp4(const void* q, const void* scales, size_t rows, siz
   return launched(name, nrq::launch_mx_dequantize(q, scales, rows, cols, dst, dtype, dst_stride, (hipStream_t)stream));
 }
 
+int nrq_matmul_mxfp4_workspace(size_t rows, size_t cols, size_t batch, size_t* bytes) {
+  return mx_workspace("nrq_matmul_mxfp4_workspace", rows, cols, batch, bytes, matmul_bytes);
+}
+
 int nrq_dev_matmul_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, const void* w_scales, const void* x,
-                         const void* x_scales, size_t rows, size_t cols, size_t batch, void* stream) {
+                         const void* x_scales, size_t rows, size_t cols, size_t batch, void* workspace,
+                         size_t workspace_bytes, void* stream) {
   static const char* name = "nrq_dev_matmul_mxfp4";
   int rc;
   if (rows == 0 || batch == 0) return device_check(name, stream);
   if ((rc = mx_product_check(name, y, dtype, y_stride, w, w_scales, rows, cols, batch))) return rc;
   if (cols && (!x || !x_scales)) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(x, 16)) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
+  if ((rc = workspace_check(name, workspace, workspace_bytes, matmul_bytes(rows, cols, batch)))) return rc;
   if ((rc = device_check(name, stream))) return rc;
-  return mx_matmul(name, y, dtype, y_stride, w, w_scales, x, x_scales, rows, cols, batch, stream);
+  return mx_matmul(name, y, dtype, y_stride, w, w_scales, x, x_scales, rows, cols, batch, workspace, stream);
 }
 
 int nrq_linear_mxfp4_workspace(size_t rows, size_t cols, size_t batch, size_t* bytes) {
-  static const char* name = "nrq_linear_mxfp4_workspace";
-  if (!bytes) return fail(NRQ_ERR_ARG, name, "null pointer");
-  int rc = mx_check(name, rows, cols);
-  if (rc) return rc;
-  if (batch > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "batch of %zu (at most 2^20)", batch);
-  // the product's workgroups quantize few values for themselves
-  *bytes = linear_bytes(rows, cols, batch);
-  return NRQ_OK;
+  return mx_workspace("nrq_linear_mxfp4_workspace", rows, cols, batch, bytes, linear_bytes);
 }
 
 int nrq_dev_linear_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, const void* w_scales, const void* x,
@@ -353,13 +368,14 @@ int nrq_dev_linear_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, co
   if ((rc = device_check(name, stream))) return rc;
   if (cols && nrq::mx_linear_fits((int)rows, (int)cols, (int)batch)) {
     nrq::MxMatmul L{y,         dtype,      y_stride,   (const uint8_t*)w, (const uint8_t*)w_scales, nullptr, nullptr,
-                    (int)rows, (int)cols, (int)batch, (hipStream_t)stream};
+                    (int)rows, (int)cols, (int)batch, (hipStream_t)stream, nullptr};
     return launched(name, nrq::launch_mx_linear(L, x, x_dtype, x_stride));
   }
   uint8_t* xs = (uint8_t*)workspace + up16(batch * (cols / 2));
   if (cols && (rc = launched(name, nrq::launch_mx_quantize(x, x_dtype, batch, cols, x_stride, workspace, xs, (hipStream_t)stream))))
     return rc;
-  return mx_matmul(name, y, dtype, y_stride, w, w_scales, workspace, xs, rows, cols, batch, stream);
+  return mx_matmul(name, y, dtype, y_stride, w, w_scales, workspace, xs, rows, cols, batch,
+                   (uint8_t*)workspace + linear_own(cols, batch), stream);
 }
 
 }  // extern "C"

@@ -84,7 +84,10 @@ struct MxMatmul {
   const uint8_t *w, *ws, *x, *xs;
   int rows, cols, batch;
   hipStream_t stream;
+  void* workspace;
 };
+size_t mx_matmul_workspace(int rows, int cols, int batch);
+size_t mx_gemm_workspace(int rows, int cols, int batch);
 hipError_t launch_mx_matmul(const MxMatmul& L);
 bool mx_linear_fits(int rows, int cols, int batch);  // whether launch_mx_linear takes the activation as it is
 hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64_t stride);

@@ -266,7 +266,15 @@ BIND(matmul_mxfp4, 5) {
   const Mx x = mx(tensor(a[3], "x"), tensor(a[4], "x_scales"), "x, x_scales", dev);
   VALUE_CHECK(x.cols == w.cols && (size_t)y.size(0) == x.rows && (size_t)y.size(1) == w.rows, "y ", y.sizes(),
               ": x is [", x.rows, ", ", x.cols, "], w [", w.rows, ", ", w.cols, "]");
-  return nrq_dev_matmul_mxfp4(on(y, "y", dev), kind(y, "y"), y.stride(0), w.q, w.s, x.q, x.s, w.rows, w.cols, x.rows, stream);
+  void* yp = on(y, "y", dev);
+  const int yk = kind(y, "y");
+  size_t need;
+  const int rc = nrq_matmul_mxfp4_workspace(w.rows, w.cols, x.rows, &need);
+  if (rc) return rc;
+  at::Tensor ws;
+  if (need) ws = workspace(need, y);
+  return nrq_dev_matmul_mxfp4(yp, yk, y.stride(0), w.q, w.s, x.q, x.s, w.rows, w.cols, x.rows,
+                              need ? ws.data_ptr() : nullptr, need, stream);
 }
 
 // y, w, w_scales, x

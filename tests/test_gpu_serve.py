@@ -778,6 +778,28 @@ def test_mx_matmul(gpu, kind, batch, rows, cols):
     assert torch.equal(z, y)
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(65, 1, 2048), (70, 131, 9728), (130, 700, 2080), (200, 1000, 3136), (129, 515, 8192),
+                                             (500, 2500, 4096), (80, 8200, 1088), (17, 2561, 5120), (64, 40, 20032)])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_mx_matmul_in_parts(gpu, kind, batch, rows, cols):
+    """Few tiles behind long rows, which several workgroups share: into odd rows and aligned ones, the same bits."""
+    import torch
+
+    from nightrun_amd import serve
+
+    g = gen(batch + rows + cols)
+    w, ws = mx_random(g, rows, cols)
+    x, xs = mx_random(g, batch, cols)
+    wide = torch.full((batch, rows + 6), 3.0, dtype=dt(kind), device="cuda")
+    y, z = wide[:, 1:1 + rows], torch.empty(batch, rows, dtype=dt(kind), device="cuda")
+    args = [t.cuda() for t in (w, ws, x, xs)]
+    serve.matmul_mxfp4(y, *args)
+    check_product(y, unpack(x), xs.numpy(), unpack(w), ws.numpy(), kind)
+    assert torch.all(wide[:, :1] == 3) and torch.all(wide[:, 1 + rows:] == 3)
+    serve.matmul_mxfp4(z, *args)
+    assert torch.equal(z, y)
+
+
 @pytest.mark.parametrize("kind,cols", [("f32", 2080), ("bf16", 2560), ("f16", 4032)])
 def test_mx_matmul_tiles_of_256(gpu, kind, cols):
     """Sizes for which the larger tiles are taken, with rows and tokens that end inside one; odd output rows."""
@@ -794,13 +816,13 @@ def test_mx_matmul_tiles_of_256(gpu, kind, cols):
     serve.matmul_mxfp4(y, w.cuda(), ws.cuda(), x.cuda(), xs.cuda())
     check_product(y, unpack(x), xs.numpy(), unpack(w), ws.numpy(), kind)
     assert torch.all(wide[:, :1] == 3) and torch.all(wide[:, 1 + rows:] == 3)
-    few = torch.empty(20, rows, dtype=dt(kind), device="cuda")  # the same sums in the same order on the smaller ones
-    serve.matmul_mxfp4(few, w.cuda(), ws.cuda(), x[:20].cuda(), xs[:20].cuda())
-    assert torch.equal(few, y[:20])
+    few = torch.empty(520, rows, dtype=dt(kind), device="cuda")  # the same sums in the same order on the smaller ones
+    serve.matmul_mxfp4(few, w.cuda(), ws.cuda(), x[:520].cuda(), xs[:520].cuda())
+    assert torch.equal(few, y[:520])
 
 
 @pytest.mark.parametrize("batch,rows,cols", [(1, 20, 96), (3, 40, 160), (70, 200, 96), (70, 200, 416), (70, 200, 480), (130, 130, 544),
-                                             (70, 300, 2080), (1030, 8201, 2080)])
+                                             (70, 300, 2080), (1030, 8201, 2080), (90, 131, 9728)])
 def test_mx_matmul_nan_rows_stay_alone(gpu, batch, rows, cols):
     """A row of w, or a token, whose scales are all NaN: its outputs are NaN, no other changes."""
     import torch

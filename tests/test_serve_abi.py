@@ -18,7 +18,7 @@ def test_symbols():
     from nightrun_amd import _lib
 
     names = re.findall(r"^int (nrq_\w+)\(", open(HEADER).read(), flags=re.M)
-    assert sorted(names) == sorted(_lib.SERVE_SIGNATURES) and len(names) == 11
+    assert sorted(names) == sorted(_lib.SERVE_SIGNATURES) and len(names) == 12
     L = C.CDLL(_lib.LIB_PATH)
     for n in names:
         assert hasattr(L, n), n
@@ -97,7 +97,8 @@ def _dequant():
 
 
 def _matmul():
-    return dict(y=P, dtype=0, ldy=40, w=P, ws=P, x=P, xs=P, rows=40, cols=64, batch=5, stream=None)
+    return dict(y=P, dtype=0, ldy=40, w=P, ws=P, x=P, xs=P, rows=40, cols=64, batch=5, wk=None, wk_bytes=0,
+                stream=None)
 
 
 def _linear():
@@ -165,6 +166,7 @@ REFUSED = [
     ("nrq_dev_matmul_mxfp4", dict(x=P + 8), ARG, "aligned"),
     ("nrq_dev_matmul_mxfp4", dict(w=None), ARG, "null"),
     ("nrq_dev_matmul_mxfp4", dict(batch=(1 << 20) + 1), UNSUPPORTED, "batch"),
+    ("nrq_dev_matmul_mxfp4", dict(ldy=2560, rows=2560, cols=9728, batch=128), ARG, "workspace"),
     ("nrq_dev_linear_mxfp4", dict(x_dtype=5), ARG, "unknown type"),
     ("nrq_dev_linear_mxfp4", dict(wk_bytes=100), ARG, "workspace"),
     ("nrq_dev_linear_mxfp4", dict(x=None), ARG, "null"),
@@ -208,6 +210,12 @@ def test_workspaces():
     assert L.nrq_linear_mxfp4_workspace(40, 64, 505, C.byref(n)) == 0 and n.value == 505 * 32 + 1024
     assert L.nrq_linear_mxfp4_workspace(40, 64, 5, C.byref(n)) == 0 and n.value == 0  # quantized where it is used
     assert L.nrq_linear_mxfp4_workspace(40, 65, 5, C.byref(n)) == SHAPE
+    assert L.nrq_matmul_mxfp4_workspace(40, 65, 5, C.byref(n)) == SHAPE
+    assert L.nrq_matmul_mxfp4_workspace(40, 64, 5, C.byref(n)) == 0 and n.value == 0
+    # planes of sums where few tiles share long rows
+    assert L.nrq_matmul_mxfp4_workspace(2556, 9728, 128, C.byref(n)) == 0 and n.value % (128 * 2560 * 4) == 0 < n.value
+    planes = n.value
+    assert L.nrq_linear_mxfp4_workspace(2556, 9728, 128, C.byref(n)) == 0 and n.value == planes + 128 * 9728 * 17 // 32
     assert L.nrq_verify_workspace(3, 5000, C.byref(n)) == 0 and 0 < n.value <= 3 * 5000 * 16
     assert L.nrq_paged_attention_workspace(3, 1, 32, _kv(), C.byref(n)) == 0 and n.value >= 4 * 130 * 4
     assert L.nrq_paged_attention_workspace(3, 1, 33, _kv(), C.byref(n)) == SHAPE
