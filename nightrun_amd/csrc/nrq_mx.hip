@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t mx_quantize8(float* f, uint32_t* scale) {
   return r;
 }
 
-constexpr int kMxOwn = 16384;  // values that a product's workgroups quantize for themselves
+constexpr int kMxOwn = 16384;  // values that a workgroup of four waves quantizes for itself
 constexpr int kMxAhead = 2;  // accesses of a thread that are on their way together
 
 // Eight values an access, four lanes a block: cols / 8 is a multiple of four and a workgroup
@@ -170,15 +170,15 @@ __device__ __forceinline__ void mx_store(void* y, int dtype, int64_t at, int n, 
     put4((__bf16*)y, at, n, v);
 }
 
-// Tiles of 16 rows of w by 16 NT tokens. A workgroup's four waves take every
-// fourth step of 128 columns and add up in LDS; it goes from one row tile to another, the next
+// Tiles of 16 rows of w by 16 NT tokens. A workgroup's W waves take every
+// W-th step of 128 columns and add up in LDS; it goes from one row tile to another, the next
 // weights on their way while these are multiplied. With X the activation is not in MXFP4
 // yet but [batch][cols] of X: every workgroup quantizes it once into LDS, behind the loads of its
 // first weights, which saves a launch (for a token or a few: see mx_linear_fits).
-template <int NT, int U, typename X>
-__global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, const X* act, int64_t stride, int wide) {
+template <int NT, int U, int W, typename X>
+__global__ __launch_bounds__(64 * W) void mx_matvec_kernel(MxMatmul L, int tiles, const X* act, int64_t stride, int wide) {
   constexpr bool kOwn = !__is_same(X, void);
-  __shared__ f32x4 part[2][4][NT][64];
+  __shared__ f32x4 part[2][W][NT][64];
   extern __shared__ __align__(16) uint8_t own[];  // with X: [batch][cols / 2], then [batch][cols / 32]
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   const int blocks = L.cols / 32, steps = (blocks + 3) / 4;
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, c
 #pragma unroll
     for (int u = 0; u < U; u++) {
       // blocks behind the last read the last again, no load is conditional; they are cleared when used
-      const int64_t b = r + min(4 * (s0 + 4 * u) + g, blocks - 1);
+      const int64_t b = r + min(4 * (s0 + W * u) + g, blocks - 1);
       a[u] = mx_block(L.w + b * 16, L.ws + b);
     }
   };
@@ -211,11 +211,11 @@ __global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, c
     float f[2][8];
     const int t = threadIdx.x;
     value(min(t, items - 1), f[0]);
-    value(min(t + 256, items - 1), f[1]);
+    value(min(t + 64 * W, items - 1), f[1]);
     load(blockIdx.x, w);
     if (t < items) put(t, f[0]);
-    if (t + 256 < items) put(t + 256, f[1]);
-    for (int k = t + 512; k < items; k += 256) {
+    if (t + 64 * W < items) put(t + 64 * W, f[1]);
+    for (int k = t + 128 * W; k < items; k += 64 * W) {
       value(k, f[0]);
       put(k, f[0]);
     }
@@ -229,17 +229,17 @@ __global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, c
     f32x4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = f32x4{0, 0, 0, 0};
-    for (int s0 = w; s0 < steps; s0 += 4 * U) {
+    for (int s0 = w; s0 < steps; s0 += W * U) {
       MxBlock now[U];
 #pragma unroll
       for (int u = 0; u < U; u++) now[u] = a[u];
-      if (s0 + 4 * U < steps)
-        load(tile, s0 + 4 * U);
+      if (s0 + W * U < steps)
+        load(tile, s0 + W * U);
       else if (tile + (int)gridDim.x < tiles)
         load(tile + gridDim.x, w);
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int b = 4 * (s0 + 4 * u) + g;
+        const int b = 4 * (s0 + W * u) + g;
         const bool none = b >= blocks;
         if (none) now[u] = MxBlock{{0, 0, 0, 0}, 127};
 #pragma unroll
@@ -258,10 +258,12 @@ __global__ __launch_bounds__(256) void mx_matvec_kernel(MxMatmul L, int tiles, c
 #pragma unroll
     for (int t = 0; t < NT; t++) p[w][t][lane] = acc[t];
     __syncthreads();
-    if (w != (round & 3)) continue;
+    if (w != (round & (W - 1))) continue;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const f32x4 y = ((p[0][t][lane] + p[1][t][lane]) + p[2][t][lane]) + p[3][t][lane];
+      f32x4 y = p[0][t][lane];
+#pragma unroll
+      for (int k = 1; k < W; k++) y += p[k][t][lane];
       const int tok = (blockIdx.y * NT + t) * 16 + i, r = tile * 16 + 4 * g;
       if (tok < L.batch && r < L.rows) mx_store(L.y, L.dtype, tok * L.ldy + r, L.rows - r, y);
     }
@@ -275,16 +277,28 @@ inline unsigned mx_matvec_grid(int tiles) {
   return (unsigned)((tiles + rounds - 1) / rounds);
 }
 
+// Eight waves a workgroup, where there are no more workgroups than CUs and rows long enough for them, else four: 2048 x
+// 8192 by one and four tokens takes 6.2 and 10.3 us with eight, 7.3 and 12.1 with four, 2560 x 9728 by one 6.8 and 7.7.
 // Steps of a wave on their way together (U): four or five, whichever divides its steps with less rest (2048 columns
 // are four steps a wave, 2560 five: with five for both, 128256 x 2048 takes 42 us for 38).
-template <typename X>
-void matvec_t(const MxMatmul& L, size_t lds, const X* x, int64_t stride, int wide) {
-  const int tiles = (L.rows + 15) / 16, steps = (L.cols + 511) / 512;
+template <int W, typename X>
+void matvec_w(const MxMatmul& L, size_t lds, const X* x, int64_t stride, int wide) {
+  const int tiles = (L.rows + 15) / 16, steps = (L.cols + 128 * W - 1) / (128 * W);
   const dim3 grid(mx_matvec_grid(tiles));
   if ((steps + 3) / 4 * 4 < (steps + 4) / 5 * 5)
-    hipLaunchKernelGGL((mx_matvec_kernel<1, 4, X>), grid, dim3(256), lds, L.stream, L, tiles, x, stride, wide);
+    hipLaunchKernelGGL((mx_matvec_kernel<1, 4, W, X>), grid, dim3(64 * W), lds, L.stream, L, tiles, x, stride, wide);
   else
-    hipLaunchKernelGGL((mx_matvec_kernel<1, 5, X>), grid, dim3(256), lds, L.stream, L, tiles, x, stride, wide);
+    hipLaunchKernelGGL((mx_matvec_kernel<1, 5, W, X>), grid, dim3(64 * W), lds, L.stream, L, tiles, x, stride, wide);
+}
+
+inline bool mx_wide(int rows, int cols) { return rows <= 16 * 256 && cols >= 4096; }
+
+template <typename X>
+void matvec_t(const MxMatmul& L, size_t lds, const X* x, int64_t stride, int wide) {
+  if (mx_wide(L.rows, L.cols))
+    matvec_w<8>(L, lds, x, stride, wide);
+  else
+    matvec_w<4>(L, lds, x, stride, wide);
 }
 
 template <typename T>
@@ -351,11 +365,11 @@ static bool mx_wants_gemm(int rows, int cols, int batch) {
   return cols >= 64 && (batch > 64 || (batch > 16 && (rows >= 8192 || cols >= 4096)) || (batch > 3 && rows >= 32768));
 }
 
-// A token or a few are quantized by every workgroup of the product, up to 16384 values: 9728 x 2560 by one, four,
-// eight tokens takes 6.3, 7.7, 10.1 us so and 9.7, 10.2, 10.1 in two launches, 2560 x 9728 by one and two 8.2, 10.8 and
-// 10.1, 10.1.
+// A token or a few are quantized by every workgroup of the product, up to 16384 values, twice as many by one of eight
+// waves: 9728 x 2560 by one, four, eight tokens takes 6.3, 7.7, 10.1 us so and 9.7, 10.2, 10.1 in two launches, 4096 x 4096
+// by eight and twelve 7.3, 9.3 and 9.8, 10.0, 2048 x 8192 by four and eight 10.0, 13.9 and 10.4, 10.7.
 bool mx_linear_fits(int rows, int cols, int batch) {
-  return batch <= 16 && (int64_t)cols * batch <= kMxOwn && !mx_wants_gemm(rows, cols, batch);
+  return batch <= 16 && (int64_t)cols * batch <= (mx_wide(rows, cols) ? 2 * kMxOwn : kMxOwn) && !mx_wants_gemm(rows, cols, batch);
 }
 
 hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64_t stride) {
@@ -378,7 +392,7 @@ hipError_t launch_mx_matmul(const MxMatmul& L) {
   if (tokens == 1)
     matvec_t<void>(L, 0, nullptr, 0, 0);
   else
-    hipLaunchKernelGGL((mx_matvec_kernel<4, 2, void>), dim3(mx_matvec_grid(tiles), (tokens + 3) / 4), dim3(256), 0,
+    hipLaunchKernelGGL((mx_matvec_kernel<4, 2, 4, void>), dim3(mx_matvec_grid(tiles), (tokens + 3) / 4), dim3(256), 0,
                        L.stream, L, tiles, (const void*)nullptr, (int64_t)0, 0);
   return hipGetLastError();
 }
