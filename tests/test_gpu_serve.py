@@ -800,6 +800,39 @@ def test_mx_matmul_in_parts(gpu, kind, batch, rows, cols):
     assert torch.equal(z, y)
 
 
+def test_mx_parts_in_graphs_on_two_streams(gpu):
+    """Products whose sums go through a workspace, captured, replayed at once: each has its own."""
+    import torch
+
+    from nightrun_amd import serve
+
+    sizes = [(70, 2560, 9728), (130, 700, 8192)]
+    calls = []
+    for batch, rows, cols in sizes:
+        g = gen(rows)
+        w, ws = (t.cuda() for t in mx_random(g, rows, cols))
+        x = torch.randn(batch, cols, generator=g).cuda()
+        y = torch.empty(batch, rows, device="cuda")
+        serve.linear_mxfp4(y, w, ws, x)
+        graph = torch.cuda.CUDAGraph()
+        want = y.clone()
+        with torch.cuda.graph(graph):
+            serve.linear_mxfp4(y, w, ws, x)
+        calls.append((graph, y, want, (w, ws, x), torch.cuda.Stream()))
+    for _ in range(4):
+        for _, y, *_ in calls:
+            y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for graph, *_, stream in calls:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        (w, ws, x) = calls[0][3]
+        z = torch.empty_like(calls[0][1])
+        serve.linear_mxfp4(z, w, ws, x)  # eager work beside them
+        torch.cuda.synchronize()
+        assert torch.equal(z, calls[0][2]) and all(torch.equal(y, want) for _, y, want, *_ in calls)
+
+
 @pytest.mark.parametrize("kind,cols", [("f32", 2080), ("bf16", 2560), ("f16", 4032)])
 def test_mx_matmul_tiles_of_256(gpu, kind, cols):
     """Sizes for which the larger tiles are taken, with rows and tokens that end inside one; odd output rows."""
