@@ -539,7 +539,7 @@ __global__ __attribute__((aligned(kDecodeEntry))) __launch_bounds__(NT) void att
       const int t = min(c * C + tl, n - 1);
       const uint32_t dst = __builtin_amdgcn_readfirstlane(
           (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint4*)(vring + (size_t)slot * npc + wbase));
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(vc + kvi(t, i0)) : "memory");
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(vc + kvi(t, i0)) : "memory");
     }
   };
   // this wave's DMAs for the older of its two outstanding chunks are done

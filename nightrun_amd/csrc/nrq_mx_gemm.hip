@@ -34,12 +34,12 @@ __device__ const uint32_t mx_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0
 
 // 16 bytes a lane from memory to LDS, lane after lane from byte address m0 (wave-uniform)
 __device__ __forceinline__ void mx_dma16(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
 }
 
 // the same from `at` bytes behind a wave-uniform address
 __device__ __forceinline__ void mx_dma16(const uint8_t* g, uint32_t at, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m0), "v"(at), "s"(g) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(m0), "v"(at), "s"(g) : "memory");
 }
 
 template <int S>

@@ -27,11 +27,11 @@ namespace nrq {
 namespace {
 
 __device__ __forceinline__ void ws_dma4(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(m0), "v"(g) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(m0), "v"(g) : "memory");
 }
 
 __device__ __forceinline__ void ws_dma16(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
 }
 
 template <int N>
@@ -350,7 +350,7 @@ static_assert(kWgChainWork <= 256, "the workspace fits the smallest add array");
 __host__ __device__ inline size_t ws_norm_floats(int n) { return 3 * (size_t)n; }
 
 __device__ __forceinline__ void ws_dma16_g(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
 }
 
 // The fused Q8_0 kernels start on 4 KB boundaries (kDecodeEntry, nrq_device.h); the others
