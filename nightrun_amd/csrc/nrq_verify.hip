@@ -121,8 +121,9 @@ __global__ __launch_bounds__(kVerNT) void verify_sums_kernel(VerArgs A) {
   }
 }
 
-// Sums over the workgroup's threads up to and before each; one thread's `upto` is the next one's
-// `before` to the bit, so that exactly one thread holds a point between them.
+// Sums over the workgroup's threads up to and before each. The lanes add in different orders, so that the sums need
+// not grow with the thread to the last bit, not even behind the last weight: more than one thread may find a point
+// between its two. Who draws is the first thread with weight whose `upto` is above the point, and that one alone.
 struct VerSum {
   double before, upto, total;
 };
@@ -146,9 +147,21 @@ __device__ __forceinline__ VerSum ver_scan(double own, double* lds) {
   return VerSum{before + y, before + x, all};
 }
 
+// The workgroup's first thread for which `on` holds, kVerNT if there is none.
+__device__ __forceinline__ int ver_first(bool on, int* lds) {
+  const int w = threadIdx.x >> 6;
+  const unsigned long long m = __ballot(on);
+  if ((threadIdx.x & 63) == 0) lds[w] = m ? 64 * w + __ffsll(m) - 1 : kVerNT;
+  __syncthreads();
+  int t = kVerNT;
+#pragma unroll
+  for (int i = 0; i < kVerNT / 64; i++) t = min(t, lds[i]);
+  return t;
+}
+
 __global__ __launch_bounds__(kVerNT) void verify_draw_kernel(VerArgs A) {
   __shared__ double lds[3][kVerNT / 64], base;
-  __shared__ int found, last[2], drawn;
+  __shared__ int first[2][kVerNT / 64], found, last[2], drawn;
   const VerifyLaunch& L = A.L;
   const int b = blockIdx.x, t = threadIdx.x;
   double* sums = A.sums + (int64_t)b * A.spans;
@@ -178,18 +191,21 @@ __global__ __launch_bounds__(kVerNT) void verify_draw_kernel(VerArgs A) {
     }
     c = ver_scan(own, lds[1]);
   }
-  // the first span whose cumulative sum is above the point
-  const double point = u * c.total;
-  if (c.before <= point && c.upto > point) {
+  // the first span with weight whose cumulative sum is above the point; a uniform of 1 has none (its product with
+  // the sum may be an ulp below what another lane's order gives)
+  const double point = u < 1.0 ? u * c.total : INFINITY;
+  if (t == ver_first(own > 0.0 && c.upto > point, first[0])) {
     double before = c.before;
-    int i = s0;
-    for (; i + 1 < s1; i++) {
+    int at = -1;
+    for (int i = s0; i < s1; i++) {
       const double s = sums[i];
+      if (!(s > 0.0)) continue;
+      at = i;
+      base = before;
       if (before + s > point) break;
       before += s;
     }
-    found = i;
-    base = before;
+    found = at;  // where rounding leaves the point behind the run, its last span with weight
   }
   __syncthreads();
   int span = found;
@@ -217,7 +233,7 @@ __global__ __launch_bounds__(kVerNT) void verify_draw_kernel(VerArgs A) {
 #pragma unroll
     for (int i = 0; i < kVerPer; i++)
       if (w[i] > 0.0) lastw = v0 + i;
-    if (e.before <= point1 && e.upto > point1) {
+    if (t == ver_first(s > 0.0 && e.upto > point1, first[1])) {
       double at = e.before;
       int v = -1;
 #pragma unroll

@@ -1153,3 +1153,52 @@ def test_serving_step_on_a_stream(gpu):
     s.run(stream=st)
     st.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(s.results(), want))
+
+
+# ---- draws at the end of the sum and at its borders ---------------------------------------------------
+
+
+@pytest.mark.parametrize("vocab,rows", [(32000, 300), (50257, 300), (151936, 200), (300001, 80)])
+def test_verify_draw_of_1_takes_the_last_weight(gpu, vocab, rows):
+    """Dense rows, whose sums round: a last uniform of 1 has no cumulative sum above it in any order of adding up."""
+    import torch
+
+    from nightrun_amd import serve
+
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    t = torch.softmax(2.5 * torch.randn(rows, 1, vocab, device="cuda", generator=g), -1)
+    t[::3, 0, -vocab // 3:] = 0.0  # whole spans without weight at the end
+    u = torch.full((rows, 1), 1.0, device="cuda")
+    u[1::5] = 1.5
+    tokens, accepted = (torch.full(n, 99, dtype=torch.int32, device="cuda") for n in ((rows, 1), (rows,)))
+    serve.verify_drafts(tokens, accepted, t, None, torch.zeros(rows, 0, dtype=torch.int32, device="cuda"), u)
+    v = torch.arange(vocab, device="cuda")
+    assert torch.equal(tokens[:, 0].long(), torch.where(t[:, 0] > 0, v, -1).amax(1))
+
+
+@pytest.mark.parametrize("vocab,some", [(32000, None), (151936, None), (600001, None), (600001, 40), (262145, 3), (5000, 7)])
+def test_verify_draws_lie_between_their_sums(gpu, vocab, some):
+    """Any uniform: the token drawn has weight, and the point lies between the sums before and through it, within the
+    rounding of three sums (the point's, theirs, the definition's) of up to 2^20 terms in 64 bits, each off by at most 2^20 * 2^-53 of the
+    whole. Rows of `some` tokens only have most of their spans empty."""
+    import torch
+
+    from nightrun_amd import serve
+
+    rows = 64
+    g = torch.Generator(device="cuda").manual_seed(vocab + (some or 0))
+    t = torch.softmax(2.5 * torch.randn(rows, 1, vocab, device="cuda", generator=g), -1)
+    if some:
+        keep = torch.zeros(rows, 1, vocab, device="cuda")
+        keep.scatter_(2, torch.randint(0, vocab, (rows, 1, some), device="cuda", generator=g), 1.0)
+        t = t * keep
+    u = torch.rand(rows, 1, device="cuda", generator=g)
+    u[:6, 0] = torch.tensor([0.0, 2.0 ** -149, 2.0 ** -24, 1 - 2.0 ** -24, 1 - 2.0 ** -23, 0.5])
+    tokens, accepted = (torch.full(n, 99, dtype=torch.int32, device="cuda") for n in ((rows, 1), (rows,)))
+    serve.verify_drafts(tokens, accepted, t, None, torch.zeros(rows, 0, dtype=torch.int32, device="cuda"), u)
+    p = f64(t)[:, 0]
+    c = np.cumsum(p, 1)
+    at, i = tokens[:, 0].cpu().numpy(), np.arange(rows)
+    assert np.all(at >= 0) and np.all(p[i, at] > 0)
+    point, slack = f64(u)[:, 0] * c[:, -1], 3 * 2.0 ** -33 * c[:, -1]
+    assert np.all(c[i, at] > point - slack) and np.all(c[i, at] - p[i, at] <= point + slack)
