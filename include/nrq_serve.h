@@ -140,7 +140,8 @@ int nrq_dev_verify_drafts(int32_t *tokens, int32_t *accepted, const float *targe
  * HIP allocation). s - 127 = floor(log2(largest magnitude)) - 2,
  * at least -127 (also for zeros); values to the nearest of those (ties to the even
  * code), at most 6. A block with an infinity or a NaN is s = 255 (NaN
- * throughout) with zeros. */
+ * throughout) with zeros. Here and in the functions below an output that shares memory with
+ * an input or another output is refused; columns of one matrix do not. */
 int nrq_dev_quantize_mxfp4(const void *src, int dtype, size_t rows, size_t cols, int64_t src_stride, void *q,
                            void *scales, void *stream);
 /* The values of such blocks, rounded to `dtype`; dst rows dst_stride apart. */

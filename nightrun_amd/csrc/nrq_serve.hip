@@ -10,6 +10,7 @@
 #include "../../include/nrq.h"
 #include "../../include/nrq_serve.h"
 #include "nrq_launch.h"
+#include "nrq_rows.h"
 #include "nrq_serve_launch.h"
 
 namespace {
@@ -164,6 +165,23 @@ int mx_product_check(const char* name, const void* y, int dtype, int64_t ldy, co
   return NRQ_OK;
 }
 
+// What a call of the MXFP4 functions writes shares no byte with what it reads or with another output: workgroups
+// read while others write. Asked last, where the memory is known to be the device's.
+nrq::Rows strided(const void* p, size_t n, int64_t stride, size_t cols, int dtype) {
+  return nrq::Rows{p, n, stride, cols, (int)bytes_of(dtype)};
+}
+nrq::Rows packed(const void* q, size_t rows, size_t cols) { return nrq::Rows{q, 1, 0, rows * (cols / 2)}; }
+nrq::Rows packed_scales(const void* s, size_t rows, size_t cols) { return nrq::Rows{s, 1, 0, rows * (cols / 32)}; }
+int apart_check(const char* name, std::initializer_list<nrq::Rows> out, std::initializer_list<nrq::Rows> in) {
+  for (const nrq::Rows* o = out.begin(); o != out.end(); o++) {
+    for (const nrq::Rows& i : in)
+      if (nrq::rows_meet(*o, i)) return fail(NRQ_ERR_ARG, name, "output and input overlap");
+    for (const nrq::Rows* p = o + 1; p != out.end(); p++)
+      if (nrq::rows_meet(*o, *p)) return fail(NRQ_ERR_ARG, name, "outputs overlap");
+  }
+  return NRQ_OK;
+}
+
 int mx_workspace(const char* name, size_t rows, size_t cols, size_t batch, size_t* bytes,
                  size_t (*need)(size_t, size_t, size_t)) {
   if (!bytes) return fail(NRQ_ERR_ARG, name, "null pointer");
@@ -315,6 +333,9 @@ int nrq_dev_quantize_mxfp4(const void* src, int dtype, size_t rows, size_t cols,
   if (!src || !q || !scales) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(src, bytes_of(dtype)) || !aligned(q, 16)) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
   if ((rc = device_check(name, stream))) return rc;
+  if ((rc = apart_check(name, {packed(q, rows, cols), packed_scales(scales, rows, cols)},
+                        {strided(src, rows, src_stride, cols, dtype)})))
+    return rc;
   return launched(name, nrq::launch_mx_quantize(src, dtype, rows, cols, src_stride, q, scales, (hipStream_t)stream));
 }
 
@@ -329,6 +350,9 @@ int nrq_dev_dequantize_mxfp4(const void* q, const void* scales, size_t rows, siz
   if (!aligned(dst, bytes_of(dtype)) || !aligned(q, 16)) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
   if (rows > 1 && dst_stride < (int64_t)cols) return fail(NRQ_ERR_ARG, name, "output rows overlap");
   if ((rc = device_check(name, stream))) return rc;
+  if ((rc = apart_check(name, {strided(dst, rows, dst_stride, cols, dtype)},
+                        {packed(q, rows, cols), packed_scales(scales, rows, cols)})))
+    return rc;
   return launched(name, nrq::launch_mx_dequantize(q, scales, rows, cols, dst, dtype, dst_stride, (hipStream_t)stream));
 }
 
@@ -347,6 +371,10 @@ int nrq_dev_matmul_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, co
   if (!aligned(x, 16)) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
   if ((rc = workspace_check(name, workspace, workspace_bytes, matmul_bytes(rows, cols, batch)))) return rc;
   if ((rc = device_check(name, stream))) return rc;
+  if ((rc = apart_check(name, {strided(y, batch, y_stride, rows, dtype)},
+                        {packed(w, rows, cols), packed_scales(w_scales, rows, cols), packed(x, batch, cols),
+                         packed_scales(x_scales, batch, cols)})))
+    return rc;
   return mx_matmul(name, y, dtype, y_stride, w, w_scales, x, x_scales, rows, cols, batch, workspace, stream);
 }
 
@@ -366,6 +394,10 @@ int nrq_dev_linear_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, co
   if (!aligned(x, bytes_of(x_dtype))) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
   if ((rc = workspace_check(name, workspace, workspace_bytes, linear_bytes(rows, cols, batch)))) return rc;
   if ((rc = device_check(name, stream))) return rc;
+  if ((rc = apart_check(name, {strided(y, batch, y_stride, rows, dtype)},
+                        {packed(w, rows, cols), packed_scales(w_scales, rows, cols),
+                         strided(x, batch, x_stride, cols, x_dtype)})))
+    return rc;
   if (cols && nrq::mx_linear_fits((int)rows, (int)cols, (int)batch)) {
     nrq::MxMatmul L{y,         dtype,      y_stride,   (const uint8_t*)w, (const uint8_t*)w_scales, nullptr, nullptr,
                     (int)rows, (int)cols, (int)batch, (hipStream_t)stream, nullptr};

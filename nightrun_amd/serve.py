@@ -10,7 +10,9 @@ on `stream` (default: torch's current stream) and may be captured into a graph; 
 workspace comes from torch's allocator on that stream, so captured graphs and
 streams never share one. Tensors live on the library's device, which is the
 current one. Wrong types, shapes, layouts or devices raise ValueError before anything
-is launched, shapes that the library refuses NrPanic, anything else it refuses NrqError.
+is launched, shapes that the library refuses NrPanic, anything else it refuses NrqError: an output of
+the MXFP4 functions that shares memory with an input, for one. rope() and rope_append() may run in place (y is x or q, with
+the same strides); no other output may overlap an input.
 """
 from __future__ import annotations
 

@@ -1202,3 +1202,48 @@ def test_verify_draws_lie_between_their_sums(gpu, vocab, some):
     assert np.all(at >= 0) and np.all(p[i, at] > 0)
     point, slack = f64(u)[:, 0] * c[:, -1], 3 * 2.0 ** -33 * c[:, -1]
     assert np.all(c[i, at] > point - slack) and np.all(c[i, at] - p[i, at] <= point + slack)
+
+
+# ---- outputs over inputs ------------------------------------------------------------------------------
+
+
+def test_mx_outputs_over_inputs_are_refused(gpu):
+    """Workgroups read what others have written by then. Columns of one matrix beside each other are no overlap."""
+    import torch
+
+    from nightrun_amd import NrqError, serve
+
+    def f16(t, rows, cols):  # the first bytes of t as another matrix
+        return t.view(-1).view(torch.uint8)[:rows * cols * 2].view(torch.float16).view(rows, cols)
+
+    g = gen(11)
+    n = 512
+    w, ws = (t.cuda() for t in mx_random(g, n, n))
+    kept = w.clone()
+    for batch in (1, 5, 70):  # in one launch, in two
+        both = normal(g, batch, 2 * n)
+        x, y = both[:, :n], both[:, n:]
+        before = both.clone()
+        for out in (x, both[:, n // 2:n // 2 + n], both[:, n - 1:2 * n - 1], f16(both, batch, n), f16(w, 1, n).expand(batch, n)):
+            if out.stride(0) == 0 and batch > 1:
+                continue
+            with pytest.raises(NrqError, match="overlap"):
+                serve.linear_mxfp4(out, w, ws, x)
+        assert torch.equal(both, before) and torch.equal(w, kept)
+        serve.linear_mxfp4(y, w, ws, x)
+        alone = torch.empty(batch, n, device="cuda")
+        serve.linear_mxfp4(alone, w, ws, x.contiguous())
+        assert torch.equal(y, alone) and torch.equal(x, before[:, :n])
+    x, xs = (t.cuda() for t in mx_random(g, 3, n))
+    for t in (w, ws, x, xs):
+        with pytest.raises(NrqError, match="overlap"):
+            serve.matmul_mxfp4(f16(t, 3, 8), w[:8], ws[:8], x, xs)
+    src, s = normal(g, 8, n), torch.empty(8, n // 32, dtype=torch.uint8, device="cuda")
+    q = torch.empty(8, n // 2, dtype=torch.uint8, device="cuda")
+    for out, scales in ((src.view(torch.uint8).view(-1)[:q.numel()].view(q.shape), s), (q, q.view(-1)[:s.numel()].view(s.shape))):
+        with pytest.raises(NrqError, match="overlap"):
+            serve.quantize_mxfp4(src, out, scales)
+    serve.quantize_mxfp4(src, q, s)
+    for t in (q, s):
+        with pytest.raises(NrqError, match="overlap"):
+            serve.dequantize_mxfp4(q[:1, :32], s[:1, :2], f16(t, 1, 64))
