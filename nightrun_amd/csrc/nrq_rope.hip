@@ -189,16 +189,23 @@ hipError_t launch_t(const RopeLaunch& L) {
   // be full; with few tokens their rows are spread over more workgroups, an access a thread in each.
   int t = kRopeNT / L.nf;
   t = t < 1 ? 1 : (t > kRopeTokens ? kRopeTokens : t);
-  if (t > (L.tokens + 2047) / 2048) t = (L.tokens + 2047) / 2048;
+  if (t > (L.tokens - 1) / 2048 + 1) t = (L.tokens - 1) / 2048 + 1;
   const int64_t work = (int64_t)t * (L.heads + (APPEND ? 2 * L.kv.n_kv : 0)) * L.hd;
-  const int tw = (L.tokens + t - 1) / t;
+  const int tw = (L.tokens - 1) / t + 1;
   int64_t gy = tw >= 512 ? 1 : (512 + tw - 1) / tw;
   if (gy * kRopeNT * V > work) gy = work < kRopeNT * V ? 1 : work / (kRopeNT * V);
-  const dim3 grid(tw, (unsigned)gy);
-  if (wide)
-    hipLaunchKernelGGL((rope_kernel<T, C, V, APPEND>), grid, dim3(kRopeNT), 0, L.stream, L, t);
-  else
-    hipLaunchKernelGGL((rope_kernel<T, C, 1, APPEND>), grid, dim3(kRopeNT), 0, L.stream, L, t);
+  const int64_t most = (int64_t)t << 23;  // tokens of a launch: a grid has fewer than 2^32 threads
+  for (int64_t t0 = 0; t0 < L.tokens; t0 += most) {
+    RopeLaunch P = L;
+    P.tokens = (int)(L.tokens - t0 < most ? L.tokens - t0 : most);
+    P.x = (const T*)L.x + t0 * L.xt, P.y = (T*)L.y + t0 * L.yt, P.pos = L.pos + t0;
+    if (APPEND) P.k = (const T*)L.k + t0 * L.kt, P.v = (const T*)L.v + t0 * L.vt, P.seq = L.seq + t0;
+    const dim3 grid((P.tokens - 1) / t + 1, (unsigned)gy);
+    if (wide)
+      hipLaunchKernelGGL((rope_kernel<T, C, V, APPEND>), grid, dim3(kRopeNT), 0, L.stream, P, t);
+    else
+      hipLaunchKernelGGL((rope_kernel<T, C, 1, APPEND>), grid, dim3(kRopeNT), 0, L.stream, P, t);
+  }
   return hipGetLastError();
 }
 

@@ -1247,3 +1247,43 @@ def test_mx_outputs_over_inputs_are_refused(gpu):
     for t in (q, s):
         with pytest.raises(NrqError, match="overlap"):
             serve.dequantize_mxfp4(q[:1, :32], s[:1, :2], f16(t, 1, 64))
+
+
+# ---- sizes past one launch ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("append", [False, True])
+def test_rope_more_tokens_than_a_grid_has_threads_for(gpu, append):
+    """2^31 - 1 tokens (the most) of one head of two, of which a launch takes at most 64 * 2^23: all tokens share one
+    input row; the positions run through a page of outputs that are checked at the launches' borders and at random."""
+    import torch
+
+    from nightrun_amd import serve
+
+    n, span = 2 ** 31 - 1, 1 << 20
+    x = torch.tensor([[[1.0, 0.5]]], dtype=torch.float16, device="cuda").expand(n, 1, 2)
+    y = torch.full((n, 1, 2), 9.0, dtype=torch.float16, device="cuda")
+    pos = torch.arange(span, dtype=torch.int32, device="cuda").repeat(n // span + 1)[:n]
+    f = torch.tensor([0.25], device="cuda")
+    if append:
+        seq = torch.full((n,), -1, dtype=torch.int32, device="cuda")  # padding but for two, which lie in two launches
+        at = torch.tensor([5, n - 1], device="cuda")
+        seq[at] = 0
+        table = torch.arange(span // 2 ** 14, dtype=torch.int32, device="cuda").view(1, -1)
+        kp, vp = (torch.zeros(span // 2 ** 14, 1, 2 ** 14, 8, dtype=torch.float16, device="cuda")[..., :2] for _ in range(2))
+        serve.rope_append(y, x, x, x, pos, seq, f, kp, vp, table)
+    else:
+        at = torch.cat([torch.tensor([0, 1, n - 1]), torch.arange(1, 4) * 2 ** 29, torch.arange(1, 4) * 2 ** 29 - 1,
+                        torch.randint(0, n, (100000,), generator=gen(3))]).cuda()
+        serve.rope(y, x, pos, f)
+        assert int((y[:, 0, 0] == 9).sum()) == 0
+    p = pos[at].double().cpu().numpy()
+    want, m = turn(np.tile([[[1.0, 0.5]]], (len(p), 1, 1)), p, [0.25], False, 1.0)
+    tol = rope_tolerance(want, m, "f16", span)
+    assert np.all(np.abs(f64(y[at]) - want) <= tol)
+    if append:
+        assert bool((y[6:n - 1] == 9).all())
+        got = f64(kp)[:, 0].reshape(-1, 2)[p.astype(int)]
+        assert np.all(np.abs(got - want[:, 0]) <= tol[:, 0])
+        assert np.array_equal(f64(vp)[:, 0].reshape(-1, 2)[p.astype(int)], np.tile([1.0, 0.5], (2, 1)))
+        assert int((vp != 0).any(-1).sum()) == 2
