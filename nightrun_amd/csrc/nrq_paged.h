@@ -35,7 +35,7 @@
 namespace nrq {
 
 constexpr int kPaNT = 256;        // threads: four waves
-constexpr int kTile = 128;        // positions of a tile, 32 a wave
+constexpr int kTile = kPagedTile;  // positions of a tile, 32 a wave
 constexpr int kPaMaxWgs = 768;
 constexpr float kLog2e = 1.44269504088896341f;
 

@@ -5,8 +5,13 @@ namespace nrq {
 
 hipError_t launch_paged_bf16(const PagedAttnLaunch& L);
 
+size_t paged_attn_units(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd) {
+  const size_t rows = n_new * (heads / n_kv), per = pa_per(hd, rows);
+  return seqs * n_kv * ((rows + per - 1) / per);
+}
+
 size_t paged_attn_workspace(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd) {
-  const size_t rows = n_new * (heads / n_kv), per = pa_per(hd, rows), units = seqs * n_kv * ((rows + per - 1) / per);
+  const size_t rows = n_new * (heads / n_kv), per = pa_per(hd, rows), units = paged_attn_units(seqs, n_new, heads, n_kv, hd);
   return 2 * (size_t)kPaMaxWgs * (rows < per ? rows : per) * ((size_t)hd * sizeof(float) + sizeof(float2)) + 16 +
          units * sizeof(int4);
 }

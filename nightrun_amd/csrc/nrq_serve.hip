@@ -276,6 +276,11 @@ int nrq_dev_paged_attention(void* out, const void* q, int dtype, size_t n_new, s
   if ((double)table->seqs * (double)(n_new * heads) * ((double)held / 128 + 1) >= 2147483647.0)
     return fail(NRQ_ERR_UNSUPPORTED, name, "%d sequences of %d pages of %d: too much work for a call", table->seqs,
                 table->width, kv->page_size);
+  // the join takes a workgroup of 256 threads for each unit, and a grid has fewer than 2^32 of them
+  if (nrq::paged_attn_units((size_t)table->seqs, n_new, heads, kv->n_kv_heads, kv->head_dim) >= (size_t)1 << 24 &&
+      held > nrq::kPagedTile)
+    return fail(NRQ_ERR_UNSUPPORTED, name, "%d sequences of %zu rows of %zu heads: too much work for a call", table->seqs,
+                n_new, heads);
   const size_t e = bytes_of(dtype);
   if (!aligned(out, e) || !aligned(q, e) || !aligned(lens, 4) || !aligned(counts, 4) || !aligned(lse, 4))
     return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");

@@ -56,6 +56,8 @@ struct PagedAttnLaunch {
   void* workspace;
   hipStream_t stream;
 };
+constexpr int kPagedTile = 128;  // positions of a tile; where a sequence holds no more there is no join
+size_t paged_attn_units(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd);
 size_t paged_attn_workspace(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd);
 hipError_t launch_paged_attn(const PagedAttnLaunch& L);
 

@@ -297,3 +297,19 @@ def test_line(page, total, wgs):
     for g in some:
         w = page.owner(g, total, wgs)
         assert 0 <= w < wgs and starts[w] <= g < starts[w + 1], (g, w)
+
+
+# ---- sizes that no launch takes ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("seqs,width,fits", [(2 ** 21, 9, False), (2 ** 21 - 1, 9, True), (2 ** 21, 8, True), (2 ** 23, 8, True)])
+def test_attention_units(seqs, width, fits):
+    """Eight units a sequence; 2^24 need a grid of 2^32 threads where sequences hold more than a tile of 128."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("checks the no-GPU failure path")
+    rc, msg = _call("nrq_dev_paged_attention", _attend(), n_new=1, ws_bytes=1 << 40, strides=_i64(8192, 4096, 128, 4096, 4096, 128),
+                    table=_table(seqs=seqs, width=width, stride=width))
+    assert rc == (NOT_INIT if fits else UNSUPPORTED), (rc, msg)
+    assert fits or "too much" in msg
