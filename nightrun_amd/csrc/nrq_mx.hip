@@ -335,6 +335,9 @@ void linear_t(const MxMatmul& L, const void* x, int64_t stride) {
 
 }  // namespace
 
+// Grids of fewer than 2^24 workgroups of 256 threads: a launch takes fewer than 2^32 threads.
+bool mx_quantize_fits(size_t rows, size_t cols) { return (double)rows * (double)(cols / 8) <= 256.0 * kMxAhead * 16777215.0; }
+
 hipError_t launch_mx_quantize(const void* src, int dtype, size_t rows, size_t cols, int64_t stride, void* q, void* s,
                               hipStream_t st) {
   if (dtype == kF32)
@@ -381,6 +384,8 @@ hipError_t launch_mx_linear(const MxMatmul& L, const void* x, int x_dtype, int64
     linear_t<__bf16>(L, x, stride);
   return hipGetLastError();
 }
+
+bool mx_matmul_fits(int rows, int cols, int batch) { return !mx_wants_gemm(rows, cols, batch) || mx_gemm_fits(rows, cols, batch); }
 
 size_t mx_matmul_workspace(int rows, int cols, int batch) {
   return mx_wants_gemm(rows, cols, batch) ? mx_gemm_workspace(rows, cols, batch) : 0;

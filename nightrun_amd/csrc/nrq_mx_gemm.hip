@@ -529,6 +529,11 @@ hipError_t gemm_t(const MxMatmul& L) {
 
 }  // namespace
 
+// The kernel of few columns takes a workgroup of 256 threads for each tile, of which a launch takes fewer than 2^24.
+bool mx_gemm_fits(int rows, int cols, int batch) {
+  return (cols > 384 && cols <= 1 << 26) || (int64_t)((rows + 127) / 128) * ((batch + 127) / 128) <= (1 << 24) - 8;
+}
+
 size_t mx_gemm_workspace(int rows, int cols, int batch) {
   const int parts = gemm_parts(rows, cols, batch);
   return parts > 1 ? (size_t)parts * batch * gemm_ld(rows) * sizeof(float) : 0;

@@ -131,8 +131,16 @@ bool paged_hd(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || 
 
 int mx_check(const char* name, size_t rows, size_t cols) {
   if (cols % 32) return fail(NRQ_ERR_SHAPE, name, "%zu columns are not a multiple of 32", cols);
-  if (rows > INT_MAX || cols > INT_MAX - 1024) return fail(NRQ_ERR_UNSUPPORTED, name, "dimension exceeds 2^31");
+  // both are rounded up to tiles in 32 bits
+  if (rows > INT_MAX - 1024 || cols > INT_MAX - 1024) return fail(NRQ_ERR_UNSUPPORTED, name, "dimension exceeds 2^31");
   return NRQ_OK;
+}
+
+int mx_quant_check(const char* name, size_t rows, size_t cols) {
+  int rc = mx_check(name, rows, cols);
+  if (!rc && !nrq::mx_quantize_fits(rows, cols))
+    return fail(NRQ_ERR_UNSUPPORTED, name, "%zu rows of %zu columns: more than 2^36 values", rows, cols);
+  return rc;
 }
 
 size_t matmul_bytes(size_t rows, size_t cols, size_t batch) {
@@ -159,6 +167,8 @@ int mx_product_check(const char* name, const void* y, int dtype, int64_t ldy, co
   if (rc) return rc;
   if (!bytes_of(dtype)) return fail(NRQ_ERR_ARG, name, "unknown type %d", dtype);
   if (batch > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "batch of %zu (at most 2^20)", batch);
+  if (!nrq::mx_matmul_fits((int)rows, (int)cols, (int)batch))
+    return fail(NRQ_ERR_UNSUPPORTED, name, "%zu rows by %zu tokens: too many for a launch", rows, batch);
   if (!y || (cols && (!w || !ws))) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(y, bytes_of(dtype)) || !aligned(w, 16)) return fail(NRQ_ERR_ARG, name, "pointer not aligned");
   if (batch > 1 && ldy < (int64_t)rows) return fail(NRQ_ERR_ARG, name, "output rows overlap");
@@ -332,7 +342,7 @@ int nrq_dev_quantize_mxfp4(const void* src, int dtype, size_t rows, size_t cols,
                            void* scales, void* stream) {
   static const char* name = "nrq_dev_quantize_mxfp4";
   int rc;
-  if ((rc = mx_check(name, rows, cols))) return rc;
+  if ((rc = mx_quant_check(name, rows, cols))) return rc;
   if (!bytes_of(dtype)) return fail(NRQ_ERR_ARG, name, "unknown type %d", dtype);
   if (rows == 0 || cols == 0) return device_check(name, stream);
   if (!src || !q || !scales) return fail(NRQ_ERR_ARG, name, "null pointer");
@@ -348,7 +358,7 @@ int nrq_dev_dequantize_mxfp4(const void* q, const void* scales, size_t rows, siz
                              int64_t dst_stride, void* stream) {
   static const char* name = "nrq_dev_dequantize_mxfp4";
   int rc;
-  if ((rc = mx_check(name, rows, cols))) return rc;
+  if ((rc = mx_quant_check(name, rows, cols))) return rc;
   if (!bytes_of(dtype)) return fail(NRQ_ERR_ARG, name, "unknown type %d", dtype);
   if (rows == 0 || cols == 0) return device_check(name, stream);
   if (!dst || !q || !scales) return fail(NRQ_ERR_ARG, name, "null pointer");
@@ -394,6 +404,7 @@ int nrq_dev_linear_mxfp4(void* y, int dtype, int64_t y_stride, const void* w, co
   int rc;
   if (rows == 0 || batch == 0) return device_check(name, stream);
   if ((rc = mx_product_check(name, y, dtype, y_stride, w, w_scales, rows, cols, batch))) return rc;
+  if ((rc = mx_quant_check(name, batch, cols))) return rc;
   if (!bytes_of(x_dtype)) return fail(NRQ_ERR_ARG, name, "unknown type %d", x_dtype);
   if (cols && !x) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(x, bytes_of(x_dtype))) return fail(NRQ_ERR_ARG, name, "pointer not aligned");

@@ -75,6 +75,7 @@ struct VerifyLaunch {
 size_t verify_workspace(size_t seqs, size_t vocab);
 hipError_t launch_verify(const VerifyLaunch& L);
 
+bool mx_quantize_fits(size_t rows, size_t cols);  // whether a grid holds the values
 hipError_t launch_mx_quantize(const void* src, int dtype, size_t rows, size_t cols, int64_t stride, void* q, void* s,
                               hipStream_t stream);
 hipError_t launch_mx_dequantize(const void* q, const void* s, size_t rows, size_t cols, void* dst, int dtype,
@@ -88,6 +89,8 @@ struct MxMatmul {
   hipStream_t stream;
   void* workspace;
 };
+bool mx_matmul_fits(int rows, int cols, int batch);  // whether a grid holds the tiles
+bool mx_gemm_fits(int rows, int cols, int batch);
 size_t mx_matmul_workspace(int rows, int cols, int batch);
 size_t mx_gemm_workspace(int rows, int cols, int batch);
 hipError_t launch_mx_matmul(const MxMatmul& L);

@@ -313,3 +313,28 @@ def test_attention_units(seqs, width, fits):
                     table=_table(seqs=seqs, width=width, stride=width))
     assert rc == (NOT_INIT if fits else UNSUPPORTED), (rc, msg)
     assert fits or "too much" in msg
+
+
+@pytest.mark.parametrize("name,change,fits", [
+    ("nrq_dev_quantize_mxfp4", dict(rows=2 ** 30, cols=64, stride=64), False),
+    ("nrq_dev_quantize_mxfp4", dict(rows=2 ** 30 - 64, cols=64, stride=64), True),
+    ("nrq_dev_quantize_mxfp4", dict(rows=2 ** 31 - 1023, cols=32, stride=32), False),
+    ("nrq_dev_dequantize_mxfp4", dict(rows=2 ** 30, cols=64, stride=64), False),
+    ("nrq_dev_dequantize_mxfp4", dict(rows=2 ** 30 - 64, cols=64, stride=64), True),
+    ("nrq_dev_matmul_mxfp4", dict(rows=2 ** 31 - 1, batch=1), False),  # rounded up to tiles it would be negative
+    ("nrq_dev_matmul_mxfp4", dict(rows=2 ** 31 - 1, cols=0, batch=1), False),
+    ("nrq_dev_matmul_mxfp4", dict(rows=2 ** 31 - 1025, batch=1), True),
+    ("nrq_dev_matmul_mxfp4", dict(rows=2 ** 30, batch=129, ldy=2 ** 30), False),  # 2^24 tiles
+    ("nrq_dev_matmul_mxfp4", dict(rows=2 ** 30 - 1024, batch=129, ldy=2 ** 30), True),
+    ("nrq_dev_linear_mxfp4", dict(rows=40, cols=2 ** 16 + 64, batch=2 ** 20, wk_bytes=2 ** 40), False),  # the activation's values
+    ("nrq_dev_linear_mxfp4", dict(rows=2 ** 31 - 1, batch=1), False),
+    ("nrq_dev_linear_mxfp4", dict(rows=2 ** 30, batch=129, ldy=2 ** 30), False),
+    ("nrq_dev_linear_mxfp4", dict(rows=2 ** 30 - 1024, batch=128, ldy=2 ** 30), True)])
+def test_mx_sizes(name, change, fits):
+    """Sizes that a launch does not hold are refused, those below them are not."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("checks the no-GPU failure path")
+    rc, msg = _call(name, CALLS[name](), **change)
+    assert rc == (NOT_INIT if fits else UNSUPPORTED), (rc, msg)
