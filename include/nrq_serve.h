@@ -95,7 +95,8 @@ int nrq_dev_rope_append(void *y, const void *q, const void *k, const void *v, in
  * to nothing gives zeros. What the cache holds at positions that a row does not
  * attend to, infinities and NaN too, does not reach it. lse (or NULL):
  * f32 [table.seqs][n_new][heads] contiguous, log sum_t exp(scale q.k_t), -inf for nothing.
- * out may not overlap q. Scores, softmax and sums are in 32 bits. The results depend on how the work
+ * out may not overlap q. Scores, softmax and sums are in 32 bits; in products with an f16 cache, queries of another type
+ * and the weights of the softmax are within 2^-23 of their value, or 2^-37 of the largest. The results depend on how the work
  * is split, never on the order in which it runs: the same call gives the same
  * bits.
  * workspace: nrq_paged_attention_workspace bytes, 16-byte aligned, its contents

@@ -26,9 +26,9 @@
 //   hd / 16 dimensions of those eight positions and turns the 8 x hd / 16 block around.
 // The cache's 16-bit values go into the matrix instructions as they are. f32
 // queries go in as sums of 16-bit pieces (scaled by a power of two so that none
-// is lost in subnormals), and so do the f32 weights: two f16 pieces keep 22 bits,
-// three bf16 pieces 24, two bf16 pieces 16 (for 16-bit outputs, whose own
-// rounding is 2^-9).
+// is lost in subnormals), and so do the f32 weights: three bf16 pieces are an f32 value, two f16 pieces are within
+// 2^-23 of it (or 2^-37 of the largest). With two bf16 pieces, 2^-17, outputs that cancel would show it; the third takes
+// 48 sequences of up to 6000 from 127.0 us to 127.6, thirteen of 9000 by five tokens from 68.4 to 71.1 (bf16).
 #include "nrq_page.h"
 #include "nrq_serve_launch.h"
 
@@ -118,7 +118,7 @@ template <>
 struct PaType<_Float16> {
   typedef _Float16 v8 __attribute__((ext_vector_type(8)));
   static constexpr int kId = kF16;
-  static constexpr int kPieces = 2;  // of an f32 value: 22 bits
+  static constexpr int kPieces = 2;  // of an f32 value
   static constexpr uint32_t kExp = 0x7c00u;
   static constexpr float kOffset = 12.0f;  // weights up to 2^12: pieces down to 2^-36 of the largest
   static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) {
@@ -284,10 +284,11 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
   }
 }
 
-// T: the cache's type; HD; NT: groups of 16 rows; NQ, NP: pieces of a query and of a weight.
-template <typename T, int HD, int NT, int NQ, int NP>
+// T: the cache's type; HD; NT: groups of 16 rows; NQ: pieces of a query.
+template <typename T, int HD, int NT, int NQ>
 __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArgs A) {
   typedef typename PaType<T>::v8 v8;
+  constexpr int NP = PaType<T>::kPieces;  // of a weight
   constexpr int KS = HD / 32;  // steps of K
   constexpr int DV = HD / 16;  // dimensions of a lane's values
   constexpr int OS = 16 * NT + 1;  // row stride of the exchange: odd
@@ -597,7 +598,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs A) {
         none ? -INFINITY : (mm - PaType<T>::kOffset + log2f(l)) * 0.69314718055994531f;
 }
 
-template <typename T, int HD, int NT, int NQ, int NP>
+template <typename T, int HD, int NT, int NQ>
 hipError_t pa_launch(PaArgs& A) {
   const int64_t units = (int64_t)A.units_per_seq * A.L.table.seqs;
   const int64_t tiles = ((int64_t)A.L.table.width * A.L.kv.page_size + kTile - 1) / kTile;
@@ -607,7 +608,7 @@ hipError_t pa_launch(PaArgs& A) {
   A.part_o = (float*)A.L.workspace;
   A.part_ml = (float2*)(A.part_o + (size_t)2 * A.wgs * A.slots * HD);
   A.share = (int4*)(((uintptr_t)(A.part_ml + (size_t)2 * A.wgs * A.slots) + 15) & ~(uintptr_t)15);
-  hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ, NP>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
+  hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
   if (tiles > 1)
     hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)units, A.slots), dim3(256), 0, A.L.stream, A);
   return hipGetLastError();
@@ -628,8 +629,8 @@ hipError_t pa_launch_hd(const PagedAttnLaunch& L) {
   A.wide_q = ((uintptr_t)L.q & 15) == 0 && L.qb % v == 0 && L.qt % v == 0 && L.qh % v == 0;
   const bool same = L.dtype == PaType<T>::kId;
   if constexpr (HD <= 128)
-    if (A.per == 32) return same ? pa_launch<T, HD, 2, 1, 2>(A) : pa_launch<T, HD, 2, kMany, kMany>(A);
-  return same ? pa_launch<T, HD, 1, 1, 2>(A) : pa_launch<T, HD, 1, kMany, kMany>(A);
+    if (A.per == 32) return same ? pa_launch<T, HD, 2, 1>(A) : pa_launch<T, HD, 2, kMany>(A);
+  return same ? pa_launch<T, HD, 1, 1>(A) : pa_launch<T, HD, 1, kMany>(A);
 }
 
 template <typename T>

@@ -1287,3 +1287,47 @@ def test_rope_more_tokens_than_a_grid_has_threads_for(gpu, append):
         assert np.all(np.abs(got - want[:, 0]) <= tol[:, 0])
         assert np.array_equal(f64(vp)[:, 0].reshape(-1, 2)[p.astype(int)], np.tile([1.0, 0.5], (2, 1)))
         assert int((vp != 0).any(-1).sum()) == 2
+
+
+# ---- weights of the softmax in 32 bits ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("new", [1, 3])
+def test_attention_weights_keep_32_bits(gpu, new):
+    """bf16 throughout. Three positions weigh 1, a fourth p = exp(-c s); in dimension h the values are minus the first two
+    bf16 pieces of head h's p, and 1: what is left is the third piece. Values whose third piece is 2^-18.5 and more.
+
+    The numerator is off by: 3 u of the exponent (at most 1 in units of log2) in its unit and product, 2 u in the exponential,
+    and 12 products of at most 2 added up, each sum rounded or cut: 24 u for rounding. In all 29 u, below 2^-18.5 / 1.4."""
+    import torch
+
+    from nightrun_amd import serve
+
+    def bf(x):
+        return torch.tensor(x, dtype=torch.float64).bfloat16().double().numpy()
+
+    seqs, heads, hd, s = 16, 8, 64, 0.69
+    scale = float(np.float32(s))
+    c = np.concatenate([(128 + np.arange(128)) / 256, 1 - np.arange(1, 100) / 256.0])
+    c = c[c >= 0.5]
+    p = np.exp(-c * scale)
+    third = p - bf(p) - bf(p - bf(p))
+    c = c[np.abs(third) >= 2.0 ** -18.5]
+    assert len(c) >= 5
+    pick = np.random.default_rng(2).integers(0, len(c), (seqs, heads))
+    cc = c[pick]
+    p = np.exp(-cc * scale)
+    one, two = bf(p), bf(p - bf(p))
+    q = np.zeros((seqs, new, heads, hd))
+    q[..., 0] = cc[:, None]
+    k, v = np.zeros((seqs, 1, 16, hd)), np.zeros((seqs, 1, 16, hd))
+    k[:, 0, 3, 0] = -1.0
+    v[:, 0, 0, :heads], v[:, 0, 1, :heads], v[:, 0, 3, :heads] = -one, -two, 1.0
+    qd, kd, vd = (torch.from_numpy(x).to(torch.bfloat16).cuda() for x in (q, k, v))
+    y = torch.empty_like(qd)
+    table = torch.arange(seqs, dtype=torch.int32, device="cuda").view(-1, 1)
+    serve.paged_attention(y, qd, kd, vd, table, torch.full((seqs,), 4, dtype=torch.int32, device="cuda"), scale)
+    got = f64(y)[:, -1][:, np.arange(heads), np.arange(heads)]
+    want = (p - one - two) / (3 + p)
+    assert np.all(np.abs(want) >= 2.0 ** -18.5 / 4)
+    assert np.all(np.abs(got - want) <= 29 * U / (3 + p) + half_step("bf16") * np.abs(want))
