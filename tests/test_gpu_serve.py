@@ -1331,3 +1331,147 @@ def test_attention_weights_keep_32_bits(gpu, new):
     want = (p - one - two) / (3 + p)
     assert np.all(np.abs(want) >= 2.0 ** -18.5 / 4)
     assert np.all(np.abs(got - want) <= 29 * U / (3 + p) + half_step("bf16") * np.abs(want))
+
+
+# ---- prompts: hundreds and thousands of new tokens ------------------------------------------------------
+
+
+def dense_attention(q, k, v, lens, counts, scale, window):
+    """(out, bound, lse, bound of lse) in 64 bits on the device: k, v [seqs, kv, width, hd]. The bound is that of
+    attention(); the logarithm of the sum is off by the scores' d, by (T + 8) u of the sum, and by 4 u of itself for the
+    maximum's and the logarithm's changes of unit, each at most the larger of the maximum and the result."""
+    import torch
+
+    seqs, new, heads, hd = q.shape
+    kv, width = k.shape[1], k.shape[2]
+    group = heads // kv
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    lse = torch.full(q.shape[:3], -math.inf, dtype=torch.float64, device="cuda")
+    ltol = torch.zeros_like(lse)
+    t = torch.arange(width, device="cuda")
+    for b in range(seqs):
+        n = counts[b]
+        p = lens[b] - n + torch.arange(n, device="cuda")
+        ok = (t <= p[:, None]) & (t < lens[b])
+        if window:
+            ok &= t > p[:, None] - window
+        seen = ok.any(1)
+        for h in range(heads):
+            qq, kk, vv = q[b, :n, h], k[b, h // group], v[b, h // group]
+            s = (qq @ kk.t()) * scale
+            size = torch.where(ok, (qq.abs() @ kk.t().abs()) * abs(scale), 0.0).amax(1)
+            big = torch.where(ok, s.abs(), 0.0).amax(1)
+            d = (hd + 4) * U * size + 3 * U * big
+            s = torch.where(ok, s, -math.inf)
+            top = torch.where(seen, s.amax(1), 0.0)
+            w = torch.exp(s - top[:, None])
+            total = torch.where(seen, w.sum(1), 1.0)
+            terms = ok.sum(1)
+            out[b, :n, h] = (w @ vv) / total[:, None]
+            weight = (w @ vv.abs()) / total[:, None]
+            tol[b, :n, h] = weight * (2 * torch.expm1(2 * d) + 2 * (terms + 8) * U)[:, None]
+            lse[b, :n, h] = torch.where(seen, top + torch.log(total), -math.inf)
+            ltol[b, :n, h] = 2 * d + (terms + 8) * U + 4 * U * (1 + torch.maximum(top.abs(), torch.log(total)))
+    return out, tol, lse, ltol
+
+
+@pytest.mark.parametrize("hd,heads,kv,new,lens,window,counts", [
+    (256, 8, 2, 37, [300, 37, 20], 0, None), (256, 4, 4, 300, [311, 129], 100, [300, 17]), (96, 10, 2, 130, [400, 131, 7], 0, None),
+    (96, 3, 1, 515, [515], 64, None), (32, 8, 1, 260, [600, 260], 0, [260, 0]), (32, 4, 4, 33, [33, 4000], 1000, None),
+    (64, 32, 8, 513, [513, 1030], 0, None), (128, 16, 4, 700, [701, 699, 1500], 333, [700, 512, 1]), (64, 8, 2, 4096, [4096], 0, None),
+    (128, 4, 1, 2000, [5000], 1024, None)])
+@pytest.mark.parametrize("kind,cache", [("f32", "f16"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16")])
+def test_attention_prompts(gpu, hd, heads, kv, new, lens, window, counts, kind, cache):
+    """Many row tiles a head, more rows than positions, positions that only later rows see."""
+    import torch
+
+    from nightrun_amd import serve
+
+    size, seqs = 24, len(lens)
+    g = torch.Generator(device="cuda").manual_seed(hd + new)
+    width = -(-max(lens) // size) + 1
+    table = torch.randperm(seqs * width + 3, device="cuda", generator=g)[:seqs * width].to(torch.int32).view(seqs, width)
+    kp, vp = (torch.full((seqs * width + 3, kv, size, hd), math.inf, dtype=dt(cache), device="cuda") for _ in range(2))
+    k, v = (torch.randn(seqs, kv, width * size, hd, device="cuda", generator=g).to(dt(cache)) for _ in range(2))
+    for b in range(seqs):  # behind the length there are infinities
+        t = torch.arange(lens[b], device="cuda")
+        for rows, pages in ((k, kp), (v, vp)):
+            pages[table[b].long()[t // size], :, t % size] = rows[b, :, :lens[b]].transpose(0, 1)
+    q = (1.5 * torch.randn(seqs, new, heads, hd, device="cuda", generator=g)).to(dt(kind))
+    y = torch.full_like(q, 11.0)
+    lse = torch.full((seqs, new, heads), 12.0, device="cuda")
+    serve.paged_attention(y, q, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), hd ** -0.5, window=window,
+                          counts=None if counts is None else torch.tensor(counts, dtype=torch.int32, device="cuda"), lse=lse)
+    use = counts or [new] * seqs
+    want, tol, wl, ltol = dense_attention(q.double(), k.double(), v.double(), lens, use, hd ** -0.5, window)
+    # the weights' pieces (within 2^-23) and the queries' (counted in hd + 4), the output's rounding
+    tol += 2.0 ** -22 * v.double().abs().max() + half_step(kind) * want.abs()
+    for b in range(seqs):
+        n = use[b]
+        assert torch.all((y[b, :n].double() - want[b, :n]).abs() <= tol[b, :n])
+        assert torch.all(y[b, n:] == 11) and torch.all(lse[b, n:] == 12)
+        none = torch.isneginf(wl[b, :n])
+        assert torch.equal(torch.isneginf(lse[b, :n]), none) and torch.all(y[b, :n][none] == 0)
+        assert torch.all(((lse[b, :n].double() - wl[b, :n]).abs() <= ltol[b, :n]) | none)
+
+
+@pytest.mark.parametrize("kind,cache", sorted(PIECES))
+@pytest.mark.parametrize("hd,lens,heads,kv", [(128, [1, 3, 200, 1000, 5000], 8, 2), (64, [20000], 4, 1), (256, [700, 64], 2, 1)])
+def test_attention_log_sums(gpu, kind, cache, hd, lens, heads, kv):
+    """The logarithm of the sum of exponentials to its rounding, with scores of a few units and of hundreds."""
+    import torch
+
+    from nightrun_amd import serve
+
+    for scale in (hd ** -0.5, 1.0):
+        c = Cache(gen(hd), lens, kv, hd, 16, cache)
+        kp, vp, table, ln = c.dev()
+        q = normal(gen(hd + 1), len(lens), 1, heads, hd, kind=kind, scale=1.5)
+        y, lse = torch.empty_like(q), torch.empty(len(lens), 1, heads, device="cuda")
+        serve.paged_attention(y, q, kp, vp, table, ln, scale, lse=lse)
+        k, v = (torch.zeros(len(lens), kv, max(lens), hd, dtype=torch.float64, device="cuda") for _ in range(2))
+        for b, n in enumerate(lens):
+            k[b, :, :n], v[b, :, :n] = c.k[b].double().cuda().transpose(0, 1), c.v[b].double().cuda().transpose(0, 1)
+        want, tol, wl, ltol = dense_attention(q.double(), k, v, lens, [1] * len(lens), scale, 0)
+        assert torch.all((lse.double() - wl).abs() <= ltol)
+        tol += 2.0 ** -22 * v.abs().max() + half_step(kind) * want.abs()
+        assert torch.all((y.double() - want).abs() <= tol)
+
+
+# ---- MXFP4 at the ends of the scales -------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 40, 2560), (5, 20, 96), (40, 70, 640), (70, 200, 96), (70, 200, 512), (70, 131, 9728), (300, 260, 2080)])
+def test_mx_products_of_least_and_largest_scales(gpu, batch, rows, cols):
+    """Scale bytes from 0 and up to 254: the scale of a product is the sum of both, whatever each is. Bytes past 255 start
+    again at 0, so that some products are below all that 32 bits hold: there each block's sum and each addition is off by at
+    most half of 2^-149, the step of the subnormal numbers, beside what check_product() allows."""
+    import torch
+
+    from nightrun_amd import serve
+
+    g = gen(rows + cols)
+    (w, ws), (x, xs) = mx_random(g, rows, cols), mx_random(g, batch, cols)
+    for a, b in ((0, 250), (250, 0), (0, 240), (2, 252)):
+        sw, sx = ws - ws.min() + a, xs - xs.min() + b  # 13 bytes from a and from b on
+        sw, sx = sw.clamp(max=254), sx.clamp(max=254)
+        y = torch.empty(batch, rows, device="cuda")
+        serve.matmul_mxfp4(y, w.cuda(), sw.cuda(), x.cuda(), sx.cuda())
+        vx, vw = mx_values(unpack(x), sx.numpy()), mx_values(unpack(w), sw.numpy())
+        want, size = vx @ vw.T, np.abs(vx) @ np.abs(vw).T
+        assert np.all(np.abs(f64(y) - want) <= (cols // 32 + 2) * (U * size + 2.0 ** -149) + half_step("f32") * np.abs(want))
+
+
+def test_mx_values_back_to_their_codes(gpu):
+    """What every code stands for at the scales 2^-125 to 2^125 comes back as the definition has it."""
+    import torch
+
+    from nightrun_amd import serve
+
+    q = torch.arange(16, dtype=torch.uint8).repeat(251, 2)
+    packed = (q[:, 0::2] | q[:, 1::2] << 4).contiguous().cuda()
+    s = torch.arange(2, 253, dtype=torch.uint8).view(251, 1).cuda()
+    y = torch.empty(251, 32, device="cuda")
+    serve.dequantize_mxfp4(packed, s, y)
+    fine = mx_values(q.numpy().astype(int), s.cpu().numpy()).astype(np.float32)
+    assert np.array_equal(y.cpu().numpy(), fine)
