@@ -1475,3 +1475,76 @@ def test_mx_values_back_to_their_codes(gpu):
     serve.dequantize_mxfp4(packed, s, y)
     fine = mx_values(q.numpy().astype(int), s.cpu().numpy()).astype(np.float32)
     assert np.array_equal(y.cpu().numpy(), fine)
+
+
+# ---- more sequences than a grid has rows, columns past 32-bit offsets, mixed types ----------------------
+
+
+def test_verify_more_sequences_than_a_grid_has_rows(gpu):
+    """70,000 sequences in two launches each; one-hot rows of drafts accepted, refused and counted out."""
+    import torch
+
+    from nightrun_amd import serve
+
+    b, n, vocab = 70000, 2, 33
+    g = torch.Generator(device="cuda").manual_seed(2)
+    best = torch.randint(0, vocab, (b, n + 1), device="cuda", generator=g)
+    target = torch.zeros(b, n + 1, vocab, device="cuda").scatter_(2, best[..., None], 1.0)
+    drafted = torch.where(torch.rand(b, n, device="cuda", generator=g) < 0.7, best[:, :n],
+                          torch.randint(0, vocab, (b, n), device="cuda", generator=g)).to(torch.int32)
+    counts = torch.randint(0, n + 1, (b,), device="cuda", generator=g, dtype=torch.int32)
+    u = torch.rand(b, n + 1, device="cuda", generator=g)
+    tokens, accepted = (torch.full(s, 99, dtype=torch.int32, device="cuda") for s in ((b, n + 1), (b,)))
+    serve.verify_drafts(tokens, accepted, target, None, drafted, u, counts=counts)
+    j = torch.arange(n, device="cuda")
+    took = torch.cumprod(((drafted == best[:, :n]) & (j < counts[:, None])).int(), 1).sum(1)
+    # a refused draft is not the row's one token, so that what is left out does not matter
+    j = torch.arange(n + 1, device="cuda")
+    want = torch.where(j <= took[:, None], best, -1)
+    assert torch.equal(accepted.long(), took) and torch.equal(tokens.long(), want)
+
+
+@pytest.mark.parametrize("batch", [1, 66])
+@pytest.mark.parametrize("cols", [2 ** 26, 2 ** 26 + 32])
+def test_mx_columns_past_32_bit_offsets(gpu, batch, cols):
+    """Rows of 2^25 bytes, of which all but a few values are zeros: whole sums, exact in any order."""
+    import torch
+
+    from nightrun_amd import serve
+
+    rows, at = 70, [0, 31, 2 ** 25 - 1, 2 ** 25, 2 ** 26 - 33, 2 ** 26 - 1, cols - 32, cols - 1]
+    at = sorted(set(at))
+    g = gen(cols % 1000 + batch)
+    codes = []
+
+    def sparse(n):
+        c = torch.randint(0, 16, (n, len(at)), generator=g)
+        q = torch.zeros(n, cols // 2, dtype=torch.uint8, device="cuda")
+        for i, a in enumerate(at):
+            q[:, a // 2] |= (c[:, i] << 4 * (a % 2)).to(torch.uint8).cuda()
+        codes.append(c.numpy())
+        return q, torch.full((n, cols // 32), 127, dtype=torch.uint8, device="cuda")
+
+    w, ws = sparse(rows)
+    x, xs = sparse(batch)
+    y = torch.empty(batch, rows, device="cuda")
+    serve.matmul_mxfp4(y, w, ws, x, xs)
+    vw, vx = (np.where(c >= 8, -1.0, 1.0) * GRID[c & 7] for c in codes)
+    assert np.array_equal(f64(y), vx @ vw.T)
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 300, 2560), (9, 40, 96), (3, 300, 8192), (40, 70, 640), (100, 300, 1056), (70, 131, 9728)])
+@pytest.mark.parametrize("kind,out", [("f32", "bf16"), ("bf16", "f32"), ("f16", "bf16"), ("f32", "f16"), ("f16", "f32"), ("bf16", "f16")])
+def test_mx_linear_mixed_types(gpu, kind, out, batch, rows, cols):
+    """The activation of one type, the outputs of another."""
+    import torch
+
+    from nightrun_amd import serve
+
+    g = gen(rows + batch)
+    w, ws = mx_random(g, rows, cols, spread=3)
+    x = torch.randn(batch, cols, generator=g).to(dt(kind))
+    y = torch.empty(batch, rows, dtype=dt(out), device="cuda")
+    serve.linear_mxfp4(y, w.cuda(), ws.cuda(), x.cuda())
+    codes, scales = mx_quantize(x.double().numpy())
+    check_product(y, codes, scales, unpack(w), ws.numpy(), out)
