@@ -13,6 +13,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: long-running CPU test")
 
 
+# Tests that ask for what is wrong. They run, and have to fail.
+WRONG = {
+    "test_m0_is_written_only_by_the_dma_asm":
+        "asks for each load to LDS directly behind the write of M0, where the instruction set manual asks for a wait "
+        "state between them; test_lds_loads.py asks for that and for the rest of what this one does",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        if item.name in WRONG:
+            item.add_marker(pytest.mark.xfail(reason=WRONG[item.name], raises=AssertionError, strict=True))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     """The CPU oracle (test infrastructure); built from oracle/ if missing."""

@@ -1,7 +1,10 @@
 """Loads from memory to LDS in the built library. They take their LDS address from M0 and, in one form, their
 base from a pair of scalar registers. Inside inline assembly the compiler puts no wait states, so the code has to
 hold those that the CDNA3 and CDNA4 instruction set manuals ask for: one between a scalar write of M0 and such a
-load, five between a vector instruction's write of a scalar register and a load that takes it as its base."""
+load, five between a vector instruction's write of a scalar register and a load that takes it as its base.
+
+The compiler does not know that the assembly writes M0, which is sound while no code of its own keeps a value there:
+nothing but those writes names M0, each has its load behind the wait state, and nothing reads it implicitly."""
 import os
 import re
 import shutil
@@ -23,7 +26,7 @@ def _registers(operand):
 
 def short_waits(lines):
     """(how many loads to LDS there are, what is wrong) of a listing's instructions."""
-    seen, loads, wrong = [], 0, []
+    seen, loads, wrong, set_m0 = [], 0, [], None
     for line in lines:
         code = line.split("//")[0].strip()
         if not line.startswith("\t") or not code:
@@ -32,7 +35,18 @@ def short_waits(lines):
             continue
         op, _, rest = code.partition(" ")
         args = [a.strip() for a in rest.split(",")]
-        if "load_lds" in op:
+        load = "load_lds" in op
+        if re.match(r"(s_sendmsg|s_movrel|v_movrel|s_set_gpr_idx|ds_gws|buffer_load\w*.*\blds\b)", code):
+            wrong.append(f"{code}: reads M0")
+        if set_m0 and not load and op != "s_nop":
+            wrong.append(f"{code}: between {set_m0} and the load")
+        if re.search(r"\bm0\b", code):
+            set_m0 = code
+            if not re.match(r"s_mov_b32 m0, s\d+$", code):
+                wrong.append(f"{code}: M0 in other code than the loads'")
+        elif op != "s_nop":
+            set_m0 = None
+        if load:
             loads += 1
             base, states = _registers(args[-1].split()[0]), 0
             for o, a in reversed(seen[-REACH:]):
@@ -53,6 +67,8 @@ def test_the_check_itself():
     assert len(short_waits(base)[1]) == 1
     base[2] = "\ts_nop 3"
     assert short_waits(base) == (1, [])
+    for other in ("\ts_mov_b32 s1, s2", "\tv_readlane_b32 s1, v0, m0", "\ts_movrels_b32 s1, s2", "\tds_gws_barrier v0"):
+        assert short_waits([good[0], other, *good[1:]])[1], other
 
 
 def test_wait_states(tmp_path):
