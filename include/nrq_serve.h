@@ -14,7 +14,9 @@
  * are in elements; the last dimension of every tensor is contiguous. Integers
  * that live on the device (lengths, positions, table entries, drafted tokens)
  * cannot be refused: what each function does with those out of range is said
- * there, and none reads or writes outside the tensors.
+ * there, and none reads or writes outside the tensors. Refused are, before
+ * anything is launched: a current device or a stream of another device than
+ * nrq_init's (NRQ_ERR_ARG), and sizes past what a call can take (NRQ_ERR_UNSUPPORTED).
  */
 #ifndef NRQ_SERVE_H
 #define NRQ_SERVE_H
@@ -83,7 +85,7 @@ int nrq_dev_rope_append(void *y, const void *q, const void *k, const void *v, in
  * NRQ_BF16), strides = {q sequence, q token, q head, out sequence, out token, out
  * head}; heads is a multiple of the KV heads, query head h reads KV head h /
  * (heads / n_kv_heads). head_dim is 32, 64, 96, 128 or 256; a table holds at
- * most 2^30 positions of a sequence.
+ * most 2^30 positions of a sequence; n_new heads is at most 2^20.
  *   lens[b]: positions of sequence b, its new tokens' among them (their keys and
  *     values are in the cache already); below 0 is 0, more than the table holds
  *     is what it holds.

@@ -270,8 +270,9 @@ __global__ __launch_bounds__(64 * W) void mx_matvec_kernel(MxMatmul L, int tiles
   }
 }
 
-// Workgroups for `tiles` row tiles: all of them up to 2048, else few enough that each has as many (128256 x 2048
-// by eight tokens: 51 us, 62 with one tile a workgroup; 19456 x 2560 by one is all of them: 7.8, with 768 8.9).
+// Workgroups for `tiles` row tiles: all of them up to 2048, else few enough that each has as many (65536 x 4096
+// by one and three tokens: 35.8 and 41.4 us, 36.6 and 47.3 with one tile a workgroup; 128256 x 2048 by one 35.6 and 35.3, by
+// three 38.5 and 40.9; 19456 x 2560 by one is all of them: 7.8, with 768 8.9).
 inline unsigned mx_matvec_grid(int tiles) {
   const int rounds = (tiles + 2047) / 2048;
   return (unsigned)((tiles + rounds - 1) / rounds);
@@ -280,7 +281,7 @@ inline unsigned mx_matvec_grid(int tiles) {
 // Eight waves a workgroup, where there are no more workgroups than CUs and rows long enough for them, else four: 2048 x
 // 8192 by one and four tokens takes 6.2 and 10.3 us with eight, 7.3 and 12.1 with four, 2560 x 9728 by one 6.8 and 7.7.
 // Steps of a wave on their way together (U): four or five, whichever divides its steps with less rest (2048 columns
-// are four steps a wave, 2560 five: with five for both, 128256 x 2048 takes 42 us for 38).
+// are four steps a wave, 2560 five: 128256 x 2048 by one takes 35.7 us with four and 41.9 with five, 19456 x 2560 10.1 and 7.3).
 template <int W, typename X>
 void matvec_w(const MxMatmul& L, size_t lds, const X* x, int64_t stride, int wide) {
   const int tiles = (L.rows + 15) / 16, steps = (L.cols + 128 * W - 1) / (128 * W);

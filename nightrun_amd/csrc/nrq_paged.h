@@ -13,8 +13,10 @@
 // A unit's keys and values are read once for all its rows, and that read bounds the kernel where
 // there is enough of it: 196,608 positions of two sequences (8 KV heads of 128, f16, 805 MB)
 // take 140 to 147 us, 5.5 to 5.75 TB/s, as fast as the card reads at all; 48 sequences of up to 6000 (603 MB)
-// 125 us, 4.8 TB/s. With five new tokens, 4 query heads each, a unit has 20 rows in two row tiles, and the f32
-// weights' second piece doubles its products: 13 sequences under a window of 4096 take 55 us, 3.3 TB/s. One
+// 127 us, 4.8 TB/s. 13 sequences under a window of 4096 (178 MB) take 43 us for one new token, 49 for four (16 rows of f32
+// queries, one row tile) and 55 for five (20 rows in two); with 16-bit queries 42, 47 and 53. A workgroup has five or six tiles
+// of them, so that the chain before the first (length, page, queries, keys) and the join weigh most: the waves
+// wait for memory 59% of their time, the matrix units work 8% of theirs. One
 // sequence of 1000 positions takes 10 us: two launches and the chain of length, page, key and value.
 //
 // Per tile each of the four waves takes 32 positions of keys and values straight from
