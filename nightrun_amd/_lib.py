@@ -105,6 +105,19 @@ SERVE_SIGNATURES = {
     "nrq_dev_linear_mxfp4": ([_vp, _i, _i64, _vp, _vp, _vp, _i, _i64, _sz, _sz, _sz, _vp, _sz, _vp], _i),
 }
 
+# symbols of include/nrq_tree.h
+TREE_SIGNATURES = {
+    "nrq_dev_norm_rope": ([_vp, _vp, _i, _sz, _sz, _sz, _vp, _vp, _f, _vp, _vp, _sz, _i, _f, _vp], _i),
+    "nrq_dev_norm_rope_append": ([_vp, _vp, _vp, _vp, _i, _sz, _sz, _vp, _i, _vp, _vp, _f, _vp, _vp, _vp, _vp, _sz, _i,
+                                  _f, _vp, _vp, _vp], _i),
+    "nrq_tree_attention_workspace": ([_sz, _sz, _sz, _vp, _szp], _i),
+    "nrq_dev_tree_attention": ([_vp, _vp, _i, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _vp, _f, C.c_int32, _vp, _vp, _sz, _vp],
+                               _i),
+    "nrq_verify_tree_workspace": ([_sz, _sz, _szp], _i),
+    "nrq_dev_verify_tree": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _vp], _i),
+    "nrq_dev_keep_path": ([_vp, _sz, _i64, _vp, _vp, _vp, _vp, _vp, _sz, _vp], _i),
+}
+
 
 class NrqError(RuntimeError):
     def __init__(self, code: int, msg: str):
@@ -133,7 +146,7 @@ def lib():
         import torch  # noqa: F401
 
         L = C.CDLL(LIB_PATH)
-        for name, (args, res) in {**SIGNATURES, **SERVE_SIGNATURES}.items():
+        for name, (args, res) in {**SIGNATURES, **SERVE_SIGNATURES, **TREE_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.argtypes, fn.restype = args, res
         _lib = L

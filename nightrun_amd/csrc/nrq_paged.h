@@ -33,6 +33,7 @@
 // 48 sequences of up to 6000 from 127.0 us to 127.6, thirteen of 9000 by five tokens from 68.4 to 71.1 (bf16).
 #include "nrq_page.h"
 #include "nrq_serve_launch.h"
+#include "nrq_tree_mask.h"
 
 namespace nrq {
 
@@ -238,20 +239,49 @@ struct PaTile {
 // Workgroups a CU holds: registers for the tile, the accumulators and the queries.
 constexpr int pa_resident(int hd, int nt) { return hd > 128 ? 1 : (nt == 2 || hd > 96 ? 2 : 3); }
 
+// What the nodes of a tree see: lane j holds node j's.
+struct PaTree {
+  uint64_t above;  // the node and those above it, as far as the window reaches
+  int depth;
+};
+__device__ __forceinline__ PaTree pa_tree(const PagedAttnLaunch& L, int b, int n) {
+  const int lane = threadIdx.x & 63;
+  const int parent = lane < n ? tree_parent(L.parents[(int64_t)b * L.n_new + lane], lane) : -1;
+  PaTree t{lane < n ? 1ull << lane : 0, 0};
+  for (int a = lane < n ? lane : -1;;) {  // parents come first, so that this ends
+    const int up = __shfl(parent, a & 63);
+    a = a < 0 ? -1 : up;
+    if (!__any(a >= 0)) return t;
+    if (a >= 0) {
+      t.depth++;
+      if (L.window == 0 || t.depth < L.window) t.above |= 1ull << a;
+    }
+  }
+}
+__device__ __forceinline__ PaTree pa_node(const PaTree& t, int j) {
+  const uint32_t lo = __shfl((uint32_t)t.above, j), hi = __shfl((uint32_t)(t.above >> 32), j);
+  return PaTree{(uint64_t)hi << 32 | lo, __shfl(t.depth, j)};
+}
+
 // The same stretch of one wave without matrix instructions, position by position and row by
 // row, for values that hold an infinity or a NaN: there the products of weights
 // that are 0 (rows that do not see a position) or of the pieces of a weight would give
 // NaN. Dimension lane + 64 e is the lane's.
-template <typename T, int HD>
+template <typename T, int HD, bool TREE>
 __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int row0, int rows, int p0, int stop, int len,
                                       int n, float* ex_o, float (*ex_ml)[2], int os) {
   constexpr int E = (HD + 63) / 64;
   const PagedAttnLaunch& L = A.L;
   const int lane = threadIdx.x & 63;
   const int* pages = L.table.pages + b * L.table.stride;
+  PaTree tree;
+  if (TREE) tree = pa_tree(L, b, n);
   for (int r = 0; r < rows; r++) {
-    const int rr = row0 + r, tok = rr / A.group, hi = len - n + tok;
-    const int lo = L.window > 0 ? max(0, hi - L.window + 1) : 0;
+    const int rr = row0 + r, tok = rr / A.group;
+    PaTree node;
+    if (TREE) node = pa_node(tree, tok);
+    const int hi = TREE ? len - 1 : len - n + tok, own = TREE ? len - n + node.depth : hi;
+    const int lo = L.window > 0 ? max(0, own - L.window + 1) : 0;
     const int64_t qa = b * L.qb + tok * L.qt + (head * A.group + rr - tok * A.group) * L.qh;
     float q[E], o[E], m = -INFINITY, l = 0;
     for (int e = 0; e < E; e++) {
@@ -264,8 +294,9 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
                                  : (float)((const __bf16*)L.q)[qa + d];
     }
     for (int t0 = p0; t0 < stop; t0 += kTile)
-      for (int t = max(t0, lo); t < min(t0 + 32, hi + 1); t++) {
-        const uint32_t place = pa_place(L, pages, t, lo, min(len, hi + 1));
+      for (int t = max(t0, TREE ? 0 : lo); t < min(t0 + 32, hi + 1); t++) {
+        if (TREE && !(tree_sees(node.above, t, len - n) & 1 && (t >= lo || t >= len - n))) continue;
+        const uint32_t place = pa_place(L, pages, t, TREE ? 0 : lo, min(len, hi + 1));
         if (place == kNoPlace) continue;
         const int64_t at = (int64_t)place * 8 + head * L.kv.head_stride;
         float s = 0;
@@ -287,7 +318,7 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
 }
 
 // T: the cache's type; HD; NT: groups of 16 rows; NQ: pieces of a query.
-template <typename T, int HD, int NT, int NQ>
+template <typename T, int HD, int NT, int NQ, bool TREE>
 __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArgs A) {
   typedef typename PaType<T>::v8 v8;
   constexpr int NP = PaType<T>::kPieces;  // of a weight
@@ -320,10 +351,11 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       A.share[b * A.units_per_seq + unit] =
           make_int4(blockIdx.x, whole ? (int)blockIdx.x : line_owner(at + sq.tiles - 1, total, wgs), rows, 0);
     if (rows > 0) {
-      const int first_hi = sq.len - sq.n + row0 / A.group;                // what the unit's first
-      const int last_hi = sq.len - sq.n + (row0 + rows - 1) / A.group;    // and last row see
+      // what the unit's first and last row see; of a tree the positions before it, and any of it
+      const int first_hi = TREE ? sq.len - sq.n - 1 : sq.len - sq.n + row0 / A.group;
+      const int last_hi = TREE ? sq.len - 1 : sq.len - sq.n + (row0 + rows - 1) / A.group;
       const int last_lo = L.window > 0 ? max(0, last_hi - L.window + 1) : 0;
-      const int begin = L.window > 0 ? max(0, first_hi - L.window + 1) : 0, end = min(sq.len, last_hi + 1);
+      const int begin = L.window > 0 ? max(0, first_hi - L.window + (TREE ? 2 : 1)) : 0, end = min(sq.len, last_hi + 1);
       const int* pages = L.table.pages + b * L.table.stride;
       const uint16_t* kp = L.kv.k + head * L.kv.head_stride;
       const uint16_t* vp = L.kv.v + head * L.kv.head_stride;
@@ -382,10 +414,19 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       __syncthreads();
       float to_log2[NT];  // what brings a row's products to log2 units
       int lo[NT], hi[NT];  // what the row sees
+      uint64_t above[NT];
+      PaTree tree;
+      if (TREE) tree = pa_tree(L, b, sq.n);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         to_log2[n] = unit_log2[16 * n + c];
-        hi[n] = sq.len - sq.n + min(row0 + 16 * n + c, sq.n * A.group - 1) / A.group;
+        const int tok = min(row0 + 16 * n + c, sq.n * A.group - 1) / A.group;
+        hi[n] = sq.len - sq.n + tok;
+        if (TREE) {
+          const PaTree node = pa_node(tree, tok);
+          above[n] = node.above;
+          hi[n] = sq.len - sq.n + node.depth;  // as far as the window goes
+        }
         lo[n] = L.window > 0 ? max(0, hi[n] - L.window + 1) : 0;
       }
 
@@ -429,7 +470,11 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
             float s[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) s[i] = x[n][i >> 2][i & 3] * to_log2[n];
-            if (!inside) {
+            if (TREE && !inside) {
+              const uint32_t base = sq.len - sq.n, sees = tree_sees(above[n], p0, base) & tree_from(lo[n], p0, base) & live;
+#pragma unroll
+              for (int i = 0; i < 8; i++) s[i] = sees >> ((i < 4 ? 0 : 16) + 4 * g + (i & 3)) & 1 ? s[i] : -INFINITY;
+            } else if (!inside) {
 #pragma unroll
               for (int i = 0; i < 8; i++) {
                 const int o = (i < 4 ? 0 : 16) + 4 * g + (i & 3), p = p0 + o;
@@ -488,7 +533,7 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       }
       __syncthreads();  // the queries are read
       if (__any(sum != sum)) {
-        pa_plain<T, HD>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, sq.len,
+        pa_plain<T, HD, TREE>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, sq.len,
                         sq.n, ex_o[w], ex_ml[w], OS);
       } else {
 #pragma unroll
@@ -600,7 +645,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs A) {
         none ? -INFINITY : (mm - PaType<T>::kOffset + log2f(l)) * 0.69314718055994531f;
 }
 
-template <typename T, int HD, int NT, int NQ>
+template <typename T, int HD, int NT, int NQ, bool TREE>
 hipError_t pa_launch(PaArgs& A) {
   const int64_t units = (int64_t)A.units_per_seq * A.L.table.seqs;
   const int64_t tiles = ((int64_t)A.L.table.width * A.L.kv.page_size + kTile - 1) / kTile;
@@ -610,13 +655,13 @@ hipError_t pa_launch(PaArgs& A) {
   A.part_o = (float*)A.L.workspace;
   A.part_ml = (float2*)(A.part_o + (size_t)2 * A.wgs * A.slots * HD);
   A.share = (int4*)(((uintptr_t)(A.part_ml + (size_t)2 * A.wgs * A.slots) + 15) & ~(uintptr_t)15);
-  hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
+  hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ, TREE>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
   if (tiles > 1)
     hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)units, A.slots), dim3(256), 0, A.L.stream, A);
   return hipGetLastError();
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool TREE>
 hipError_t pa_launch_hd(const PagedAttnLaunch& L) {
   constexpr int kMany = PaType<T>::kPieces;
   PaArgs A;
@@ -631,18 +676,18 @@ hipError_t pa_launch_hd(const PagedAttnLaunch& L) {
   A.wide_q = ((uintptr_t)L.q & 15) == 0 && L.qb % v == 0 && L.qt % v == 0 && L.qh % v == 0;
   const bool same = L.dtype == PaType<T>::kId;
   if constexpr (HD <= 128)
-    if (A.per == 32) return same ? pa_launch<T, HD, 2, 1>(A) : pa_launch<T, HD, 2, kMany>(A);
-  return same ? pa_launch<T, HD, 1, 1>(A) : pa_launch<T, HD, 1, kMany>(A);
+    if (A.per == 32) return same ? pa_launch<T, HD, 2, 1, TREE>(A) : pa_launch<T, HD, 2, kMany, TREE>(A);
+  return same ? pa_launch<T, HD, 1, 1, TREE>(A) : pa_launch<T, HD, 1, kMany, TREE>(A);
 }
 
-template <typename T>
+template <typename T, bool TREE>
 hipError_t pa_launch_type(const PagedAttnLaunch& L) {
   switch (L.kv.hd) {
-    case 32: return pa_launch_hd<T, 32>(L);
-    case 64: return pa_launch_hd<T, 64>(L);
-    case 96: return pa_launch_hd<T, 96>(L);
-    case 128: return pa_launch_hd<T, 128>(L);
-    default: return pa_launch_hd<T, 256>(L);
+    case 32: return pa_launch_hd<T, 32, TREE>(L);
+    case 64: return pa_launch_hd<T, 64, TREE>(L);
+    case 96: return pa_launch_hd<T, 96, TREE>(L);
+    case 128: return pa_launch_hd<T, 128, TREE>(L);
+    default: return pa_launch_hd<T, 256, TREE>(L);
   }
 }
 

@@ -12,36 +12,13 @@
 // token takes as long as a launch does.
 #include "nrq_page.h"
 #include "nrq_serve_launch.h"
+#include "nrq_turn.h"
 
 namespace nrq {
 namespace {
 
 constexpr int kRopeNT = 256;
 constexpr int kRopePairs = 512;  // pairs of the tokens of a workgroup: 4 KiB of LDS
-
-__device__ __forceinline__ float2 sincos_turn(int pos, float freq) {
-  const double quarter = (double)pos * (double)freq * 0.63661977236758134308;  // 2 / pi
-  const double n = rint(quarter);
-  const float x = (float)(quarter - n) * 1.57079632679489662f;
-  const int q = (int)(long long)n & 3;
-  const float z = x * x;
-  float s = fmaf(z, 1.0f / 362880, -1.0f / 5040);
-  s = fmaf(z, s, 1.0f / 120);
-  s = fmaf(z, s, -1.0f / 6);
-  s = fmaf(x * z, s, x);
-  float c = fmaf(z, -1.0f / 3628800, 1.0f / 40320);
-  c = fmaf(z, c, -1.0f / 720);
-  c = fmaf(z, c, 1.0f / 24);
-  c = fmaf(z, c, -0.5f);
-  c = fmaf(z, c, 1.0f);
-  const float a = q & 1 ? s : c, b = q & 1 ? c : s;  // magnitudes of cosine and sine
-  return make_float2(q == 1 || q == 2 ? -a : a, q >= 2 ? -b : b);
-}
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T v[V];
-};
 
 constexpr int kRopeTokens = 64;  // tokens of a workgroup at most
 constexpr int kRopeAhead = 4;    // rows of a thread whose loads are on their way together

@@ -55,6 +55,7 @@ struct PagedAttnLaunch {
   float* lse;
   void* workspace;
   hipStream_t stream;
+  const int* parents = nullptr;  // [seqs][n_new]: the new tokens are a tree's nodes (launch_tree_attn)
 };
 constexpr int kPagedTile = 128;  // positions of a tile; where a sequence holds no more there is no join
 size_t paged_attn_units(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd);
@@ -71,9 +72,13 @@ struct VerifyLaunch {
   int seqs, n_new, vocab;
   void* workspace;
   hipStream_t stream;
+  const int* parents = nullptr;  // [seqs][n_new]: the drafted tokens are a tree's nodes (launch_verify_tree)
+  int* path = nullptr;
 };
 size_t verify_workspace(size_t seqs, size_t vocab);
 hipError_t launch_verify(const VerifyLaunch& L);
+size_t verify_tree_workspace(size_t seqs, size_t vocab);
+hipError_t launch_verify_tree(const VerifyLaunch& L);
 
 bool mx_quantize_fits(size_t rows, size_t cols);  // whether a grid holds the values
 hipError_t launch_mx_quantize(const void* src, int dtype, size_t rows, size_t cols, int64_t stride, void* q, void* s,

@@ -1,0 +1,252 @@
+// C ABI of the operators for trees of drafts (declared in include/nrq_tree.h): argument
+// checks, then one or two kernel launches on the caller's stream.
+#include "../../include/nrq_tree.h"
+
+#include "nrq_rows.h"
+#include "nrq_serve_check.h"
+#include "nrq_tree_launch.h"
+
+namespace {
+
+// A tensor of up to three dimensions of rows, for the question whether two share memory. Exact where the rows of both
+// are those of one dimension once dimensions without gaps between them are taken together; else two that lie
+// between one another count as sharing.
+struct Extent {
+  const void* first;
+  size_t len;  // elements of a row
+  int size;    // bytes of one
+  Dim d[3];
+};
+
+nrq::Rows as_rows(const Extent& e) {
+  nrq::Rows r{e.first, 1, 0, e.len, e.size};
+  Dim d[3];
+  int n = 0;
+  for (const Dim& x : e.d) {
+    if (x.n == 0) return nrq::Rows{e.first, 0, 0, 0, e.size};
+    if (x.n == 1 || x.stride == 0) continue;
+    int i = n++;
+    for (; i > 0 && (d[i - 1].stride < 0 ? -d[i - 1].stride : d[i - 1].stride) > (x.stride < 0 ? -x.stride : x.stride); i--)
+      d[i] = d[i - 1];
+    d[i] = x;
+  }
+  // all but the outermost: from their least address to their greatest
+  __int128 low = 0, high = (__int128)e.len;
+  for (int i = 0; i + 1 < n; i++) {
+    const __int128 span = (__int128)d[i].stride * (__int128)(d[i].n - 1);
+    (span < 0 ? low : high) += span;
+  }
+  if (high - low > (__int128)INT64_MAX / 16) high = low + INT64_MAX / 16;  // past any memory
+  r.first = (const char*)e.first + (int64_t)(low * e.size);
+  r.len = (size_t)(high - low);
+  if (n) r.n = d[n - 1].n, r.stride = d[n - 1].stride;
+  return r;
+}
+
+bool meet(const Extent& a, const Extent& b) { return nrq::rows_meet(as_rows(a), as_rows(b)); }
+
+Extent whole(const void* p, size_t n, int size) { return Extent{p, p ? n : 0, size, {{0, 1}, {0, 1}, {0, 1}}}; }
+
+int apart_from(const char* name, const Extent& out, std::initializer_list<Extent> others) {
+  for (const Extent& o : others)
+    if (o.first && meet(out, o)) return fail(NRQ_ERR_ARG, name, "an output shares memory with an input or another output");
+  return NRQ_OK;
+}
+
+Extent heads_of(const void* p, int dtype, size_t tokens, int64_t ts, size_t heads, int64_t hs, size_t hd) {
+  return Extent{p, hd, (int)bytes_of(dtype), {{ts, tokens}, {hs, heads}, {0, 1}}};
+}
+
+int norm_check(const char* name, float eps, const float* wq, const float* wk) {
+  if (!(eps >= 0.0f) || eps > 3e38f) return fail(NRQ_ERR_ARG, name, "eps of %g", (double)eps);
+  if (!aligned(wq, 4) || !aligned(wk, 4)) return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
+  return NRQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nrq_dev_norm_rope(void* y, const void* x, int dtype, size_t tokens, size_t heads, size_t head_dim,
+                      const int64_t strides[4], const float* weight, float eps, const int32_t* pos,
+                      const float* freqs, size_t n_freqs, int style, float scale, void* stream) {
+  static const char* name = "nrq_dev_norm_rope";
+  int rc;
+  if (tokens == 0 || heads == 0) return device_check(name, stream);
+  if (!strides) return fail(NRQ_ERR_ARG, name, "null pointer");
+  nrq::NormRopeLaunch N{};
+  nrq::RopeLaunch& L = N.r;
+  L.y = y, L.x = x, L.dtype = dtype, L.pos = pos, L.freqs = freqs;
+  L.xt = strides[0], L.xh = strides[1], L.yt = strides[2], L.yh = strides[3];
+  if ((rc = rope_check(name, L, tokens, heads, head_dim, n_freqs, style))) return rc;
+  if ((rc = norm_check(name, eps, weight, nullptr))) return rc;
+  L.tokens = (int)tokens, L.heads = (int)heads, L.hd = (int)head_dim, L.nf = (int)n_freqs;
+  L.neox = style == NRQ_ROPE_NEOX, L.scale = scale, L.stream = (hipStream_t)stream;
+  N.norm = true, N.wq = weight, N.eps = eps;
+  if ((rc = device_check(name, stream))) return rc;
+  const Extent out = heads_of(y, dtype, tokens, L.yt, heads, L.yh, head_dim);
+  if (y != x && (rc = apart_from(name, out, {heads_of(x, dtype, tokens, L.xt, heads, L.xh, head_dim)}))) return rc;
+  if ((rc = apart_from(name, out, {whole(weight, head_dim, 4), whole(pos, tokens, 4), whole(freqs, n_freqs, 4)}))) return rc;
+  return launched(name, nrq::launch_norm_rope(N));
+}
+
+int nrq_dev_norm_rope_append(void* y, const void* q, const void* k, const void* v, int dtype, size_t tokens,
+                             size_t heads, const int64_t strides[8], int norm, const float* q_weight,
+                             const float* k_weight, float eps, const int32_t* pos, const int32_t* seq,
+                             const int32_t* at, const float* freqs, size_t n_freqs, int style, float scale,
+                             const nrq_paged_kv* kv, const nrq_page_table* table, void* stream) {
+  static const char* name = "nrq_dev_norm_rope_append";
+  int rc;
+  nrq::NormRopeLaunch N{};
+  nrq::RopeLaunch& L = N.r;
+  if (!table) return fail(NRQ_ERR_ARG, name, "null table");
+  if ((rc = kv_check(name, kv, table, &L.kv, &L.table))) return rc;
+  if (heads == 0) return fail(NRQ_ERR_SHAPE, name, "no heads");
+  if (tokens == 0) return device_check(name, stream);
+  if (!strides || !k || !v || !seq) return fail(NRQ_ERR_ARG, name, "null pointer");
+  L.y = y, L.x = q, L.k = k, L.v = v, L.dtype = dtype, L.pos = pos, L.seq = seq, L.freqs = freqs;
+  L.xt = strides[0], L.xh = strides[1], L.kt = strides[2], L.kh = strides[3];
+  L.vt = strides[4], L.vh = strides[5], L.yt = strides[6], L.yh = strides[7];
+  const size_t hd = (size_t)kv->head_dim, n_kv = (size_t)kv->n_kv_heads;
+  if ((rc = rope_check(name, L, tokens, heads, hd, n_freqs, style))) return rc;
+  if (n_kv * hd > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "%d KV heads", kv->n_kv_heads);
+  if (!apart(hd, {{kv->page_stride, (size_t)kv->n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, (size_t)kv->page_size}}))
+    return fail(NRQ_ERR_ARG, name, "the cache's positions overlap");
+  if (!aligned(k, bytes_of(dtype)) || !aligned(v, bytes_of(dtype)) || !aligned(seq, 4) || !aligned(at, 4))
+    return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
+  if (norm && (rc = norm_check(name, eps, q_weight, k_weight))) return rc;
+  L.tokens = (int)tokens, L.heads = (int)heads, L.hd = (int)hd, L.nf = (int)n_freqs;
+  L.neox = style == NRQ_ROPE_NEOX, L.scale = scale, L.stream = (hipStream_t)stream;
+  N.norm = norm != 0, N.wq = q_weight, N.wk = k_weight, N.eps = eps, N.at = at;
+  if ((rc = device_check(name, stream))) return rc;
+  const Extent qe = heads_of(q, dtype, tokens, L.xt, heads, L.xh, hd), ke = heads_of(k, dtype, tokens, L.kt, n_kv, L.kh, hd),
+               ve = heads_of(v, dtype, tokens, L.vt, n_kv, L.vh, hd), ye = heads_of(y, dtype, tokens, L.yt, heads, L.yh, hd);
+  if (y != q && (rc = apart_from(name, ye, {qe}))) return rc;
+  if ((rc = apart_from(name, ye, {ke, ve}))) return rc;
+  for (const void* pool : {kv->k, kv->v}) {
+    const Extent c{pool, hd, 2, {{kv->page_stride, (size_t)kv->n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, (size_t)kv->page_size}}};
+    if ((rc = apart_from(name, c, {qe, ke, ve, ye}))) return rc;
+  }
+  return launched(name, nrq::launch_norm_rope(N));
+}
+
+int nrq_tree_attention_workspace(size_t seqs, size_t n_new, size_t heads, const nrq_paged_kv* kv, size_t* bytes) {
+  static const char* name = "nrq_tree_attention_workspace";
+  if (!bytes || !kv) return fail(NRQ_ERR_ARG, name, "null pointer");
+  if (kv->n_kv_heads < 1 || heads < 1 || heads % kv->n_kv_heads)
+    return fail(NRQ_ERR_SHAPE, name, "%zu heads over %d KV heads", heads, kv->n_kv_heads);
+  if (!paged_hd(kv->head_dim)) return fail(NRQ_ERR_UNSUPPORTED, name, "heads of %d", kv->head_dim);
+  if (n_new > nrq::kTreeMost) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu nodes (at most 64)", n_new);
+  *bytes = nrq::tree_attn_workspace(seqs, n_new, heads, kv->n_kv_heads, kv->head_dim);
+  return NRQ_OK;
+}
+
+int nrq_dev_tree_attention(void* out, const void* q, int dtype, size_t n_new, size_t heads, const int64_t strides[6],
+                           const nrq_paged_kv* kv, const nrq_page_table* table, const int32_t* lens,
+                           const int32_t* parents, const int32_t* counts, float scale, int32_t window, float* lse,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  static const char* name = "nrq_dev_tree_attention";
+  int rc;
+  nrq::PagedAttnLaunch L{};
+  if (n_new > nrq::kTreeMost) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu nodes (at most 64)", n_new);
+  if ((rc = attn_check(name, out, q, dtype, n_new, heads, strides, kv, table, lens, counts, scale, window, lse, &L))) return rc;
+  if (!L.out) return device_check(name, stream);  // nothing to do
+  if (!parents) return fail(NRQ_ERR_ARG, name, "null pointer");
+  if (!aligned(parents, 4)) return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
+  const size_t need = nrq::tree_attn_workspace((size_t)table->seqs, n_new, heads, kv->n_kv_heads, kv->head_dim);
+  if ((rc = workspace_check(name, workspace, workspace_bytes, need))) return rc;
+  L.parents = parents, L.workspace = workspace, L.stream = (hipStream_t)stream;
+  if ((rc = device_check(name, stream))) return rc;
+  const size_t hd = (size_t)kv->head_dim, seqs = (size_t)table->seqs, e = bytes_of(dtype);
+  const Extent oe{out, hd, (int)e, {{L.ob, seqs}, {L.ot, n_new}, {L.oh, heads}}}, we = whole(workspace, need, 1),
+               se = whole(lse, seqs * n_new * heads, 4);
+  const Extent in[] = {{q, hd, (int)e, {{L.qb, seqs}, {L.qt, n_new}, {L.qh, heads}}},
+                       whole(lens, seqs, 4),
+                       whole(parents, seqs * n_new, 4),
+                       whole(counts, seqs, 4),
+                       {table->pages, (size_t)table->width, 4, {{table->stride, seqs}, {0, 1}, {0, 1}}}};
+  for (const Extent& i : in)
+    for (const Extent* o : {&oe, &we, &se})
+      if (o->first && (rc = apart_from(name, *o, {i}))) return rc;
+  if ((rc = apart_from(name, oe, {we, se})) || (lse && (rc = apart_from(name, se, {we})))) return rc;
+  return launched(name, nrq::launch_tree_attn(L));
+}
+
+int nrq_verify_tree_workspace(size_t seqs, size_t vocab, size_t* bytes) {
+  if (!bytes) return fail(NRQ_ERR_ARG, "nrq_verify_tree_workspace", "null pointer");
+  *bytes = nrq::verify_tree_workspace(seqs, vocab);
+  return NRQ_OK;
+}
+
+int nrq_dev_verify_tree(int32_t* tokens, int32_t* path, int32_t* accepted, const float* target,
+                        const int64_t strides[2], const int32_t* drafted, const int32_t* parents,
+                        const float* uniforms, const int32_t* counts, size_t seqs, size_t n_new, size_t vocab,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  static const char* name = "nrq_dev_verify_tree";
+  int rc;
+  if (n_new > nrq::kTreeMost) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu nodes (at most 64)", n_new);
+  if (n_new < 1) return fail(NRQ_ERR_SHAPE, name, "a tree without a root");
+  if (vocab < 1) return fail(NRQ_ERR_SHAPE, name, "empty vocabulary");
+  if (vocab > (size_t)1 << 30 || seqs > (size_t)1 << 24)
+    return fail(NRQ_ERR_UNSUPPORTED, name, "%zu sequences, vocabulary of %zu", seqs, vocab);
+  if (seqs == 0) return device_check(name, stream);
+  if (!strides || !tokens || !path || !accepted || !target || !drafted || !parents || !uniforms)
+    return fail(NRQ_ERR_ARG, name, "null pointer");
+  const void* words[] = {tokens, path, accepted, target, drafted, parents, uniforms, counts};
+  for (const void* p : words)
+    if (!aligned(p, 4)) return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
+  const size_t need = nrq::verify_tree_workspace(seqs, vocab), all = seqs * n_new;
+  if ((rc = workspace_check(name, workspace, workspace_bytes, need))) return rc;
+  nrq::VerifyLaunch L{tokens,   accepted, target, nullptr,    strides[0], strides[1], 0,         0,
+                      drafted,  uniforms, counts, (int)seqs, (int)n_new, (int)vocab, workspace, (hipStream_t)stream,
+                      parents,  path};
+  if ((rc = device_check(name, stream))) return rc;
+  const Extent out[] = {whole(tokens, all, 4), whole(path, all, 4), whole(accepted, seqs, 4), whole(workspace, need, 1)};
+  const Extent in[] = {{target, vocab, 4, {{strides[0], seqs}, {strides[1], n_new}, {0, 1}}},
+                       whole(drafted, all, 4), whole(parents, all, 4), whole(uniforms, all, 4), whole(counts, seqs, 4)};
+  for (int i = 0; i < 4; i++) {
+    for (const Extent& e : in)
+      if ((rc = apart_from(name, out[i], {e}))) return rc;
+    for (int j = 0; j < i; j++)
+      if ((rc = apart_from(name, out[i], {out[j]}))) return rc;
+  }
+  return launched(name, nrq::launch_verify_tree(L));
+}
+
+int nrq_dev_keep_path(int32_t* new_lens, size_t layers, int64_t layer_stride, const nrq_paged_kv* kv,
+                      const nrq_page_table* table, const int32_t* lens, const int32_t* path, const int32_t* counts,
+                      size_t n_new, void* stream) {
+  static const char* name = "nrq_dev_keep_path";
+  int rc;
+  nrq::KeepLaunch L{};
+  if (!table) return fail(NRQ_ERR_ARG, name, "null table");
+  if ((rc = kv_check(name, kv, table, &L.kv, &L.table))) return rc;
+  if (n_new > nrq::kTreeMost) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu nodes (at most 64)", n_new);
+  const size_t n_kv = (size_t)kv->n_kv_heads, hd = (size_t)kv->head_dim, seqs = (size_t)table->seqs;
+  if (n_kv * hd > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "%d KV heads of %d", kv->n_kv_heads, kv->head_dim);
+  if (layers > (size_t)1 << 12) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu layers (at most 4096)", layers);
+  if ((double)layers * (double)n_kv * (double)hd > 1073741824.0)
+    return fail(NRQ_ERR_UNSUPPORTED, name, "%zu layers of %d KV heads of %d", layers, kv->n_kv_heads, kv->head_dim);
+  const int64_t held = (int64_t)table->width * kv->page_size;  // positions of a sequence at most
+  if (held > (int64_t)1 << 30) return fail(NRQ_ERR_UNSUPPORTED, name, "%lld positions of a sequence (at most 2^30)", (long long)held);
+  if (seqs == 0) return device_check(name, stream);
+  if (!new_lens || !lens || (n_new && !path)) return fail(NRQ_ERR_ARG, name, "null pointer");
+  if (!aligned(new_lens, 4) || !aligned(lens, 4) || !aligned(path, 4) || !aligned(counts, 4))
+    return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
+  if (layers > 1 && (layer_stride < 0 || layer_stride % 8)) return fail(NRQ_ERR_ARG, name, "layer stride is not a multiple of 8");
+  if (!apart(hd, {{layer_stride, layers},
+                  {kv->page_stride, (size_t)kv->n_pages},
+                  {kv->head_stride, n_kv},
+                  {kv->pos_stride, (size_t)kv->page_size}}))
+    return fail(NRQ_ERR_ARG, name, "the caches' positions overlap");
+  L.new_lens = new_lens, L.layers = (int)layers, L.layer_stride = layers > 1 ? layer_stride : 0;
+  L.lens = lens, L.path = path, L.counts = counts, L.n_new = (int)n_new, L.stream = (hipStream_t)stream;
+  if ((rc = device_check(name, stream))) return rc;
+  if ((rc = apart_from(name, whole(new_lens, seqs, 4),
+                       {whole(lens, seqs, 4), whole(path, seqs * n_new, 4), whole(counts, seqs, 4),
+                        {table->pages, (size_t)table->width, 4, {{table->stride, seqs}, {0, 1}, {0, 1}}}})))
+    return rc;
+  return launched(name, nrq::launch_keep(L));
+}
+
+}  // extern "C"

@@ -1,6 +1,6 @@
 // nightrun_amd._serve: what nightrun_amd/serve.py calls. Takes torch tensors
 // apart, checks types, shapes, layouts and devices (ValueError) and calls the C
-// ABI (include/nrq_serve.h) on torch's current stream; returns its status. In C++
+// ABI (include/nrq_serve.h, include/nrq_tree.h) on torch's current stream; returns its status. In C++
 // because a decode step's calls last a few microseconds each, which is what a dozen
 // attribute reads and a ctypes call take in Python.
 #include <Python.h>
@@ -13,7 +13,7 @@
 #include <stdexcept>
 #include <string>
 
-#include "../../include/nrq_serve.h"
+#include "../../include/nrq_tree.h"
 
 namespace {
 
@@ -154,11 +154,20 @@ BIND(rope, 6) {
                       (float)number(a[5]), stream);
 }
 
-// y, q, k, v, pos, seq, freqs, k_pages, v_pages, table, neox, scale
-BIND(rope_append, 12) {
+// what an append takes apart
+struct Append {
+  void *y, *q, *k, *v;
+  int dtype;
+  size_t tokens, heads;
+  int64_t s[8];
+  const int32_t *pos, *seq;
+  nrq_paged_kv kv;
+  nrq_page_table t;
+};
+Append append(PyObject* const* a, PyObject* po, PyObject* so, PyObject* kpo, PyObject* vpo, PyObject* to, long dev) {
   const at::Tensor &y = tensor(a[0], "y"), &q = tensor(a[1], "q"), &k = tensor(a[2], "k"), &v = tensor(a[3], "v"),
-                   &pos = tensor(a[4], "pos"), &seq = tensor(a[5], "seq"), &f = tensor(a[6], "freqs"),
-                   &kp = tensor(a[7], "k_pages"), &vp = tensor(a[8], "v_pages"), &tab = tensor(a[9], "table");
+                   &pos = tensor(po, "pos"), &seq = tensor(so, "seq"), &kp = tensor(kpo, "k_pages"),
+                   &vp = tensor(vpo, "v_pages"), &tab = tensor(to, "table");
   rows(q, "q", 3);
   rows(k, "k", 3);
   rows(v, "v", 3);
@@ -171,15 +180,61 @@ BIND(rope_append, 12) {
                   k.size(2) == q.size(2) && q.size(2) == kv.head_dim,
               "k: got ", k.scalar_type(), " ", k.sizes(), " with q ", q.scalar_type(), " ", q.sizes(), " and pages ",
               kp.sizes());
-  const int64_t s[8] = {q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), y.stride(0), y.stride(1)};
-  return nrq_dev_rope_append(on(y, "y", dev), on(q, "q", dev), on(k, "k", dev), on(v, "v", dev), kind(q, "q"),
-                             q.size(0), q.size(1), s, ints(pos, "pos", dev, {q.size(0)}),
-                             ints(seq, "seq", dev, {q.size(0)}), freqs(f, dev), f.numel(), (int)integer(a[10]),
-                             (float)number(a[11]), &kv, &t, stream);
+  return Append{on(y, "y", dev), on(q, "q", dev), on(k, "k", dev), on(v, "v", dev), kind(q, "q"), (size_t)q.size(0),
+                (size_t)q.size(1),
+                {q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), y.stride(0), y.stride(1)},
+                ints(pos, "pos", dev, {q.size(0)}), ints(seq, "seq", dev, {q.size(0)}), kv, t};
 }
 
-// y, q, k_pages, v_pages, table, lens, scale, window, counts or None, lse or None
-BIND(paged_attention, 10) {
+// y, q, k, v, pos, seq, freqs, k_pages, v_pages, table, neox, scale
+BIND(rope_append, 12) {
+  const Append p = append(a, a[4], a[5], a[7], a[8], a[9], dev);
+  const at::Tensor& f = tensor(a[6], "freqs");
+  return nrq_dev_rope_append(p.y, p.q, p.k, p.v, p.dtype, p.tokens, p.heads, p.s, p.pos, p.seq, freqs(f, dev), f.numel(),
+                             (int)integer(a[10]), (float)number(a[11]), &p.kv, &p.t, stream);
+}
+
+// f32 [head_dim], contiguous, or None
+const float* weight(PyObject* o, const char* what, int64_t hd, long dev) {
+  return o == Py_None ? nullptr : (const float*)exactly(tensor(o, what), what, dev, at::kFloat, {hd});
+}
+
+// y, x, weight or None, pos, freqs, eps, neox, scale
+BIND(norm_rope, 8) {
+  const at::Tensor &y = tensor(a[0], "y"), &x = tensor(a[1], "x"), &pos = tensor(a[3], "pos"), &f = tensor(a[4], "freqs");
+  rows(x, "x", 3);
+  rows(y, "y", 3);
+  same(y, x, "y");
+  const int64_t s[4] = {x.stride(0), x.stride(1), y.stride(0), y.stride(1)};
+  return nrq_dev_norm_rope(on(y, "y", dev), on(x, "x", dev), kind(x, "x"), x.size(0), x.size(1), x.size(2), s,
+                           weight(a[2], "weight", x.size(2), dev), (float)number(a[5]), ints(pos, "pos", dev, {x.size(0)}),
+                           freqs(f, dev), f.numel(), (int)integer(a[6]), (float)number(a[7]), stream);
+}
+
+// y, q, k, v, norm, q_weight or None, k_weight or None, pos, seq, freqs, k_pages, v_pages, table, eps, neox, scale, at or None
+BIND(norm_rope_append, 17) {
+  const Append p = append(a, a[7], a[8], a[10], a[11], a[12], dev);
+  const at::Tensor& f = tensor(a[9], "freqs");
+  const int32_t* at = a[16] == Py_None ? nullptr : ints(tensor(a[16], "at"), "at", dev, {(int64_t)p.tokens});
+  return nrq_dev_norm_rope_append(p.y, p.q, p.k, p.v, p.dtype, p.tokens, p.heads, p.s, (int)integer(a[4]),
+                                  weight(a[5], "q_weight", p.kv.head_dim, dev), weight(a[6], "k_weight", p.kv.head_dim, dev),
+                                  (float)number(a[13]), p.pos, p.seq, at, freqs(f, dev), f.numel(), (int)integer(a[14]),
+                                  (float)number(a[15]), &p.kv, &p.t, stream);
+}
+
+// what an attention takes apart
+struct Attend {
+  void *y, *q;
+  int dtype;
+  size_t seqs, n, heads;
+  int64_t s[6];
+  nrq_paged_kv kv;
+  nrq_page_table t;
+  const int32_t *lens, *counts;
+  int32_t window;
+  float* lse;
+};
+Attend attend(PyObject* const* a, PyObject* wo, PyObject* co, PyObject* lo, long dev) {
   const at::Tensor &y = tensor(a[0], "y"), &q = tensor(a[1], "q"), &kp = tensor(a[2], "k_pages"),
                    &vp = tensor(a[3], "v_pages"), &tab = tensor(a[4], "table"), &lens = tensor(a[5], "lens");
   rows(q, "q", 4);
@@ -189,22 +244,38 @@ BIND(paged_attention, 10) {
   const nrq_page_table t = page_table(tab, dev);
   VALUE_CHECK(t.seqs == q.size(0) && kv.head_dim == q.size(3), "q ", q.sizes(), " does not go with pages ", kp.sizes(),
               " and table ", tab.sizes());
-  const size_t n = q.size(1), heads = q.size(2);
-  const int32_t* counts = a[8] == Py_None ? nullptr : ints(tensor(a[8], "counts"), "counts", dev, {q.size(0)});
+  const int32_t* counts = co == Py_None ? nullptr : ints(tensor(co, "counts"), "counts", dev, {q.size(0)});
   float* lse = nullptr;
-  if (a[9] != Py_None)
-    lse = (float*)exactly(tensor(a[9], "lse"), "lse", dev, at::kFloat, {q.size(0), q.size(1), q.size(2)});
+  if (lo != Py_None) lse = (float*)exactly(tensor(lo, "lse"), "lse", dev, at::kFloat, {q.size(0), q.size(1), q.size(2)});
   const int32_t* len = ints(lens, "lens", dev, {q.size(0)});
-  const long window = integer(a[7]);
+  const long window = integer(wo);
   VALUE_CHECK(window >= 0 && window <= INT32_MAX, "window: ", window);
-  void *yp = on(y, "y", dev), *qp = on(q, "q", dev);
+  return Attend{on(y, "y", dev), on(q, "q", dev), kind(q, "q"), (size_t)q.size(0), (size_t)q.size(1), (size_t)q.size(2),
+                {q.stride(0), q.stride(1), q.stride(2), y.stride(0), y.stride(1), y.stride(2)},
+                kv, t, len, counts, (int32_t)window, lse};
+}
+
+// y, q, k_pages, v_pages, table, lens, scale, window, counts or None, lse or None
+BIND(paged_attention, 10) {
+  const Attend p = attend(a, a[7], a[8], a[9], dev);
   size_t need;
-  const int rc = nrq_paged_attention_workspace(q.size(0), n, heads, &kv, &need);
+  const int rc = nrq_paged_attention_workspace(p.seqs, p.n, p.heads, &p.kv, &need);
   if (rc) return rc;
-  const at::Tensor ws = workspace(need, q);
-  const int64_t s[6] = {q.stride(0), q.stride(1), q.stride(2), y.stride(0), y.stride(1), y.stride(2)};
-  return nrq_dev_paged_attention(yp, qp, kind(q, "q"), n, heads, s, &kv, &t, len, counts, (float)number(a[6]),
-                                 (int32_t)window, lse, ws.data_ptr(), need, stream);
+  const at::Tensor ws = workspace(need, tensor(a[1], "q"));
+  return nrq_dev_paged_attention(p.y, p.q, p.dtype, p.n, p.heads, p.s, &p.kv, &p.t, p.lens, p.counts, (float)number(a[6]),
+                                 p.window, p.lse, ws.data_ptr(), need, stream);
+}
+
+// y, q, k_pages, v_pages, table, lens, parents, scale, window, counts or None, lse or None
+BIND(tree_attention, 11) {
+  const Attend p = attend(a, a[8], a[9], a[10], dev);
+  const int32_t* parents = ints(tensor(a[6], "parents"), "parents", dev, {(int64_t)p.seqs, (int64_t)p.n});
+  size_t need;
+  const int rc = nrq_tree_attention_workspace(p.seqs, p.n, p.heads, &p.kv, &need);
+  if (rc) return rc;
+  const at::Tensor ws = workspace(need, tensor(a[1], "q"));
+  return nrq_dev_tree_attention(p.y, p.q, p.dtype, p.n, p.heads, p.s, &p.kv, &p.t, p.lens, parents, p.counts,
+                                (float)number(a[7]), p.window, p.lse, ws.data_ptr(), need, stream);
 }
 
 // tokens, accepted, target, draft or None, drafted, uniforms, counts or None
@@ -235,6 +306,50 @@ BIND(verify_drafts, 7) {
   if (rc) return rc;
   const at::Tensor ws = workspace(need, target);
   return nrq_dev_verify_drafts(tp, ap, p, dp, s, xp, up, counts, b, r - 1, vocab, ws.data_ptr(), need, stream);
+}
+
+// tokens, path, accepted, target, drafted, parents, uniforms, counts or None
+BIND(verify_tree, 8) {
+  const at::Tensor& target = tensor(a[3], "target");
+  rows(target, "target", 3);
+  const int64_t b = target.size(0), r = target.size(1), vocab = target.size(2);
+  VALUE_CHECK(target.scalar_type() == at::kFloat && r > 0, "target: expected float32 [sequences, nodes, vocabulary]");
+  int32_t* tp = (int32_t*)ints(tensor(a[0], "tokens"), "tokens", dev, {b, r});
+  int32_t* pp = (int32_t*)ints(tensor(a[1], "path"), "path", dev, {b, r});
+  int32_t* ap = (int32_t*)ints(tensor(a[2], "accepted"), "accepted", dev, {b});
+  const int32_t* xp = ints(tensor(a[4], "drafted"), "drafted", dev, {b, r});
+  const int32_t* parents = ints(tensor(a[5], "parents"), "parents", dev, {b, r});
+  const float* up = (const float*)exactly(tensor(a[6], "uniforms"), "uniforms", dev, at::kFloat, {b, r});
+  const int32_t* counts = a[7] == Py_None ? nullptr : ints(tensor(a[7], "counts"), "counts", dev, {b});
+  const float* p = (const float*)on(target, "target", dev);
+  const int64_t s[2] = {target.stride(0), target.stride(1)};
+  size_t need;
+  const int rc = nrq_verify_tree_workspace(b, vocab, &need);
+  if (rc) return rc;
+  const at::Tensor ws = workspace(need, target);
+  return nrq_dev_verify_tree(tp, pp, ap, p, s, xp, parents, up, counts, b, r, vocab, ws.data_ptr(), need, stream);
+}
+
+// new_lens, k_pages, v_pages, table, lens, path, counts or None; pages with or without the layers in front
+BIND(keep_path, 7) {
+  const at::Tensor &kp = tensor(a[1], "k_pages"), &vp = tensor(a[2], "v_pages"), &path = tensor(a[5], "path");
+  const bool deep = kp.dim() == 5;
+  VALUE_CHECK(vp.dim() == kp.dim(), "k_pages and v_pages differ in type, shape or strides");
+  size_t layers = 1;
+  int64_t stride = 0;
+  if (deep) {
+    VALUE_CHECK(kp.size(0) == vp.size(0) && kp.stride(0) == vp.stride(0), "k_pages and v_pages differ in type, shape or strides");
+    layers = kp.size(0), stride = kp.stride(0);
+  }
+  const nrq_page_table t = page_table(tensor(a[3], "table"), dev);
+  VALUE_CHECK(path.dim() == 2, "path: expected [sequences, nodes], got ", path.sizes());
+  int32_t* np = (int32_t*)ints(tensor(a[0], "new_lens"), "new_lens", dev, {t.seqs});
+  const int32_t* lp = ints(tensor(a[4], "lens"), "lens", dev, {t.seqs});
+  const int32_t* pp = ints(path, "path", dev, {t.seqs, path.size(1)});
+  const int32_t* counts = a[6] == Py_None ? nullptr : ints(tensor(a[6], "counts"), "counts", dev, {t.seqs});
+  VALUE_CHECK(layers > 0, "k_pages: no layers");
+  const nrq_paged_kv kv = deep ? paged(kp.select(0, 0), vp.select(0, 0), dev) : paged(kp, vp, dev);
+  return nrq_dev_keep_path(np, layers, stride, &kv, &t, lp, pp, counts, path.size(1), stream);
 }
 
 // src, q, scales
@@ -300,7 +415,9 @@ BIND(linear_mxfp4, 4) {
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(rope),           METHOD(rope_append),      METHOD(paged_attention),
                          METHOD(verify_drafts),  METHOD(quantize_mxfp4),   METHOD(dequantize_mxfp4),
-                         METHOD(matmul_mxfp4),   METHOD(linear_mxfp4),     {nullptr, nullptr, 0, nullptr}};
+                         METHOD(matmul_mxfp4),   METHOD(linear_mxfp4),     METHOD(norm_rope),
+                         METHOD(norm_rope_append), METHOD(tree_attention), METHOD(verify_tree),
+                         METHOD(keep_path),      {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_serve", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,197 @@
+"""include/nrq_tree.h without a GPU: its symbols, what it refuses, and what a node of a tree sees
+(csrc/nrq_tree_mask.h compiled for the host)."""
+import ctypes as C
+import os
+import random
+import re
+import subprocess
+
+import pytest
+
+from tests.test_serve_abi import _call, _i64, _kv, _table
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "nrq_tree.h")
+ARG, SHAPE, UNSUPPORTED, NOT_INIT = -1, -2, -4, -5
+P = 1 << 20  # aligned addresses that nothing reads, 2^32 apart
+
+
+def at(i):
+    return P + (i << 32)
+
+
+def test_symbols():
+    from nightrun_amd import _lib
+
+    names = re.findall(r"^int (nrq_\w+)\(", open(HEADER).read(), flags=re.M)
+    assert sorted(names) == sorted(_lib.TREE_SIGNATURES) and len(names) == 7
+    L = C.CDLL(_lib.LIB_PATH)
+    for n in names:
+        assert hasattr(L, n), n
+
+
+def test_header_is_plain_c(tmp_path):
+    src = tmp_path / "t.c"
+    src.write_text('#include "nrq_tree.h"\nint main(void) { return sizeof(nrq_paged_kv) == 64 ? 0 : 1; }\n')
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.dirname(HEADER), str(src), "-o",
+                    str(tmp_path / "t")], check=True)
+
+
+def _norm():
+    return dict(y=at(0), x=at(1), dtype=0, tokens=5, heads=4, hd=128, strides=_i64(512, 128, 512, 128), weight=at(2),
+                eps=1e-6, pos=at(3), freqs=at(4), nf=64, style=1, scale=1.0, stream=None)
+
+
+def _append():
+    return dict(y=at(0), q=at(1), k=at(2), v=at(3), dtype=0, tokens=5, heads=32,
+                strides=_i64(4096, 128, 1024, 128, 1024, 128, 4096, 128), norm=1, q_weight=at(4), k_weight=at(5),
+                eps=1e-6, pos=at(6), seq=at(7), at=at(8), freqs=at(9), nf=64, style=0, scale=1.0,
+                kv=_kv(k=at(10), v=at(11)), table=_table(), stream=None)
+
+
+def _attend():
+    return dict(out=at(0), q=at(1), dtype=0, n_new=2, heads=32, strides=_i64(8192, 4096, 128, 8192, 4096, 128),
+                kv=_kv(), table=_table(pages=at(2)), lens=at(3), parents=at(4), counts=None, scale=0.1, window=0,
+                lse=None, ws=at(5), ws_bytes=1 << 30, stream=None)
+
+
+def _verify():
+    return dict(tokens=at(0), path=at(1), accepted=at(2), target=at(3), strides=_i64(4000, 1000), drafted=at(4),
+                parents=at(5), uniforms=at(6), counts=None, seqs=2, n_new=4, vocab=1000, ws=at(7), ws_bytes=1 << 20,
+                stream=None)
+
+
+def _keep():
+    return dict(new_lens=at(0), layers=2, layer_stride=10 * 8 * 16 * 128, kv=_kv(), table=_table(pages=at(1)),
+                lens=at(2), path=at(3), counts=None, n_new=8, stream=None)
+
+
+CALLS = {"nrq_dev_norm_rope": _norm, "nrq_dev_norm_rope_append": _append, "nrq_dev_tree_attention": _attend,
+         "nrq_dev_verify_tree": _verify, "nrq_dev_keep_path": _keep}
+
+REFUSED = [
+    ("nrq_dev_norm_rope", dict(dtype=1), ARG, "unknown type"),
+    ("nrq_dev_norm_rope", dict(eps=-1e-6), ARG, "eps"),
+    ("nrq_dev_norm_rope", dict(eps=float("nan")), ARG, "eps"),
+    ("nrq_dev_norm_rope", dict(eps=float("inf")), ARG, "eps"),
+    ("nrq_dev_norm_rope", dict(weight=P + 2), ARG, "aligned"),
+    ("nrq_dev_norm_rope", dict(nf=65), SHAPE, "frequencies"),
+    ("nrq_dev_norm_rope", dict(tokens=1 << 31), UNSUPPORTED, "tokens"),
+    ("nrq_dev_norm_rope", dict(strides=None), ARG, "null"),
+    ("nrq_dev_norm_rope", dict(pos=None), ARG, "null"),
+    ("nrq_dev_norm_rope", dict(strides=_i64(512, 128, 512, 64)), ARG, "overlap"),
+    ("nrq_dev_norm_rope", dict(y=at(1), strides=_i64(1024, 128, 512, 128)), ARG, "in place"),
+    ("nrq_dev_norm_rope_append", dict(eps=-1.0), ARG, "eps"),
+    ("nrq_dev_norm_rope_append", dict(k_weight=P + 1), ARG, "aligned"),
+    ("nrq_dev_norm_rope_append", dict(at=P + 2), ARG, "aligned"),
+    ("nrq_dev_norm_rope_append", dict(seq=None), ARG, "null"),
+    ("nrq_dev_norm_rope_append", dict(v=None), ARG, "null"),
+    ("nrq_dev_norm_rope_append", dict(table=None), ARG, "null"),
+    ("nrq_dev_norm_rope_append", dict(heads=0), SHAPE, "no heads"),
+    ("nrq_dev_norm_rope_append", dict(kv=_kv(pos_stride=64)), ARG, "overlap"),
+    ("nrq_dev_norm_rope_append", dict(kv=_kv(dtype=0)), ARG, "type"),
+    ("nrq_dev_tree_attention", dict(n_new=65), UNSUPPORTED, "64"),
+    ("nrq_dev_tree_attention", dict(parents=None), ARG, "null"),
+    ("nrq_dev_tree_attention", dict(parents=P + 2), ARG, "aligned"),
+    ("nrq_dev_tree_attention", dict(heads=31), SHAPE, "31 heads"),
+    ("nrq_dev_tree_attention", dict(window=-1), ARG, "window"),
+    ("nrq_dev_tree_attention", dict(kv=_kv(head_dim=80)), UNSUPPORTED, "heads of 80"),
+    ("nrq_dev_tree_attention", dict(ws_bytes=100), ARG, "workspace of 100"),
+    ("nrq_dev_tree_attention", dict(ws=None), ARG, "workspace"),
+    ("nrq_dev_tree_attention", dict(strides=_i64(8192, 4096, 128, 8192, 4096, 120)), ARG, "overlap"),
+    ("nrq_dev_tree_attention", dict(lens=None), ARG, "null"),
+    ("nrq_dev_verify_tree", dict(n_new=65), UNSUPPORTED, "64"),
+    ("nrq_dev_verify_tree", dict(n_new=0), SHAPE, "root"),
+    ("nrq_dev_verify_tree", dict(vocab=0), SHAPE, "vocabulary"),
+    ("nrq_dev_verify_tree", dict(path=None), ARG, "null"),
+    ("nrq_dev_verify_tree", dict(parents=None), ARG, "null"),
+    ("nrq_dev_verify_tree", dict(uniforms=P + 2), ARG, "aligned"),
+    ("nrq_dev_verify_tree", dict(ws_bytes=8), ARG, "workspace"),
+    ("nrq_dev_keep_path", dict(n_new=65), UNSUPPORTED, "64"),
+    ("nrq_dev_keep_path", dict(layers=4097), UNSUPPORTED, "layers"),
+    ("nrq_dev_keep_path", dict(layer_stride=12), ARG, "multiple of 8"),
+    ("nrq_dev_keep_path", dict(layer_stride=1024), ARG, "overlap"),
+    ("nrq_dev_keep_path", dict(path=None), ARG, "null"),
+    ("nrq_dev_keep_path", dict(new_lens=None), ARG, "null"),
+    ("nrq_dev_keep_path", dict(lens=P + 1), ARG, "aligned"),
+    ("nrq_dev_keep_path", dict(table=_table(width=2 ** 26 + 1, stride=2 ** 27)), UNSUPPORTED, "2^30"),
+]
+
+
+@pytest.mark.parametrize("name,change,code,text", REFUSED, ids=[f"{n[8:]}-{'-'.join(c)}-{i}" for i, (n, c, _, _) in
+                                                               enumerate(REFUSED)])
+def test_refusals(name, change, code, text):
+    rc, msg = _call(name, CALLS[name](), **change)
+    assert rc == code and text in msg and msg.startswith(name), (rc, msg)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_without_a_device(name):
+    """Good arguments: refused for want of nrq_init, never a silent fallback."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("checks the no-GPU failure path")
+    assert _call(name, CALLS[name]())[0] == NOT_INIT
+    nothing = {"nrq_dev_tree_attention": "n_new", "nrq_dev_verify_tree": "seqs", "nrq_dev_keep_path": "n_new"}
+    assert _call(name, CALLS[name](), **{nothing.get(name, "tokens"): 0})[0] == NOT_INIT
+
+
+def test_workspaces():
+    from nightrun_amd import _lib
+
+    L, n = _lib.lib(), C.c_size_t()
+    assert L.nrq_verify_tree_workspace(3, 5000, C.byref(n)) == 0 and 0 < n.value <= 3 * 5000 * 16
+    assert L.nrq_verify_tree_workspace(3, 5000, None) == ARG
+    assert L.nrq_tree_attention_workspace(3, 8, 32, _kv(), C.byref(n)) == 0 and n.value >= 4 * 130 * 4
+    assert L.nrq_tree_attention_workspace(3, 65, 32, _kv(), C.byref(n)) == UNSUPPORTED
+    assert L.nrq_tree_attention_workspace(3, 8, 33, _kv(), C.byref(n)) == SHAPE
+    assert L.nrq_tree_attention_workspace(3, 8, 32, _kv(), None) == ARG
+
+
+# ---- what a node sees -----------------------------------------------------------------------------
+
+
+@pytest.fixture(scope="module")
+def mask(tmp_path_factory):
+    d = tmp_path_factory.mktemp("mask")
+    src = d / "mask.cpp"
+    src.write_text('''#include "nrq_tree_mask.h"
+extern "C" {
+int parent(int p, int j) { return nrq::tree_parent(p, j); }
+uint32_t sees(uint64_t above, int p0, int base) { return nrq::tree_sees(above, p0, base); }
+uint32_t from(int lo, int p0, int base) { return nrq::tree_from(lo, p0, base); }
+}
+''')
+    so = d / "mask.so"
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-Wall", "-Werror", "-fsanitize=undefined",
+                    "-fno-sanitize-recover", "-static-libubsan", "-I", os.path.join(ROOT, "nightrun_amd", "csrc"),
+                    str(src), "-o", str(so)], check=True)
+    L = C.CDLL(str(so))
+    L.sees.argtypes, L.sees.restype = [C.c_uint64, C.c_int, C.c_int], C.c_uint32
+    getattr(L, "from").restype = C.c_uint32
+    return L
+
+
+def test_parents(mask):
+    for j in range(64):
+        for p in (-2 ** 31, -1, 0, j - 1, j, j + 1, 63, 64, 2 ** 31 - 1):
+            assert mask.parent(p, j) == (p if 0 <= p < j else -1)
+
+
+def test_bits(mask):
+    """Every bit of every 32 positions around the tree, trees before position 0 and at the largest positions among them."""
+    rng = random.Random(3)
+    low = getattr(mask, "from")
+    for base in (-64, -40, -1, 0, 1, 31, 32, 33, 100, 2 ** 30, 2 ** 30 - 64):
+        for _ in range(40):
+            above = rng.getrandbits(64)
+            lo = rng.choice([0, base, base - 1, base - 40, base + 3, base + 70, 2 ** 30, rng.randint(0, 200)])
+            lo = max(lo, 0)
+            for p0 in {max(0, base + d) for d in (-70, -64, -33, -32, -31, -16, -1, 0, 1, 16, 31, 32, 33, 63, 64, 65, 90)}:
+                s, f = mask.sees(above, p0, base), low(lo, p0, base)
+                for i in range(32):
+                    t = p0 + i
+                    r = t - base
+                    assert s >> i & 1 == (1 if r < 0 else (above >> r & 1 if r < 64 else 0)), (above, p0, base, i)
+                    assert f >> i & 1 == int(t >= lo or r >= 0), (lo, p0, base, i)
