@@ -115,6 +115,27 @@ __device__ __forceinline__ void pa_store(void* o, int dtype, int64_t at, float v
     ((__bf16*)o)[at] = (__bf16)v;
 }
 
+// Four of a row, together where `wide`.
+template <typename T>
+__device__ __forceinline__ void pa_put4(T* o, bool wide, const float* v) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  const t4 x = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+  if (wide) {
+    *(t4*)o = x;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = x[i];
+  }
+}
+__device__ __forceinline__ void pa_store4(void* o, int dtype, int64_t at, bool wide, const float* v) {
+  if (dtype == kF32)
+    pa_put4((float*)o + at, wide, v);
+  else if (dtype == kF16)
+    pa_put4((_Float16*)o + at, wide, v);
+  else
+    pa_put4((__bf16*)o + at, wide, v);
+}
+
 template <typename T>
 struct PaType;
 template <>
@@ -264,12 +285,12 @@ __device__ __forceinline__ PaTree pa_node(const PaTree& t, int j) {
 }
 
 // The same stretch of one wave without matrix instructions, position by position and row by
-// row, for values that hold an infinity or a NaN: there the products of weights
+// row, 32 positions of every `step`, for values that hold an infinity or a NaN: there the products of weights
 // that are 0 (rows that do not see a position) or of the pieces of a weight would give
 // NaN. Dimension lane + 64 e is the lane's.
 template <typename T, int HD, bool TREE>
-__device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int row0, int rows, int p0, int stop, int len,
-                                      int n, float* ex_o, float (*ex_ml)[2], int os) {
+__device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int row0, int rows, int p0, int stop, int step,
+                                      int len, int n, float* ex_o, float (*ex_ml)[2], int os) {
   constexpr int E = (HD + 63) / 64;
   const PagedAttnLaunch& L = A.L;
   const int lane = threadIdx.x & 63;
@@ -293,7 +314,7 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
                : L.dtype == kF16 ? (float)((const _Float16*)L.q)[qa + d]
                                  : (float)((const __bf16*)L.q)[qa + d];
     }
-    for (int t0 = p0; t0 < stop; t0 += kTile)
+    for (int t0 = p0; t0 < stop; t0 += step)
       for (int t = max(t0, TREE ? 0 : lo); t < min(t0 + 32, hi + 1); t++) {
         if (TREE && !(tree_sees(node.above, t, len - n) & 1 && (t >= lo || t >= len - n))) continue;
         const uint32_t place = pa_place(L, pages, t, TREE ? 0 : lo, min(len, hi + 1));
@@ -533,8 +554,8 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       }
       __syncthreads();  // the queries are read
       if (__any(sum != sum)) {
-        pa_plain<T, HD, TREE>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, sq.len,
-                        sq.n, ex_o[w], ex_ml[w], OS);
+        pa_plain<T, HD, TREE>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, kTile,
+                        sq.len, sq.n, ex_o[w], ex_ml[w], OS);
       } else {
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -645,6 +666,28 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PaArgs A) {
         none ? -INFINITY : (mm - PaType<T>::kOffset + log2f(l)) * 0.69314718055994531f;
 }
 
+// The line of a call whose units are `per` rows.
+inline PaArgs pa_args(const PagedAttnLaunch& L, int per) {
+  PaArgs A;
+  A.L = L;
+  A.group = L.heads / L.kv.n_kv;
+  A.rows = L.n_new * A.group;
+  A.per = per;
+  A.row_tiles = (A.rows + per - 1) / per;
+  A.units_per_seq = L.kv.n_kv * A.row_tiles;
+  A.slots = A.rows < per ? A.rows : per;
+  const int v = L.dtype == kF32 ? 4 : 8;
+  A.wide_q = ((uintptr_t)L.q & 15) == 0 && L.qb % v == 0 && L.qt % v == 0 && L.qh % v == 0;
+  return A;
+}
+
+// Parts for the join, of A.wgs workgroups.
+inline void pa_workspace(PaArgs& A, int hd) {
+  A.part_o = (float*)A.L.workspace;
+  A.part_ml = (float2*)(A.part_o + (size_t)2 * A.wgs * A.slots * hd);
+  A.share = (int4*)(((uintptr_t)(A.part_ml + (size_t)2 * A.wgs * A.slots) + 15) & ~(uintptr_t)15);
+}
+
 template <typename T, int HD, int NT, int NQ, bool TREE>
 hipError_t pa_launch(PaArgs& A) {
   const int64_t units = (int64_t)A.units_per_seq * A.L.table.seqs;
@@ -652,9 +695,7 @@ hipError_t pa_launch(PaArgs& A) {
   const int64_t most = units * (tiles > 0 ? tiles : 1), fill = 256 * pa_resident(HD, NT);
   static_assert(256 * pa_resident(HD, NT) <= kPaMaxWgs, "workspace");
   A.wgs = (int)(most < fill ? most : fill);
-  A.part_o = (float*)A.L.workspace;
-  A.part_ml = (float2*)(A.part_o + (size_t)2 * A.wgs * A.slots * HD);
-  A.share = (int4*)(((uintptr_t)(A.part_ml + (size_t)2 * A.wgs * A.slots) + 15) & ~(uintptr_t)15);
+  pa_workspace(A, HD);
   hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ, TREE>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
   if (tiles > 1)
     hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)units, A.slots), dim3(256), 0, A.L.stream, A);
@@ -664,16 +705,7 @@ hipError_t pa_launch(PaArgs& A) {
 template <typename T, int HD, bool TREE>
 hipError_t pa_launch_hd(const PagedAttnLaunch& L) {
   constexpr int kMany = PaType<T>::kPieces;
-  PaArgs A;
-  A.L = L;
-  A.group = L.heads / L.kv.n_kv;
-  A.rows = L.n_new * A.group;
-  A.per = pa_per(HD, A.rows);
-  A.row_tiles = (A.rows + A.per - 1) / A.per;
-  A.units_per_seq = L.kv.n_kv * A.row_tiles;
-  A.slots = A.rows < A.per ? A.rows : A.per;
-  const int v = L.dtype == kF32 ? 4 : 8;
-  A.wide_q = ((uintptr_t)L.q & 15) == 0 && L.qb % v == 0 && L.qt % v == 0 && L.qh % v == 0;
+  PaArgs A = pa_args(L, pa_per(HD, (size_t)L.n_new * (L.heads / L.kv.n_kv)));
   const bool same = L.dtype == PaType<T>::kId;
   if constexpr (HD <= 128)
     if (A.per == 32) return same ? pa_launch<T, HD, 2, 1, TREE>(A) : pa_launch<T, HD, 2, kMany, TREE>(A);

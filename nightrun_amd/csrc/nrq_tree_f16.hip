@@ -1,17 +1,21 @@
 // Attention of a tree's nodes over an f16 cache, and the dispatch by the cache's type.
-#include "nrq_paged.h"
-#include "nrq_tree_launch.h"
+#include "nrq_tree_attn.h"
 
 namespace nrq {
 
 hipError_t launch_tree_bf16(const PagedAttnLaunch& L);
 
 size_t tree_attn_workspace(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd) {
-  return paged_attn_workspace(seqs, n_new, heads, n_kv, hd);
+  const size_t rows = n_new * (heads / n_kv);
+  const size_t few = paged_attn_workspace(seqs, n_new, heads, n_kv, hd);
+  if (rows <= ta_few(hd)) return few;
+  // units of 64 rows at least, parts of 256 at most
+  const size_t units = seqs * n_kv * ((rows + 63) / 64), slots = rows < 256 ? rows : 256;
+  return 2 * (size_t)kTaWgs * slots * ((size_t)hd * sizeof(float) + sizeof(float2)) + 16 + units * sizeof(int4);
 }
 
 hipError_t launch_tree_attn(const PagedAttnLaunch& L) {
-  return L.kv.dtype == kF16 ? pa_launch_type<_Float16, true>(L) : launch_tree_bf16(L);
+  return L.kv.dtype == kF16 ? ta_launch_type<_Float16>(L) : launch_tree_bf16(L);
 }
 
 }  // namespace nrq
