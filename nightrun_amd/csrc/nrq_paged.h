@@ -50,6 +50,7 @@ struct PaArgs {
   int wgs;
   int slots;            // rows of a unit that there are: min(rows, per)
   int wide_q;           // q in 16-byte loads
+  int setup;            // tiles that the beginning of a unit counts for in the line, beside its own
   float* part_o;        // [2 * wgs][slots][hd]
   float2* part_ml;      // [2 * wgs][slots]: maximum (log2 units), sum
   int4* share;          // [units]: first and last workgroup, rows
@@ -75,9 +76,10 @@ struct PaLine {
 };
 __device__ __forceinline__ PaLine pa_line(const PaArgs& A, int wg) {
   const int lane = threadIdx.x & 63, seqs = A.L.table.seqs;
-  const int mine = lane < seqs ? pa_seq(A.L, lane).tiles * A.units_per_seq : 0;
+  auto length = [&](int b) { return (pa_seq(A.L, b).tiles + A.setup) * A.units_per_seq; };
+  const int mine = lane < seqs ? length(lane) : 0;
   int t = mine;
-  for (int b = lane + 64; b < seqs; b += 64) t += pa_seq(A.L, b).tiles * A.units_per_seq;
+  for (int b = lane + 64; b < seqs; b += 64) t += length(b);
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) t += __shfl_xor(t, m);
   PaLine p;
@@ -86,7 +88,7 @@ __device__ __forceinline__ PaLine pa_line(const PaArgs& A, int wg) {
   p.at = wg < p.wgs ? line_start(wg, p.total, p.wgs) : p.total;
   int base = 0;
   for (int b0 = 0; b0 < seqs; b0 += 64) {
-    const int own = b0 == 0 ? mine : (b0 + lane < seqs ? pa_seq(A.L, b0 + lane).tiles * A.units_per_seq : 0);
+    const int own = b0 == 0 ? mine : (b0 + lane < seqs ? length(b0 + lane) : 0);
     int sum = own;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -265,9 +267,12 @@ struct PaTree {
   uint64_t above;  // the node and those above it, as far as the window reaches
   int depth;
 };
-__device__ __forceinline__ PaTree pa_tree(const PagedAttnLaunch& L, int b, int n) {
+__device__ __forceinline__ int pa_parent(const PagedAttnLaunch& L, int b, int n) {
   const int lane = threadIdx.x & 63;
-  const int parent = lane < n ? tree_parent(L.parents[(int64_t)b * L.n_new + lane], lane) : -1;
+  return lane < n ? L.parents[(int64_t)b * L.n_new + lane] : -1;
+}
+__device__ __forceinline__ PaTree pa_tree(const PagedAttnLaunch& L, int parent_, int n) {
+  const int lane = threadIdx.x & 63, parent = tree_parent(parent_, lane);
   PaTree t{lane < n ? 1ull << lane : 0, 0};
   for (int a = lane < n ? lane : -1;;) {  // parents come first, so that this ends
     const int up = __shfl(parent, a & 63);
@@ -296,7 +301,7 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
   const int lane = threadIdx.x & 63;
   const int* pages = L.table.pages + b * L.table.stride;
   PaTree tree;
-  if (TREE) tree = pa_tree(L, b, n);
+  if (TREE) tree = pa_tree(L, pa_parent(L, b, n), n);
   for (int r = 0; r < rows; r++) {
     const int rr = row0 + r, tok = rr / A.group;
     PaTree node;
@@ -437,7 +442,7 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       int lo[NT], hi[NT];  // what the row sees
       uint64_t above[NT];
       PaTree tree;
-      if (TREE) tree = pa_tree(L, b, sq.n);
+      if (TREE) tree = pa_tree(L, pa_parent(L, b, sq.n), sq.n);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         to_log2[n] = unit_log2[16 * n + c];
@@ -676,6 +681,7 @@ inline PaArgs pa_args(const PagedAttnLaunch& L, int per) {
   A.row_tiles = (A.rows + per - 1) / per;
   A.units_per_seq = L.kv.n_kv * A.row_tiles;
   A.slots = A.rows < per ? A.rows : per;
+  A.setup = 0;
   const int v = L.dtype == kF32 ? 4 : 8;
   A.wide_q = ((uintptr_t)L.q & 15) == 0 && L.qb % v == 0 && L.qt % v == 0 && L.qh % v == 0;
   return A;

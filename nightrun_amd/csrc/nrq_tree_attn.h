@@ -22,6 +22,7 @@
 namespace nrq {
 
 constexpr int kTaWgs = 256;  // workgroups: one a CU
+constexpr int kTaSetup = 2;  // what the beginning and the end of a unit cost, in tiles
 
 // Rows of a KV head that nrq_paged.h takes: one unit of its.
 inline size_t ta_few(int hd) { return hd <= 128 ? 32 : 16; }
@@ -57,23 +58,69 @@ __device__ __forceinline__ u32x2 ta_read_tr(const uint8_t* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)p));
 }
 
+__device__ const uint32_t ta_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
+
+// 16 bytes a lane from memory to LDS, lane after lane from byte address m0 (wave-uniform)
+__device__ __forceinline__ void ta_dma16(const void* g, uint32_t m0) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(g) : "memory");
+}
+
+// The pieces of eight weights, as pa_split() has them, in fewer instructions: conversions by twos, the rest of a
+// value in one fused step.
+template <typename T, int N>
+__device__ __forceinline__ void ta_split(const float* f, typename PaType<T>::v8* out) {
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) r[i] = f[i];
+#pragma unroll
+  for (int k = 0; k < N; k++)
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const t2 x = __builtin_convertvector((f2{r[i], r[i + 1]}), t2);
+      out[k][i] = x[0], out[k][i + 1] = x[1];
+      if (k + 1 < N) r[i] = fmaf((float)x[0], -1.0f, r[i]), r[i + 1] = fmaf((float)x[1], -1.0f, r[i + 1]);
+    }
+}
+
 // W waves, WR of them side by side over the rows, TP positions of a stage.
 template <int HD, int W, int WR, int TP>
 struct TaShape {
   static constexpr int kNT = 64 * W, kWP = W / WR, kRows = 32 * WR;
   static constexpr int kChunks = HD / 8;                     // 16-byte chunks of a row
-  static constexpr int kK = HD * 2 + 16;                     // bytes from row to row: an odd number of chunks
-  static constexpr int kV = HD * 2 + (HD % 64 == 0 ? 64 : 0);
-  static constexpr int kStage = TP * (kK + kV);
-  static constexpr int kLoads = TP * kChunks / kNT;          // chunks of a thread
+  static constexpr int kRow = HD * 2;                        // bytes
+  static constexpr int kStage = 2 * TP * kRow;               // keys, then values
+  static constexpr int kLoads = TP * kChunks / kNT;          // chunks of a thread, of keys and of values
   static constexpr int kAcc = HD / 2;                        // accumulators of a lane
-  // waves that hand their results to the first of their rows, 16 accumulators of a lane at a time
+  // waves that hand their results to the first of their rows
   static constexpr int kJoin = (W - WR) * 64 * kAcc * 4;
   static constexpr int kPlain = W * HD * 9 * 4;              // the plain way: 8 rows of a wave at a time
   static constexpr int kMost = kJoin > kPlain ? kJoin : kPlain;
   static constexpr int kLds = 2 * kStage > kMost ? 2 * kStage : kMost;
   static_assert(TP * kChunks % kNT == 0 && (TP == 64 || TP == 128) && TP / 32 >= kWP, "stages");
-  static_assert(kK % 32 == 16 && kV % 128 == 64, "rows without bank conflicts");
+
+  // Where chunk c of a row's keys lies in the row: 16 rows from any on have it on 16 different places of the 64 banks.
+  static __device__ __forceinline__ int key_chunk(int row, int c) {
+    if constexpr (HD % 128 == 0) return c ^ (row & 15);
+    if constexpr (HD == 64) return c ^ (row >> 1 & 7);
+    if constexpr (HD == 32) return c ^ (row >> 2 & 3);
+    const int x = c + (row >> 2 & 3);  // rows of 12 chunks
+    return x < kChunks ? x : x - kChunks;
+  }
+  // The chunk of a row's keys that lies at place p.
+  static __device__ __forceinline__ int key_at(int row, int p) {
+    if constexpr (HD != 96) return key_chunk(row, p);
+    const int x = p - (row >> 2 & 3);
+    return x < 0 ? x + kChunks : x;
+  }
+  // The same for values, both ways: the 64 bytes that hold a dimension of four rows from a multiple of 4 on lie in
+  // four different quarters of the banks.
+  static __device__ __forceinline__ int value_chunk(int row, int c) {
+    if constexpr (HD % 128 == 0) return c ^ (row & 3) << 2;
+    if constexpr (HD == 64) return c ^ (row >> 1 & 1) << 2;
+    return c;
+  }
 };
 
 template <typename T, int HD, int W, int WR, int TP, int NQ, int NP>
@@ -87,6 +134,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
   const int wr = w % WR, wp = w / WR;
 
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)shared;
+
   const PaLine line = pa_line(A, blockIdx.x);
   const int total = line.total, wgs = line.wgs;
   if ((int)blockIdx.x >= wgs) return;
@@ -94,16 +143,17 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
   const int stop = line_start(blockIdx.x + 1, total, wgs);
   while (at < stop) {
     const SeqSpan sq = pa_seq(L, b);
-    const int unit = (at - first) / sq.tiles;
-    const int t_begin = at - first - unit * sq.tiles;
-    const int t_end = min(sq.tiles, t_begin + (stop - at));
+    // a unit's place in the line: what its beginning costs, then its tiles
+    const int length = sq.tiles + A.setup, unit = (at - first) / length;
+    const int v_begin = at - first - unit * length, v_end = min(length, v_begin + (stop - at));
+    const int t_begin = max(0, v_begin - A.setup), t_end = max(0, v_end - A.setup);
     const int head = unit / A.row_tiles, rt = unit - head * A.row_tiles;
     const int row0 = rt * Sh::kRows, rows = min(Sh::kRows, sq.n * A.group - row0);
     const bool whole = t_begin == 0 && t_end == sq.tiles;
-    if (t_begin == 0 && threadIdx.x == 0)
+    if (t_begin == 0 && t_end > 0 && threadIdx.x == 0)
       A.share[b * A.units_per_seq + unit] =
-          make_int4(blockIdx.x, whole ? (int)blockIdx.x : line_owner(at + sq.tiles - 1, total, wgs), rows, 0);
-    if (rows > 0) {
+          make_int4(blockIdx.x, whole ? (int)blockIdx.x : line_owner(first + (unit + 1) * length - 1, total, wgs), rows, 0);
+    if (rows > 0 && t_begin < t_end) {
       const int base = sq.len - sq.n;
       const int begin = L.window > 0 ? max(0, base - L.window + 1) : 0, end = sq.len;
       const int last_lo = L.window > 0 ? max(0, end - L.window) : 0;  // what the deepest node may see first
@@ -113,49 +163,71 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
       const int s_begin = sq.start + t_begin * kTile;  // the stretch's first position
       const int stages = (t_end - t_begin) * (kTile / TP);
 
-      // ---- the way of a stage: places (a lane has those of positions lane and lane + 64), loads, LDS
-      uint32_t place[2];
-      u32x4 lk[Sh::kLoads], lv[Sh::kLoads];
-      uint32_t on = 0;             // of the loads in registers, those of a place
-      uint64_t live[2] = {0, 0};   // of the stage in registers
-      auto find = [&](int st) {
-        place[0] = place[1] = kNoPlace;
-        if (st < stages) {
-          place[0] = pa_place(L, pages, s_begin + st * TP + lane, begin, end);
-          if (TP > 64) place[1] = pa_place(L, pages, s_begin + st * TP + 64 + lane, begin, end);
+      // ---- the way of a stage: a lane asks for the pages of positions lane and lane + 64, one stage later has their
+      // places and the loads go out, another stage later what they brought goes to LDS. The pages are asked for before
+      // the loads and looked at behind them: loads come back in order, and a wait for a page right after it is asked for were one for
+      // all loads before it.
+      constexpr int kHalf = TP / 64;
+      uint32_t column[kHalf], within[kHalf], page[kHalf], place[kHalf];
+      uint64_t asked[kHalf];
+      const uint32_t size = L.kv.page_size, steps = TP / size, rest = TP - steps * size;
+#pragma unroll
+      for (int i = 0; i < kHalf; i++) {
+        const uint32_t t = s_begin + 64 * i + lane;
+        column[i] = t / size, within[i] = t - column[i] * size;
+      }
+      uint64_t live[2] = {0, 0};   // of the stage on its way
+      auto ask = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < kHalf; i++) {
+          const int t = s_begin + st * TP + 64 * i + lane;
+          const bool ok = st < stages && t >= begin && t < end && column[i] < (uint32_t)L.table.width;
+          asked[i] = __ballot(ok);
+          page[i] = 0;
+          if (asked[i]) page[i] = pages[ok ? column[i] : 0];  // where any is, the table has a column
         }
       };
-      auto load = [&]() {
+      auto look = [&]() {  // behind ask()
+#pragma unroll
+        for (int i = 0; i < kHalf; i++) {
+          const bool ok = (asked[i] >> lane & 1) && page[i] < (uint32_t)L.kv.n_pages;
+          place[i] = ok ? page[i] * L.kv.page_stride8 + within[i] * L.kv.pos_stride8 : kNoPlace;
+          column[i] += steps, within[i] += rest;
+          if (within[i] >= size) within[i] -= size, column[i]++;
+        }
+      };
+      auto load = [&](int st) {
         live[0] = __ballot(place[0] != kNoPlace);
-        live[1] = TP > 64 ? __ballot(place[1] != kNoPlace) : 0;
-        on = 0;
-        if (!(live[0] | live[1])) return;  // the pool may be empty
+        live[1] = kHalf > 1 ? __ballot(place[kHalf - 1] != kNoPlace) : 0;
+        if (!(live[0] | live[1])) return;
+        const uint32_t to = lds + (st & 1) * Sh::kStage + w * 1024;
 #pragma unroll
         for (int i = 0; i < Sh::kLoads; i++) {
-          const int e = (int)threadIdx.x + Sh::kNT * i, row = e / Sh::kChunks, ch = e - row * Sh::kChunks;
+          const int e = (int)threadIdx.x + Sh::kNT * i, row = e / Sh::kChunks, at_ = e - row * Sh::kChunks;
           uint32_t p = __shfl((int)place[0], row & 63);
-          if (TP > 64) {
-            const uint32_t q = __shfl((int)place[1], row & 63);
-            p = row < 64 ? p : q;
+          if (kHalf > 1) {
+            const uint32_t p1 = __shfl((int)place[kHalf - 1], row & 63);
+            p = row < 64 ? p : p1;
           }
-          // positions without a place read the pool's first: no load is conditional
-          on |= p != kNoPlace ? 1u << i : 0;
-          const uint64_t o = (uint64_t)(p == kNoPlace ? 0 : p) * 8 + 8 * ch;
-          lk[i] = *(const u32x4*)(kp + o);
-          lv[i] = *(const u32x4*)(vp + o);
+          // positions without a place are zeros: weights of 0 would not clear what a page holds, a NaN
+          const uint64_t o = (uint64_t)p * 8;
+          const uint16_t* fk = p == kNoPlace ? (const uint16_t*)ta_zeros : kp + (o + 8 * Sh::key_at(row, at_));
+          const uint16_t* fv = p == kNoPlace ? (const uint16_t*)ta_zeros : vp + (o + 8 * Sh::value_chunk(row, at_));
+          ta_dma16(fk, to + Sh::kNT * 16 * i);
+          ta_dma16(fv, to + Sh::kNT * 16 * i + TP * Sh::kRow);
         }
       };
-      find(0);
-      load();
-      find(1);
-
+      __syncthreads();  // what the unit before left in LDS is read
+      ask(0);
       // ---- queries: lane l has 8 dimensions of each 16 of row l % 32
       const int r = min(row0 + 32 * wr + c, sq.n * A.group - 1), tok = r / A.group;
       const int64_t qa = b * L.qb + tok * L.qt + (head * A.group + r - tok * A.group) * L.qh + 8 * h;
       v8 q[KS][NQ];
-      float to_log2 = L.scale * kLog2e;  // what brings the row's products to log2 units
+      PaTree node;  // what the row sees
+      float to_log2 = fabsf(L.scale) * kLog2e;  // what brings the row's products to log2 units; its sign goes into the queries
       {
         float big = 0.0f, f[KS][8];
+        const int parent = pa_parent(L, b, sq.n);
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           if (NQ == 1)
@@ -166,25 +238,39 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
             pa_load8((const _Float16*)L.q + qa + 16 * s, A.wide_q, f[s]);
           else
             pa_load8((const __bf16*)L.q + qa + 16 * s, A.wide_q, f[s]);
+        }
+        // pages, parents and queries are on their way together; the first stage's loads go out as soon as its pages are there
+        __builtin_amdgcn_sched_barrier(0);
+        look();
+        ask(1);
+        load(0);
+        __builtin_amdgcn_sched_barrier(0);
+        node = pa_node(pa_tree(L, parent, sq.n), tok);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
 #pragma unroll
           for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(f[s][i]));
-        }
-        float up = 1.0f;
+        float up = L.scale < 0.0f ? -1.0f : 1.0f;
         if (NQ > 1) {  // the largest magnitude of the row to [2^13, 2^14)
           big = fmaxf(big, __shfl_xor(big, 32));
           const int e = min(max((int)(__float_as_uint(big) >> 23), 27), 253);  // small rows: as if 2^-100
-          up = __uint_as_float((uint32_t)(267 - e) << 23);
-          to_log2 *= 1.0f / up;
+          const float by = __uint_as_float((uint32_t)(267 - e) << 23);
+          up *= by;
+          to_log2 *= 1.0f / by;
         }
+        if (to_log2 == 0.0f) up = 0.0f, to_log2 = 1.0f;  // times 0, a masked score were NaN
 #pragma unroll
         for (int s = 0; s < KS; s++) {
 #pragma unroll
           for (int i = 0; i < 8; i++) f[s][i] *= up;
           pa_split<T, NQ>(f[s], q[s]);
         }
+        // they are here before the stages begin: a wait for them in the loop would be one for the next stage's loads too
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+          for (int k = 0; k < NQ; k++) asm volatile("" : "+v"(q[s][k]));
       }
-      // ---- what the row sees
-      const PaTree node = pa_node(pa_tree(L, b, sq.n), tok);
       const int lo = L.window > 0 ? max(0, base + node.depth - L.window + 1) : 0;
 
       float m = -INFINITY, l = 0.0f;
@@ -194,55 +280,60 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
 #pragma unroll
         for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
 
-      __syncthreads();  // what the unit before left in LDS is read
       for (int st = 0; st < stages; st++) {
-        uint8_t* sk = shared + (st & 1) * Sh::kStage;
-        uint8_t* sv = sk + TP * Sh::kK;
+        const uint8_t* sk = shared + (st & 1) * Sh::kStage;
+        const uint8_t* sv = sk + TP * Sh::kRow;
         const uint64_t now[2] = {live[0], live[1]};
-        if (now[0] | now[1]) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the stage is there
+        __syncthreads();                                  // and so are the others', who have read the stage before it
+        look();
+        ask(st + 2);
+        load(st + 1);
+        if (!(now[0] | now[1])) continue;
+        constexpr int US = TP / 32 / WP;  // of 32 positions, the wave's
+        u32x4 ka[KS];
+        auto read_k = [&](int u0) {
+          const int row = 32 * (u0 * WP + wp) + c;
 #pragma unroll
-          for (int i = 0; i < Sh::kLoads; i++) {
-            const int e = (int)threadIdx.x + Sh::kNT * i, row = e / Sh::kChunks, ch = e - row * Sh::kChunks;
-            const bool has = on >> i & 1;
-            u32x4 x = lv[i];
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = has ? x[k] : 0u;  // weights of 0 would not clear a NaN
-            *(u32x4*)(sk + row * Sh::kK + 16 * ch) = lk[i];
-            *(u32x4*)(sv + row * Sh::kV + 16 * ch) = x;
-          }
-        }
-        load();  // the next stage's; its places are known
-        find(st + 2);
-        __syncthreads();
-#pragma unroll
-        for (int u0 = 0; u0 < TP / 32 / WP; u0++) {
+          for (int s = 0; s < KS; s++) ka[s] = *(const u32x4*)(sk + row * Sh::kRow + 16 * Sh::key_chunk(row, 2 * s + h));
+        };
+        read_k(0);
+#pragma unroll 1
+        for (int u0 = 0; u0 < US; u0++) {
           const int u = u0 * WP + wp, p0 = s_begin + st * TP + 32 * u;
           const uint32_t here = (uint32_t)((u < 2 ? now[0] : now[1]) >> (32 * (u & 1)));
-          if (!here) continue;
           f32x16 x;
 #pragma unroll
           for (int i = 0; i < 16; i++) x[i] = 0.0f;
-          const uint8_t* ka = sk + (32 * u + c) * Sh::kK + 16 * h;
 #pragma unroll
-          for (int s = 0; s < KS; s++) {
-            const u32x4 a = *(const u32x4*)(ka + 32 * s);
+          for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int k = NQ - 1; k >= 0; k--) x = TaType<T>::mfma(__builtin_bit_cast(v8, a), q[s][k], x);
-          }
-          float s[16];
+            for (int k = NQ - 1; k >= 0; k--) x = TaType<T>::mfma(__builtin_bit_cast(v8, ka[s]), q[s][k], x);
+          // reads run ahead of the products that take them: the first values' over the softmax, the next keys' over the values'
+          const int vrow = 4 * h + (lane >> 2 & 3), vbyte = (lane & 1) * 8;  // the row's low bits are the same 8 rows on
+          const uint8_t* va = sv + (32 * u + vrow) * Sh::kRow + vbyte;
+          u32x4 vt[2][2];
+          auto read_v = [&](int d) {
+            const uint8_t* y = va + 16 * Sh::value_chunk(vrow, 4 * d + (lane >> 4 & 1) * 2 + (lane >> 1 & 1));
 #pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = x[i] * to_log2;
+            for (int k = 0; k < 2; k++) {
+              const u32x2 y0 = ta_read_tr(y + 16 * k * Sh::kRow), y1 = ta_read_tr(y + (16 * k + 8) * Sh::kRow);
+              vt[d & 1][k] = u32x4{y0[0], y0[1], y1[0], y1[1]};
+            }
+          };
+          read_v(0);
+          __builtin_amdgcn_sched_barrier(0);
           if (!(here == 0xffffffffu && p0 + 31 < base && p0 >= last_lo)) {
-            const uint32_t sees = tree_sees(node.above, p0, base) & tree_from(lo, p0, base) & here;
+            const uint32_t sees = tree_sees(node.above, p0, base) & tree_from(lo, p0, base) & here, mine = sees >> (4 * h);
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = sees >> (8 * (i >> 2) + 4 * h + (i & 3)) & 1 ? s[i] : -INFINITY;
+            for (int i = 0; i < 16; i++) x[i] = mine & 1u << (8 * (i >> 2) + (i & 3)) ? x[i] : -INFINITY;
           }
           // ---- running maximum and sum
-          float top = s[0];
+          float top = x[0];
 #pragma unroll
-          for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+          for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
           top = fmaxf(top, __shfl_xor(top, 32));
-          const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
+          const float mn = fmaxf(m, top * to_log2), ref = mn == -INFINITY ? 0.0f : mn;
           if (__any(mn > m)) {
             const float by = __builtin_amdgcn_exp2f(m - ref);
             l *= by;
@@ -252,28 +343,29 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
               for (int i = 0; i < 16; i++) acc[d][i] *= by;
             m = mn;
           }
+          const float less = PaType<T>::kOffset - ref;
           v8 pp[2][NP];
 #pragma unroll
           for (int k = 0; k < 2; k++) {
             float p[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-              p[i] = __builtin_amdgcn_exp2f(s[8 * k + i] - ref + PaType<T>::kOffset);
+              p[i] = __builtin_amdgcn_exp2f(fmaf(x[8 * k + i], to_log2, less));
               l += p[i];
             }
-            pa_split<T, NP>(p, pp[k]);
+            ta_split<T, NP>(p, pp[k]);
           }
           // ---- O^T += V^T P^T
-          const uint8_t* va = sv + (32 * u + 4 * h + (lane >> 2 & 3)) * Sh::kV + (16 * (lane >> 4 & 1) + 4 * (lane & 3)) * 2;
+          if (u0 + 1 < US) read_k(u0 + 1);
 #pragma unroll
-          for (int d = 0; d < DB; d++)
+          for (int d = 0; d < DB; d++) {
+            if (d + 1 < DB) read_v(d + 1);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-              const u32x2 y0 = ta_read_tr(va + 64 * d + 16 * k * Sh::kV), y1 = ta_read_tr(va + 64 * d + (16 * k + 8) * Sh::kV);
-              const u32x4 a = {y0[0], y0[1], y1[0], y1[1]};
+            for (int k = 0; k < 2; k++)
 #pragma unroll
-              for (int j = NP - 1; j >= 0; j--) acc[d] = TaType<T>::mfma(__builtin_bit_cast(v8, a), pp[k][j], acc[d]);
-            }
+              for (int j = NP - 1; j >= 0; j--) acc[d] = TaType<T>::mfma(__builtin_bit_cast(v8, vt[d & 1][k]), pp[k][j], acc[d]);
+          }
         }
       }
       l += __shfl_xor(l, 32);
@@ -360,13 +452,14 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
           const int hh = head * A.group + r - tok * A.group;
           const int64_t o = b * L.ob + tok * L.ot + hh * L.oh + 4 * h;
           const bool none = m == -INFINITY && l == 0.0f;
+          const float by = 1.0f / l;
 #pragma unroll
           for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
               float y[4];
 #pragma unroll
-              for (int j = 0; j < 4; j++) y[j] = none ? 0.0f : acc[d][4 * i + j] / l;
+              for (int j = 0; j < 4; j++) y[j] = none ? 0.0f : acc[d][4 * i + j] * by;
               pa_store4(L.out, L.dtype, o + 32 * d + 8 * i, wide_o, y);
             }
           if (L.lse && h == 0)
@@ -375,12 +468,61 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
         }
       }
     }
-    at += t_end - t_begin;
-    if (at == first + sq.tiles * A.units_per_seq) {
+    at += v_end - v_begin;
+    if (at == first + length * A.units_per_seq) {
       first = at;
       b++;
     }
   }
+}
+
+// The stretches of a unit that several workgroups shared, in order: 16 lanes a row, 16 rows a workgroup.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void tree_join_kernel(PaArgs A, int wide_o) {
+  constexpr int E = HD / 16, F = E % 4 ? 2 : 4;  // dimensions of a lane, F side by side
+  const PagedAttnLaunch& L = A.L;
+  const int u = blockIdx.x, b = u / A.units_per_seq, unit = u - b * A.units_per_seq;
+  const int4 share = A.share[u];
+  const int r = 16 * blockIdx.y + (threadIdx.x >> 4), c = threadIdx.x & 15, w0 = share.x, n = share.y - w0 + 1;
+  if (n < 2 || r >= share.z) return;
+  const int head = unit / A.row_tiles, rr = (unit - head * A.row_tiles) * A.per + r;
+  auto slot = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * A.slots + r; };
+  float mm = -INFINITY;
+  for (int k = c; k < n; k += 16) mm = fmaxf(mm, A.part_ml[slot(k)].x);
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) mm = fmaxf(mm, __shfl_xor(mm, x, 16));
+  const float ref = mm == -INFINITY ? 0.0f : mm;
+  float o[E], l = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = 0;
+#pragma unroll 4
+  for (int k = 0; k < n; k++) {
+    const int64_t s = slot(k);
+    const float2 x = A.part_ml[s];
+    const float by = __builtin_amdgcn_exp2f(x.x - ref);
+    l += x.y * by;
+    const float* p = A.part_o + s * HD + F * c;
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] += p[e / F * 16 * F + e % F] * by;
+  }
+  const int tok = rr / A.group, h = head * A.group + rr - tok * A.group;
+  const bool none = mm == -INFINITY && l == 0.0f;
+  const float by = 1.0f / l;
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = none ? 0.0f : o[e] * by;
+  const int64_t at = b * L.ob + tok * L.ot + h * L.oh + F * c;
+#pragma unroll
+  for (int e = 0; e < E; e += F) {
+    if constexpr (F == 4) {
+      pa_store4(L.out, L.dtype, at + e / F * 16 * F, wide_o, o + e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < F; i++) pa_store(L.out, L.dtype, at + e / F * 16 * F + i, o[e + i]);
+    }
+  }
+  if (L.lse && c == 0)
+    L.lse[((int64_t)b * L.n_new + tok) * L.heads + h] =
+        none ? -INFINITY : (mm - PaType<T>::kOffset + log2f(l)) * 0.69314718055994531f;
 }
 
 template <typename T, int HD, int W, int WR, int TP, int NQ, int NP>
@@ -388,14 +530,15 @@ hipError_t ta_launch(const PagedAttnLaunch& L) {
   PaArgs A = pa_args(L, 32 * WR);
   const int64_t units = (int64_t)A.units_per_seq * L.table.seqs;
   const int64_t tiles = ((int64_t)L.table.width * L.kv.page_size + kTile - 1) / kTile;
-  const int64_t most = units * (tiles > 0 ? tiles : 1);
+  A.setup = kTaSetup;
+  const int64_t most = units * ((tiles > 0 ? tiles : 1) + A.setup);
   A.wgs = (int)(most < kTaWgs ? most : kTaWgs);
   pa_workspace(A, HD);
   const int v = L.dtype == kF32 ? 4 : 2;  // four values are stored together
   const int wide_o = ((uintptr_t)L.out & (v == 4 ? 15 : 7)) == 0 && L.ob % 4 == 0 && L.ot % 4 == 0 && L.oh % 4 == 0;
   hipLaunchKernelGGL((tree_kernel<T, HD, W, WR, TP, NQ, NP>), dim3(A.wgs), dim3(64 * W), 0, L.stream, A, wide_o);
   if (tiles > 1)
-    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)units, A.slots), dim3(256), 0, L.stream, A);
+    hipLaunchKernelGGL((tree_join_kernel<T, HD>), dim3((unsigned)units, (A.slots + 15) / 16), dim3(256), 0, L.stream, A, wide_o);
   return hipGetLastError();
 }
 
@@ -408,7 +551,7 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
     if (rows > 64) return ta_launch<T, HD, 4, 4, 64, NQ, NP>(L);
     return ta_launch<T, HD, 4, 2, 64, NQ, NP>(L);
   } else {
-    constexpr int kTP = (HD == 128 && NQ == 2) ? 64 : 128;  // registers for a stage of 64 beside the queries' pieces
+    constexpr int kTP = 128;  // registers for a stage of 64 beside the queries' pieces
     if (rows > 128) return ta_launch<T, HD, 8, 8, kTP, NQ, NP>(L);
     if (rows > 64) return ta_launch<T, HD, 8, 4, kTP, NQ, NP>(L);
     return ta_launch<T, HD, 8, 2, 128, NQ, NP>(L);
