@@ -53,10 +53,11 @@ struct TaType<__bf16> {
 // Four positions of one dimension: of 16 lanes, lanes 4 r .. 4 r + 3 name 16 consecutive values of row r, lane i gets
 // the i-th of each of the four rows.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x2 ta_read_tr(const uint8_t* p) {
+__device__ __forceinline__ u32x2 ta_read_tr(uint32_t at) {
   typedef __attribute__((address_space(3))) s16x4* lds;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)p));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)at));
 }
+__device__ __forceinline__ u32x4 ta_read(uint32_t at) { return *(__attribute__((address_space(3))) u32x4*)at; }
 
 __device__ const uint32_t ta_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
 
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
   typedef TaShape<HD, W, WR, TP> Sh;
   typedef typename PaType<T>::v8 v8;
   constexpr int KS = HD / 16, DB = HD / 32, WP = Sh::kWP;
-  __shared__ __align__(16) uint8_t shared[Sh::kLds];
+  __shared__ __align__(512) uint8_t shared[Sh::kLds];  // rows of a stage begin at multiples of their size
   __shared__ float ex_ml[W][32][2];
   const PagedAttnLaunch& L = A.L;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 31, h = lane >> 5;
@@ -281,8 +282,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
         for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
 
       for (int st = 0; st < stages; st++) {
-        const uint8_t* sk = shared + (st & 1) * Sh::kStage;
-        const uint8_t* sv = sk + TP * Sh::kRow;
+        const uint32_t sk = lds + (st & 1) * Sh::kStage, sv = sk + TP * Sh::kRow;
         const uint64_t now[2] = {live[0], live[1]};
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the stage is there
         __syncthreads();                                  // and so are the others', who have read the stage before it
@@ -291,13 +291,22 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
         load(st + 1);
         if (!(now[0] | now[1])) continue;
         constexpr int US = TP / 32 / WP;  // of 32 positions, the wave's
-        u32x4 ka[KS];
-        auto read_k = [&](int u0) {
-          const int row = 32 * (u0 * WP + wp) + c;
+        // the first half of the keys is read ahead, the second while the first is multiplied
+        constexpr int KH = KS / 2;
+        u32x4 ka[KH], kb[KH];
+        auto read_k = [&](int u, int half, u32x4* k) {
+          const int row = 32 * u + c;
+          const uint32_t line = sk + row * Sh::kRow;
 #pragma unroll
-          for (int s = 0; s < KS; s++) ka[s] = *(const u32x4*)(sk + row * Sh::kRow + 16 * Sh::key_chunk(row, 2 * s + h));
+          for (int s = 0; s < KH; s++) {
+            const int ch = 2 * (KH * half + s);
+            if constexpr (HD == 96)
+              k[s] = ta_read(line + 16 * Sh::key_chunk(row, ch + h));
+            else  // the chunk's bits and the row's
+              k[s] = ta_read((line + 16 * Sh::key_chunk(row, h)) ^ (16 * ch));
+          }
         };
-        read_k(0);
+        read_k(wp, 0, ka);
 #pragma unroll 1
         for (int u0 = 0; u0 < US; u0++) {
           const int u = u0 * WP + wp, p0 = s_begin + st * TP + 32 * u;
@@ -305,16 +314,20 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
           f32x16 x;
 #pragma unroll
           for (int i = 0; i < 16; i++) x[i] = 0.0f;
+          read_k(u, 1, kb);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int k = NQ - 1; k >= 0; k--) x = TaType<T>::mfma(__builtin_bit_cast(v8, ka[s]), q[s][k], x);
+            for (int k = NQ - 1; k >= 0; k--)
+              x = TaType<T>::mfma(__builtin_bit_cast(v8, s < KH ? ka[s % KH] : kb[s % KH]), q[s][k], x);
           // reads run ahead of the products that take them: the first values' over the softmax, the next keys' over the values'
-          const int vrow = 4 * h + (lane >> 2 & 3), vbyte = (lane & 1) * 8;  // the row's low bits are the same 8 rows on
-          const uint8_t* va = sv + (32 * u + vrow) * Sh::kRow + vbyte;
+          const int vrow = 4 * h + (lane >> 2 & 3);  // its low bits are the same 8 rows on
+          const uint32_t va = sv + (32 * u + vrow) * Sh::kRow + (lane & 1) * 8 +
+                              16 * Sh::value_chunk(vrow, (lane >> 4 & 1) * 2 + (lane >> 1 & 1));
           u32x4 vt[2][2];
           auto read_v = [&](int d) {
-            const uint8_t* y = va + 16 * Sh::value_chunk(vrow, 4 * d + (lane >> 4 & 1) * 2 + (lane >> 1 & 1));
+            const uint32_t y = HD == 96 ? va + 64 * d : va ^ (64 * d);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
               const u32x2 y0 = ta_read_tr(y + 16 * k * Sh::kRow), y1 = ta_read_tr(y + (16 * k + 8) * Sh::kRow);
@@ -356,7 +369,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
             ta_split<T, NP>(p, pp[k]);
           }
           // ---- O^T += V^T P^T
-          if (u0 + 1 < US) read_k(u0 + 1);
+          if (u0 + 1 < US) read_k(u + WP, 0, ka);
 #pragma unroll
           for (int d = 0; d < DB; d++) {
             if (d + 1 < DB) read_v(d + 1);
