@@ -35,6 +35,7 @@ template <typename T>
 struct TaType;
 template <>
 struct TaType<_Float16> {
+  static constexpr float kRoom = 3.0f;  // weights up to 2^15
   typedef PaType<_Float16>::v8 v8;
   typedef _Float16 v4 __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
@@ -43,6 +44,7 @@ struct TaType<_Float16> {
 };
 template <>
 struct TaType<__bf16> {
+  static constexpr float kRoom = 16.0f;  // as many bits at any size
   typedef PaType<__bf16>::v8 v8;
   typedef __bf16 v4 __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
@@ -346,8 +348,12 @@ __global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_
 #pragma unroll
           for (int i = 1; i < 16; i++) top = fmaxf(top, x[i]);
           top = fmaxf(top, __shfl_xor(top, 32));
-          const float mn = fmaxf(m, top * to_log2), ref = mn == -INFINITY ? 0.0f : mn;
-          if (__any(mn > m)) {
+          // the weights' unit 2^m follows the maximum only where it is left behind by more than the weights' type has room for:
+          // the accumulators are brought to another unit a few times a stretch, not in every other tile
+          const float mn = fmaxf(m, top * to_log2);
+          const bool behind = __any(mn > m + TaType<T>::kRoom);
+          const float ref = behind ? (mn == -INFINITY ? 0.0f : mn) : (m == -INFINITY ? 0.0f : m);
+          if (behind) {
             const float by = __builtin_amdgcn_exp2f(m - ref);
             l *= by;
 #pragma unroll
