@@ -21,8 +21,8 @@
 
 namespace nrq {
 
-constexpr int kTaWgs = 256;  // workgroups: one a CU
-constexpr int kTaSetup = 2;  // what the beginning and the end of a unit cost, in tiles
+constexpr int kTaCus = 256;
+constexpr int kTaSetup = 3;  // what the beginning and the end of a unit cost, in tiles
 
 // Rows of a KV head that nrq_paged.h takes: one unit of its.
 inline size_t ta_few(int hd) { return hd <= 128 ? 32 : 16; }
@@ -126,8 +126,11 @@ struct TaShape {
   }
 };
 
+// Waves of a SIMD: registers for the accumulators and the queries' pieces.
+constexpr int ta_waves(int hd, int nq) { return hd > 128 || nq > 2 ? 1 : 2; }
+
 template <typename T, int HD, int W, int WR, int TP, int NQ, int NP>
-__global__ __launch_bounds__(64 * W, W / 4) void tree_kernel(PaArgs A, int wide_o) {
+__global__ __launch_bounds__(64 * W, ta_waves(HD, NQ)) void tree_kernel(PaArgs A, int wide_o) {
   typedef TaShape<HD, W, WR, TP> Sh;
   typedef typename PaType<T>::v8 v8;
   constexpr int KS = HD / 16, DB = HD / 32, WP = Sh::kWP;
@@ -551,7 +554,8 @@ hipError_t ta_launch(const PagedAttnLaunch& L) {
   const int64_t tiles = ((int64_t)L.table.width * L.kv.page_size + kTile - 1) / kTile;
   A.setup = kTaSetup;
   const int64_t most = units * ((tiles > 0 ? tiles : 1) + A.setup);
-  A.wgs = (int)(most < kTaWgs ? most : kTaWgs);
+  constexpr int kWgs = kTaCus * ta_waves(HD, NQ) * 4 / W;  // what the card holds
+  A.wgs = (int)(most < kWgs ? most : kWgs);
   pa_workspace(A, HD);
   const int v = L.dtype == kF32 ? 4 : 2;  // four values are stored together
   const int wide_o = ((uintptr_t)L.out & (v == 4 ? 15 : 7)) == 0 && L.ob % 4 == 0 && L.ot % 4 == 0 && L.oh % 4 == 0;
@@ -570,10 +574,11 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
     if (rows > 64) return ta_launch<T, HD, 4, 4, 64, NQ, NP>(L);
     return ta_launch<T, HD, 4, 2, 64, NQ, NP>(L);
   } else {
-    constexpr int kTP = 128;  // registers for a stage of 64 beside the queries' pieces
-    if (rows > 128) return ta_launch<T, HD, 8, 8, kTP, NQ, NP>(L);
-    if (rows > 64) return ta_launch<T, HD, 8, 4, kTP, NQ, NP>(L);
-    return ta_launch<T, HD, 8, 2, 128, NQ, NP>(L);
+    // more than 128 rows: one workgroup a CU; else two, one of which multiplies while the other begins or ends a unit
+    constexpr int kTP = HD == 128 || HD == 96 ? 64 : 128;
+    if (rows > 128) return ta_launch<T, HD, 8, 8, HD == 96 ? 128 : kTP, NQ, NP>(L);
+    if (rows > 64) return ta_launch<T, HD, 4, 4, kTP, NQ, NP>(L);
+    return ta_launch<T, HD, 4, 2, kTP, NQ, NP>(L);
   }
 }
 
