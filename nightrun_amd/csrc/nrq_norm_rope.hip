@@ -23,18 +23,36 @@ struct NrArgs {
   int lanes;   // of a row: a power of two, at most 64
   int pairs;   // items that rotate
   int items;   // of a row
+  float inv;   // 1 / head_dim
 };
 
-// Where a row comes from and goes to.
+// Where a row comes from and goes to, and its values: d and d1 of the lane's items.
+template <typename T, int V, int K>
 struct NrRow {
-  const void* from;  // nullptr: none
-  void* to;
+  Vec<T, V> a[K], b[K];
+  void* to;  // nullptr: nowhere
   int kind;  // 0: q, 1: k, 2: v
   int tok;
 };
 
+// The sum over a group of lanes, a power of two of them, the same in each. A lane whose quad has one sum finds the
+// other quad's mirrored in the eight lanes, and so on.
+template <int CTRL>
+__device__ __forceinline__ float nr_dpp(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 15, 15, true));
+}
+__device__ __forceinline__ float nr_sum(float s, int lanes) {
+  if (lanes > 1) s += nr_dpp<0xb1>(s);   // the neighbour in a pair
+  if (lanes > 2) s += nr_dpp<0x4e>(s);   // the other pair of a quad
+  if (lanes > 4) s += nr_dpp<0x141>(s);  // mirrored in eight lanes
+  if (lanes > 8) s += nr_dpp<0x140>(s);  // mirrored in sixteen
+  if (lanes > 16) s += __shfl_xor(s, 16);
+  if (lanes > 32) s += __shfl_xor(s, 32);
+  return s;
+}
+
 // T: the rows' type, C: the cache's, V: elements of an access (16 bytes of T, or 1 where strides, addresses
-// or the rotated part do not allow it), K: items of a lane at most, A: rows of a lane on their way together.
+// or the rotated part do not allow it), K: items of a lane at most, A: rows of a lane in a turn, the next turn's on their way.
 template <typename T, typename C, int V, int K, int A, bool APPEND, bool NORM>
 __global__ __launch_bounds__(kNrNT) void norm_rope_kernel(NrArgs P) {
   __shared__ float2 cs[kNrPairs];
@@ -42,19 +60,6 @@ __global__ __launch_bounds__(kNrNT) void norm_rope_kernel(NrArgs P) {
   __shared__ bool pad[kNrTokens];
   const RopeLaunch& L = P.L.r;
   const int t0 = blockIdx.x * P.tpw, nt = min(P.tpw, L.tokens - t0), half = L.nf;
-  for (int i = threadIdx.x; i < nt * half; i += kNrNT) {
-    const float2 v = sincos_turn(L.pos[t0 + i / half], L.freqs[i % half]);
-    cs[i] = make_float2(v.x * L.scale, v.y * L.scale);
-  }
-  if (APPEND)
-    for (int i = threadIdx.x; i < nt; i += kNrNT) {
-      const int seq = L.seq[t0 + i], at = P.L.at ? P.L.at[t0 + i] : L.pos[t0 + i];
-      const bool p = seq < 0 || seq >= L.table.seqs || at < 0;
-      pad[i] = p;
-      place[i] = p ? kNoPlace
-                   : page_place(L.table.pages + seq * L.table.stride, L.table.width, L.kv.page_size, L.kv.n_pages,
-                                L.kv.page_stride8, L.kv.pos_stride8, at);
-    }
   const int heads = APPEND ? L.heads + 2 * L.kv.n_kv : L.heads;
   const int across = kNrNT / P.lanes, lane = threadIdx.x & (P.lanes - 1);
   const int step = across * gridDim.y, dt = step / heads, dh = step - dt * heads;
@@ -70,6 +75,56 @@ __global__ __launch_bounds__(kNrNT) void norm_rope_kernel(NrArgs P) {
     two[k] = turning[k] && (L.neox || V == 1);
     d1[k] = two[k] ? (L.neox ? d[k] + half : d[k] + 1) : d[k];
   }
+  int r = (int)threadIdx.x / P.lanes + across * blockIdx.y, tt = r / heads, h = r - tt * heads;
+  // a turn's rows; also padding's, which are not stored
+  auto fetch = [&](NrRow<T, V, K>* row) {
+#pragma unroll
+    for (int j = 0; j < A; j++) {
+      NrRow<T, V, K>& w = row[j];
+      const T* from = nullptr;
+      w.kind = -1, w.tok = min(tt, nt - 1);
+      const int t = t0 + tt;
+      if (tt < nt) {
+        if (!APPEND || h < L.heads) {
+          w.kind = 0;
+          from = (const T*)L.x + t * L.xt + h * L.xh;
+          w.to = (T*)L.y + t * L.yt + h * L.yh;
+        } else {
+          const bool isk = h < L.heads + L.kv.n_kv;
+          const int hh = h - L.heads - (isk ? 0 : L.kv.n_kv);
+          w.kind = isk ? 1 : 2;
+          from = isk ? (const T*)L.k + t * L.kt + hh * L.kh : (const T*)L.v + t * L.vt + hh * L.vh;
+          w.to = (C*)(isk ? L.kv.k : L.kv.v) + hh * L.kv.head_stride;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        w.a[k] = w.b[k] = Vec<T, V>{};
+        if (from && lane + P.lanes * k < P.items) {
+          w.a[k] = *(const Vec<T, V>*)(from + d[k]);
+          if (two[k]) w.b[k] = *(const Vec<T, V>*)(from + d1[k]);
+        }
+      }
+      h += dh;
+      tt += dt;
+      if (h >= heads) h -= heads, tt++;
+    }
+  };
+  NrRow<T, V, K> first[A], second[A];
+  fetch(first);  // on their way while the angles are formed
+  for (int i = threadIdx.x; i < nt * half; i += kNrNT) {
+    const float2 v = sincos_turn(L.pos[t0 + i / half], L.freqs[i % half]);
+    cs[i] = make_float2(v.x * L.scale, v.y * L.scale);
+  }
+  if (APPEND)
+    for (int i = threadIdx.x; i < nt; i += kNrNT) {
+      const int seq = L.seq[t0 + i], at = P.L.at ? P.L.at[t0 + i] : L.pos[t0 + i];
+      const bool p = seq < 0 || seq >= L.table.seqs || at < 0;
+      pad[i] = p;
+      place[i] = p ? kNoPlace
+                   : page_place(L.table.pages + seq * L.table.stride, L.table.width, L.kv.page_size, L.kv.n_pages,
+                                L.kv.page_stride8, L.kv.pos_stride8, at);
+    }
   // one item a lane: its weights stay in registers
   float wq[2][V], wk[2][V];
   if (NORM && K == 1 && lane < P.items) {
@@ -84,68 +139,38 @@ __global__ __launch_bounds__(kNrNT) void norm_rope_kernel(NrArgs P) {
     }
   }
   __syncthreads();
-  int r = (int)threadIdx.x / P.lanes + across * blockIdx.y, tt = r / heads, h = r - tt * heads;
-  // every lane of a wave takes the same number of turns: the shuffles below want all of them
-  const int turns = (nt * heads + step * A - 1) / (step * A);
-  for (int n = 0; n < turns; n++) {
-    Vec<T, V> a[A][K], b[A][K];
-    NrRow row[A];
+  auto finish = [&](const NrRow<T, V, K>* row) {
 #pragma unroll
     for (int j = 0; j < A; j++) {
-      NrRow& w = row[j];
-      w.from = nullptr, w.to = nullptr, w.kind = 0, w.tok = min(tt, nt - 1);
-      if (tt < nt) {
-        const int t = t0 + tt;
-        if (!APPEND || h < L.heads) {
-          if (!APPEND || !pad[tt]) {
-            w.from = (const T*)L.x + t * L.xt + h * L.xh;
-            w.to = (T*)L.y + t * L.yt + h * L.yh;
-          }
-        } else if (place[tt] != kNoPlace) {
-          const bool isk = h < L.heads + L.kv.n_kv;
-          const int hh = h - L.heads - (isk ? 0 : L.kv.n_kv);
-          w.kind = isk ? 1 : 2;
-          w.from = isk ? (const T*)L.k + t * L.kt + hh * L.kh : (const T*)L.v + t * L.vt + hh * L.vh;
-          w.to = (C*)(isk ? L.kv.k : L.kv.v) + (uint64_t)place[tt] * 8 + hh * L.kv.head_stride;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < K; k++) {
-        a[j][k] = b[j][k] = Vec<T, V>{};
-        if (w.from && lane + P.lanes * k < P.items) {
-          a[j][k] = *(const Vec<T, V>*)((const T*)w.from + d[k]);
-          if (two[k]) b[j][k] = *(const Vec<T, V>*)((const T*)w.from + d1[k]);
-        }
-      }
-      h += dh;
-      tt += dt;
-      if (h >= heads) h -= heads, tt++;
-    }
-#pragma unroll
-    for (int j = 0; j < A; j++) {
-      const NrRow& w = row[j];
+      const NrRow<T, V, K>& w = row[j];
       float by = 1.0f;
-      if (NORM) {
+      if (NORM) {  // all lanes of the wave
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
           for (int i = 0; i < V; i++) {
-            const float x0 = (float)a[j][k].v[i], x1 = (float)b[j][k].v[i];  // zero without a second access
+            const float x0 = (float)w.a[k].v[i], x1 = (float)w.b[k].v[i];  // zero without a second access
             s = fmaf(x0, x0, s);
             s = fmaf(x1, x1, s);
           }
-        for (int m = 1; m < P.lanes; m <<= 1) s += __shfl_xor(s, m);
-        by = 1.0f / sqrtf(s / (float)L.hd + P.L.eps);
+        const float mean = nr_sum(s, P.lanes) * P.inv + P.L.eps;
+        // the instruction is within a step of the value, but takes a subnormal mean for zero
+        by = mean >= 0x1p-126f ? __builtin_amdgcn_rsqf(mean) : 1.0f / sqrtf(mean);
       }
-      if (!w.from) continue;
+      void* to = w.to;
+      if (w.kind < 0) continue;
+      if (APPEND) {
+        if (w.kind == 0 ? pad[w.tok] : place[w.tok] == kNoPlace) continue;
+        if (w.kind > 0) to = (C*)to + (uint64_t)place[w.tok] * 8;
+      }
       const float2* cw = cs + w.tok * half;
 #pragma unroll
       for (int k = 0; k < K; k++) {
         if (lane + P.lanes * k >= P.items) continue;
         float o0[V], o1[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) o0[i] = (float)a[j][k].v[i], o1[i] = (float)b[j][k].v[i];
+        for (int i = 0; i < V; i++) o0[i] = (float)w.a[k].v[i], o1[i] = (float)w.b[k].v[i];
         if (!APPEND || w.kind != 2) {
           if (NORM) {
             const bool isk = APPEND && w.kind == 1;
@@ -183,25 +208,34 @@ __global__ __launch_bounds__(kNrNT) void norm_rope_kernel(NrArgs P) {
           Vec<T, V> v;
 #pragma unroll
           for (int i = 0; i < V; i++) v.v[i] = (T)o0[i];
-          *(Vec<T, V>*)((T*)w.to + d[k]) = v;
+          *(Vec<T, V>*)((T*)to + d[k]) = v;
           if (two[k]) {
 #pragma unroll
             for (int i = 0; i < V; i++) v.v[i] = (T)o1[i];
-            *(Vec<T, V>*)((T*)w.to + d1[k]) = v;
+            *(Vec<T, V>*)((T*)to + d1[k]) = v;
           }
         } else {
           Vec<C, V> v;
 #pragma unroll
           for (int i = 0; i < V; i++) v.v[i] = (C)o0[i];
-          *(Vec<C, V>*)((C*)w.to + d[k]) = v;
+          *(Vec<C, V>*)((C*)to + d[k]) = v;
           if (two[k]) {
 #pragma unroll
             for (int i = 0; i < V; i++) v.v[i] = (C)o1[i];
-            *(Vec<C, V>*)((C*)w.to + d1[k]) = v;
+            *(Vec<C, V>*)((C*)to + d1[k]) = v;
           }
         }
       }
     }
+  };
+  // every lane of a wave takes the same number of turns: the sums want all of them
+  const int turns = (nt * heads + step * A - 1) / (step * A);
+  for (int n = 0; n < turns; n += 2) {
+    if (n + 1 < turns) fetch(second);
+    finish(first);
+    if (n + 1 >= turns) break;
+    if (n + 2 < turns) fetch(first);
+    finish(second);
   }
 }
 
@@ -248,11 +282,12 @@ hipError_t nr_launch_t(const NormRopeLaunch& N) {
   const int v = wide ? V : 1, rest0 = 2 * L.nf / v;
   P.pairs = L.neox ? L.nf / v : (v == 1 ? L.nf : rest0);
   P.items = P.pairs + L.hd / v - rest0;
+  P.inv = 1.0f / (float)L.hd;
   P.lanes = 1;
   while (P.lanes < P.items && P.lanes < 64) P.lanes *= 2;
   // heads of 1024: 256 accesses of 4, or 1023 of 1 (where all but two dimensions are copied)
   if (!wide) return nr_launch<T, C, 1, 16, 1, APPEND, NORM>(P);
-  if (P.items <= 64) return nr_launch<T, C, V, 1, 4, APPEND, NORM>(P);
+  if (P.items <= 64) return nr_launch<T, C, V, 1, 2, APPEND, NORM>(P);
   return nr_launch<T, C, V, 4, 1, APPEND, NORM>(P);
 }
 
