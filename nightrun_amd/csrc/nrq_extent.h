@@ -1,0 +1,88 @@
+// Whether tensors of several dimensions share memory, for the argument checks and (compiled alone by a host compiler)
+// for the tests.
+#pragma once
+
+#include "nrq_rows.h"
+
+namespace nrq {
+
+struct Dim {
+  int64_t stride;  // elements
+  size_t n;
+};
+
+// A tensor of up to three dimensions of rows, for the question whether two share memory. Exact where both come down to
+// rows of one dimension, once dimensions that follow one another without gaps, or at one distance, are taken together; else two
+// that lie between one another count as sharing.
+struct Extent {
+  const void* first;
+  size_t len;  // elements of a row
+  int size;    // bytes of one
+  Dim d[3];
+};
+
+inline Rows as_rows(const Extent& e) {
+  Dim d[3];
+  int n = 0;
+  typedef __int128 wide;
+  wide low = 0, len = (wide)e.len;
+  for (const Dim& x : e.d) {
+    if (x.n == 0) return Rows{e.first, 0, 0, 0, e.size};
+    if (x.n == 1 || x.stride == 0) continue;
+    Dim y = x;
+    if (y.stride < 0) {  // from its other end
+      low += (wide)y.stride * (wide)(y.n - 1);
+      y.stride = y.stride == INT64_MIN ? INT64_MAX : -y.stride;
+    }
+    int i = n++;
+    for (; i > 0 && d[i - 1].stride > y.stride; i--) d[i] = d[i - 1];
+    d[i] = y;
+  }
+  int at = 0;  // dimensions d[at] .. d[n - 1] are left
+  while (at < n && (wide)d[at].stride <= len) len += (wide)d[at].stride * (wide)(d[at].n - 1), at++;
+  while (n - at > 1) {
+    Dim &x = d[at], &y = d[at + 1];
+    if ((wide)y.stride == (wide)x.stride * (wide)x.n) {
+      x.n *= y.n;
+      if (n - at > 2) y = d[at + 2];
+      n--;
+    } else {
+      len += (wide)x.stride * (wide)(x.n - 1), at++;
+    }
+  }
+  const wide past = (wide)INT64_MAX / 16;  // any memory
+  if (len > past) len = past;
+  Rows r{(const char*)e.first + (int64_t)(low * e.size), 1, 0, (size_t)len, e.size};
+  if (at < n) r.n = d[at].n, r.stride = d[at].stride;
+  return r;
+}
+
+// From the least address of a tensor to behind its greatest; what overflows reaches everywhere.
+struct Range {
+  uintptr_t low, high;
+};
+inline Range range_of(const Extent& e) {
+  const uintptr_t all = ~(uintptr_t)0;
+  int64_t low = 0, high = (int64_t)e.len;
+  bool over = e.len > (size_t)INT64_MAX;
+  for (const Dim& x : e.d) {
+    if (x.n == 0) return Range{1, 0};
+    int64_t span;
+    over |= x.n > (size_t)INT64_MAX || __builtin_mul_overflow(x.stride, (int64_t)(x.n - 1), &span);
+    if (over) return Range{0, all};
+    over |= __builtin_add_overflow(span < 0 ? low : high, span, span < 0 ? &low : &high);
+  }
+  if (e.len == 0) return Range{1, 0};
+  int64_t from, to;
+  over |= __builtin_mul_overflow(low, (int64_t)e.size, &from) || __builtin_mul_overflow(high, (int64_t)e.size, &to);
+  if (over || (uintptr_t)e.first < (uintptr_t)-from || (uintptr_t)e.first > all - (uintptr_t)to) return Range{0, all};
+  return Range{(uintptr_t)e.first + from, (uintptr_t)e.first + to};
+}
+
+// Whether they do, or lie between one another as as_rows() cannot tell apart.
+inline bool extents_meet(const Extent& a, const Extent& b) {
+  const Range x = range_of(a), y = range_of(b);
+  return x.low < y.high && y.low < x.high && rows_meet(as_rows(a), as_rows(b));
+}
+
+}  // namespace nrq

@@ -54,7 +54,7 @@ __device__ __forceinline__ float nr_sum(float s, int lanes) {
 // T: the rows' type, C: the cache's, V: elements of an access (16 bytes of T, or 1 where strides, addresses
 // or the rotated part do not allow it), K: items of a lane at most, A: rows of a lane in a turn, the next turn's on their way.
 template <typename T, typename C, int V, int K, int A, bool APPEND, bool NORM>
-__global__ __launch_bounds__(kNrNT) void norm_rope_kernel(NrArgs P) {
+__global__ __launch_bounds__(kNrNT, K == 1 && V > 1 ? 4 : 1) void norm_rope_kernel(NrArgs P) {
   __shared__ float2 cs[kNrPairs];
   __shared__ uint32_t place[kNrTokens];
   __shared__ bool pad[kNrTokens];
@@ -242,11 +242,11 @@ __global__ __launch_bounds__(kNrNT) void norm_rope_kernel(NrArgs P) {
 template <typename T, typename C, int V, int K, int A, bool APPEND, bool NORM>
 hipError_t nr_launch(NrArgs& P) {
   const RopeLaunch& L = P.L.r;
-  // Tokens of a workgroup: as many as make one angle a thread, fewer where the card (2048 workgroups) would not
+  // Tokens of a workgroup: as many as make one angle a thread, fewer where the card (1024 workgroups) would not
   // be full; with few tokens their rows are spread over more workgroups, a row a group of lanes in each.
   int t = kNrNT / L.nf;
   t = t < 1 ? 1 : (t > kNrTokens ? kNrTokens : t);
-  if (t > (L.tokens - 1) / 2048 + 1) t = (L.tokens - 1) / 2048 + 1;
+  if (t > (L.tokens - 1) / 1024 + 1) t = (L.tokens - 1) / 1024 + 1;
   P.tpw = t;
   const int64_t rows = (int64_t)t * (L.heads + (APPEND ? 2 * L.kv.n_kv : 0)), across = kNrNT / P.lanes;
   const int tw = (L.tokens - 1) / t + 1;

@@ -10,6 +10,7 @@
 
 #include "../../include/nrq.h"
 #include "../../include/nrq_serve.h"
+#include "nrq_extent.h"
 #include "nrq_launch.h"
 #include "nrq_serve_launch.h"
 
@@ -79,10 +80,7 @@ int kv_check(const char* name, const nrq_paged_kv* kv, const nrq_page_table* tab
 }
 
 // Rows written must not overlap: sorted by their strides, each dimension steps over all of the ones inside it.
-struct Dim {
-  int64_t stride;
-  size_t n;
-};
+using nrq::Dim;
 bool apart(size_t row, std::initializer_list<Dim> dims) {
   Dim d[4];
   int count = 0;

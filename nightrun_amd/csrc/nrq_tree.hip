@@ -2,54 +2,35 @@
 // checks, then one or two kernel launches on the caller's stream.
 #include "../../include/nrq_tree.h"
 
-#include "nrq_rows.h"
+#include "nrq_extent.h"
 #include "nrq_serve_check.h"
 #include "nrq_tree_launch.h"
 
 namespace {
 
-// A tensor of up to three dimensions of rows, for the question whether two share memory. Exact where the rows of both
-// are those of one dimension once dimensions without gaps between them are taken together; else two that lie
-// between one another count as sharing.
-struct Extent {
-  const void* first;
-  size_t len;  // elements of a row
-  int size;    // bytes of one
-  Dim d[3];
-};
-
-nrq::Rows as_rows(const Extent& e) {
-  nrq::Rows r{e.first, 1, 0, e.len, e.size};
-  Dim d[3];
-  int n = 0;
-  for (const Dim& x : e.d) {
-    if (x.n == 0) return nrq::Rows{e.first, 0, 0, 0, e.size};
-    if (x.n == 1 || x.stride == 0) continue;
-    int i = n++;
-    for (; i > 0 && (d[i - 1].stride < 0 ? -d[i - 1].stride : d[i - 1].stride) > (x.stride < 0 ? -x.stride : x.stride); i--)
-      d[i] = d[i - 1];
-    d[i] = x;
-  }
-  // all but the outermost: from their least address to their greatest
-  __int128 low = 0, high = (__int128)e.len;
-  for (int i = 0; i + 1 < n; i++) {
-    const __int128 span = (__int128)d[i].stride * (__int128)(d[i].n - 1);
-    (span < 0 ? low : high) += span;
-  }
-  if (high - low > (__int128)INT64_MAX / 16) high = low + INT64_MAX / 16;  // past any memory
-  r.first = (const char*)e.first + (int64_t)(low * e.size);
-  r.len = (size_t)(high - low);
-  if (n) r.n = d[n - 1].n, r.stride = d[n - 1].stride;
-  return r;
-}
-
-bool meet(const Extent& a, const Extent& b) { return nrq::rows_meet(as_rows(a), as_rows(b)); }
+using nrq::Extent;
+using nrq::Range;
+using nrq::as_rows;
+using nrq::range_of;
 
 Extent whole(const void* p, size_t n, int size) { return Extent{p, p ? n : 0, size, {{0, 1}, {0, 1}, {0, 1}}}; }
 
-int apart_from(const char* name, const Extent& out, std::initializer_list<Extent> others) {
-  for (const Extent& o : others)
-    if (o.first && meet(out, o)) return fail(NRQ_ERR_ARG, name, "an output shares memory with an input or another output");
+// Refuses outputs that share memory with one another or with inputs; those that are not there (nullptr) share none.
+// Ranges that do not meet, as a rule, are told apart without more.
+int apart_from(const char* name, std::initializer_list<Extent> out, std::initializer_list<Extent> in) {
+  Range r[16];
+  const Extent* e[16];
+  size_t n = 0;
+  const size_t outs = out.size();
+  for (const auto* list : {&out, &in})
+    for (const Extent& x : *list) {
+      e[n] = &x;
+      r[n++] = x.first ? range_of(x) : Range{1, 0};
+    }
+  for (size_t i = 0; i < outs; i++)
+    for (size_t j = i + 1; j < n; j++)
+      if (r[i].low < r[j].high && r[j].low < r[i].high && nrq::rows_meet(as_rows(*e[i]), as_rows(*e[j])))
+        return fail(NRQ_ERR_ARG, name, "an output shares memory with an input or another output");
   return NRQ_OK;
 }
 
@@ -84,9 +65,11 @@ int nrq_dev_norm_rope(void* y, const void* x, int dtype, size_t tokens, size_t h
   L.neox = style == NRQ_ROPE_NEOX, L.scale = scale, L.stream = (hipStream_t)stream;
   N.norm = true, N.wq = weight, N.eps = eps;
   if ((rc = device_check(name, stream))) return rc;
-  const Extent out = heads_of(y, dtype, tokens, L.yt, heads, L.yh, head_dim);
-  if (y != x && (rc = apart_from(name, out, {heads_of(x, dtype, tokens, L.xt, heads, L.xh, head_dim)}))) return rc;
-  if ((rc = apart_from(name, out, {whole(weight, head_dim, 4), whole(pos, tokens, 4), whole(freqs, n_freqs, 4)}))) return rc;
+  // in place the input is left out
+  if ((rc = apart_from(name, {heads_of(y, dtype, tokens, L.yt, heads, L.yh, head_dim)},
+                       {heads_of(y != x ? x : nullptr, dtype, tokens, L.xt, heads, L.xh, head_dim),
+                        whole(weight, head_dim, 4), whole(pos, tokens, 4), whole(freqs, n_freqs, 4)})))
+    return rc;
   return launched(name, nrq::launch_norm_rope(N));
 }
 
@@ -119,14 +102,18 @@ int nrq_dev_norm_rope_append(void* y, const void* q, const void* k, const void* 
   L.neox = style == NRQ_ROPE_NEOX, L.scale = scale, L.stream = (hipStream_t)stream;
   N.norm = norm != 0, N.wq = q_weight, N.wk = k_weight, N.eps = eps, N.at = at;
   if ((rc = device_check(name, stream))) return rc;
+  const size_t n_pages = (size_t)kv->n_pages, size = (size_t)kv->page_size;
   const Extent qe = heads_of(q, dtype, tokens, L.xt, heads, L.xh, hd), ke = heads_of(k, dtype, tokens, L.kt, n_kv, L.kh, hd),
-               ve = heads_of(v, dtype, tokens, L.vt, n_kv, L.vh, hd), ye = heads_of(y, dtype, tokens, L.yt, heads, L.yh, hd);
-  if (y != q && (rc = apart_from(name, ye, {qe}))) return rc;
-  if ((rc = apart_from(name, ye, {ke, ve}))) return rc;
-  for (const void* pool : {kv->k, kv->v}) {
-    const Extent c{pool, hd, 2, {{kv->page_stride, (size_t)kv->n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, (size_t)kv->page_size}}};
-    if ((rc = apart_from(name, c, {qe, ke, ve, ye}))) return rc;
-  }
+               ve = heads_of(v, dtype, tokens, L.vt, n_kv, L.vh, hd), ye = heads_of(y, dtype, tokens, L.yt, heads, L.yh, hd),
+               ck{kv->k, hd, 2, {{kv->page_stride, n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, size}}},
+               cv{kv->v, hd, 2, {{kv->page_stride, n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, size}}};
+  const Extent at_ = whole(at, tokens, 4), wq = whole(norm ? q_weight : nullptr, hd, 4), wk = whole(norm ? k_weight : nullptr, hd, 4),
+               pe = whole(pos, tokens, 4), se = whole(seq, tokens, 4), fe = whole(freqs, n_freqs, 4);
+  const Extent none{};  // in place the queries are left out
+  if ((rc = apart_from(name, {ye}, {y != q ? qe : none, ck, cv, ke, ve, pe, se, at_, fe, wq, wk})) ||
+      (rc = apart_from(name, {ck}, {y != q ? qe : none, ke, ve, pe, se, at_, fe, wq, wk})) ||
+      (rc = apart_from(name, {cv}, {y != q ? qe : none, ke, ve, pe, se, at_, fe, wq, wk})))
+    return rc;
   return launched(name, nrq::launch_norm_rope(N));
 }
 
@@ -158,17 +145,16 @@ int nrq_dev_tree_attention(void* out, const void* q, int dtype, size_t n_new, si
   L.parents = parents, L.workspace = workspace, L.stream = (hipStream_t)stream;
   if ((rc = device_check(name, stream))) return rc;
   const size_t hd = (size_t)kv->head_dim, seqs = (size_t)table->seqs, e = bytes_of(dtype);
-  const Extent oe{out, hd, (int)e, {{L.ob, seqs}, {L.ot, n_new}, {L.oh, heads}}}, we = whole(workspace, need, 1),
-               se = whole(lse, seqs * n_new * heads, 4);
-  const Extent in[] = {{q, hd, (int)e, {{L.qb, seqs}, {L.qt, n_new}, {L.qh, heads}}},
-                       whole(lens, seqs, 4),
-                       whole(parents, seqs * n_new, 4),
-                       whole(counts, seqs, 4),
-                       {table->pages, (size_t)table->width, 4, {{table->stride, seqs}, {0, 1}, {0, 1}}}};
-  for (const Extent& i : in)
-    for (const Extent* o : {&oe, &we, &se})
-      if (o->first && (rc = apart_from(name, *o, {i}))) return rc;
-  if ((rc = apart_from(name, oe, {we, se})) || (lse && (rc = apart_from(name, se, {we})))) return rc;
+  if ((rc = apart_from(name,
+                       {{out, hd, (int)e, {{L.ob, seqs}, {L.ot, n_new}, {L.oh, heads}}},
+                        whole(workspace, need, 1),
+                        whole(lse, seqs * n_new * heads, 4)},
+                       {{q, hd, (int)e, {{L.qb, seqs}, {L.qt, n_new}, {L.qh, heads}}},
+                        whole(lens, seqs, 4),
+                        whole(parents, seqs * n_new, 4),
+                        whole(counts, seqs, 4),
+                        {table->pages, (size_t)table->width, 4, {{table->stride, seqs}, {0, 1}, {0, 1}}}})))
+    return rc;
   return launched(name, nrq::launch_tree_attn(L));
 }
 
@@ -201,15 +187,10 @@ int nrq_dev_verify_tree(int32_t* tokens, int32_t* path, int32_t* accepted, const
                       drafted,  uniforms, counts, (int)seqs, (int)n_new, (int)vocab, workspace, (hipStream_t)stream,
                       parents,  path};
   if ((rc = device_check(name, stream))) return rc;
-  const Extent out[] = {whole(tokens, all, 4), whole(path, all, 4), whole(accepted, seqs, 4), whole(workspace, need, 1)};
-  const Extent in[] = {{target, vocab, 4, {{strides[0], seqs}, {strides[1], n_new}, {0, 1}}},
-                       whole(drafted, all, 4), whole(parents, all, 4), whole(uniforms, all, 4), whole(counts, seqs, 4)};
-  for (int i = 0; i < 4; i++) {
-    for (const Extent& e : in)
-      if ((rc = apart_from(name, out[i], {e}))) return rc;
-    for (int j = 0; j < i; j++)
-      if ((rc = apart_from(name, out[i], {out[j]}))) return rc;
-  }
+  if ((rc = apart_from(name, {whole(tokens, all, 4), whole(path, all, 4), whole(accepted, seqs, 4), whole(workspace, need, 1)},
+                       {{target, vocab, 4, {{strides[0], seqs}, {strides[1], n_new}, {0, 1}}},
+                        whole(drafted, all, 4), whole(parents, all, 4), whole(uniforms, all, 4), whole(counts, seqs, 4)})))
+    return rc;
   return launched(name, nrq::launch_verify_tree(L));
 }
 
@@ -242,7 +223,7 @@ int nrq_dev_keep_path(int32_t* new_lens, size_t layers, int64_t layer_stride, co
   L.new_lens = new_lens, L.layers = (int)layers, L.layer_stride = layers > 1 ? layer_stride : 0;
   L.lens = lens, L.path = path, L.counts = counts, L.n_new = (int)n_new, L.stream = (hipStream_t)stream;
   if ((rc = device_check(name, stream))) return rc;
-  if ((rc = apart_from(name, whole(new_lens, seqs, 4),
+  if ((rc = apart_from(name, {whole(new_lens, seqs, 4)},
                        {whole(lens, seqs, 4), whole(path, seqs * n_new, 4), whole(counts, seqs, 4),
                         {table->pages, (size_t)table->width, 4, {{table->stride, seqs}, {0, 1}, {0, 1}}}})))
     return rc;

@@ -195,3 +195,101 @@ def test_bits(mask):
                     r = t - base
                     assert s >> i & 1 == (1 if r < 0 else (above >> r & 1 if r < 64 else 0)), (above, p0, base, i)
                     assert f >> i & 1 == int(t >= lo or r >= 0), (lo, p0, base, i)
+
+
+# ---- which tensors share memory -----------------------------------------------------------------
+
+
+@pytest.fixture(scope="module")
+def extent(tmp_path_factory):
+    d = tmp_path_factory.mktemp("extent")
+    src = d / "extent.cpp"
+    src.write_text('''#include "nrq_extent.h"
+extern "C" int meet(const int64_t* a, const int64_t* b) {
+  const int64_t* p[2] = {a, b};
+  nrq::Extent e[2];
+  for (int i = 0; i < 2; i++)
+    e[i] = nrq::Extent{(const void*)p[i][0], (size_t)p[i][1], (int)p[i][2],
+                       {{p[i][3], (size_t)p[i][4]}, {p[i][5], (size_t)p[i][6]}, {p[i][7], (size_t)p[i][8]}}};
+  return nrq::extents_meet(e[0], e[1]);
+}
+''')
+    so = d / "extent.so"
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-Wall", "-Werror", "-fsanitize=undefined",
+                    "-fno-sanitize-recover", "-static-libubsan", "-I", os.path.join(ROOT, "nightrun_amd", "csrc"),
+                    str(src), "-o", str(so)], check=True)
+    L = C.CDLL(str(so))
+    return lambda a, b: bool(L.meet((C.c_int64 * 9)(*a), (C.c_int64 * 9)(*b)))
+
+
+def _bytes(first, length, size, *dims):
+    out = {0}
+    for stride, n in dims:
+        out = {o + stride * i for o in out for i in range(n)}
+    return {first + (o + k) * size + e for o in out for k in range(length) for e in range(size)}
+
+
+def test_extents_never_miss(extent):
+    """Whatever shares a byte is found; what is apart in ranges is left alone."""
+    rng = random.Random(11)
+    met = apart = 0
+    for _ in range(20000):
+        a, b = ([4000 + rng.randint(-200, 200), rng.choice([0, 1, 2, 4, 8]), rng.choice([1, 2, 4])] +
+                [x for _ in range(3) for x in (rng.choice([-24, -8, 0, 3, 8, 16, 24, 64, 130]), rng.choice([0, 1, 1, 2, 3]))]
+                for _ in range(2))
+        x, y = (_bytes(e[0], e[1], e[2], *zip(e[3::2], e[4::2])) for e in (a, b))
+        got = extent(a, b)
+        assert got == extent(b, a)
+        if x & y:
+            met += 1
+            assert got, (a, b)
+        elif not x or not y or max(x) < min(y) or max(y) < min(x):
+            apart += 1
+            assert not got, (a, b)
+    assert met > 500 and apart > 2000
+
+
+def test_extents_of_layouts(extent):
+    """Layouts of one tensor: slices of a projection, keys and values of one pool, heads between heads."""
+    base = 1 << 40
+
+    def e(first, length, *dims, size=2):
+        dims = list(dims) + [(0, 1)] * (3 - len(dims))
+        return [base + first * size, length, size] + [x for d in dims for x in d]
+
+    t, h, kv, hd = 100, 32, 8, 128
+    row = (h + 2 * kv) * hd
+    q, k, v = e(0, hd, (row, t), (hd, h)), e(h * hd, hd, (row, t), (hd, kv)), e((h + kv) * hd, hd, (row, t), (hd, kv))
+    for i, x in enumerate((q, k, v)):
+        for j, y in enumerate((q, k, v)):
+            assert extent(x, y) == (i == j)
+    assert extent(q, e(h * hd - 1, hd, (row, t), (hd, kv)))
+    p, size = 50, 16
+    one = 2 * kv * size * hd  # [pages][2][heads][positions][hd], [pages][positions][2][heads][hd]
+    pools = ([(one, p), (size * hd, kv), (hd, size)], kv * size * hd), ([(one, p), (hd, kv), (2 * kv * hd, size)], kv * hd)
+    for dims, off in pools:
+        assert not extent(e(0, hd, *dims), e(off, hd, *dims))
+        assert extent(e(0, hd, *dims), e(off - 1, hd, *dims))
+    extent(e(0, hd, (2 ** 62, 3)), e(hd, hd, (-2 ** 62, 7)))  # past any memory: either answer, no overflow
+    assert extent(e(0, hd, (0, 5)), e(1, hd))
+    assert not extent(e(0, hd, (row, 0)), e(0, hd))
+
+
+SHARED = [
+    ("nrq_dev_norm_rope", "y", "x", 128), ("nrq_dev_norm_rope", "y", "weight", 0), ("nrq_dev_norm_rope", "y", "freqs", 0),
+    ("nrq_dev_norm_rope_append", "y", "k", 0), ("nrq_dev_norm_rope_append", "y", "pos", 0),
+    ("nrq_dev_tree_attention", "out", "q", 0), ("nrq_dev_tree_attention", "ws", "q", 0), ("nrq_dev_tree_attention", "out", "lens", 0),
+    ("nrq_dev_verify_tree", "tokens", "path", 0), ("nrq_dev_verify_tree", "path", "parents", 0),
+    ("nrq_dev_verify_tree", "accepted", "uniforms", 4), ("nrq_dev_keep_path", "new_lens", "lens", 0),
+]
+
+
+@pytest.mark.parametrize("name,out,other,by", SHARED)
+def test_overlaps_reach_the_check(name, out, other, by):
+    """Asked last, behind the device: without one the arguments are otherwise good."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("checks the no-GPU failure path")
+    a = CALLS[name]()
+    assert _call(name, a, **{out: a[other] + by})[0] == NOT_INIT
