@@ -386,6 +386,8 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       const uint16_t* kp = L.kv.k + head * L.kv.head_stride;
       const uint16_t* vp = L.kv.v + head * L.kv.head_stride;
       const int pw = sq.start + 32 * w + (lane & 31);  // the lane's position in the first tile
+      int parent = -1;
+      if (TREE) parent = pa_parent(L, b, sq.n);  // on its way with the pages
       uint32_t here = pa_place(L, pages, pw + t_begin * kTile, begin, end);
       PaTile<HD> tile;
       uint32_t live = (uint32_t)__ballot(here != kNoPlace), next = kNoPlace, next_live = 0;
@@ -442,7 +444,7 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       int lo[NT], hi[NT];  // what the row sees
       uint64_t above[NT];
       PaTree tree;
-      if (TREE) tree = pa_tree(L, pa_parent(L, b, sq.n), sq.n);
+      if (TREE) tree = pa_tree(L, parent, sq.n);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         to_log2[n] = unit_log2[16 * n + c];
