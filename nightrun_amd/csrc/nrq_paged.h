@@ -320,7 +320,7 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
                                  : (float)((const __bf16*)L.q)[qa + d];
     }
     for (int t0 = p0; t0 < stop; t0 += step)
-      for (int t = max(t0, TREE ? 0 : lo); t < min(t0 + 32, hi + 1); t++) {
+      for (int t = max(t0, TREE ? min(lo, max(len - n, 0)) : lo); t < min(t0 + 32, hi + 1); t++) {
         if (TREE && !(tree_sees(node.above, t, len - n) & 1 && (t >= lo || t >= len - n))) continue;
         const uint32_t place = pa_place(L, pages, t, TREE ? 0 : lo, min(len, hi + 1));
         if (place == kNoPlace) continue;
@@ -344,7 +344,7 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
 }
 
 // T: the cache's type; HD; NT: groups of 16 rows; NQ: pieces of a query.
-template <typename T, int HD, int NT, int NQ, bool TREE>
+template <typename T, int HD, int NT, int NQ>
 __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArgs A) {
   typedef typename PaType<T>::v8 v8;
   constexpr int NP = PaType<T>::kPieces;  // of a weight
@@ -377,17 +377,14 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       A.share[b * A.units_per_seq + unit] =
           make_int4(blockIdx.x, whole ? (int)blockIdx.x : line_owner(at + sq.tiles - 1, total, wgs), rows, 0);
     if (rows > 0) {
-      // what the unit's first and last row see; of a tree the positions before it, and any of it
-      const int first_hi = TREE ? sq.len - sq.n - 1 : sq.len - sq.n + row0 / A.group;
-      const int last_hi = TREE ? sq.len - 1 : sq.len - sq.n + (row0 + rows - 1) / A.group;
+      const int first_hi = sq.len - sq.n + row0 / A.group;                // what the unit's first
+      const int last_hi = sq.len - sq.n + (row0 + rows - 1) / A.group;    // and last row see
       const int last_lo = L.window > 0 ? max(0, last_hi - L.window + 1) : 0;
-      const int begin = L.window > 0 ? max(0, first_hi - L.window + (TREE ? 2 : 1)) : 0, end = min(sq.len, last_hi + 1);
+      const int begin = L.window > 0 ? max(0, first_hi - L.window + 1) : 0, end = min(sq.len, last_hi + 1);
       const int* pages = L.table.pages + b * L.table.stride;
       const uint16_t* kp = L.kv.k + head * L.kv.head_stride;
       const uint16_t* vp = L.kv.v + head * L.kv.head_stride;
       const int pw = sq.start + 32 * w + (lane & 31);  // the lane's position in the first tile
-      int parent = -1;
-      if (TREE) parent = pa_parent(L, b, sq.n);  // on its way with the pages
       uint32_t here = pa_place(L, pages, pw + t_begin * kTile, begin, end);
       PaTile<HD> tile;
       uint32_t live = (uint32_t)__ballot(here != kNoPlace), next = kNoPlace, next_live = 0;
@@ -442,19 +439,10 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       __syncthreads();
       float to_log2[NT];  // what brings a row's products to log2 units
       int lo[NT], hi[NT];  // what the row sees
-      uint64_t above[NT];
-      PaTree tree;
-      if (TREE) tree = pa_tree(L, parent, sq.n);
 #pragma unroll
       for (int n = 0; n < NT; n++) {
         to_log2[n] = unit_log2[16 * n + c];
-        const int tok = min(row0 + 16 * n + c, sq.n * A.group - 1) / A.group;
-        hi[n] = sq.len - sq.n + tok;
-        if (TREE) {
-          const PaTree node = pa_node(tree, tok);
-          above[n] = node.above;
-          hi[n] = sq.len - sq.n + node.depth;  // as far as the window goes
-        }
+        hi[n] = sq.len - sq.n + min(row0 + 16 * n + c, sq.n * A.group - 1) / A.group;
         lo[n] = L.window > 0 ? max(0, hi[n] - L.window + 1) : 0;
       }
 
@@ -498,11 +486,7 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
             float s[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) s[i] = x[n][i >> 2][i & 3] * to_log2[n];
-            if (TREE && !inside) {
-              const uint32_t base = sq.len - sq.n, sees = tree_sees(above[n], p0, base) & tree_from(lo[n], p0, base) & live;
-#pragma unroll
-              for (int i = 0; i < 8; i++) s[i] = sees >> ((i < 4 ? 0 : 16) + 4 * g + (i & 3)) & 1 ? s[i] : -INFINITY;
-            } else if (!inside) {
+            if (!inside) {
 #pragma unroll
               for (int i = 0; i < 8; i++) {
                 const int o = (i < 4 ? 0 : 16) + 4 * g + (i & 3), p = p0 + o;
@@ -561,7 +545,7 @@ __global__ __launch_bounds__(kPaNT, pa_resident(HD, NT)) void paged_kernel(PaArg
       }
       __syncthreads();  // the queries are read
       if (__any(sum != sum)) {
-        pa_plain<T, HD, TREE>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, kTile,
+        pa_plain<T, HD, false>(A, b, head, row0, rows, sq.start + t_begin * kTile + 32 * w, sq.start + t_end * kTile, kTile,
                         sq.len, sq.n, ex_o[w], ex_ml[w], OS);
       } else {
 #pragma unroll
@@ -696,7 +680,7 @@ inline void pa_workspace(PaArgs& A, int hd) {
   A.share = (int4*)(((uintptr_t)(A.part_ml + (size_t)2 * A.wgs * A.slots) + 15) & ~(uintptr_t)15);
 }
 
-template <typename T, int HD, int NT, int NQ, bool TREE>
+template <typename T, int HD, int NT, int NQ>
 hipError_t pa_launch(PaArgs& A) {
   const int64_t units = (int64_t)A.units_per_seq * A.L.table.seqs;
   const int64_t tiles = ((int64_t)A.L.table.width * A.L.kv.page_size + kTile - 1) / kTile;
@@ -704,30 +688,30 @@ hipError_t pa_launch(PaArgs& A) {
   static_assert(256 * pa_resident(HD, NT) <= kPaMaxWgs, "workspace");
   A.wgs = (int)(most < fill ? most : fill);
   pa_workspace(A, HD);
-  hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ, TREE>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
+  hipLaunchKernelGGL((paged_kernel<T, HD, NT, NQ>), dim3(A.wgs), dim3(kPaNT), 0, A.L.stream, A);
   if (tiles > 1)
     hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3((unsigned)units, A.slots), dim3(256), 0, A.L.stream, A);
   return hipGetLastError();
 }
 
-template <typename T, int HD, bool TREE>
+template <typename T, int HD>
 hipError_t pa_launch_hd(const PagedAttnLaunch& L) {
   constexpr int kMany = PaType<T>::kPieces;
   PaArgs A = pa_args(L, pa_per(HD, (size_t)L.n_new * (L.heads / L.kv.n_kv)));
   const bool same = L.dtype == PaType<T>::kId;
   if constexpr (HD <= 128)
-    if (A.per == 32) return same ? pa_launch<T, HD, 2, 1, TREE>(A) : pa_launch<T, HD, 2, kMany, TREE>(A);
-  return same ? pa_launch<T, HD, 1, 1, TREE>(A) : pa_launch<T, HD, 1, kMany, TREE>(A);
+    if (A.per == 32) return same ? pa_launch<T, HD, 2, 1>(A) : pa_launch<T, HD, 2, kMany>(A);
+  return same ? pa_launch<T, HD, 1, 1>(A) : pa_launch<T, HD, 1, kMany>(A);
 }
 
-template <typename T, bool TREE>
+template <typename T>
 hipError_t pa_launch_type(const PagedAttnLaunch& L) {
   switch (L.kv.hd) {
-    case 32: return pa_launch_hd<T, 32, TREE>(L);
-    case 64: return pa_launch_hd<T, 64, TREE>(L);
-    case 96: return pa_launch_hd<T, 96, TREE>(L);
-    case 128: return pa_launch_hd<T, 128, TREE>(L);
-    default: return pa_launch_hd<T, 256, TREE>(L);
+    case 32: return pa_launch_hd<T, 32>(L);
+    case 64: return pa_launch_hd<T, 64>(L);
+    case 96: return pa_launch_hd<T, 96>(L);
+    case 128: return pa_launch_hd<T, 128>(L);
+    default: return pa_launch_hd<T, 256>(L);
   }
 }
 

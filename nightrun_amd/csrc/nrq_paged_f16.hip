@@ -17,7 +17,7 @@ size_t paged_attn_workspace(size_t seqs, size_t n_new, size_t heads, int n_kv, i
 }
 
 hipError_t launch_paged_attn(const PagedAttnLaunch& L) {
-  return L.kv.dtype == kF16 ? pa_launch_type<_Float16, false>(L) : launch_paged_bf16(L);
+  return L.kv.dtype == kF16 ? pa_launch_type<_Float16>(L) : launch_paged_bf16(L);
 }
 
 }  // namespace nrq

@@ -140,6 +140,9 @@ int nrq_dev_tree_attention(void* out, const void* q, int dtype, size_t n_new, si
   if (!L.out) return device_check(name, stream);  // nothing to do
   if (!parents) return fail(NRQ_ERR_ARG, name, "null pointer");
   if (!aligned(parents, 4)) return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
+  if (nrq::tree_attn_line((size_t)table->seqs, n_new, heads, kv->n_kv_heads, (int64_t)table->width * kv->page_size) >= 2147483647.0)
+    return fail(NRQ_ERR_UNSUPPORTED, name, "%d sequences of %d pages of %d: too much work for a call", table->seqs,
+                table->width, kv->page_size);
   const size_t need = nrq::tree_attn_workspace((size_t)table->seqs, n_new, heads, kv->n_kv_heads, kv->head_dim);
   if ((rc = workspace_check(name, workspace, workspace_bytes, need))) return rc;
   L.parents = parents, L.workspace = workspace, L.stream = (hipStream_t)stream;

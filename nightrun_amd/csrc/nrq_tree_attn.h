@@ -24,9 +24,6 @@ namespace nrq {
 constexpr int kTaCus = 256;
 constexpr int kTaSetup = 3;  // what the beginning and the end of a unit cost, in tiles
 
-// Rows of a KV head that nrq_paged.h takes: one unit of its.
-inline size_t ta_few(int hd) { return hd <= 128 ? 32 : 16; }
-
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -294,7 +291,7 @@ __global__ __launch_bounds__(64 * W, ta_waves(HD, NQ)) void tree_kernel(PaArgs A
         look();
         ask(st + 2);
         load(st + 1);
-        if (!(now[0] | now[1])) continue;
+        if (!(now[0] | now[1]) || 32 * wr >= rows) continue;
         constexpr int US = TP / 32 / WP;  // of 32 positions, the wave's
         // the first half of the keys is read ahead, the second while the first is multiplied
         constexpr int KH = KS / 2;
@@ -570,14 +567,17 @@ hipError_t ta_launch(const PagedAttnLaunch& L) {
 template <typename T, int HD, int NQ, int NP>
 hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
   const int rows = L.n_new * (L.heads / L.kv.n_kv);
+  // units of as many rows as leave each workgroup three tiles, as far as the table goes
+  const int64_t tiles = (int64_t)L.table.seqs * L.kv.n_kv * (((int64_t)L.table.width * L.kv.page_size + kTile - 1) / kTile);
+  auto fills = [&](int per, int wgs) { return tiles * ((rows + per - 1) / per) >= 3 * wgs; };
   if constexpr (HD > 128 || NQ > 2) {
-    if (rows > 64) return ta_launch<T, HD, 4, 4, 64, NQ, NP>(L);
+    if (rows > 64 && fills(128, kTaCus)) return ta_launch<T, HD, 4, 4, 64, NQ, NP>(L);
     return ta_launch<T, HD, 4, 2, 64, NQ, NP>(L);
   } else {
     // more than 128 rows: one workgroup a CU; else two, one of which multiplies while the other begins or ends a unit
     constexpr int kTP = HD == 128 || HD == 96 ? 64 : 128;
-    if (rows > 128) return ta_launch<T, HD, 8, 8, HD == 96 ? 128 : kTP, NQ, NP>(L);
-    if (rows > 64) return ta_launch<T, HD, 4, 4, kTP, NQ, NP>(L);
+    if (rows > 128 && fills(256, kTaCus)) return ta_launch<T, HD, 8, 8, HD == 96 ? 128 : kTP, NQ, NP>(L);
+    if (rows > 64 && fills(128, 2 * kTaCus)) return ta_launch<T, HD, 4, 4, kTP, NQ, NP>(L);
     return ta_launch<T, HD, 4, 2, kTP, NQ, NP>(L);
   }
 }
@@ -585,7 +585,6 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
 template <typename T, int HD>
 hipError_t ta_launch_hd(const PagedAttnLaunch& L) {
   constexpr int kMany = PaType<T>::kPieces;
-  if ((size_t)L.n_new * (L.heads / L.kv.n_kv) <= ta_few(HD)) return pa_launch_hd<T, HD, true>(L);
   // a weight's pieces: two are within 2^-17 of it (bf16), far below a rounding of a 16-bit output
   if (L.dtype == PaType<T>::kId) return ta_launch_rows<T, HD, 1, 2>(L);
   return ta_launch_rows<T, HD, kMany, kMany>(L);

@@ -5,12 +5,14 @@ namespace nrq {
 
 hipError_t launch_tree_bf16(const PagedAttnLaunch& L);
 
+double tree_attn_line(size_t seqs, size_t n_new, size_t heads, int n_kv, int64_t held) {
+  return (double)(seqs * n_kv * ((n_new * (heads / n_kv) + 63) / 64)) * ((double)held / kTile + 1 + kTaSetup);
+}
+
 size_t tree_attn_workspace(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd) {
   const size_t rows = n_new * (heads / n_kv);
-  const size_t few = paged_attn_workspace(seqs, n_new, heads, n_kv, hd);
-  if (rows <= ta_few(hd)) return few;
-  // units of 64 rows at least; two parts a workgroup, of 128 rows at most where a CU has two of them, else of 256
-  const size_t units = seqs * n_kv * ((rows + 63) / 64), slots = rows <= 128 ? 2 * rows : (rows < 256 ? rows : 256);
+  // units of 64 rows at least; two parts a workgroup, of 128 rows at most where a CU has two workgroups, else of 256
+  const size_t units = seqs * n_kv * ((rows + 63) / 64), slots = rows <= 128 ? 2 * rows : 256;
   return 2 * (size_t)kTaCus * slots * ((size_t)hd * sizeof(float) + sizeof(float2)) + 16 + units * sizeof(int4);
 }
 

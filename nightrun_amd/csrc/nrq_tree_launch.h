@@ -15,6 +15,7 @@ struct NormRopeLaunch {
 };
 hipError_t launch_norm_rope(const NormRopeLaunch& L);
 
+double tree_attn_line(size_t seqs, size_t n_new, size_t heads, int n_kv, int64_t held);  // tiles of all units at most
 size_t tree_attn_workspace(size_t seqs, size_t n_new, size_t heads, int n_kv, int hd);
 hipError_t launch_tree_attn(const PagedAttnLaunch& L);
 

@@ -149,6 +149,21 @@ def test_workspaces():
     assert L.nrq_tree_attention_workspace(3, 8, 32, _kv(), None) == ARG
 
 
+@pytest.mark.parametrize("seqs,width,fits", [(2 ** 20, 2048, True), (2 ** 20, 16128, True), (2 ** 20, 16366, False), (2 ** 20, 16384, False)])
+def test_tree_attention_line(seqs, width, fits):
+    """One node, one head over one: a sequence is its tiles and what the beginning of a unit counts for; 2^31 of them are
+    no int."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("checks the no-GPU failure path")
+    rc, msg = _call("nrq_dev_tree_attention", _attend(), n_new=1, heads=1, ws_bytes=1 << 40,
+                    strides=_i64(128, 128, 128, 128, 128, 128),
+                    kv=_kv(n_kv_heads=1, page_stride=16 * 128), table=_table(pages=at(2), seqs=seqs, width=width, stride=width))
+    assert rc == (NOT_INIT if fits else UNSUPPORTED), (rc, msg)
+    assert fits or "too much" in msg
+
+
 # ---- what a node sees -----------------------------------------------------------------------------
 
 
