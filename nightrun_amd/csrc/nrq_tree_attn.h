@@ -599,7 +599,7 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
 template <typename T, int HD>
 hipError_t ta_launch_hd(const PagedAttnLaunch& L) {
   constexpr int kMany = PaType<T>::kPieces;
-  // A weight's pieces: with bf16 outputs two, within 2^-17 of it, where a rounding of the output is 2^-9 (and what cancels to a hundredth
+  // A weight's pieces: with bf16 outputs two, within 2^-17 of it, where a rounding of the output is 2^-8 (and what cancels to a hundredth
   // keeps it); a third would be a third more products. f32 outputs take three, which are all of its bits.
   if (L.dtype == PaType<T>::kId) return ta_launch_rows<T, HD, 1, 2>(L);
   return ta_launch_rows<T, HD, kMany, kMany>(L);

@@ -475,6 +475,108 @@ def test_tree_strides_and_far_offsets(gpu, new):
     assert np.all(got == 2.0)
 
 
+@pytest.mark.parametrize("heads,kv,new,hd,kind,cache", [(64, 1, 64, 64, "bf16", "bf16"), (24, 1, 64, 128, "f32", "f16"), (7, 1, 64, 32, "f16", "f16"),
+                                                        (20, 1, 64, 128, "f32", "bf16"), (16, 1, 64, 256, "f16", "f16"), (9, 3, 64, 96, "bf16", "bf16")])
+def test_tree_many_rows(gpu, heads, kv, new, hd, kind, cache):
+    """Several units for a KV head, the last of them not full, over a sequence that fills the card and short ones."""
+    lens = [9000 if hd < 256 else 4000, 64, 200]
+    c = Cache(gen(hd), lens, kv, hd, 16, cache)
+    check_tree(c, kind, cache, trees(heads, 3, new), heads)
+
+
+@pytest.mark.parametrize("size", [3, 200, 1000])
+@pytest.mark.parametrize("new", [5, 40])
+def test_tree_page_sizes(gpu, size, new):
+    """Pages longer than a stage, pages that end anywhere in it; a table with room for far more than there is."""
+    c = Cache(gen(size), [700, 128 + new, 256, 64 + new], 2, 128, size, "f16", width=4096 // size + 1)
+    check_tree(c, "f16", "f16", trees(size, 4, new), 8)
+    check_tree(c, "f32", "f16", trees(size, 4, new), 2, window=77)
+
+
+@pytest.mark.parametrize("new", [4, 40])
+def test_tree_one_pool_and_wide_table(gpu, new):
+    """Keys and values side by side in one pool; the table is a part of a wider one."""
+    import torch
+
+    from nightrun_amd import serve
+
+    c = Cache(gen(new), [300, new, 129], 2, 64, 16, "bf16")
+    t = trees(new, 3, new)
+    want = check_tree(c, "bf16", "bf16", t, 8)
+    kp, vp, table, lens = c.dev()
+    for both in (torch.stack((kp, vp), 1), torch.stack((kp.transpose(1, 2), vp.transpose(1, 2)), 2)):
+        k, v = (both[:, 0], both[:, 1]) if both.shape[1] == 2 else (both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2))
+        wide = torch.full((3, c.width + 5), -1, dtype=torch.int32, device="cuda")
+        wide[:, 2:2 + c.width] = table
+        q = normal(gen(1), 3, new, 8, 64, kind="bf16", scale=1.5)
+        y = torch.empty_like(q)
+        serve.tree_attention(y, q, k, v, wide[:, 2:2 + c.width], lens, torch.from_numpy(t).cuda(), 0.125)
+        assert torch.equal(y, want)
+        # the append and the move into such pools
+        x = normal(gen(2), 3, 12, 64, kind="bf16")
+        f = torch.from_numpy(freqs(32)).cuda()
+        pos = lens - new
+        seq = torch.arange(3, dtype=torch.int32, device="cuda")
+        out = torch.empty(3, 8, 64, dtype=torch.bfloat16, device="cuda")
+        k2, v2 = kp.clone(), vp.clone()
+        serve.norm_rope_append(out, x[:, :8], x[:, 8:10], x[:, 10:], None, None, pos, seq, f, k2, v2, table)
+        serve.norm_rope_append(out, x[:, :8], x[:, 8:10], x[:, 10:], None, None, pos, seq, f, k, v, wide[:, 2:2 + c.width])
+        assert torch.equal(k.nan_to_num(9), k2.nan_to_num(9)) and torch.equal(v.nan_to_num(9), v2.nan_to_num(9))
+        path = torch.full((3, new), -1, dtype=torch.int32, device="cuda")
+        path[:, 0], path[:, 1] = 1, new - 1
+        a, b = torch.empty_like(lens), torch.empty_like(lens)
+        serve.keep_path(a, k2, v2, table, lens, path)
+        serve.keep_path(b, k, v, wide[:, 2:2 + c.width], lens, path)
+        assert torch.equal(a, b) and torch.equal(k.nan_to_num(9), k2.nan_to_num(9)) and torch.equal(v.nan_to_num(9), v2.nan_to_num(9))
+
+
+@pytest.mark.parametrize("kind,cache,hd", [("f16", "f16", 128), ("f32", "f16", 64), ("f32", "bf16", 128), ("bf16", "bf16", 256)])
+def test_tree_bad_queries_stay_alone(gpu, kind, cache, hd):
+    """Queries with an infinity or a NaN: their rows alone."""
+    import torch
+
+    from nightrun_amd import serve
+
+    c = Cache(gen(hd), [400, 90], 2, hd, 16, cache)
+    t = trees(3, 2, 20)
+    q = normal(gen(5), 2, 20, 8, hd, kind=kind, scale=1.5)
+    want, tol, _, _ = tree_attention(f64(q), c, t, [20, 20], hd ** -0.5, 0)
+    tol += PIECES[kind, cache] * max(float(v.abs().max()) for v in c.v) + half_step(kind) * np.abs(want)
+    q[0, 3, 1, 7], q[1, 19, 7, hd - 1] = float("nan"), float("inf")
+    kp, vp, table, lens = c.dev()
+    y = torch.empty_like(q)
+    serve.tree_attention(y, q, kp, vp, table, lens, torch.from_numpy(t).cuda(), hd ** -0.5)
+    got = f64(y)
+    bad = np.zeros(got.shape[:3], bool)
+    bad[0, 3, 1] = bad[1, 19, 7] = True
+    assert np.all(np.abs(got - want)[~bad] <= tol[~bad]) and not np.isfinite(got[bad]).any()
+
+
+def test_norm_rope_more_tokens_than_a_grid_has_threads_for(gpu):
+    """2^29 tokens and some are two launches: rows around the seam and at the ends."""
+    import torch
+
+    from nightrun_amd import serve
+
+    n = 2 ** 29 + 77
+    x = torch.tensor([[[3.0, 4.0]]], device="cuda", dtype=torch.bfloat16).expand(n, 1, 2)
+    pos = torch.zeros(n, dtype=torch.int32, device="cuda")
+    at = [0, 1, 2 ** 29 - 1, 2 ** 29, 2 ** 29 + 1, n - 1]
+    for i, p in enumerate(at):
+        pos[p] = i + 1
+    y = torch.zeros(n, 1, 2, dtype=torch.bfloat16, device="cuda")
+    f = torch.ones(1, device="cuda")
+    serve.norm_rope(y, x, None, pos, f)
+    r = math.sqrt(12.5 + 1e-6)
+    for i, p in enumerate(at):
+        c, s_ = math.cos(i + 1), math.sin(i + 1)
+        w = np.array([3 * c - 4 * s_, 3 * s_ + 4 * c]) / r
+        assert np.all(np.abs(f64(y[p, 0]) - w) <= half_step("bf16") * np.abs(w) + 1e-6)
+    w = torch.tensor([3 / r, 4 / r], device="cuda").bfloat16()
+    bad = (y[:, 0] != w).any(-1)
+    assert int(bad.sum()) == len(at)
+
+
 # ---- acceptance of a path ---------------------------------------------------------------------------
 
 
