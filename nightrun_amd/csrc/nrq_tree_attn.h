@@ -16,12 +16,12 @@
 // show no conflicts.
 //
 // What bounds it. Two sequences of 65,536 and 131,072 positions by 64 nodes (256 rows a KV head of 128, f16; 805 MB, 206 GFLOP, 309 with the
-// weights in two pieces) take 355 us, 13 of them the join: the matrix units work half of the clocks, vector instructions the other half, and the
+// weights in two pieces) take 351 us, 10 of them the join: the matrix units work half of the clocks, vector instructions the other half, and the
 // clock is down to 1.75 GHz, the power limit; without its loads it would take 300. Orders of instructions, priorities and stages that
 // keep both busier change nothing there. 64 rows a wave halve the reads of LDS but leave the 256 registers that
-// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, 307 MB) 97 us: 86 and the
+// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, 307 MB) 97 to 100 us: 86 and the
 // join; a unit's beginning and end (its length, pages, queries and first stage in sequence, its parts) are a third of it. 13 sequences under a window
-// of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 76. One sequence of 1001 positions by 8 nodes 13.4: two launches, one tile a workgroup.
+// of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 73. One sequence of 1001 positions by 8 nodes 13.4: two launches, one tile a workgroup.
 #pragma once
 
 #include "nrq_paged.h"
@@ -33,6 +33,10 @@ constexpr int kTaCus = 256;
 // What the beginning and the end of a unit cost, in tiles: stretches of many short units are as long as those of a few long ones. 24
 // sequences of 250 to 6000 positions by 32 nodes take 156, 127, 114, 115 us with 0, 1, 2, 3, 119 with 5; 13 of one length 91, 85, 81, 79 and 80.
 constexpr int kTaSetup = 3;
+// Workgroups of a unit, on average, from which on the join takes a row a workgroup, 16 stretches side by side, else four rows, four
+// stretches side by side: one KV head over 131,072 positions by 4 nodes 36.7 us so, 51.8 the other way (92.8 with one after the
+// other); two sequences of 8 heads (16 workgroups a unit) 345 and 334, 24 by 32 nodes (three) 124 and 108.
+constexpr int kTaShared = 32;
 
 namespace {
 
@@ -505,17 +509,22 @@ __global__ __launch_bounds__(64 * W, ta_waves(HD, NQ)) void tree_kernel(PaArgs A
   }
 }
 
-// The stretches of a unit that several workgroups shared, in order: 16 lanes a row, 16 rows a workgroup.
-template <typename T, int HD>
+// The stretches of a unit that several workgroups shared: 16 lanes a row and G groups of them, each of which takes every
+// G-th stretch; what they have is added up in order.
+template <typename T, int HD, int G>
 __global__ __launch_bounds__(256) void tree_join_kernel(PaArgs A, int wide_o) {
   constexpr int E = HD / 16, F = E % 4 ? 2 : 4;  // dimensions of a lane, F side by side
+  constexpr int R = 16 / G;                      // rows
+  __shared__ float ex_o[G > 1 ? G : 1][R][G > 1 ? HD : 1], ex_l[G][R];
   const PagedAttnLaunch& L = A.L;
   const int u = blockIdx.x, b = u / A.units_per_seq, unit = u - b * A.units_per_seq;
   const int4 share = A.share[u];
-  const int r = 16 * blockIdx.y + (threadIdx.x >> 4), c = threadIdx.x & 15, w0 = share.x, n = share.y - w0 + 1;
-  if (n < 2 || r >= share.z) return;
+  const int c = threadIdx.x & 15, g = (threadIdx.x >> 4) % G, rw = threadIdx.x / (16 * G), r = R * blockIdx.y + rw;
+  const int w0 = share.x, n = share.y - w0 + 1;
+  if (n < 2 || R * (int)blockIdx.y >= share.z) return;
+  const bool on = r < share.z;
   const int head = unit / A.row_tiles, rr = (unit - head * A.row_tiles) * A.per + r;
-  auto slot = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * A.slots + r; };
+  auto slot = [&](int k) { return (int64_t)(2 * (w0 + k) + (k == 0 ? 1 : 0)) * A.slots + (on ? r : 0); };
   float mm = -INFINITY;
   for (int k = c; k < n; k += 16) mm = fmaxf(mm, A.part_ml[slot(k)].x);
 #pragma unroll
@@ -525,7 +534,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(PaArgs A, int wide_o) {
 #pragma unroll
   for (int e = 0; e < E; e++) o[e] = 0;
 #pragma unroll 4
-  for (int k = 0; k < n; k++) {
+  for (int k = g; k < n; k += G) {
     const int64_t s = slot(k);
     const float2 x = A.part_ml[s];
     const float by = __builtin_amdgcn_exp2f(x.x - ref);
@@ -534,6 +543,20 @@ __global__ __launch_bounds__(256) void tree_join_kernel(PaArgs A, int wide_o) {
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] += p[e / F * 16 * F + e % F] * by;
   }
+  if constexpr (G > 1) {
+#pragma unroll
+    for (int e = 0; e < E; e++) ex_o[g][rw][16 * e + c] = o[e];
+    if (c == 0) ex_l[g][rw] = l;
+    __syncthreads();
+    if (g > 0) return;
+#pragma unroll
+    for (int k = 1; k < G; k++) {
+      l += ex_l[k][rw];
+#pragma unroll
+      for (int e = 0; e < E; e++) o[e] += ex_o[k][rw][16 * e + c];
+    }
+  }
+  if (!on) return;
   const int tok = rr / A.group, h = head * A.group + rr - tok * A.group;
   const bool none = mm == -INFINITY && l == 0.0f;
   const float by = 1.0f / l;
@@ -567,8 +590,10 @@ hipError_t ta_launch(const PagedAttnLaunch& L) {
   const int v = L.dtype == kF32 ? 4 : 2;  // four values are stored together
   const int wide_o = ((uintptr_t)L.out & (v == 4 ? 15 : 7)) == 0 && L.ob % 4 == 0 && L.ot % 4 == 0 && L.oh % 4 == 0;
   hipLaunchKernelGGL((tree_kernel<T, HD, W, WR, TP, NQ, NP>), dim3(A.wgs), dim3(64 * W), 0, L.stream, A, wide_o);
-  if (tiles > 1)
-    hipLaunchKernelGGL((tree_join_kernel<T, HD>), dim3((unsigned)units, (A.slots + 15) / 16), dim3(256), 0, L.stream, A, wide_o);
+  if (tiles > 1 && A.wgs >= kTaShared * units)
+    hipLaunchKernelGGL((tree_join_kernel<T, HD, 16>), dim3((unsigned)units, A.slots), dim3(256), 0, L.stream, A, wide_o);
+  else if (tiles > 1)
+    hipLaunchKernelGGL((tree_join_kernel<T, HD, 4>), dim3((unsigned)units, (A.slots + 3) / 4), dim3(256), 0, L.stream, A, wide_o);
   return hipGetLastError();
 }
 
