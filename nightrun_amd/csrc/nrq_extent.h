@@ -79,9 +79,8 @@ inline Range range_of(const Extent& e) {
   return Range{(uintptr_t)e.first + from, (uintptr_t)e.first + to};
 }
 
-// Whether they do, or lie between one another as as_rows() cannot tell apart.
-inline bool extents_meet(const Extent& a, const Extent& b) {
-  const Range x = range_of(a), y = range_of(b);
+// Whether two tensors of these ranges share memory, or lie between one another as as_rows() cannot tell apart.
+inline bool extents_meet(const Extent& a, const Range& x, const Extent& b, const Range& y) {
   return x.low < y.high && y.low < x.high && rows_meet(as_rows(a), as_rows(b));
 }
 

@@ -10,7 +10,6 @@ namespace {
 
 using nrq::Extent;
 using nrq::Range;
-using nrq::as_rows;
 using nrq::range_of;
 
 Extent whole(const void* p, size_t n, int size) { return Extent{p, p ? n : 0, size, {{0, 1}, {0, 1}, {0, 1}}}; }
@@ -29,7 +28,7 @@ int apart_from(const char* name, std::initializer_list<Extent> out, std::initial
     }
   for (size_t i = 0; i < outs; i++)
     for (size_t j = i + 1; j < n; j++)
-      if (r[i].low < r[j].high && r[j].low < r[i].high && nrq::rows_meet(as_rows(*e[i]), as_rows(*e[j])))
+      if (nrq::extents_meet(*e[i], r[i], *e[j], r[j]))
         return fail(NRQ_ERR_ARG, name, "an output shares memory with an input or another output");
   return NRQ_OK;
 }

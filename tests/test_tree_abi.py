@@ -226,7 +226,7 @@ extern "C" int meet(const int64_t* a, const int64_t* b) {
   for (int i = 0; i < 2; i++)
     e[i] = nrq::Extent{(const void*)p[i][0], (size_t)p[i][1], (int)p[i][2],
                        {{p[i][3], (size_t)p[i][4]}, {p[i][5], (size_t)p[i][6]}, {p[i][7], (size_t)p[i][8]}}};
-  return nrq::extents_meet(e[0], e[1]);
+  return nrq::extents_meet(e[0], nrq::range_of(e[0]), e[1], nrq::range_of(e[1]));
 }
 ''')
     so = d / "extent.so"
