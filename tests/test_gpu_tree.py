@@ -552,6 +552,37 @@ def test_tree_bad_queries_stay_alone(gpu, kind, cache, hd):
     assert np.all(np.abs(got - want)[~bad] <= tol[~bad]) and not np.isfinite(got[bad]).any()
 
 
+@pytest.mark.parametrize("kind,cache,hd,heads,kv,new", [("bf16", "bf16", 64, 8, 1, 40), ("f32", "bf16", 128, 4, 1, 50), ("f16", "f16", 256, 4, 1, 30),
+                                                        ("f32", "f16", 96, 3, 1, 64), ("f16", "f16", 32, 4, 2, 20), ("bf16", "bf16", 128, 4, 1, 64),
+                                                        ("f32", "bf16", 256, 2, 1, 9)])
+def test_tree_infinities_in_every_shape(gpu, kind, cache, hd, heads, kv, new):
+    """An infinity in one node's values, which its descendants see and no other: with every number of rows and pieces, over
+    positions that several workgroups share."""
+    import torch
+
+    from nightrun_amd import serve
+
+    lens = [new + 600, new + 3, 130 + new]
+    c = Cache(gen(hd + new), lens, kv, hd, 16, cache)
+    t = trees(new, 3, new)
+    q = normal(gen(3), 3, new, heads, hd, kind=kind, scale=1.5)
+    want, tol, _, _ = tree_attention(f64(q), c, t, [new] * 3, hd ** -0.5, 0)
+    tol += PIECES[kind, cache] * max(float(v.abs().max()) for v in c.v) + half_step(kind) * np.abs(want)
+    node = new // 3
+    for b, n in enumerate(lens):
+        p = n - new + node
+        c.vp[int(c.table[b, p // 16]), :, p % 16, hd - 1] = float("inf")
+    kp, vp, table, lens_ = c.dev()
+    y = torch.empty_like(q)
+    serve.tree_attention(y, q, kp, vp, table, lens_, torch.from_numpy(t).cuda(), hd ** -0.5)
+    got = f64(y)
+    for b in range(3):
+        for j in range(new):
+            below = node in way(t[b], j)
+            assert np.all(np.abs(got[b, j] - want[b, j])[:, :hd - below] <= tol[b, j][:, :hd - below]), (b, j)
+            assert np.all(np.isposinf(got[b, j, :, hd - 1])) == below, (b, j)
+
+
 def test_norm_rope_more_tokens_than_a_grid_has_threads_for(gpu):
     """2^29 tokens and some are two launches: rows around the seam and at the ends."""
     import torch
