@@ -16,12 +16,12 @@
 // show no conflicts.
 //
 // What bounds it. Two sequences of 65,536 and 131,072 positions by 64 nodes (256 rows a KV head of 128, f16; 805 MB, 206 GFLOP, 309 with the
-// weights in two pieces) take 351 us, 10 of them the join: the matrix units work half of the clocks, vector instructions the other half, and the
+// weights in two pieces) take 351 to 358 us, 10 of them the join: the matrix units work half of the clocks, vector instructions the other half, and the
 // clock is down to 1.75 GHz, the power limit; without its loads it would take 300. Orders of instructions, priorities and stages that
 // keep both busier change nothing there. 64 rows a wave halve the reads of LDS but leave the 256 registers that
-// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, 307 MB) 97 to 100 us: 86 and the
+// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, 307 MB) 97 to 102 us: 86 and the
 // join; a unit's beginning and end (its length, pages, queries and first stage in sequence, its parts) are a third of it. 13 sequences under a window
-// of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 73. One sequence of 1001 positions by 8 nodes 13.4: two launches, one tile a workgroup.
+// of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 73 to 77. One sequence of 1001 positions by 8 nodes 13.4: two launches, one tile a workgroup.
 #pragma once
 
 #include "nrq_paged.h"
