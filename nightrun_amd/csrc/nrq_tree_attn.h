@@ -19,8 +19,8 @@
 // weights in two pieces) take 351 to 358 us, 10 of them the join: the matrix units work half of the clocks, vector instructions the other half, and the
 // clock is down to 1.75 GHz, the power limit; without its loads it would take 300. Orders of instructions, priorities and stages that
 // keep both busier change nothing there. 64 rows a wave halve the reads of LDS but leave the 256 registers that
-// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, 307 MB) 97 to 102 us: 86 and the
-// join; a unit's beginning and end (its length, pages, queries and first stage in sequence, its parts) are a third of it. 13 sequences under a window
+// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, bf16, 307 MB) 112 to 116 us, 99 with the weights in two pieces instead of
+// three, which left them 16 bits; a unit's beginning and end (its length, pages, queries and first stage in sequence, its parts) are a third of it. 13 sequences under a window
 // of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 73 to 77. One sequence of 1001 positions by 8 nodes 13.4: two launches, one tile a workgroup.
 #pragma once
 
@@ -140,10 +140,11 @@ struct TaShape {
 // Waves of a SIMD: registers for the accumulators and the queries' pieces.
 constexpr int ta_waves(int hd, int nq) { return hd > 128 || nq > 2 ? 1 : 2; }
 
-template <typename T, int HD, int W, int WR, int TP, int NQ, int NP>
+template <typename T, int HD, int W, int WR, int TP, int NQ>
 __global__ __launch_bounds__(64 * W, ta_waves(HD, NQ)) void tree_kernel(PaArgs A, int wide_o) {
   typedef TaShape<HD, W, WR, TP> Sh;
   typedef typename PaType<T>::v8 v8;
+  constexpr int NP = PaType<T>::kPieces;  // of a weight: f32 values, as in nrq_paged.h
   constexpr int KS = HD / 16, DB = HD / 32, WP = Sh::kWP;
   __shared__ __align__(512) uint8_t shared[Sh::kLds];  // rows of a stage begin at multiples of their size
   __shared__ float ex_ml[W][32][2];
@@ -577,7 +578,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(PaArgs A, int wide_o) {
         none ? -INFINITY : (mm - PaType<T>::kOffset + log2f(l)) * 0.69314718055994531f;
 }
 
-template <typename T, int HD, int W, int WR, int TP, int NQ, int NP>
+template <typename T, int HD, int W, int WR, int TP, int NQ>
 hipError_t ta_launch(const PagedAttnLaunch& L) {
   PaArgs A = pa_args(L, 32 * WR);
   const int64_t units = (int64_t)A.units_per_seq * L.table.seqs;
@@ -589,7 +590,7 @@ hipError_t ta_launch(const PagedAttnLaunch& L) {
   pa_workspace(A, HD);
   const int v = L.dtype == kF32 ? 4 : 2;  // four values are stored together
   const int wide_o = ((uintptr_t)L.out & (v == 4 ? 15 : 7)) == 0 && L.ob % 4 == 0 && L.ot % 4 == 0 && L.oh % 4 == 0;
-  hipLaunchKernelGGL((tree_kernel<T, HD, W, WR, TP, NQ, NP>), dim3(A.wgs), dim3(64 * W), 0, L.stream, A, wide_o);
+  hipLaunchKernelGGL((tree_kernel<T, HD, W, WR, TP, NQ>), dim3(A.wgs), dim3(64 * W), 0, L.stream, A, wide_o);
   if (tiles > 1 && A.wgs >= kTaShared * units)
     hipLaunchKernelGGL((tree_join_kernel<T, HD, 16>), dim3((unsigned)units, A.slots), dim3(256), 0, L.stream, A, wide_o);
   else if (tiles > 1)
@@ -599,7 +600,7 @@ hipError_t ta_launch(const PagedAttnLaunch& L) {
 
 // Units of as many rows as there are, up to what a workgroup's registers hold: 32 a wave, of eight waves on two a SIMD, or
 // where a row takes more registers (heads of 256, queries in three pieces) of four.
-template <typename T, int HD, int NQ, int NP>
+template <typename T, int HD, int NQ>
 hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
   const int rows = L.n_new * (L.heads / L.kv.n_kv);
   // Units of as many rows as leave each workgroup three tiles, as far as the table goes (the lengths are on the device). One sequence by 64
@@ -608,26 +609,23 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
   const int64_t tiles = (int64_t)L.table.seqs * L.kv.n_kv * (((int64_t)L.table.width * L.kv.page_size + kTile - 1) / kTile);
   auto fills = [&](int per, int wgs) { return tiles * ((rows + per - 1) / per) >= 3 * wgs; };
   if constexpr (HD > 128 || NQ > 2) {
-    if (rows > 64 && fills(128, kTaCus)) return ta_launch<T, HD, 4, 4, 64, NQ, NP>(L);
-    return ta_launch<T, HD, 4, 2, 64, NQ, NP>(L);
+    if (rows > 64 && fills(128, kTaCus)) return ta_launch<T, HD, 4, 4, 64, NQ>(L);
+    return ta_launch<T, HD, 4, 2, 64, NQ>(L);
   } else {
     // More than 128 rows: one workgroup of eight waves a CU (two long sequences by 64 nodes 359 us, in two units of 128 rows 414, in four
     // of 64 531). Else two of four waves, one of which multiplies while the other begins or ends a unit (24 sequences by 32 nodes
     // 96 us, with one of eight waves 104).
     constexpr int kTP = HD == 128 || HD == 96 ? 64 : 128;
-    if (rows > 128 && fills(256, kTaCus)) return ta_launch<T, HD, 8, 8, HD == 96 ? 128 : kTP, NQ, NP>(L);
-    if (rows > 64 && fills(128, 2 * kTaCus)) return ta_launch<T, HD, 4, 4, kTP, NQ, NP>(L);
-    return ta_launch<T, HD, 4, 2, kTP, NQ, NP>(L);
+    if (rows > 128 && fills(256, kTaCus)) return ta_launch<T, HD, 8, 8, HD == 96 ? 128 : kTP, NQ>(L);
+    if (rows > 64 && fills(128, 2 * kTaCus)) return ta_launch<T, HD, 4, 4, kTP, NQ>(L);
+    return ta_launch<T, HD, 4, 2, kTP, NQ>(L);
   }
 }
 
 template <typename T, int HD>
 hipError_t ta_launch_hd(const PagedAttnLaunch& L) {
-  constexpr int kMany = PaType<T>::kPieces;
-  // A weight's pieces: with bf16 outputs two, within 2^-17 of it, where a rounding of the output is 2^-8 (and what cancels to a hundredth
-  // keeps it); a third would be a third more products. f32 outputs take three, which are all of its bits.
-  if (L.dtype == PaType<T>::kId) return ta_launch_rows<T, HD, 1, 2>(L);
-  return ta_launch_rows<T, HD, kMany, kMany>(L);
+  if (L.dtype == PaType<T>::kId) return ta_launch_rows<T, HD, 1>(L);
+  return ta_launch_rows<T, HD, PaType<T>::kPieces>(L);
 }
 
 template <typename T>

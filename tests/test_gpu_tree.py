@@ -583,6 +583,54 @@ def test_tree_infinities_in_every_shape(gpu, kind, cache, hd, heads, kv, new):
             assert np.all(np.isposinf(got[b, j, :, hd - 1])) == below, (b, j)
 
 
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("new,width", [(1, 1), (3, 1), (12, 1), (40, 3), (12, 900), (40, 900)])
+def test_tree_weights_keep_32_bits(gpu, hd, new, width):
+    """bf16 throughout, outputs that cancel. Three positions before the tree weigh 1, a fourth p = exp(-c s), the nodes nothing; in
+    dimension h the values are minus the first two bf16 pieces of head h's p, and 1: what is left is the third piece. Values whose third
+    piece is 2^-18.5 and more. Wide tables (whose columns are no pages) bring in the units of 128 and 256 rows.
+
+    The numerator is off by: 3 u of the exponent (at most 1 in units of log2) in its unit and product, 2 u in the exponential,
+    and 12 products of at most 2 added up, each sum rounded or cut: 24 u for rounding. In all 29 u, below 2^-18.5 / 1.4. The sum of the
+    weights, its reciprocal and the product with it: less than 8 u of the output."""
+    import torch
+
+    from nightrun_amd import serve
+
+    def bf(x):
+        return torch.tensor(x, dtype=torch.float64).bfloat16().double().numpy()
+
+    seqs, heads, s = 16, 8, 0.69
+    scale = float(np.float32(s))
+    c = np.concatenate([(128 + np.arange(128)) / 256, 1 - np.arange(1, 100) / 256.0])
+    c = c[c >= 0.5]
+    p = np.exp(-c * scale)
+    third = p - bf(p) - bf(p - bf(p))
+    c = c[np.abs(third) >= 2.0 ** -18.5]
+    assert len(c) >= 5
+    cc = c[np.random.default_rng(2).integers(0, len(c), (seqs, heads))]
+    p = np.exp(-cc * scale)
+    one, two = bf(p), bf(p - bf(p))
+    q = np.zeros((seqs, new, heads, hd))
+    q[..., 0] = cc[:, None]
+    pages = -(-(4 + new) // 16)
+    k, v = np.zeros((seqs, pages * 16, hd)), np.zeros((seqs, pages * 16, hd))
+    k[:, 3, 0] = -1.0
+    k[:, 4:, 0] = -1000.0
+    v[:, 0, :heads], v[:, 1, :heads], v[:, 3, :heads] = -one, -two, 1.0
+    qd = torch.from_numpy(q).to(torch.bfloat16).cuda()
+    kd, vd = (torch.from_numpy(x).to(torch.bfloat16).view(seqs * pages, 1, 16, hd).cuda() for x in (k, v))
+    table = torch.full((seqs, width), -1, dtype=torch.int32)
+    table[:, :pages] = torch.arange(seqs * pages, dtype=torch.int32).view(seqs, pages)
+    y = torch.empty_like(qd)
+    serve.tree_attention(y, qd, kd, vd, table.cuda(), torch.full((seqs,), 4 + new, dtype=torch.int32, device="cuda"),
+                         torch.from_numpy(trees(new, seqs, new)).cuda(), scale)
+    got = f64(y)[:, :, np.arange(heads), np.arange(heads)]
+    want = ((p - one - two) / (3 + p))[:, None]
+    assert np.all(np.abs(want) >= 2.0 ** -18.5 / 4)
+    assert np.all(np.abs(got - want) <= 29 * U / (3 + p[:, None]) + (half_step("bf16") + 8 * U) * np.abs(want))
+
+
 def test_norm_rope_more_tokens_than_a_grid_has_threads_for(gpu):
     """2^29 tokens and some are two launches: rows around the seam and at the ends."""
     import torch
