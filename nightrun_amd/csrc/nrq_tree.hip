@@ -208,7 +208,9 @@ int nrq_dev_keep_path(int32_t* new_lens, size_t layers, int64_t layer_stride, co
   const size_t n_kv = (size_t)kv->n_kv_heads, hd = (size_t)kv->head_dim, seqs = (size_t)table->seqs;
   if (n_kv * hd > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "%d KV heads of %d", kv->n_kv_heads, kv->head_dim);
   if (layers > (size_t)1 << 12) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu layers (at most 4096)", layers);
-  if ((double)layers * (double)n_kv * (double)hd > 1073741824.0)
+  // a thread has eight dimensions (the last of a head fewer) of keys or values, and the threads of a sequence are an int
+  const double threads = 2.0 * (double)layers * (double)n_kv * (double)((hd + 7) / 8);
+  if ((double)layers * (double)n_kv * (double)hd > 1073741824.0 || threads > (double)(INT_MAX - 255))
     return fail(NRQ_ERR_UNSUPPORTED, name, "%zu layers of %d KV heads of %d", layers, kv->n_kv_heads, kv->head_dim);
   const int64_t held = (int64_t)table->width * kv->page_size;  // positions of a sequence at most
   if (held > (int64_t)1 << 30) return fail(NRQ_ERR_UNSUPPORTED, name, "%lld positions of a sequence (at most 2^30)", (long long)held);

@@ -164,6 +164,23 @@ def test_tree_attention_line(seqs, width, fits):
     assert fits or "too much" in msg
 
 
+@pytest.mark.parametrize("layers,n_kv,hd,fits", [(1024, 2 ** 20, 1, False), (1024, 2 ** 20 - 1, 1, True), (4096, 2 ** 18, 1, False),
+                                                 (4096, 2 ** 18 - 1, 1, True), (1024, 2 ** 19, 2, True), (4096, 2 ** 15, 8, True),
+                                                 (1024, 1, 2 ** 20, True)])
+def test_keep_path_items(layers, n_kv, hd, fits):
+    """A thread has eight dimensions of a head's keys or values in a layer: the last are fewer, but a thread. 2^31 of those are no int."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("checks the no-GPU failure path")
+    head = -(-hd // 8) * 8
+    kv = _kv(k=at(10), v=at(2 ** 15), n_pages=2, page_size=1, n_kv_heads=n_kv, head_dim=hd, head_stride=head,
+             pos_stride=n_kv * head, page_stride=n_kv * head)
+    rc, msg = _call("nrq_dev_keep_path", _keep(), layers=layers, layer_stride=2 * n_kv * head, kv=kv)
+    assert rc == (NOT_INIT if fits else UNSUPPORTED), (rc, msg)
+    assert fits or "layers of" in msg
+
+
 # ---- what a node sees -----------------------------------------------------------------------------
 
 
