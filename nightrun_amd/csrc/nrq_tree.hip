@@ -207,6 +207,7 @@ int nrq_dev_keep_path(int32_t* new_lens, size_t layers, int64_t layer_stride, co
   if (n_new > nrq::kTreeMost) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu nodes (at most 64)", n_new);
   const size_t n_kv = (size_t)kv->n_kv_heads, hd = (size_t)kv->head_dim, seqs = (size_t)table->seqs;
   if (n_kv * hd > (size_t)1 << 20) return fail(NRQ_ERR_UNSUPPORTED, name, "%d KV heads of %d", kv->n_kv_heads, kv->head_dim);
+  if (seqs > (size_t)1 << 30) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu sequences (at most 2^30)", seqs);
   if (layers > (size_t)1 << 12) return fail(NRQ_ERR_UNSUPPORTED, name, "%zu layers (at most 4096)", layers);
   // a thread has eight dimensions (the last of a head fewer) of keys or values, and the threads of a sequence are an int
   const double threads = 2.0 * (double)layers * (double)n_kv * (double)((hd + 7) / 8);

@@ -181,6 +181,18 @@ def test_keep_path_items(layers, n_kv, hd, fits):
     assert fits or "layers of" in msg
 
 
+@pytest.mark.parametrize("seqs,fits", [(2 ** 30, True), (2 ** 30 + 1, False), (2 ** 31 - 1, False)])
+def test_keep_path_sequences(seqs, fits):
+    """Launches go from sequence to sequence in steps of up to 2^15 of them: behind the last, that is an int too."""
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("checks the no-GPU failure path")
+    rc, msg = _call("nrq_dev_keep_path", _keep(), n_new=0, table=_table(pages=at(1), seqs=seqs, width=0, stride=0))
+    assert rc == (NOT_INIT if fits else UNSUPPORTED), (rc, msg)
+    assert fits or "sequences" in msg
+
+
 # ---- what a node sees -----------------------------------------------------------------------------
 
 
