@@ -33,7 +33,8 @@ int nrq_dev_norm_rope(void *y, const void *x, int dtype, size_t tokens, size_t h
  * as they are (weights and eps are not used). at (or NULL: pos) has the cache position of each token, where it
  * is not the rotary one; then pos may be any int32. A token whose seq is outside [0, table.seqs) or whose place at[t] is
  * negative is padding, one whose place is behind the table, or on no page, is rotated but not appended. y may be q (then with the
- * same strides); it shares no memory with q otherwise, nor with k or v, and the cache none with either. */
+ * same strides); it shares no memory with q otherwise, nor with any other input, the cache none with either, and
+ * its keys none with its values. */
 int nrq_dev_norm_rope_append(void *y, const void *q, const void *k, const void *v, int dtype, size_t tokens,
                              size_t heads, const int64_t strides[8], int norm, const float *q_weight,
                              const float *k_weight, float eps, const int32_t *pos, const int32_t *seq,

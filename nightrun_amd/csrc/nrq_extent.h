@@ -84,4 +84,43 @@ inline bool extents_meet(const Extent& a, const Range& x, const Extent& b, const
   return x.low < y.high && y.low < x.high && rows_meet(as_rows(a), as_rows(b));
 }
 
+// Whether a tensor and another of the same layout at `other` share memory, where no two rows of one overlap (each dimension steps
+// over all of the smaller ones'). Exact, wherever one lies in the other: rows meet where their distance, less than a row,
+// is the tensors' and some steps of each dimension. A dimension's steps leave what the smaller ones span, less than its stride,
+// so that there are two numbers of them at most.
+inline bool copies_meet(const Extent& e, const void* other) {
+  typedef __int128 wide;
+  struct Step {
+    wide stride, most;  // bytes; steps either way
+  } d[sizeof e.d / sizeof e.d[0]];
+  int n = 0;
+  wide span = (wide)e.len * e.size;  // of what is smaller, beside the row's first byte
+  for (const Dim& x : e.d) {
+    if (x.n == 0) return false;
+    if (x.n == 1) continue;
+    int i = n++;
+    const Step y{(wide)(x.stride < 0 ? -(wide)x.stride : (wide)x.stride) * e.size, (wide)(x.n - 1)};
+    for (; i > 0 && d[i - 1].stride > y.stride; i--) d[i] = d[i - 1];
+    d[i] = y;
+    span += y.stride * y.most;
+  }
+  if (e.len == 0) return false;
+  struct Search {
+    const Step* d;
+    bool meet(int n, wide off, wide span) const {
+      if (off >= span || -off >= span) return false;
+      if (n == 0) return true;
+      const Step& x = d[n - 1];
+      const wide rest = span - x.stride * x.most;
+      if (x.stride == 0) return meet(n - 1, off, rest);
+      wide k = -(off + rest - 1) / x.stride;  // near the least with off + k stride > -rest
+      k = k - 1 < -x.most ? -x.most : k - 1;
+      for (; k <= x.most && off + k * x.stride < rest; k++)
+        if (meet(n - 1, off + k * x.stride, rest)) return true;
+      return false;
+    }
+  };
+  return Search{d}.meet(n, (wide)(uintptr_t)other - (wide)(uintptr_t)e.first, span);
+}
+
 }  // namespace nrq

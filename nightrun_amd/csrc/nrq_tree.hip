@@ -37,6 +37,10 @@ Extent heads_of(const void* p, int dtype, size_t tokens, int64_t ts, size_t head
   return Extent{p, hd, (int)bytes_of(dtype), {{ts, tokens}, {hs, heads}, {0, 1}}};
 }
 
+Extent table_of(const nrq_page_table& t) {
+  return Extent{t.pages, (size_t)t.width, 4, {{t.stride, (size_t)t.seqs}, {0, 1}, {0, 1}}};
+}
+
 int norm_check(const char* name, float eps, const float* wq, const float* wk) {
   if (!(eps >= 0.0f) || eps > 3e38f) return fail(NRQ_ERR_ARG, name, "eps of %g", (double)eps);
   if (!aligned(wq, 4) || !aligned(wk, 4)) return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
@@ -107,12 +111,13 @@ int nrq_dev_norm_rope_append(void* y, const void* q, const void* k, const void* 
                ck{kv->k, hd, 2, {{kv->page_stride, n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, size}}},
                cv{kv->v, hd, 2, {{kv->page_stride, n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, size}}};
   const Extent at_ = whole(at, tokens, 4), wq = whole(norm ? q_weight : nullptr, hd, 4), wk = whole(norm ? k_weight : nullptr, hd, 4),
-               pe = whole(pos, tokens, 4), se = whole(seq, tokens, 4), fe = whole(freqs, n_freqs, 4);
+               pe = whole(pos, tokens, 4), se = whole(seq, tokens, 4), fe = whole(freqs, n_freqs, 4), te = table_of(*table);
   const Extent none{};  // in place the queries are left out
-  if ((rc = apart_from(name, {ye}, {y != q ? qe : none, ck, cv, ke, ve, pe, se, at_, fe, wq, wk})) ||
-      (rc = apart_from(name, {ck}, {y != q ? qe : none, ke, ve, pe, se, at_, fe, wq, wk})) ||
-      (rc = apart_from(name, {cv}, {y != q ? qe : none, ke, ve, pe, se, at_, fe, wq, wk})))
+  if ((rc = apart_from(name, {ye}, {y != q ? qe : none, ck, cv, ke, ve, pe, se, at_, fe, wq, wk, te})) ||
+      (rc = apart_from(name, {ck}, {y != q ? qe : none, ke, ve, pe, se, at_, fe, wq, wk, te})) ||
+      (rc = apart_from(name, {cv}, {y != q ? qe : none, ke, ve, pe, se, at_, fe, wq, wk, te})))
     return rc;
+  if (nrq::copies_meet(ck, kv->v)) return fail(NRQ_ERR_ARG, name, "the cache's keys share memory with its values");
   return launched(name, nrq::launch_norm_rope(N));
 }
 
@@ -155,7 +160,7 @@ int nrq_dev_tree_attention(void* out, const void* q, int dtype, size_t n_new, si
                         whole(lens, seqs, 4),
                         whole(parents, seqs * n_new, 4),
                         whole(counts, seqs, 4),
-                        {table->pages, (size_t)table->width, 4, {{table->stride, seqs}, {0, 1}, {0, 1}}}})))
+                        table_of(*table)})))
     return rc;
   return launched(name, nrq::launch_tree_attn(L));
 }
@@ -230,7 +235,7 @@ int nrq_dev_keep_path(int32_t* new_lens, size_t layers, int64_t layer_stride, co
   if ((rc = device_check(name, stream))) return rc;
   if ((rc = apart_from(name, {whole(new_lens, seqs, 4)},
                        {whole(lens, seqs, 4), whole(path, seqs * n_new, 4), whole(counts, seqs, 4),
-                        {table->pages, (size_t)table->width, 4, {{table->stride, seqs}, {0, 1}, {0, 1}}}})))
+                        table_of(*table)})))
     return rc;
   return launched(name, nrq::launch_keep(L));
 }

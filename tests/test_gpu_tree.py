@@ -1008,6 +1008,90 @@ def test_tree_refusals(gpu):
         serve.keep_path(torch.empty_like(lens), kp[None], vp, table, lens, path)
 
 
+class Arena:
+    """Arguments of a C entry in one block of memory, each at the beginning of a slot of its own. Everything is zeros: whatever a
+    call is made of them stays in their memory."""
+
+    SLOT = 4 << 20
+
+    def __init__(self, entry):
+        import torch
+
+        from nightrun_amd import _lib
+
+        _lib.init(0)
+        self.entry, self.a = entry, getattr(self, entry[len("nrq_dev_"):])()
+        self.size = {n: x[0] for n, x in self.a.items() if isinstance(x, tuple)}  # bytes, alignment
+        self.align = {n: x[1] for n, x in self.a.items() if isinstance(x, tuple)}
+        self.block = torch.zeros(len(self.size) * self.SLOT, dtype=torch.uint8, device="cuda")
+        self.at = {n: self.block.data_ptr() + i * self.SLOT for i, n in enumerate(self.size)}
+
+    def call(self, **moved):
+        """The status and what went wrong, with arguments moved to other addresses."""
+        import ctypes as C
+
+        import torch
+
+        from nightrun_amd import _lib
+        from nightrun_amd.serve import PagedKv, PageTable
+
+        self.block.zero_()
+        p, args = {**self.at, **moved}, []
+        for n, x in self.a.items():
+            if n in ("k_pages", "v_pages", "pages"):
+                continue
+            if n == "kv":
+                args.append(C.byref(PagedKv(p["k_pages"], p["v_pages"], *x)))
+            elif n == "table":
+                args.append(C.byref(PageTable(p["pages"], *x)))
+            elif n == "strides":
+                args.append((C.c_int64 * len(x))(*x))
+            else:
+                args.append(p[n] if n in p else x)
+        rc = getattr(_lib.lib(), self.entry)(*args, torch._C._cuda_getCurrentRawStream(0))
+        torch.cuda.synchronize()
+        return rc, _lib.lib().nrq_last_error().decode()
+
+    # ---- arguments in order: (bytes, alignment), or what they are; a cache's three pages of 16 positions of one head of 64
+
+    def pools(self):
+        return dict(k_pages=(6144, 16), v_pages=(6144, 16), pages=(16, 4), kv=[1024, 1024, 64, 3, 16, 1, 64, 16], table=[2, 2, 2])
+
+    def norm_rope(self):
+        return dict(y=(2048, 4), x=(2048, 4), dtype=0, tokens=4, heads=2, hd=64, strides=[128, 64, 128, 64], weight=(256, 4),
+                    eps=1e-6, pos=(16, 4), freqs=(128, 4), nf=32, style=1, scale=1.0)
+
+    def norm_rope_append(self):
+        return dict(y=(2048, 4), q=(2048, 4), k=(1024, 4), v=(1024, 4), dtype=0, tokens=4, heads=2,
+                    strides=[128, 64, 64, 64, 64, 64, 128, 64], norm=1, q_weight=(256, 4), k_weight=(256, 4), eps=1e-6,
+                    pos=(16, 4), seq=(16, 4), at=(16, 4), freqs=(128, 4), nf=32, style=1, scale=1.0, **self.pools())
+
+    def verify_tree(self):
+        return dict(tokens=(24, 4), path=(24, 4), accepted=(8, 4), target=(2400, 4), strides=[300, 100], drafted=(24, 4),
+                    parents=(24, 4), uniforms=(24, 4), counts=(8, 4), seqs=2, n_new=3, vocab=100, ws=(56, 16), ws_bytes=56)
+
+
+OUTPUTS = {"nrq_dev_norm_rope": ["y"], "nrq_dev_norm_rope_append": ["y", "k_pages", "v_pages"],
+           "nrq_dev_verify_tree": ["tokens", "path", "accepted", "ws"]}
+
+
+@pytest.mark.parametrize("entry", OUTPUTS)
+def test_tree_shared_memory(gpu, entry):
+    """Each output over the last bytes of each other argument, and right behind it: refused and taken."""
+    a = Arena(entry)
+    assert a.call()[0] == 0
+    for out in OUTPUTS[entry]:
+        for other in a.size:
+            if other == out:
+                continue
+            end, n = a.at[other] + a.size[other], a.align[out]
+            rc, text = a.call(**{out: (end - 1) // n * n})
+            assert rc == -1 and ("shares memory" in text or "share memory" in text), (out, other, rc, text)
+            assert a.call(**{out: -(-end // n) * n})[0] == 0, (out, other)
+    if "x" in a.a or "q" in a.a:
+        assert a.call(y=a.at["x" if "x" in a.a else "q"])[0] == 0  # in place
+
+
 # ---- a step of them together ---------------------------------------------------------------------------
 
 

@@ -319,6 +319,68 @@ def test_extents_of_layouts(extent):
     assert not extent(e(0, hd, (row, 0)), e(0, hd))
 
 
+@pytest.fixture(scope="module")
+def copies(tmp_path_factory):
+    d = tmp_path_factory.mktemp("copies")
+    src = d / "copies.cpp"
+    src.write_text('''#include "nrq_extent.h"
+extern "C" int meet(const int64_t* a, int64_t other) {
+  const nrq::Extent e{(const void*)a[0], (size_t)a[1], (int)a[2], {{a[3], (size_t)a[4]}, {a[5], (size_t)a[6]}, {a[7], (size_t)a[8]}}};
+  return nrq::copies_meet(e, (const void*)other);
+}
+''')
+    so = d / "copies.so"
+    subprocess.run(["g++", "-O1", "-shared", "-fPIC", "-Wall", "-Werror", "-fsanitize=undefined",
+                    "-fno-sanitize-recover", "-static-libubsan", "-I", os.path.join(ROOT, "nightrun_amd", "csrc"),
+                    str(src), "-o", str(so)], check=True)
+    L = C.CDLL(str(so))
+    return lambda a, other: bool(L.meet((C.c_int64 * 9)(*a), C.c_int64(other)))
+
+
+def test_copies_meet(copies):
+    """Keys and values of any layouts whose rows do not overlap, at any distance: exact."""
+    rng = random.Random(5)
+    met = between = 0
+    for _ in range(30000):
+        length, size = rng.choice([0, 1, 2, 4, 8]), rng.choice([1, 2])
+        span, dims = length, []
+        for _ in range(3):
+            stride, n = span + rng.choice([0, 0, 1, 8, span, 2 * span + 3]), rng.choice([0, 1, 1, 2, 3, 4])
+            dims.append((stride, n))
+            if n > 1:
+                span += stride * (n - 1)
+        rng.shuffle(dims)
+        first = 1 << 20
+        other = first + rng.randint(-size * (span + 10), size * (span + 10))
+        x = _bytes(first, length, size, *dims)
+        y = {i + other - first for i in x}
+        got = copies([first, length, size] + [v for d in dims for v in d], other)
+        assert got == bool(x & y), (length, size, dims, other - first)
+        met += got
+        between += not got and bool(x) and max(x) >= min(y) and max(y) >= min(x)
+    assert met > 3000 and between > 2000
+
+
+def test_copies_of_layouts(copies):
+    """Keys and values of one pool, some of its pages, some of its heads, at its far end; the same pool twice."""
+    base, kv, size, hd, layers, pages = 1 << 40, 8, 16, 128, 28, 1000
+
+    def e(*dims):
+        return [base, hd, 2] + [x for d in dims for x in d]
+
+    one = kv * size * hd
+    for k, off in ((e((2 * one, pages), (size * hd, kv), (hd, size)), one),  # [pages][2][heads][positions]
+                   (e((2 * one, pages), (size * hd, kv // 2), (hd, size)), one // 2),  # and half of the heads
+                   (e((2 * one, pages), (hd, kv), (2 * kv * hd, size)), kv * hd),  # [pages][positions][2][heads]
+                   (e((2 * one * (pages + 7), layers), (2 * one, pages), (hd, size * kv)), one),  # some pages of each layer
+                   (e((one, pages), (size * hd, kv), (hd, size)), one * pages), (e((2 ** 61, 4), (one, 3), (hd, size)), one * 3)):
+        gap = one - size * hd if off == one * 3 else 0  # one head's pages at the distance of all heads'
+        for sign in (1, -1):
+            assert not copies(k, base + 2 * off * sign) and not copies(k, base + 2 * (off - gap) * sign)
+            assert copies(k, base + (2 * (off - gap) - 2) * sign) and copies(k, base + 16 * sign)
+        assert copies(k, base)
+
+
 SHARED = [
     ("nrq_dev_norm_rope", "y", "x", 128), ("nrq_dev_norm_rope", "y", "weight", 0), ("nrq_dev_norm_rope", "y", "freqs", 0),
     ("nrq_dev_norm_rope_append", "y", "k", 0), ("nrq_dev_norm_rope_append", "y", "pos", 0),
