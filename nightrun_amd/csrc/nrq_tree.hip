@@ -41,6 +41,11 @@ Extent table_of(const nrq_page_table& t) {
   return Extent{t.pages, (size_t)t.width, 4, {{t.stride, (size_t)t.seqs}, {0, 1}, {0, 1}}};
 }
 
+Extent pool_of(const void* p, const nrq_paged_kv& kv) {
+  return Extent{p, (size_t)kv.head_dim, 2,
+                {{kv.page_stride, (size_t)kv.n_pages}, {kv.head_stride, (size_t)kv.n_kv_heads}, {kv.pos_stride, (size_t)kv.page_size}}};
+}
+
 int norm_check(const char* name, float eps, const float* wq, const float* wk) {
   if (!(eps >= 0.0f) || eps > 3e38f) return fail(NRQ_ERR_ARG, name, "eps of %g", (double)eps);
   if (!aligned(wq, 4) || !aligned(wk, 4)) return fail(NRQ_ERR_ARG, name, "pointer not aligned to its type");
@@ -105,11 +110,9 @@ int nrq_dev_norm_rope_append(void* y, const void* q, const void* k, const void* 
   L.neox = style == NRQ_ROPE_NEOX, L.scale = scale, L.stream = (hipStream_t)stream;
   N.norm = norm != 0, N.wq = q_weight, N.wk = k_weight, N.eps = eps, N.at = at;
   if ((rc = device_check(name, stream))) return rc;
-  const size_t n_pages = (size_t)kv->n_pages, size = (size_t)kv->page_size;
   const Extent qe = heads_of(q, dtype, tokens, L.xt, heads, L.xh, hd), ke = heads_of(k, dtype, tokens, L.kt, n_kv, L.kh, hd),
                ve = heads_of(v, dtype, tokens, L.vt, n_kv, L.vh, hd), ye = heads_of(y, dtype, tokens, L.yt, heads, L.yh, hd),
-               ck{kv->k, hd, 2, {{kv->page_stride, n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, size}}},
-               cv{kv->v, hd, 2, {{kv->page_stride, n_pages}, {kv->head_stride, n_kv}, {kv->pos_stride, size}}};
+               ck = pool_of(kv->k, *kv), cv = pool_of(kv->v, *kv);
   const Extent at_ = whole(at, tokens, 4), wq = whole(norm ? q_weight : nullptr, hd, 4), wk = whole(norm ? k_weight : nullptr, hd, 4),
                pe = whole(pos, tokens, 4), se = whole(seq, tokens, 4), fe = whole(freqs, n_freqs, 4), te = table_of(*table);
   const Extent none{};  // in place the queries are left out
@@ -160,7 +163,9 @@ int nrq_dev_tree_attention(void* out, const void* q, int dtype, size_t n_new, si
                         whole(lens, seqs, 4),
                         whole(parents, seqs * n_new, 4),
                         whole(counts, seqs, 4),
-                        table_of(*table)})))
+                        table_of(*table),
+                        pool_of(kv->k, *kv),
+                        pool_of(kv->v, *kv)})))
     return rc;
   return launched(name, nrq::launch_tree_attn(L));
 }

@@ -1066,13 +1066,26 @@ class Arena:
                     strides=[128, 64, 64, 64, 64, 64, 128, 64], norm=1, q_weight=(256, 4), k_weight=(256, 4), eps=1e-6,
                     pos=(16, 4), seq=(16, 4), at=(16, 4), freqs=(128, 4), nf=32, style=1, scale=1.0, **self.pools())
 
+    def tree_attention(self):
+        import ctypes as C
+
+        from nightrun_amd import _lib
+        from nightrun_amd.serve import PagedKv
+
+        pools, n = self.pools(), C.c_size_t()
+        kv = PagedKv(0, 0, *pools["kv"])
+        assert _lib.lib().nrq_tree_attention_workspace(2, 3, 2, C.byref(kv), C.byref(n)) == 0 and n.value < self.SLOT // 2
+        return dict(out=(3072, 4), q=(3072, 4), dtype=0, n_new=3, heads=2, strides=[384, 128, 64, 384, 128, 64], **pools,
+                    lens=(8, 4), parents=(24, 4), counts=(8, 4), scale=0.1, window=0, lse=(48, 4), ws=(n.value, 16),
+                    ws_bytes=n.value)
+
     def verify_tree(self):
         return dict(tokens=(24, 4), path=(24, 4), accepted=(8, 4), target=(2400, 4), strides=[300, 100], drafted=(24, 4),
                     parents=(24, 4), uniforms=(24, 4), counts=(8, 4), seqs=2, n_new=3, vocab=100, ws=(56, 16), ws_bytes=56)
 
 
 OUTPUTS = {"nrq_dev_norm_rope": ["y"], "nrq_dev_norm_rope_append": ["y", "k_pages", "v_pages"],
-           "nrq_dev_verify_tree": ["tokens", "path", "accepted", "ws"]}
+           "nrq_dev_tree_attention": ["out", "lse", "ws"], "nrq_dev_verify_tree": ["tokens", "path", "accepted", "ws"]}
 
 
 @pytest.mark.parametrize("entry", OUTPUTS)
@@ -1088,7 +1101,7 @@ def test_tree_shared_memory(gpu, entry):
             rc, text = a.call(**{out: (end - 1) // n * n})
             assert rc == -1 and ("shares memory" in text or "share memory" in text), (out, other, rc, text)
             assert a.call(**{out: -(-end // n) * n})[0] == 0, (out, other)
-    if "x" in a.a or "q" in a.a:
+    if "y" in a.a:
         assert a.call(y=a.at["x" if "x" in a.a else "q"])[0] == 0  # in place
 
 
