@@ -85,8 +85,9 @@ int nrq_dev_verify_tree(int32_t *tokens, int32_t *path, int32_t *accepted, const
  * ends the path. new_lens[b] (int32 [table.seqs]) = base + the number of those, at least 0. A move from or to a
  * position that is negative or on no page is left out. What was behind the new length is of no meaning.
  * Where two sequences of a call have a page in common, neither may write to it. new_lens shares no memory with the
- * inputs. n_new <= 64, at most 2^30 sequences. A layer has at most 2^20 values of a position (KV heads times head_dim, any head_dim), all layers, 4096 at
- * most, have at most 2^30, in at most 2^30 - 128 eights (the last of a head may be short). */
+ * inputs or the caches, these none with the inputs, keys none with values. n_new <= 64, at most 2^30 sequences. A layer
+ * has at most 2^20 values of a position (KV heads times head_dim, any head_dim), all layers, 4096 at most, have at most
+ * 2^30, in at most 2^30 - 128 eights (the last of a head may be short). */
 int nrq_dev_keep_path(int32_t *new_lens, size_t layers, int64_t layer_stride, const nrq_paged_kv *kv,
                       const nrq_page_table *table, const int32_t *lens, const int32_t *path, const int32_t *counts,
                       size_t n_new, void *stream);

@@ -7,22 +7,22 @@
 namespace nrq {
 
 struct Dim {
-  int64_t stride;  // elements
-  size_t n;
+  int64_t stride = 0;  // elements
+  size_t n = 1;
 };
 
-// A tensor of up to three dimensions of rows, for the question whether two share memory. Exact where both come down to
+// A tensor of up to four dimensions of rows, for the question whether two share memory. Exact where both come down to
 // rows of one dimension, once dimensions that follow one another without gaps, or at one distance, are taken together; else two
 // that lie between one another count as sharing.
 struct Extent {
   const void* first;
   size_t len;  // elements of a row
   int size;    // bytes of one
-  Dim d[3];
+  Dim d[4];
 };
 
 inline Rows as_rows(const Extent& e) {
-  Dim d[3];
+  Dim d[4];
   int n = 0;
   typedef __int128 wide;
   wide low = 0, len = (wide)e.len;
@@ -44,7 +44,7 @@ inline Rows as_rows(const Extent& e) {
     Dim &x = d[at], &y = d[at + 1];
     if ((wide)y.stride == (wide)x.stride * (wide)x.n) {
       x.n *= y.n;
-      if (n - at > 2) y = d[at + 2];
+      for (int i = at + 1; i + 1 < n; i++) d[i] = d[i + 1];
       n--;
     } else {
       len += (wide)x.stride * (wide)(x.n - 1), at++;

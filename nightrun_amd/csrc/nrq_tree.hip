@@ -12,7 +12,7 @@ using nrq::Extent;
 using nrq::Range;
 using nrq::range_of;
 
-Extent whole(const void* p, size_t n, int size) { return Extent{p, p ? n : 0, size, {{0, 1}, {0, 1}, {0, 1}}}; }
+Extent whole(const void* p, size_t n, int size) { return Extent{p, p ? n : 0, size, {}}; }
 
 // Refuses outputs that share memory with one another or with inputs; those that are not there (nullptr) share none.
 // Ranges that do not meet, as a rule, are told apart without more.
@@ -34,11 +34,11 @@ int apart_from(const char* name, std::initializer_list<Extent> out, std::initial
 }
 
 Extent heads_of(const void* p, int dtype, size_t tokens, int64_t ts, size_t heads, int64_t hs, size_t hd) {
-  return Extent{p, hd, (int)bytes_of(dtype), {{ts, tokens}, {hs, heads}, {0, 1}}};
+  return Extent{p, hd, (int)bytes_of(dtype), {{ts, tokens}, {hs, heads}}};
 }
 
 Extent table_of(const nrq_page_table& t) {
-  return Extent{t.pages, (size_t)t.width, 4, {{t.stride, (size_t)t.seqs}, {0, 1}, {0, 1}}};
+  return Extent{t.pages, (size_t)t.width, 4, {{t.stride, (size_t)t.seqs}}};
 }
 
 Extent pool_of(const void* p, const nrq_paged_kv& kv) {
@@ -200,7 +200,7 @@ int nrq_dev_verify_tree(int32_t* tokens, int32_t* path, int32_t* accepted, const
                       parents,  path};
   if ((rc = device_check(name, stream))) return rc;
   if ((rc = apart_from(name, {whole(tokens, all, 4), whole(path, all, 4), whole(accepted, seqs, 4), whole(workspace, need, 1)},
-                       {{target, vocab, 4, {{strides[0], seqs}, {strides[1], n_new}, {0, 1}}},
+                       {{target, vocab, 4, {{strides[0], seqs}, {strides[1], n_new}}},
                         whole(drafted, all, 4), whole(parents, all, 4), whole(uniforms, all, 4), whole(counts, seqs, 4)})))
     return rc;
   return launched(name, nrq::launch_verify_tree(L));
@@ -238,10 +238,13 @@ int nrq_dev_keep_path(int32_t* new_lens, size_t layers, int64_t layer_stride, co
   L.new_lens = new_lens, L.layers = (int)layers, L.layer_stride = layers > 1 ? layer_stride : 0;
   L.lens = lens, L.path = path, L.counts = counts, L.n_new = (int)n_new, L.stream = (hipStream_t)stream;
   if ((rc = device_check(name, stream))) return rc;
-  if ((rc = apart_from(name, {whole(new_lens, seqs, 4)},
-                       {whole(lens, seqs, 4), whole(path, seqs * n_new, 4), whole(counts, seqs, 4),
-                        table_of(*table)})))
+  const Extent le = whole(lens, seqs, 4), pe = whole(path, seqs * n_new, 4), ce = whole(counts, seqs, 4), te = table_of(*table);
+  Extent ck = pool_of(kv->k, *kv), cv = pool_of(kv->v, *kv);
+  ck.d[3] = cv.d[3] = {layer_stride, layers};
+  if ((rc = apart_from(name, {whole(new_lens, seqs, 4)}, {ck, cv, le, pe, ce, te})) ||
+      (rc = apart_from(name, {ck}, {le, pe, ce, te})) || (rc = apart_from(name, {cv}, {le, pe, ce, te})))
     return rc;
+  if (nrq::copies_meet(ck, kv->v)) return fail(NRQ_ERR_ARG, name, "the cache's keys share memory with its values");
   return launched(name, nrq::launch_keep(L));
 }
 

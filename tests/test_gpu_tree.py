@@ -1083,9 +1083,14 @@ class Arena:
         return dict(tokens=(24, 4), path=(24, 4), accepted=(8, 4), target=(2400, 4), strides=[300, 100], drafted=(24, 4),
                     parents=(24, 4), uniforms=(24, 4), counts=(8, 4), seqs=2, n_new=3, vocab=100, ws=(56, 16), ws_bytes=56)
 
+    def keep_path(self):
+        return dict(new_lens=(8, 4), layers=2, layer_stride=4096, **{**self.pools(), "k_pages": (14336, 16), "v_pages": (14336, 16)},
+                    lens=(8, 4), path=(24, 4), counts=(8, 4), n_new=3)
+
 
 OUTPUTS = {"nrq_dev_norm_rope": ["y"], "nrq_dev_norm_rope_append": ["y", "k_pages", "v_pages"],
-           "nrq_dev_tree_attention": ["out", "lse", "ws"], "nrq_dev_verify_tree": ["tokens", "path", "accepted", "ws"]}
+           "nrq_dev_tree_attention": ["out", "lse", "ws"], "nrq_dev_verify_tree": ["tokens", "path", "accepted", "ws"],
+           "nrq_dev_keep_path": ["new_lens", "k_pages", "v_pages"]}
 
 
 @pytest.mark.parametrize("entry", OUTPUTS)

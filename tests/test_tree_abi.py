@@ -381,6 +381,47 @@ def test_copies_of_layouts(copies):
         assert copies(k, base)
 
 
+def test_extents_of_four_dimensions(tmp_path):
+    """The caches of some layers: layers, pages, heads and positions come down to rows at one distance, whichever of them follow one
+    another without gaps. What lies beside a layer's pages in its part of memory is apart from them."""
+    src = tmp_path / "four.cpp"
+    src.write_text('''#include "nrq_extent.h"
+#include <cstdio>
+#include <initializer_list>
+int main() {
+  typedef nrq::Extent E;
+  auto meet = [](const E& a, const E& b) { return nrq::extents_meet(a, nrq::range_of(a), b, nrq::range_of(b)); };
+  const uintptr_t base = 1l << 40;
+  const int64_t hd = 128, size = 16, kv = 8, pages = 50, layers = 5, one = hd * size * kv, gap = 4096;
+  const size_t s = size, h = kv, p = pages, l = layers;
+  const int64_t layer = pages * one + gap;
+  const E dense{(void*)base, (size_t)hd, 2, {{one, p}, {size * hd, h}, {hd, s}, {layer, l}}};
+  const E rows{(void*)base, (size_t)hd, 2, {{one, p}, {hd, h}, {kv * hd, s}, {layer, l}}};
+  const E two{(void*)base, (size_t)hd, 2, {{2 * one, p}, {size * hd, h}, {hd, s}, {2 * one * pages, l}}};
+  int bad = 0;
+  for (const E& e : {dense, rows})
+    for (int i = 0; i < layers; i++) {
+      const uintptr_t end = base + 2 * (layer * i + pages * one);
+      bad += meet(E{(void*)end, (size_t)gap, 2, {}}, e) || meet(e, E{(void*)end, (size_t)gap, 2, {}});
+      bad += !meet(E{(void*)(end - 4), 1, 4, {}}, e) || !meet(e, E{(void*)(end - 4), 1, 4, {}});
+      if (i + 1 < layers) bad += !meet(E{(void*)(end + 4), (size_t)gap, 2, {}}, e);
+    }
+  for (int i = 0; i < layers * pages; i++) {  // values between the keys
+    bad += meet(E{(void*)(base + 2 * (2 * i + 1) * one), (size_t)one, 2, {}}, two);
+    bad += !meet(E{(void*)(base + 2 * (2 * i + 1) * one - 4), 1, 4, {}}, two);
+  }
+  const E copy{(void*)(base + 2 * one), (size_t)hd, 2, {{2 * one, p}, {size * hd, h}, {hd, s}, {2 * one * pages, l}}};
+  bad += meet(copy, two) || nrq::copies_meet(two, copy.first) || !nrq::copies_meet(two, (void*)(base + 2 * one - 16));
+  bad += !nrq::copies_meet(two, (void*)(base + 4 * one * pages * (layers - 1))) || nrq::copies_meet(two, (void*)(base + 4 * one * pages * layers));
+  printf("%d\\n", bad);
+  return bad != 0;
+}
+''')
+    subprocess.run(["g++", "-O1", "-Wall", "-Werror", "-fsanitize=undefined", "-fno-sanitize-recover", "-static-libubsan", "-I",
+                    os.path.join(ROOT, "nightrun_amd", "csrc"), str(src), "-o", str(tmp_path / "four")], check=True)
+    subprocess.run([str(tmp_path / "four")], check=True)
+
+
 SHARED = [
     ("nrq_dev_norm_rope", "y", "x", 128), ("nrq_dev_norm_rope", "y", "weight", 0), ("nrq_dev_norm_rope", "y", "freqs", 0),
     ("nrq_dev_norm_rope_append", "y", "k", 0), ("nrq_dev_norm_rope_append", "y", "pos", 0),
