@@ -47,7 +47,8 @@ int nrq_dev_norm_rope_append(void *y, const void *q, const void *k, const void *
  * it alone; with window > 0 only to what is less than `window` rotary positions before its own. Where lens[b] is less than the
  * nodes, those at negative positions are attended to by none. Arguments, empty rows, precision and workspace
  * (nrq_tree_attention_workspace) else as for nrq_dev_paged_attention; out and lse share no memory with the inputs or one
- * another. What an infinity or a NaN in the cache costs: rows of its KV head are done again one position after the other, so that a long
+ * another. An infinity among the values that a row attends to is the row's output, however small its weight (where its score is
+ * -infinity, a NaN). What an infinity or a NaN in the cache costs: rows of its KV head are done again one position after the other, so that a long
  * sequence takes a hundred times as long. */
 int nrq_tree_attention_workspace(size_t seqs, size_t n_new, size_t heads, const nrq_paged_kv *kv, size_t *bytes);
 int nrq_dev_tree_attention(void *out, const void *q, int dtype, size_t n_new, size_t heads, const int64_t strides[6],

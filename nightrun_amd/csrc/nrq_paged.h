@@ -289,6 +289,10 @@ __device__ __forceinline__ PaTree pa_node(const PaTree& t, int j) {
   return PaTree{(uint64_t)hi << 32 | lo, __shfl(t.depth, j)};
 }
 
+// A sum of weighted values in another unit: an infinity stays one however far the maximum has gone since, so that the outcome does
+// not go by how the positions are shared among waves and workgroups.
+__device__ __forceinline__ float pa_less(float o, float by) { return fabsf(o) == INFINITY ? o : o * by; }
+
 // The same stretch of one wave without matrix instructions, position by position and row by
 // row, 32 positions of every `step`, for values that hold an infinity or a NaN: there the products of weights
 // that are 0 (rows that do not see a position) or of the pieces of a weight would give
@@ -334,7 +338,11 @@ __device__ __forceinline__ void pa_plain(const PaArgs& A, int b, int head, int r
         const float p = __builtin_amdgcn_exp2f(s - (mn == -INFINITY ? 0.0f : mn) + PaType<T>::kOffset);
         l = l * by + p;
         for (int e = 0; e < E; e++)
-          if (64 * e + lane < HD) o[e] = o[e] * by + p * (float)((const T*)L.kv.v)[at + 64 * e + lane];
+          if (64 * e + lane < HD) {
+            const float v = (float)((const T*)L.kv.v)[at + 64 * e + lane];
+            // a weight of e^s is above zero however small, also where f32 has it as 0
+            o[e] = TREE ? pa_less(o[e], by) + (fabsf(v) == INFINITY && s > -INFINITY ? v : p * v) : o[e] * by + p * v;
+          }
         m = mn;
       }
     for (int e = 0; e < E; e++)

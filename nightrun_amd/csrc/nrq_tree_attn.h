@@ -447,26 +447,23 @@ __global__ __launch_bounds__(64 * W, ta_waves(HD, NQ)) void tree_kernel(PaArgs A
           for (int k = 1; k < WP; k++) mm = fmaxf(mm, ex_ml[wr + k * WR][c][0]);
           const float ref = mm == -INFINITY ? 0.0f : mm, own = __builtin_amdgcn_exp2f(m - ref);
           l *= own;
-          const bool none = !(own > 0.0f || ref != ref);  // saw nothing, or nothing of weight
 #pragma unroll
           for (int d = 0; d < DB; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) acc[d][i] = none ? 0.0f : acc[d][i] * own;
+            for (int i = 0; i < 16; i++) acc[d][i] = pa_less(acc[d][i], own);
 #pragma unroll
           for (int k = 1; k < WP; k++) {
             const int other = wr + k * WR;
             const float by = __builtin_amdgcn_exp2f(ex_ml[other][c][0] - ref);
             l += ex_ml[other][c][1] * by;
-            if (by > 0.0f || ref != ref) {
 #pragma unroll
-              for (int d = 0; d < DB; d++)
+            for (int d = 0; d < DB; d++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                  const f32x4 y = ex[((other - WR) * DB * 4 + 4 * d + i) * 64 + lane];
+              for (int i = 0; i < 4; i++) {
+                const f32x4 y = ex[((other - WR) * DB * 4 + 4 * d + i) * 64 + lane];
 #pragma unroll
-                  for (int j = 0; j < 4; j++) acc[d][4 * i + j] += y[j] * by;
-                }
-            }
+                for (int j = 0; j < 4; j++) acc[d][4 * i + j] += pa_less(y[j], by);
+              }
           }
           m = mm;
         }
@@ -542,7 +539,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(PaArgs A, int wide_o) {
     l += x.y * by;
     const float* p = A.part_o + s * HD + F * c;
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] += p[e / F * 16 * F + e % F] * by;
+    for (int e = 0; e < E; e++) o[e] += pa_less(p[e / F * 16 * F + e % F], by);
   }
   if constexpr (G > 1) {
 #pragma unroll

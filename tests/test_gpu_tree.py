@@ -583,6 +583,51 @@ def test_tree_infinities_in_every_shape(gpu, kind, cache, hd, heads, kv, new):
             assert np.all(np.isposinf(got[b, j, :, hd - 1])) == below, (b, j)
 
 
+@pytest.mark.parametrize("kind,cache,hd,heads,new", [("f16", "f16", 64, 1, 1), ("bf16", "bf16", 64, 8, 40), ("f32", "bf16", 128, 4, 20),
+                                                     ("f32", "f16", 128, 4, 40), ("bf16", "bf16", 128, 4, 64), ("f16", "f16", 256, 4, 30),
+                                                     ("f32", "f16", 32, 2, 5), ("bf16", "f16", 96, 1, 9)])
+def test_tree_infinities_of_little_weight(gpu, kind, cache, hd, heads, new):
+    """A weight is positive however small: an infinity that a row sees is its output, also where f32 holds no such weight, whether
+    the row's largest score is in the same 32 positions, with another wave or with another workgroup, before or behind. Infinities of
+    both signs, and a NaN, give NaN. Keys are 0 but the largest's: e^-256 of its weight for all others, so that the output is its value."""
+    import torch
+
+    from nightrun_amd import serve
+
+    n, size, pages = 3000, 16, 196
+    places = [0, 7, 31, 32, 70, 127, 128, 333, 1000, 1500, 2048, 2900]
+    pairs = [(a, b) for a in places for b in places if a != b][::3] + [(7, 31), (31, 7), (7, 32), (32, 7), (7, 70), (70, 7), (333, 1500)]
+    seqs = 8
+    g = gen(hd + new)
+    q = torch.zeros(seqs, new, heads, hd, dtype=dt(kind))
+    q[..., 0] = 16.0
+    qd, t = q.cuda(), torch.from_numpy(trees(new, seqs, new)).cuda()
+    table = torch.arange(seqs * pages, dtype=torch.int32, device="cuda").view(seqs, pages)
+    for i in range(0, len(pairs), seqs):
+        some = (pairs[i:] + pairs)[:seqs]
+        for kinds in ((1,), (-1,), (1, -1), (float("nan"),)):
+            k = torch.zeros(seqs, pages * size, hd, dtype=dt(cache))
+            v = torch.randn(seqs, pages * size, hd, generator=g).to(dt(cache))
+            want = np.zeros((seqs, hd))
+            for b, (top, at) in enumerate(some):
+                k[b, top, 0] = 16.0
+                want[b] = v[b, top].double().numpy()
+                for j, sign in enumerate(kinds):  # the second somewhere else
+                    v[b, (at + 900 * j) % n if (at + 900 * j) % n != top else top + 1, hd - 3] = sign * float("inf")
+            kp, vp = (x.view(-1, 1, size, hd).cuda() for x in (k, v))
+            y = torch.empty_like(qd)
+            serve.tree_attention(y, qd, kp, vp, table, torch.full((seqs,), n + new, dtype=torch.int32, device="cuda"), t, 1.0)
+            got = f64(y)
+            hit = got[..., hd - 3]
+            if len(kinds) == 2 or kinds[0] != kinds[0]:
+                assert np.isnan(hit).all(), (some, kinds, hit[:, 0, 0])
+            else:
+                assert np.all(hit == kinds[0] * np.inf), (some, kinds, hit[:, 0, 0])
+            got[..., hd - 3] = want[:, None, None, hd - 3]
+            tol = PIECES[kind, cache] * 8 + half_step(kind) * np.abs(want)
+            assert np.all(np.abs(got - want[:, None, None]) <= tol[:, None, None]), (some, kinds)
+
+
 @pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
 @pytest.mark.parametrize("new,width", [(1, 1), (3, 1), (12, 1), (40, 3), (12, 900), (40, 900)])
 def test_tree_weights_keep_32_bits(gpu, hd, new, width):
