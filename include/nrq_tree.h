@@ -22,7 +22,8 @@ extern "C" {
 
 /* nrq_dev_rope of normed rows: each head's row x of head_dim values becomes
  *   x / sqrt(mean of x^2 + eps) * weight
- * before it is rotated, in 32 bits throughout and rounded once. weight is f32
+ * before it is rotated, in 32 bits throughout and rounded once: a row whose squares add up to 2^128 or more becomes
+ * zeros, and a square below 2^-150 is 0. weight is f32
  * [head_dim], the same for all heads (NULL: ones). eps >= 0; a row of zeros with eps 0 gives NaN. Arguments else as
  * for nrq_dev_rope; y may be x (then with the same strides), but shares no memory with it otherwise, and none with weight, pos or freqs. */
 int nrq_dev_norm_rope(void *y, const void *x, int dtype, size_t tokens, size_t heads, size_t head_dim,
@@ -49,7 +50,8 @@ int nrq_dev_norm_rope_append(void *y, const void *q, const void *k, const void *
  * (nrq_tree_attention_workspace) else as for nrq_dev_paged_attention; out and lse share no memory with the inputs or one
  * another. An infinity among the values that a row attends to is the row's output, however small its weight (where its score is
  * -infinity, a NaN). What an infinity or a NaN in the cache costs: rows of its KV head are done again one position after the other, so that a long
- * sequence takes a hundred times as long. */
+ * sequence takes a hundred times as long. How rows are shared out goes by the table's width, as the lengths are on the device: in a
+ * table far wider than its sequences are long, short ones take up to a third longer. */
 int nrq_tree_attention_workspace(size_t seqs, size_t n_new, size_t heads, const nrq_paged_kv *kv, size_t *bytes);
 int nrq_dev_tree_attention(void *out, const void *q, int dtype, size_t n_new, size_t heads, const int64_t strides[6],
                            const nrq_paged_kv *kv, const nrq_page_table *table, const int32_t *lens,

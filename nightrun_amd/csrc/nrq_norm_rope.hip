@@ -8,9 +8,16 @@
 // before the angles are formed, and each turn's while the turn before it is finished.
 //
 // Memory bounds it: 16,381 tokens of 33 heads of 128 in f16 (277 MB both ways, read and written once as the counters show)
-// take 63.6 us, 4.35 TB/s (93 without the rows of the next turn on their way and with the sums through LDS). 1536 nodes of 32 + 8 + 8
-// heads into a bf16 cache (38 MB) take 14.2 us, twice what their bytes do: a workgroup has three turns, before them positions,
-// pages and angles. One token takes as long as a launch does.
+// take 60 to 64 us, 4.5 TB/s (93 without the rows of the next turn on their way and with the sums through LDS). 1536 nodes of 32 + 8 + 8
+// heads into a bf16 cache (38 MB) take 14.3 us, twice what their bytes do: a workgroup has two turns, the second of them half empty, and before
+// them positions, pages and angles. The append of a prompt of 4096 (101 MB) takes 23.1, 4.4 TB/s; two of its registers spill under the bound of
+// four waves a SIMD (bf16 and f16 rows). One token takes as long as a launch does.
+//
+// Rows that do not go in accesses of 16 bytes (pointers, strides, or a rotated part that ends inside one: with f16 rows and NEOX pairs one
+// of 40 dimensions, say) take several times as long: one value an access, one row of a lane in flight, and sixteen places for items, as
+// rows of 1024 need, of which a head of 128 fills two. 16,381 tokens of 32 heads of 128, f16, 40 dimensions rotated: 515 us, where
+// all 128 take 48; heads of 96 with 24 of them 461; the append of 4096 tokens 225. Without norms (a place of its own for each token)
+// that append takes 128, and 70 in nrq_rope.hip, which takes no such places and keeps four rows in flight.
 #include "nrq_page.h"
 #include "nrq_tree_launch.h"
 #include "nrq_turn.h"
@@ -247,8 +254,8 @@ __global__ __launch_bounds__(kNrNT, K == 1 && V > 1 ? 4 : 1) void norm_rope_kern
 template <typename T, typename C, int V, int K, int A, bool APPEND, bool NORM>
 hipError_t nr_launch(NrArgs& P) {
   const RopeLaunch& L = P.L.r;
-  // Tokens of a workgroup: as many as make one angle a thread, fewer where the card (1024 workgroups) would not
-  // be full (1536 nodes: 14.2 us so, 18.4 with one token a workgroup); with few tokens their rows are spread over more workgroups, a row a group of lanes in each.
+  // Tokens of a workgroup: as many as make one angle a thread, fewer where fewer than 512 to 1024 workgroups would be
+  // left (1536 nodes: 768 of them, 14.3 us; 18.4 with one token a workgroup); with few tokens their rows are spread over more workgroups, a row a group of lanes in each.
   int t = kNrNT / L.nf;
   t = t < 1 ? 1 : (t > kNrTokens ? kNrTokens : t);
   if (t > (L.tokens - 1) / 1024 + 1) t = (L.tokens - 1) / 1024 + 1;
@@ -290,7 +297,8 @@ hipError_t nr_launch_t(const NormRopeLaunch& N) {
   P.inv = 1.0f / (float)L.hd;
   P.lanes = 1;
   while (P.lanes < P.items && P.lanes < 64) P.lanes *= 2;
-  // heads of 1024: 256 accesses of 4, or 1023 of 1 (where all but two dimensions are copied)
+  // heads of 1024: 256 accesses of 4, or 1023 of 1 (where all but two dimensions are copied); the latter's kernel is
+  // every row's that is not wide (at the file's head: what that costs)
   if (!wide) return nr_launch<T, C, 1, 16, 1, APPEND, NORM>(P);
   if (P.items <= 64) return nr_launch<T, C, V, 1, 2, APPEND, NORM>(P);
   return nr_launch<T, C, V, 4, 1, APPEND, NORM>(P);

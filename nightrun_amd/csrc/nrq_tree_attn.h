@@ -4,7 +4,7 @@
 //
 // With R rows (nodes x query heads of a KV head) a position of a KV head costs 4 R head_dim operations for 4 head_dim bytes,
 // R operations a byte: groups of 32 rows that each read the keys and values for themselves ask the L2 for
-// more than it delivers (24 sequences of 64 nodes: 824 us so, 160 here). So a unit is up to 256 rows, and its keys and values
+// more than it delivers (24 sequences of 64 nodes, f16: 824 us so, 174 here). So a unit is up to 256 rows, and its keys and values
 // pass through LDS once for all of them: stage by stage, the next one on its way from memory to LDS while one is multiplied.
 //
 // A wave owns 32 rows; where there are fewer of those than waves, each takes a part of each stage's positions, and their results
@@ -19,9 +19,12 @@
 // weights in two pieces) take 351 to 358 us, 10 of them the join: the matrix units work half of the clocks, vector instructions the other half, and the
 // clock is down to 1.75 GHz, the power limit; without its loads it would take 300. Orders of instructions, priorities and stages that
 // keep both busier change nothing there. 64 rows a wave halve the reads of LDS but leave the 256 registers that
-// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, bf16, 307 MB) 112 to 116 us, 99 with the weights in two pieces instead of
-// three, which left them 16 bits; a unit's beginning and end (its length, pages, queries and first stage in sequence, its parts) are a third of it. 13 sequences under a window
-// of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 73 to 77. One sequence of 1001 positions by 8 nodes 13.4: two launches, one tile a workgroup.
+// vector instructions reach: 415. 24 sequences of up to 6000 by 32 nodes (128 rows, bf16, 307 MB) 112 to 118 us, 15 of them the join: the
+// matrix units work 40% of the clocks, vector instructions 45%; with the weights in two pieces instead of three, which left them 16 bits, 99. In f16
+// 105. What else it takes is units' beginnings and ends, one after the other: length, pages, queries and first stage, and parts that are
+// written and read again. 13 sequences under a window of 4096 by 25 nodes, f32 queries in two pieces (178 MB) 72 to 77: the same, and two to six
+// registers that spill (f32 queries over an f16 cache, heads of 128: the pieces of both leave no room). One sequence of 1001 positions by 8
+// nodes 13.7: two launches, one tile a workgroup, half of whose waves have no rows.
 #pragma once
 
 #include "nrq_paged.h"
@@ -31,11 +34,12 @@ namespace nrq {
 
 constexpr int kTaCus = 256;
 // What the beginning and the end of a unit cost, in tiles: stretches of many short units are as long as those of a few long ones. 24
-// sequences of 250 to 6000 positions by 32 nodes take 156, 127, 114, 115 us with 0, 1, 2, 3, 119 with 5; 13 of one length 91, 85, 81, 79 and 80.
+// sequences of 250 to 6000 positions by 64 nodes take 214, 182, 174, 174 us with 0, 1, 2, 3, 181 with 5 (f16), by 32 nodes 122, 107, 105, 105,
+// 108 and 128, 116, 117, 118, 121 (bf16); 13 of one length 105, 104, 102, 102, 104.
 constexpr int kTaSetup = 3;
 // Workgroups of a unit, on average, from which on the join takes a row a workgroup, 16 stretches side by side, else four rows, four
-// stretches side by side: one KV head over 131,072 positions by 4 nodes 36.7 us so, 51.8 the other way (92.8 with one after the
-// other); two sequences of 8 heads (16 workgroups a unit) 345 and 334, 24 by 32 nodes (three) 124 and 108.
+// stretches side by side: one KV head over 131,072 positions by 4 nodes 38 us so, 56 the other way (93 with one after the
+// other); two sequences of 8 heads (16 workgroups a unit) 358 and 354, 24 by 32 nodes (three) 128 and 105.
 constexpr int kTaShared = 32;
 
 namespace {
@@ -602,7 +606,7 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
   const int rows = L.n_new * (L.heads / L.kv.n_kv);
   // Units of as many rows as leave each workgroup three tiles, as far as the table goes (the lengths are on the device). One sequence by 64
   // nodes of 4 heads: 4000 positions 35 us in units of 256 rows, 28 of 64; 16,000 48 and 50; 32 nodes, 8000 positions 35 in units of
-  // 128 and 29 of 64.
+  // 128 and 29 of 64. So a table far wider than its sequences are long costs short ones: those 4000 positions take 37 in one for 131,072.
   const int64_t tiles = (int64_t)L.table.seqs * L.kv.n_kv * (((int64_t)L.table.width * L.kv.page_size + kTile - 1) / kTile);
   auto fills = [&](int per, int wgs) { return tiles * ((rows + per - 1) / per) >= 3 * wgs; };
   if constexpr (HD > 128 || NQ > 2) {
@@ -611,7 +615,7 @@ hipError_t ta_launch_rows(const PagedAttnLaunch& L) {
   } else {
     // More than 128 rows: one workgroup of eight waves a CU (two long sequences by 64 nodes 359 us, in two units of 128 rows 414, in four
     // of 64 531). Else two of four waves, one of which multiplies while the other begins or ends a unit (24 sequences by 32 nodes
-    // 96 us, with one of eight waves 104).
+    // in f16 105 us, with one of eight waves 106.5; in bf16 118 and 116).
     constexpr int kTP = HD == 128 || HD == 96 ? 64 : 128;
     if (rows > 128 && fills(256, kTaCus)) return ta_launch<T, HD, 8, 8, HD == 96 ? 128 : kTP, NQ>(L);
     if (rows > 64 && fills(128, 2 * kTaCus)) return ta_launch<T, HD, 4, 4, kTP, NQ>(L);
