@@ -1057,7 +1057,7 @@ class Arena:
     """Arguments of a C entry in one block of memory, each at the beginning of a slot of its own. Everything is zeros: whatever a
     call is made of them stays in their memory."""
 
-    SLOT = 4 << 20
+    SLOT = 8 << 20
 
     def __init__(self, entry):
         import torch
@@ -1119,9 +1119,9 @@ class Arena:
 
         pools, n = self.pools(), C.c_size_t()
         kv = PagedKv(0, 0, *pools["kv"])
-        assert _lib.lib().nrq_tree_attention_workspace(2, 3, 2, C.byref(kv), C.byref(n)) == 0 and n.value < self.SLOT // 2
-        return dict(out=(3072, 4), q=(3072, 4), dtype=0, n_new=3, heads=2, strides=[384, 128, 64, 384, 128, 64], **pools,
-                    lens=(8, 4), parents=(24, 4), counts=(8, 4), scale=0.1, window=0, lse=(48, 4), ws=(n.value, 16),
+        assert _lib.lib().nrq_tree_attention_workspace(2, 5, 2, C.byref(kv), C.byref(n)) == 0 and n.value < self.SLOT
+        return dict(out=(5120, 4), q=(5120, 4), dtype=0, n_new=5, heads=2, strides=[640, 128, 64, 640, 128, 64], **pools,
+                    lens=(8, 4), parents=(40, 4), counts=(8, 4), scale=0.1, window=0, lse=(80, 4), ws=(n.value, 16),
                     ws_bytes=n.value)
 
     def verify_tree(self):
