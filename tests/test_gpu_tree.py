@@ -583,6 +583,58 @@ def test_tree_infinities_in_every_shape(gpu, kind, cache, hd, heads, kv, new):
             assert np.all(np.isposinf(got[b, j, :, hd - 1])) == below, (b, j)
 
 
+def test_tree_broadcast_inputs(gpu):
+    """Queries that repeat, sequences of one row of the table, all pages one: strides of 0 are read like any other."""
+    import torch
+
+    from nightrun_amd import serve
+
+    g = gen(21)
+    for new in (3, 40):
+        c = Cache(gen(new), [100 + new], 2, 64, 16, "f16")
+        kp, vp, table, _ = c.dev()
+        q = normal(g, 1, 1, 4, 64, kind="f16").expand(3, new, 4, 64)
+        t = torch.from_numpy(trees(new, 3, new)).cuda()
+        lens = torch.tensor([100 + new, 64, 31 + new], dtype=torch.int32, device="cuda")
+        y, z = (torch.empty(3, new, 4, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+        serve.tree_attention(y, q, kp, vp, table.expand(3, -1), lens, t, 0.125, window=50)
+        serve.tree_attention(z, q.contiguous(), kp, vp, table.repeat(3, 1), lens, t, 0.125, window=50)
+        assert torch.equal(y, z)
+        one = kp[:1].expand(7, -1, -1, -1), vp[:1].expand(7, -1, -1, -1)
+        same = torch.zeros_like(table).expand(3, -1)
+        serve.tree_attention(y, q, *one, table.clamp(max=6).expand(3, -1), lens, t, 0.125)
+        serve.tree_attention(z, q, kp, vp, same, lens, t, 0.125)
+        assert torch.equal(y, z)
+
+
+def test_tree_more_sequences_than_a_grid_has_rows(gpu):
+    """70,000 sequences of a few positions, three in four without nodes."""
+    import torch
+
+    from nightrun_amd import serve
+
+    n = 70000
+    g = gen(22)
+    kp, vp = (torch.randn(50, 1, 4, 32, generator=g).half().cuda() for _ in range(2))
+    table = torch.randint(0, 50, (n, 2), generator=g, dtype=torch.int32).cuda()
+    lens = torch.randint(2, 9, (n,), generator=g, dtype=torch.int32).cuda()
+    counts = (2 * (torch.arange(n) % 4 == 0)).to(torch.int32).cuda()
+    q = normal(g, n, 2, 1, 32, kind="f16")
+    y = torch.full_like(q, 5.0)
+    serve.tree_attention(y, q, kp, vp, table, lens, torch.tensor([[-1, 0]], dtype=torch.int32, device="cuda").repeat(n, 1),
+                         32 ** -0.5, counts=counts)
+    some = torch.arange(0, n, 4, device="cuda")
+    k, v = (x[table[some].long()].float().reshape(len(some), 8, 32) for x in (kp, vp))
+    hi = lens[some].long()[:, None] - 2 + torch.arange(2, device="cuda")
+    s = (q[some, :, 0].float()[:, :, None] * k[:, None]).sum(-1) * 32 ** -0.5
+    w = torch.softmax(s.masked_fill(torch.arange(8, device="cuda") > hi[..., None], -math.inf), -1)
+    want = (w[..., None] * v[:, None]).sum(2)
+    # 36 products and sums of at most |s| times 4 |v| in f32 on either side, and the output's rounding
+    assert float((y[some, :, 0].float() - want).abs().max()) <= 2.0 ** -11 * 5 + 1e-4
+    y[some] = 5.0
+    assert bool((y == 5.0).all())
+
+
 @pytest.mark.parametrize("kind,cache,hd,heads,new", [("f16", "f16", 64, 1, 1), ("bf16", "bf16", 64, 8, 40), ("f32", "bf16", 128, 4, 20),
                                                      ("f32", "f16", 128, 4, 40), ("bf16", "bf16", 128, 4, 64), ("f16", "f16", 256, 4, 30),
                                                      ("f32", "f16", 32, 2, 5), ("bf16", "f16", 96, 1, 9)])
